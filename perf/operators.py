@@ -1,0 +1,372 @@
+"""The microscaled 4-bit operators and the router's balance, as cases that can be timed and compared.
+
+Five kinds, each through the entry point that a program calls:
+  quant    mx4_quantize then mx4_dequantize (rows to 4-bit values with a power-of-two scale per 32, and back)
+  linear   MX4Linear.run (4-bit weights, 16-bit rows)
+  gemm     mx4_quantize of the rows, then mx4_gemm (both operands in 4 bits)
+  moe      mx4_moe_forward (routed experts with 4-bit weights, optionally a shared expert)
+  balance  route_balance and route_balance_grad (per-expert counts, balance loss, gradient of the router logits)
+
+The format: 32 consecutive values of a row share a scale 2^(s - 127) held in a byte (255: not a number); a value is
+sign, two exponent bits and one mantissa bit (0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the even one in the low half.
+"""
+import importlib
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+# ------------------------------------------------------------------------------------------------ cases
+def listed():
+    return [
+        # the rows of a few sequences that decode together: the smallest call, all latency
+        dict(name="quant_decode", kind="quant", rows=4, k=4096, dtype="bf16"),
+        # the input of the widest projection of a 31B-class dense model, one prefill chunk (ragged)
+        dict(name="quant_prefill", kind="quant", rows=2039, k=5376, dtype="fp16"),
+        # one decode token through one projection
+        dict(name="linear_decode", kind="linear", rows=1, k=4096, n=4096, dtype="bf16", out="bf16", bias=False),
+        # a verify block of 6 tokens through the widest projection
+        dict(name="linear_verify", kind="linear", rows=6, k=5376, n=21504, dtype="fp16", out="fp32", bias=False),
+        # a ragged prompt through the widest projection, with a bias
+        dict(name="linear_prefill", kind="linear", rows=1021, k=5376, n=21504, dtype="bf16", out="bf16", bias=True),
+        # a short prompt through a fused q|k|v projection, rows quantised first
+        dict(name="gemm_short", kind="gemm", rows=77, k=4096, n=6144, dtype="bf16", out="bf16"),
+        # a full prefill chunk through the widest projection, rows quantised first: the largest dense call
+        dict(name="gemm_prefill", kind="gemm", rows=2048, k=5376, n=21504, dtype="bf16", out="bf16"),
+        # one decode token through a sparse layer of many small experts
+        dict(name="moe_decode", kind="moe", rows=1, H=2048, I=512, E=512, topk=10, shared=False, dtype="fp16",
+             act="silu"),
+        # one GPU's share of a layer of wide experts with a shared one: decode rows and a prefill chunk together
+        dict(name="moe_mixed", kind="moe", rows=260, H=7168, I=2048, E=32, topk=2, shared=True, dtype="bf16",
+             act="silu"),
+        # a prefill chunk over many small experts
+        dict(name="moe_prefill", kind="moe", rows=1024, H=2560, I=640, E=512, topk=10, shared=False, dtype="fp16",
+             act="silu"),
+        # the rows of one decode step: per-expert load while serving, sigmoid scores
+        dict(name="balance_step", kind="balance", rows=16, E=160, topk=8, score="sigmoid", padded=False),
+        # a batch of padded sequences while a router of many experts is tuned
+        dict(name="balance_batch", kind="balance", rows=32768, E=512, topk=10, score="softmax", padded=True),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _dim(rng, lo, hi):
+    return 32 * max(1, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi))) / 32)))
+
+
+def draw(rng):
+    while True:
+        kind = rng.choice(("quant", "linear", "linear", "gemm", "gemm", "moe", "moe", "balance"))
+        t = rng.choice(("fp16", "bf16"))
+        if kind == "quant":
+            c = dict(kind=kind, rows=_log(rng, 1, 4096), k=_dim(rng, 512, 21504), dtype=rng.choice(("fp16", "bf16", "fp32")))
+        elif kind == "linear":
+            n = _dim(rng, 512, 21504) if rng.random() < 0.75 else _log(rng, 500, 20000)
+            c = dict(kind=kind, rows=_log(rng, 1, 1024), k=_dim(rng, 512, 8192), n=n, dtype=t, out=rng.choice((t, "fp32")),
+                     bias=rng.random() < 0.3)
+        elif kind == "gemm":
+            c = dict(kind=kind, rows=_log(rng, 1, 2048), k=_dim(rng, 512, 8192), n=_dim(rng, 512, 21504), dtype=t,
+                     out=rng.choice((t, "fp32")))
+        elif kind == "moe":
+            E = rng.choice((8, 32, 64, 128, 160, 256, 512))
+            c = dict(kind=kind, rows=_log(rng, 1, 1024), H=_dim(rng, 1024, 7168), I=_dim(rng, 512, 2048), E=E,
+                     topk=2 if E == 8 else rng.choice((4, 8, 10)), shared=rng.random() < 0.4, dtype=t,
+                     act=rng.choice(("silu", "gelu_tanh")))
+        else:
+            E = rng.choice((8, 60, 64, 128, 160, 256, 384, 512))
+            c = dict(kind=kind, rows=_log(rng, 1, 32768), E=E, topk=2 if E == 8 else rng.choice((4, 6, 8)),
+                     score=rng.choice(("softmax", "sigmoid", "sqrt_softplus")), padded=rng.random() < 0.5)
+        # no dearer than the largest listed ones of the kind: operations, and weights to make and read
+        f = work(c)["flops"]
+        if kind == "linear" and f > 2.3e11 or kind == "gemm" and f > 4.7e11:
+            continue
+        if kind == "moe" and (f > 1.0e11 or 3 * c["H"] * c["I"] * (E + c["shared"]) > 2.6e9):
+            continue
+        if kind == "quant" and c["rows"] * c["k"] > 2039 * 5376:
+            continue
+        return c
+
+
+# ------------------------------------------------------------------------------------------------ work
+def work(case):
+    """Bytes: codes and scales of every matrix touched once (routed experts: those that a uniform routing is expected to
+    touch), rows in and out once. Operations: the products; for rows of scores and for quantising a few per value."""
+    c, r = case, case["rows"]
+    size = {"fp16": 2, "bf16": 2, "fp32": 4}
+    if c["kind"] == "quant":          # values in, values out
+        return {"bytes": 2.0 * size[c["dtype"]] * r * c["k"], "flops": 4.0 * r * c["k"]}
+    if c["kind"] in ("linear", "gemm"):
+        b = c["k"] * c["n"] * 17 / 32 + 2 * r * c["k"] + size[c["out"]] * r * c["n"]
+        return {"bytes": float(b), "flops": 2.0 * r * c["k"] * c["n"]}
+    if c["kind"] == "moe":
+        E, k, s = c["E"], c["topk"], int(c["shared"])
+        touched = E * (1 - (1 - k / E) ** r) + s
+        b = touched * 3 * c["H"] * c["I"] * 17 / 32 + 4 * r * c["H"] + 8 * r * k
+        return {"bytes": float(b), "flops": 6.0 * r * (k + s) * c["H"] * c["I"]}
+    return {"bytes": 8.0 * r * c["E"] + 4.0 * r * c["topk"] + r * c["padded"], "flops": 12.0 * r * c["E"]}
+
+
+# ------------------------------------------------------------------------------------------------ the plain forms
+def _lut(device, dtype=torch.float32):
+    return torch.tensor(VALUES + tuple(-v for v in VALUES), dtype=dtype, device=device)
+
+
+def _quantise(x):
+    """codes uint8 [..., k / 2] and scales uint8 [..., k / 32] of rows x."""
+    v = x.float().reshape(*x.shape[:-1], -1, 32)
+    top = v.abs().amax(-1, keepdim=True)
+    e = torch.where(top > 0, torch.frexp(top).exponent.float() - 3.0, torch.full_like(top, -127.0)).clamp(-127.0, 127.0)
+    a = v.abs().double() * torch.exp2(-e.double())
+    # midpoints between neighbours; at a midpoint the neighbour with the even code is taken
+    code = (a > 0.25).int() + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0)
+    code = code + 8 * (v < 0)
+    code = code.reshape(*x.shape[:-1], -1, 2)
+    return (code[..., 0] + 16 * code[..., 1]).to(torch.uint8), (e[..., 0] + 127.0).to(torch.uint8)
+
+
+def _values(codes, scales):
+    lut = _lut(codes.device)
+    v = torch.stack((lut[(codes & 15).int()], lut[(codes >> 4).int()]), -1).reshape(*scales.shape, 32)
+    return (v * torch.exp2(scales.float() - 127.0)[..., None]).reshape(*scales.shape[:-1], -1)
+
+
+def _activation(g, u, act):
+    if act == "silu":
+        return g / (1.0 + torch.exp(-g)) * u
+    return 0.5 * g * (1.0 + torch.tanh(0.7978845608028654 * (g + 0.044715 * g * g * g))) * u
+
+
+def _plain_moe(c, s):
+    x, ids, w = s["x"].float(), s["ids"].long(), s["w"]
+    r, E = x.shape[0], c["E"]
+    (gc, gs), (uc, us), (dc, ds) = s["weights"]
+    if r * c["topk"] <= 64:           # the picked experts' weights, pair by pair
+        pick = ids.reshape(-1)
+        g = torch.matmul(_values(gc[pick], gs[pick]).reshape(r, c["topk"], c["I"], c["H"]), x[:, None, :, None])[..., 0]
+        u = torch.matmul(_values(uc[pick], us[pick]).reshape(r, c["topk"], c["I"], c["H"]), x[:, None, :, None])[..., 0]
+        h = _activation(g, u, c["act"])
+        y = torch.matmul(_values(dc[pick], ds[pick]).reshape(r, c["topk"], c["H"], c["I"]), h[..., None])[..., 0]
+        out = (y * w[..., None]).sum(1)
+    else:                             # every expert over every row, weighted by zero where it was not picked
+        out = torch.zeros_like(x)
+        for e in range(E):
+            we = (w * (ids == e)).sum(1, keepdim=True)
+            h = _activation(x @ _values(gc[e], gs[e]).t(), x @ _values(uc[e], us[e]).t(), c["act"])
+            out += we * (h @ _values(dc[e], ds[e]).t())
+    if c["shared"]:
+        h = _activation(x @ _values(gc[E], gs[E]).t(), x @ _values(uc[E], us[E]).t(), c["act"])
+        out += h @ _values(dc[E], ds[E]).t()
+    return out.to(s["x"].dtype)
+
+
+def _plain_balance(c, s):
+    z, ids, E, k = s["logits"], s["ids"], c["E"], c["topk"]
+    live = s["mask"] if c["padded"] else torch.ones(z.shape[0], dtype=torch.bool, device=z.device)
+    n = live.sum()
+    counts = torch.zeros(E + 1, dtype=torch.int32, device=z.device)
+    slot = torch.where(live[:, None], ids, torch.full_like(ids, E)).reshape(-1).long()
+    counts.index_add_(0, slot, torch.ones_like(slot, dtype=torch.int32))
+    counts = counts[:E]
+    if c["score"] == "softmax":
+        sc = torch.exp(z - z.amax(1, keepdim=True))
+        inner = torch.ones_like(z)
+    elif c["score"] == "sigmoid":
+        sc = 1.0 / (1.0 + torch.exp(-z))
+        inner = 1.0 / (1.0 + torch.exp(z))
+    else:
+        sp = torch.where(z > 20.0, z, torch.log1p(torch.exp(z.clamp(max=20.0))))
+        sc = torch.sqrt(sp)
+        inner = 0.5 / (1.0 + torch.exp(-z)) / sp
+    p = sc / sc.sum(1, keepdim=True)
+    prob = (p * live[:, None]).sum(0) / n
+    frac = counts.float() * (E / (k * n.float()))
+    loss = s["coef"] * (frac * prob).sum()
+    a = s["grad"] * s["coef"] * frac / n
+    d = p * inner * (a - (p * a).sum(1, keepdim=True)) * live[:, None]
+    return {"loss": loss.reshape(1), "counts": counts, "prob": prob, "dlogits": d}
+
+
+def run(state):
+    c = state["case"]
+    if own:
+        exl3 = state["exl3"]
+        if c["kind"] == "quant":
+            return exl3.mx4_dequantize(exl3.mx4_quantize(state["x"]), DTYPES[c["dtype"]])
+        if c["kind"] == "linear":
+            y = torch.empty(c["rows"], c["n"], dtype=DTYPES[c["out"]], device="cuda")
+            state["linear"].run(state["x"], y)
+            return y
+        if c["kind"] == "gemm":
+            return exl3.mx4_gemm(exl3.mx4_quantize(state["x"]), state["weight"], out_dtype=DTYPES[c["out"]])
+        if c["kind"] == "moe":
+            return exl3.mx4_moe_forward(state["x"], state["ids"], state["w"], state["experts"], act=c["act"],
+                                        shared=c["E"] if c["shared"] else -1, out_dtype=DTYPES[c["dtype"]])
+        loss, counts, prob = exl3.route_balance(state["logits"], state["ids"], score=c["score"], mask=state["mask"],
+                                                coef=state["coef"])
+        d = exl3.route_balance_grad(state["logits"], counts, c["topk"], score=c["score"], mask=state["mask"],
+                                    coef=state["coef"], grad=state["grad"])
+        return {"loss": loss, "counts": counts, "prob": prob, "dlogits": d}
+    if c["kind"] == "quant":
+        return _values(*_quantise(state["x"])).to(DTYPES[c["dtype"]])
+    if c["kind"] == "linear":
+        y = state["x"].float() @ _values(*state["codes"]).t()
+        return (y + state["bias"].float() if c["bias"] else y).to(DTYPES[c["out"]])
+    if c["kind"] == "gemm":
+        return (_values(*_quantise(state["x"])) @ _values(*state["codes"]).t()).to(DTYPES[c["out"]])
+    if c["kind"] == "moe":
+        return _plain_moe(c, state)
+    return _plain_balance(c, state)
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(int(seed) * 7919 + 29)
+
+
+def _rows(rows, k, dtype, g):
+    """Rows as after a norm: N(0, 1), a few channels many times larger."""
+    x = torch.randn(rows, k, device="cuda", generator=g)
+    return (x * torch.exp2(torch.randn(k, device="cuda", generator=g))).to(dtype)
+
+
+def _weight(lead, n, k, g):
+    """Codes and scales of normal weights, 1 / sqrt(k) apart from a spread per row (quantised in pieces)."""
+    count = lead[0] if lead else 1
+    codes = torch.empty(count, n, k // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(count, n, k // 32, dtype=torch.uint8, device="cuda")
+    step = max(1, (1 << 26) // (n * k))
+    for i in range(0, count, step):
+        m = min(step, count - i)
+        for j in range(0, n, 8192):
+            h = min(8192, n - j)
+            v = torch.randn(m, h, k, device="cuda", generator=g)
+            v *= torch.exp2(0.5 * torch.randn(m, h, 1, device="cuda", generator=g)) / math.sqrt(k)
+            codes[i:i + m, j:j + h], scales[i:i + m, j:j + h] = _quantise(v)
+    return (codes, scales) if lead else (codes[0], scales[0])
+
+
+def prepare(case, seed):
+    c, g = case, _gen(seed)
+    s = {"case": c}
+    if own:
+        s["exl3"] = importlib.import_module("b70-inference_amd")
+    if c["kind"] == "quant":
+        s["x"] = _rows(c["rows"], c["k"], DTYPES[c["dtype"]], g)
+    elif c["kind"] in ("linear", "gemm"):
+        s["x"] = _rows(c["rows"], c["k"], DTYPES[c["dtype"]], g)
+        s["codes"] = _weight((), c["n"], c["k"], g)
+        if c["kind"] == "linear":
+            s["bias"] = torch.randn(c["n"], device="cuda", generator=g).to(DTYPES[c["dtype"]]) if c["bias"] else None
+        if own:
+            s["weight"] = s["exl3"].MX4Tensor(*s["codes"])
+            if c["kind"] == "linear":
+                s["linear"] = s["exl3"].MX4Linear(s["weight"], s["bias"])
+    elif c["kind"] == "moe":
+        E, n = c["E"], c["E"] + int(c["shared"])
+        s["x"] = torch.randn(c["rows"], c["H"], device="cuda", generator=g).to(DTYPES[c["dtype"]])
+        s["weights"] = [_weight((n,), c["I"], c["H"], g), _weight((n,), c["I"], c["H"], g), _weight((n,), c["H"], c["I"], g)]
+        score, ids = torch.topk(torch.randn(c["rows"], E, device="cuda", generator=g), c["topk"], dim=1)
+        w = torch.exp(score)
+        s["ids"], s["w"] = ids.to(torch.int32), w / w.sum(1, keepdim=True)
+        if own:
+            s["experts"] = s["exl3"].MX4Experts.stacked(*[s["exl3"].MX4Tensor(*p) for p in s["weights"]])
+    else:
+        # logits with a lean towards some experts, as a router has before it is balanced
+        lean = torch.randn(c["E"], device="cuda", generator=g)
+        s["logits"] = 1.5 * torch.randn(c["rows"], c["E"], device="cuda", generator=g) + lean
+        s["ids"] = torch.topk(s["logits"], c["topk"], dim=1)[1].to(torch.int32)
+        s["mask"] = None
+        if c["padded"]:               # sequences of up to 1024 rows, each filled to a length of its own
+            at = torch.arange(c["rows"], device="cuda")
+            full = torch.randint(1, 1025, (c["rows"] // 1024 + 1,), device="cuda", generator=g)
+            s["mask"] = (at % 1024) < full[at // 1024]
+        s["coef"] = 0.01
+        s["grad"] = torch.ones(1, device="cuda")
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ in 64 bits
+def _value64(codes, scales):
+    """The values that codes and scales stand for, from sign, exponent and mantissa bits."""
+    q = torch.cat((codes[..., None] & 15, codes[..., None] >> 4), -1).flatten(-2).to(torch.int64)
+    e, m = (q >> 1) & 3, (q & 1).double()
+    mag = torch.where(e == 0, 0.5 * m, torch.ldexp(1.0 + 0.5 * m, e - 1))
+    v = torch.where(q >= 8, -mag, mag)
+    return torch.ldexp(v, (scales.to(torch.int64) - 127).repeat_interleave(32, -1))
+
+
+def _nearest64(x):
+    """Rows x rounded to the format: the nearest value of the block's grid, the even one of two."""
+    v = x.double().unflatten(-1, (-1, 32))
+    top = v.abs().amax(-1, keepdim=True)
+    e = (torch.floor(torch.log2(torch.where(top > 0, top, torch.ones_like(top)))) - 2).clamp(-127, 127)
+    scale = torch.exp2(torch.where(top > 0, e, torch.full_like(e, -127)))
+    a = v.abs() / scale
+    # spacing of the grid at a: 0.5 below 2, 1 from 2 to 4, 2 above (torch.round takes the even multiple)
+    step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0)).to(torch.float64)
+    return (torch.sign(v) * (torch.round(a / step) * step).clamp(max=6.0) * scale).flatten(-2)
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        s = prepare(case, seed)
+    finally:
+        own = was
+    c = case
+    if c["kind"] == "quant":
+        return _nearest64(s["x"])
+    if c["kind"] in ("linear", "gemm"):
+        x = s["x"].double() if c["kind"] == "linear" else _nearest64(s["x"])
+        codes, scales = s["codes"]
+        out = torch.empty(c["rows"], c["n"], dtype=torch.float64, device="cuda")
+        for j in range(0, c["n"], 4096):
+            out[:, j:j + 4096] = torch.mm(x, _value64(codes[j:j + 4096], scales[j:j + 4096]).t())
+        if c["kind"] == "linear" and c["bias"]:
+            out += s["bias"].double()
+        return out
+    if c["kind"] == "moe":
+        x, ids, w = s["x"].double(), s["ids"].cpu(), s["w"].double()
+        out = torch.zeros_like(x)
+        for e in range(c["E"] + int(c["shared"])):
+            if e < c["E"]:
+                tok, slot = torch.nonzero(ids == e, as_tuple=True)
+                if not len(tok):
+                    continue
+                tok, slot = tok.cuda(), slot.cuda()
+                scale = w[tok, slot]
+            else:
+                tok = torch.arange(c["rows"], device="cuda")
+                scale = torch.ones(c["rows"], dtype=torch.float64, device="cuda")
+            gate, up, down = (_value64(q[e], t[e]) for q, t in s["weights"])
+            g, u = torch.mm(x[tok], gate.t()), torch.mm(x[tok], up.t())
+            if c["act"] == "silu":
+                h = g * torch.sigmoid(g) * u
+            else:
+                h = g * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)) * u
+            out.index_add_(0, tok, scale[:, None] * torch.mm(h, down.t()))
+        return out
+    z, E, k = s["logits"].double(), c["E"], c["topk"]
+    rows = torch.nonzero(s["mask"])[:, 0] if c["padded"] else torch.arange(c["rows"], device="cuda")
+    counts = torch.bincount(s["ids"][rows].reshape(-1).long(), minlength=E)
+    zr = z[rows].requires_grad_(True)
+    if c["score"] == "softmax":
+        p = torch.softmax(zr, 1)
+    else:
+        t = torch.sigmoid(zr) if c["score"] == "sigmoid" else torch.sqrt(torch.nn.functional.softplus(zr, threshold=40.0))
+        p = t / t.sum(1, keepdim=True)
+    prob = p.mean(0)
+    loss = s["coef"] * E / (k * len(rows)) * (counts.double() * prob).sum()
+    (dz,) = torch.autograd.grad(loss * s["grad"].double().sum(), zr)
+    d = torch.zeros_like(z)
+    d[rows] = dz
+    return {"loss": loss.detach().reshape(1), "counts": counts.to(torch.int32), "prob": prob.detach(), "dlogits": d}
