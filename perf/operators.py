@@ -209,9 +209,9 @@ def run(state):
         if c["kind"] == "moe":
             return exl3.mx4_moe_forward(state["x"], state["ids"], state["w"], state["experts"], act=c["act"],
                                         shared=c["E"] if c["shared"] else -1, out_dtype=DTYPES[c["dtype"]])
-        loss, counts, prob = exl3.route_balance(state["logits"], state["ids"], score=c["score"], mask=state["mask"],
-                                                coef=state["coef"])
-        d = exl3.route_balance_grad(state["logits"], counts, c["topk"], score=c["score"], mask=state["mask"],
+        loss, counts, prob, rows = exl3.route_balance(state["logits"], state["ids"], score=c["score"],
+                                                      mask=state["mask"], coef=state["coef"])
+        d = exl3.route_balance_grad(state["logits"], counts, rows, c["topk"], score=c["score"], mask=state["mask"],
                                     coef=state["coef"], grad=state["grad"])
         return {"loss": loss, "counts": counts, "prob": prob, "dlogits": d}
     if c["kind"] == "quant":
