@@ -5,6 +5,7 @@ library is missing, every op raises, so a GPU run can never silently take a non-
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -14,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("EXL3MI_LIB") or os.path.join(HERE, "libexl3mi.so")
 
 EXL3_OK, EXL3_ERR_INVALID, EXL3_ERR_UNSUPPORTED, EXL3_ERR_HIP = 0, 1, 2, 3
-EXL3_F16, EXL3_F32 = 0, 1
+EXL3_F16, EXL3_F32, EXL3_BF16 = 0, 1, 2
 EXL3_WORDS_PLANAR4, EXL3_WORDS_TILE_ORDER = 0, 1
 ACT_SILU, ACT_GELU_TANH = 0, 1
 
@@ -50,6 +51,14 @@ SIGNATURES = {
     "exl3_moe_align": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
     "exl3_route_softmax_topk": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp],
     "exl3_route_topk": [_vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _f32, _vp, _vp, _vp],
+    "exl3_mx4_quantize": [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp],
+    "exl3_mx4_dequantize": [_vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp],
+    "exl3_mx4_linear": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp],
+    "exl3_mx4_gemm": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _vp],
+    "exl3_mx4_moe_forward": [_vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _f32, _i64, _vp, _i64,
+                             _i32, _vp],
+    "exl3_route_balance": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp],
+    "exl3_route_balance_grad": [_vp, _i64, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp],
     "exl3_router_logits": [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
 }
 _RESTYPE = {"exl3_last_error": ctypes.c_char_p}
@@ -136,6 +145,23 @@ def reserve_workspace(nbytes: int, ncounters: int = 0):
 def release_workspace():
     """Free outgrown workspace buffers (synchronises; no graph captured before may be replayed afterwards)."""
     check(lib().exl3_release_workspace(), "exl3_release_workspace")
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which t's device is the current one (the library launches on, and takes its workspace from, the current
+    device)."""
+    return _same_device if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def require_same_device(what: str, *ts):
+    """GPU tensors, all on one device."""
+    require_device(*ts)
+    devs = {t.get_device() for t in ts if t is not None}
+    if len(devs) > 1:
+        raise Exl3Error(f"{what}: tensors on several devices {sorted(devs)}")
 
 
 def require_device(*ts):

@@ -1,0 +1,88 @@
+// Microscaled 4-bit values (MX4): 32 consecutive values of a row share a scale 2^(s - 127) held in a byte (255: not a
+// number); a value is sign, two exponent bits and one mantissa bit (0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the even
+// one in the low half. A matrix is codes uint8 [rows][k / 2] and scales uint8 [rows][k / 32], both row-major. Every value
+// times its scale is exact in bf16 and fp32, and in fp16 for scales 2^-23 .. 2^13.
+//
+// The gfx950 conversions take the scale's exponent bits as that byte (the mantissa is not read, exponent 0 is 2^-127),
+// round to nearest even and saturate; the scaled MFMAs take the codes as they lie in memory: lane l of a 16 x 16 x 128
+// product holds the 32 values (16 bytes, one scale) of row l & 15 that begin at 32 (l >> 4), of a 32 x 32 x 64 one those
+// of row l & 31 at 32 (l >> 5). The kernels here use that lane layout for the 16-bit MFMAs too: a lane's block of 32 is
+// four (16 x 16 x 32) or four (32 x 32 x 16) fragments of eight, both operands permuted alike along k, so a lane reads
+// whole blocks and needs one scale for each.
+#pragma once
+
+#include "exl3_device.h"
+#include "exl3_runtime.h"
+
+namespace exl3 {
+
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef int i8_t __attribute__((ext_vector_type(8)));
+
+// Type of the rows that a product takes: 16-bit values, or MX4 codes and scales.
+enum { kRowF16 = 0, kRowBF16 = 1, kRowMX4 = 2 };
+
+// Scale byte s less the power of two taken out of the matrix (fp16 rows), as the float whose exponent the conversions
+// read. A block that needs a smaller scale than 2^-127 holds zeros only (the host checks the range); 255 stays 255.
+__device__ __forceinline__ float mx4_scale(int s, int base) {
+    const int e = s - base;
+    return __builtin_bit_cast(float, (s == 255 ? 255 : e > 0 ? e : 0) << 23);
+}
+
+// Eight codes (one word) times the scale, as fp16 or bf16.
+template <int XT>
+__device__ __forceinline__ u32x4_t mx4_frag(uint32_t q, float s) {
+    u32x4_t r;
+    if constexpr (XT == kRowF16) {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 0));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 1));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 2));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 3));
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 0));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 1));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 2));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 3));
+    }
+    return r;
+}
+
+template <int XT>
+__device__ __forceinline__ f4_t mfma16(u32x4_t a, u32x4_t b, f4_t c) {
+    if constexpr (XT == kRowF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+
+// 16 x 16 x 128 product of MX4 codes (sa, sb: the lane's scale bytes).
+__device__ __forceinline__ f4_t mfma16_mx4(u32x4_t a, int sa, u32x4_t b, int sb, f4_t c) {
+    const i8_t av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i8_t bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, sa, 0, sb);
+}
+
+__device__ __forceinline__ uint16_t f2bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+__device__ __forceinline__ float bf2f(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
+
+// A value of an output or intermediate of type `dtype` (EXL3_F16, EXL3_F32, EXL3_BF16), one rounding.
+__device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype) {
+    if (dtype == EXL3_F32) reinterpret_cast<float*>(p)[i] = v;
+    else reinterpret_cast<uint16_t*>(p)[i] = dtype == EXL3_F16 ? f2h(v) : f2bf(v);
+}
+
+// Four neighbouring values at an offset that is a multiple of four from a pointer aligned to four values.
+__device__ __forceinline__ void store4_as(void* p, int64_t i, f4_t v, int dtype) {
+    if (dtype == EXL3_F32) {
+        *reinterpret_cast<f4_t*>(reinterpret_cast<float*>(p) + i) = v;
+        return;
+    }
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = dtype == EXL3_F16 ? f2h(v[j]) : f2bf(v[j]);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+
+}  // namespace exl3

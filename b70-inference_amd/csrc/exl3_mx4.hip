@@ -1,0 +1,332 @@
+// MX4 (microscaled 4-bit) quantisation, its inverse, and the dense products with MX4 weights: 16-bit rows (exl3_mx4_linear)
+// and MX4 rows (exl3_mx4_gemm).
+#include "exl3_mx4.h"
+#include "exl3_mx4_rows.h"
+
+namespace exl3 {
+
+// ================================================================================================ quantise
+// A block's scale is 2^(floor(log2 a) - 2), a its largest magnitude, so that a / scale lies in [4, 8) and the largest
+// code, 6, is within a factor 4/3 of it: the byte is a's float exponent less 2, at least 0 (subnormal a, and 0). A block
+// with an infinity or a NaN (exponent 255) has byte 255 and codes 0. Four lanes share a block, eight values each; integer maxima
+// of the magnitude bits order floats, infinities and NaNs alike. Bound by the bytes.
+template <int DT>
+struct QuantIn;
+template <>
+struct QuantIn<EXL3_F16> {
+    u32x4_t v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        v = ldg(reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(p) + i));
+    }
+    __device__ __forceinline__ uint32_t top() const {          // float bits of the largest magnitude
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, max(v[j] & 0x7FFFu, v[j] >> 16 & 0x7FFFu));
+        return __builtin_bit_cast(uint32_t, h2f((uint16_t)m));
+    }
+    __device__ __forceinline__ uint32_t codes(float s) const {
+        uint32_t q = 0;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(h2_t, (uint32_t)v[0]), s, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(h2_t, (uint32_t)v[1]), s, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(h2_t, (uint32_t)v[2]), s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(h2_t, (uint32_t)v[3]), s, 3);
+    }
+};
+template <>
+struct QuantIn<EXL3_BF16> {
+    u32x4_t v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        v = ldg(reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(p) + i));
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, max(v[j] & 0x7FFFu, v[j] >> 16 & 0x7FFFu));
+        return m << 16;
+    }
+    __device__ __forceinline__ uint32_t codes(float s) const {
+        uint32_t q = 0;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(b2_t, (uint32_t)v[0]), s, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(b2_t, (uint32_t)v[1]), s, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(b2_t, (uint32_t)v[2]), s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(b2_t, (uint32_t)v[3]), s, 3);
+    }
+};
+template <>
+struct QuantIn<EXL3_F32> {
+    f4_t a, b;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        const f4_t* q = reinterpret_cast<const f4_t*>(reinterpret_cast<const float*>(p) + i);
+        a = ldg(q);
+        b = ldg(q + 1);
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            m = max(m, max(__builtin_bit_cast(uint32_t, (float)a[j]) & 0x7FFFFFFFu,
+                           __builtin_bit_cast(uint32_t, (float)b[j]) & 0x7FFFFFFFu));
+        return m;
+    }
+    __device__ __forceinline__ uint32_t codes(float s) const {
+        uint32_t q = 0;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, a[0], a[1], s, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, a[2], a[3], s, 1);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, b[0], b[1], s, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, b[2], b[3], s, 3);
+    }
+};
+
+// Units of eight values per thread: enough loads in flight to cover the memory's latency.
+constexpr int kQuantUnits = 2;
+
+// `upr`: units of eight values per row (a multiple of 4: a block never straddles waves), `cpr` workgroups per row.
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t x_ld, int64_t upr, int cpr,
+                                                           uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    const int64_t row = blockIdx.x / (unsigned)cpr, u0 = (int64_t)(blockIdx.x % (unsigned)cpr) * (256 * kQuantUnits);
+    QuantIn<DT> in[kQuantUnits];
+#pragma unroll
+    for (int i = 0; i < kQuantUnits; ++i) {
+        const int64_t u = u0 + 256 * i + threadIdx.x;
+        in[i].load(x, row * x_ld + 8 * (u < upr ? u : upr - 1));
+    }
+#pragma unroll
+    for (int i = 0; i < kQuantUnits; ++i) {
+        const int64_t u = u0 + 256 * i + threadIdx.x;
+        uint32_t top = in[i].top();
+        top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+        const int ex = (int)(top >> 23), e = ex == 255 ? 255 : ex > 2 ? ex - 2 : 0;
+        const uint32_t q = in[i].codes(__builtin_bit_cast(float, (e == 255 ? 127 : e) << 23));
+        if (u < upr) {
+            codes[row * upr + u] = e == 255 ? 0u : q;
+            if ((u & 3) == 0) scales[(row * upr + u) >> 2] = (uint8_t)e;
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __restrict__ codes,
+                                                             const uint8_t* __restrict__ scales, int64_t upr, int cpr,
+                                                             void* __restrict__ out, int64_t out_ld) {
+    const int64_t row = blockIdx.x / (unsigned)cpr, u0 = (int64_t)(blockIdx.x % (unsigned)cpr) * (256 * kQuantUnits);
+    uint32_t q[kQuantUnits];
+    int s[kQuantUnits];
+#pragma unroll
+    for (int i = 0; i < kQuantUnits; ++i) {
+        const int64_t u = u0 + 256 * i + threadIdx.x, at = row * upr + (u < upr ? u : upr - 1);
+        q[i] = ldg(codes + at);
+        s[i] = ldg(scales + (at >> 2));
+    }
+#pragma unroll
+    for (int i = 0; i < kQuantUnits; ++i) {
+        const int64_t u = u0 + 256 * i + threadIdx.x;
+        if (u >= upr) break;
+        const float sc = mx4_scale(s[i], 0);
+        if constexpr (DT == EXL3_F32) {
+            float* o = reinterpret_cast<float*>(out) + row * out_ld + 8 * u;
+            const auto v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], sc, 0),
+                       v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], sc, 1),
+                       v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], sc, 2),
+                       v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], sc, 3);
+            reinterpret_cast<f4_t*>(o)[0] = f4_t{v0[0], v0[1], v1[0], v1[1]};
+            reinterpret_cast<f4_t*>(o)[1] = f4_t{v2[0], v2[1], v3[0], v3[1]};
+        } else {
+            *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(out) + row * out_ld + 8 * u) =
+                mx4_frag<DT == EXL3_F16 ? kRowF16 : kRowBF16>(q[i], sc);
+        }
+    }
+}
+
+// ================================================================================================ dense products
+struct Mx4Args {
+    const uint8_t* x;                  // rows: 16-bit values, or MX4 codes
+    const uint8_t* xs;                 // MX4 rows: scales
+    int64_t x_ld;                      // bytes from row to row
+    const uint8_t* w;
+    const uint8_t* ws;
+    const float* bias;                 // [n] or null
+    void* out;
+    int64_t out_ld;
+    int64_t m, n;
+    int k, base, out_dtype, vec;       // vec: four neighbouring outputs may be stored together
+};
+
+// A dense output's four neighbours n, n + 1, ... of row m: 2^base of the sum, the bias, one rounding.
+__device__ __forceinline__ void mx4_store(const Mx4Args& a, int64_t m, int64_t n, f4_t v) {
+    if (m >= a.m) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (a.base) v[q] = __builtin_ldexpf(v[q], a.base);
+        if (a.bias && n + q < a.n) v[q] += ldg(a.bias + n + q);
+    }
+    if (a.vec) {
+        if (n < a.n) store4_as(a.out, m * a.out_ld + n, v, a.out_dtype);
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (n + q < a.n) store_as(a.out, m * a.out_ld + n + q, v[q], a.out_dtype);
+}
+
+template <int XT, int NT, int MT, int U>
+__global__ __launch_bounds__(512) void mx4_rows_kernel(Mx4Args a) {
+    extern __shared__ f4_t red[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const unsigned nt = (unsigned)((a.n + 16 * NT - 1) / (16 * NT));
+    const int64_t n0 = (int64_t)(blockIdx.x % nt) * (16 * NT), m0 = (int64_t)(blockIdx.x / nt) * (16 * MT);
+    const int r = lane & 15, kb = a.k / 32;
+    const uint8_t *wq[NT], *wsc[NT], *xq[MT], *xsc[MT];
+    int base[NT];
+    f4_t acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int64_t n = n0 + 16 * i + r, nc = n < a.n ? n : a.n - 1;
+        wq[i] = a.w + nc * (a.k / 2);
+        wsc[i] = a.ws + nc * kb;
+        base[i] = a.base;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = f4_t{};
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int64_t m = m0 + 16 * j + r, mc = m < a.m ? m : a.m - 1;
+        xq[j] = a.x + mc * a.x_ld;
+        xsc[j] = XT == kRowMX4 ? a.xs + mc * kb : nullptr;
+    }
+    mx4_rows_loop<XT, NT, MT, U>(wq, wsc, base, xq, xsc, kb, wave, waves, (kb + 3) / 4, lane >> 4, acc);
+    mx4_rows_put(red, wave, lane, acc);
+    for (int t = threadIdx.x; t < NT * MT * 64; t += blockDim.x) {
+        const int l = t & 63, j = (t >> 6) % MT, i = (t >> 6) / MT;
+        mx4_store(a, m0 + 16 * j + (l & 15), n0 + 16 * i + 4 * (l >> 4), mx4_rows_sum<NT, MT>(red, waves, i, j, l));
+    }
+}
+
+typedef void (*mx4_fn)(Mx4Args);
+
+template <int XT>
+static int launch_rows(const char* name, const Mx4Args& a, hipStream_t st) {
+    const int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : a.m <= 48 ? 3 : 4, nt = mt == 1 ? 1 : 2;
+    constexpr bool q = XT == kRowMX4;
+    const mx4_fn fn = mt == 1 ? mx4_rows_kernel<XT, 1, 1, 4>
+                    : mt == 2 ? mx4_rows_kernel<XT, 2, 2, q ? 4 : 2>
+                    : mt == 3 ? mx4_rows_kernel<XT, 2, 3, q ? 4 : 1> : mx4_rows_kernel<XT, 2, 4, q ? 4 : 1>;
+    const int64_t grid = (a.n + 16 * nt - 1) / (16 * nt) * ((a.m + 16 * mt - 1) / (16 * mt));
+    EXL3_CHECK_ARG(grid <= 0x7FFFFFFF, "%s: grid too large", name);
+    const int waves = mx4_rows_waves((a.k / 32 + 3) / 4);
+    EXL3_LAUNCH(name, fn, dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * nt * mt * 1024, st, a);
+    return EXL3_OK;
+}
+
+static bool mx4_dtype(int t) { return t == EXL3_F16 || t == EXL3_F32 || t == EXL3_BF16; }
+static int elem_size(int t) { return t == EXL3_F32 ? 4 : 2; }
+
+// What both products check of their weights and output; sets those of the kernel's arguments.
+static int mx4_setup(const char* what, int64_t m, int64_t n, int64_t k, const uint8_t* w, const uint8_t* ws,
+                     const float* bias, void* C, int64_t c_ld, int c_dtype, Mx4Args& a) {
+    EXL3_CHECK_ARG(m >= 0 && n > 0 && k > 0 && k % 32 == 0 && k <= (1 << 30), "%s: bad sizes (m %lld, n %lld, k %lld; k a "
+                   "multiple of 32)", what, (long long)m, (long long)n, (long long)k);
+    EXL3_CHECK_ARG(mx4_dtype(c_dtype), "%s: the output must be fp16, bf16 or fp32", what);
+    EXL3_CHECK_ARG(c_ld >= n, "%s: output row stride %lld < n", what, (long long)c_ld);
+    EXL3_CHECK_ARG(m <= ((int64_t)1 << 40) / k && n <= ((int64_t)1 << 40) / k, "%s: operand too large", what);
+    if (m == 0) return EXL3_OK;
+    EXL3_CHECK_ARG(w && ws && C, "%s: null pointer", what);
+    EXL3_CHECK_ARG(aligned(w, 16), "%s: weight codes must be 16-byte aligned", what);
+    EXL3_CHECK_ARG(aligned(C, elem_size(c_dtype)) && (!bias || aligned(bias, 4)), "%s: misaligned output or bias", what);
+    a.w = w;
+    a.ws = ws;
+    a.bias = bias;
+    a.out = C;
+    a.out_ld = c_ld;
+    a.m = m;
+    a.n = n;
+    a.k = (int)k;
+    a.out_dtype = c_dtype;
+    a.vec = n % 4 == 0 && c_ld % 4 == 0 && aligned(C, 4 * elem_size(c_dtype));
+    return EXL3_OK;
+}
+
+}  // namespace exl3
+
+extern "C" {
+
+using namespace exl3;
+
+int exl3_mx4_quantize(const void* x, int64_t x_ld, int64_t rows, int64_t k, int x_dtype, uint8_t* codes, uint8_t* scales,
+                      void* stream) {
+    EXL3_CHECK_ARG(rows >= 0 && k > 0 && k % 32 == 0 && x_ld >= k, "exl3_mx4_quantize: bad sizes (rows %lld, k %lld, row "
+                   "stride %lld; k a multiple of 32)", (long long)rows, (long long)k, (long long)x_ld);
+    EXL3_CHECK_ARG(mx4_dtype(x_dtype), "exl3_mx4_quantize: x must be fp16, bf16 or fp32");
+    if (rows == 0) return EXL3_OK;
+    EXL3_CHECK_ARG(x && codes && scales, "exl3_mx4_quantize: null pointer");
+    EXL3_CHECK_ARG(aligned(x, 16) && (rows == 1 || x_ld * elem_size(x_dtype) % 16 == 0) && aligned(codes, 4),
+                   "exl3_mx4_quantize: rows must be 16-byte aligned and codes 4-byte");
+    EXL3_CHECK_ARG(rows <= ((int64_t)1 << 45) / x_ld, "exl3_mx4_quantize: too large");
+    if (x_ld == k) {                                           // one row of all values
+        k *= rows;
+        rows = 1;
+    }
+    const int64_t upr = k / 8, cpr = (upr + 256 * kQuantUnits - 1) / (256 * kQuantUnits);
+    EXL3_CHECK_ARG(cpr <= 0x7FFFFFFF / rows, "exl3_mx4_quantize: too large");
+    const auto fn = x_dtype == EXL3_F16 ? mx4_quantize_kernel<EXL3_F16>
+                  : x_dtype == EXL3_BF16 ? mx4_quantize_kernel<EXL3_BF16> : mx4_quantize_kernel<EXL3_F32>;
+    EXL3_LAUNCH("mx4_quantize", fn, dim3((unsigned)(rows * cpr)), dim3(256), 0, (hipStream_t)stream, x, x_ld, upr, (int)cpr,
+                reinterpret_cast<uint32_t*>(codes), scales);
+    return EXL3_OK;
+}
+
+int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t out_ld,
+                        int out_dtype, void* stream) {
+    EXL3_CHECK_ARG(rows >= 0 && k > 0 && k % 32 == 0 && out_ld >= k, "exl3_mx4_dequantize: bad sizes (rows %lld, k %lld, "
+                   "row stride %lld; k a multiple of 32)", (long long)rows, (long long)k, (long long)out_ld);
+    EXL3_CHECK_ARG(mx4_dtype(out_dtype), "exl3_mx4_dequantize: the output must be fp16, bf16 or fp32");
+    if (rows == 0) return EXL3_OK;
+    EXL3_CHECK_ARG(out && codes && scales, "exl3_mx4_dequantize: null pointer");
+    EXL3_CHECK_ARG(aligned(out, 16) && (rows == 1 || out_ld * elem_size(out_dtype) % 16 == 0) && aligned(codes, 4),
+                   "exl3_mx4_dequantize: rows must be 16-byte aligned and codes 4-byte");
+    EXL3_CHECK_ARG(rows <= ((int64_t)1 << 45) / out_ld, "exl3_mx4_dequantize: too large");
+    if (out_ld == k) {
+        k *= rows;
+        rows = 1;
+    }
+    const int64_t upr = k / 8, cpr = (upr + 256 * kQuantUnits - 1) / (256 * kQuantUnits);
+    EXL3_CHECK_ARG(cpr <= 0x7FFFFFFF / rows, "exl3_mx4_dequantize: too large");
+    const auto fn = out_dtype == EXL3_F16 ? mx4_dequantize_kernel<EXL3_F16>
+                  : out_dtype == EXL3_BF16 ? mx4_dequantize_kernel<EXL3_BF16> : mx4_dequantize_kernel<EXL3_F32>;
+    EXL3_LAUNCH("mx4_dequantize", fn, dim3((unsigned)(rows * cpr)), dim3(256), 0, (hipStream_t)stream,
+                reinterpret_cast<const uint32_t*>(codes), scales, upr, (int)cpr, out, out_ld);
+    return EXL3_OK;
+}
+
+int exl3_mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
+                    const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
+                    int c_dtype, void* stream) {
+    EXL3_CHECK_ARG(x_dtype == EXL3_F16 || x_dtype == EXL3_BF16, "exl3_mx4_linear: x must be fp16 or bf16");
+    EXL3_CHECK_ARG(x_ld >= k, "exl3_mx4_linear: x row stride %lld < k", (long long)x_ld);
+    EXL3_CHECK_ARG(scale_base >= -140 && scale_base <= 140, "exl3_mx4_linear: scale_base %d out of range", scale_base);
+    Mx4Args a{};
+    const int rc = mx4_setup("exl3_mx4_linear", m, n, k, codes, scales, bias, C, c_ld, c_dtype, a);
+    if (rc || m == 0) return rc;
+    EXL3_CHECK_ARG(x && aligned(x, 16) && (m == 1 || x_ld % 8 == 0), "exl3_mx4_linear: x rows must be 16-byte aligned");
+    EXL3_CHECK_ARG(m <= ((int64_t)1 << 45) / x_ld, "exl3_mx4_linear: operand too large");
+    a.x = reinterpret_cast<const uint8_t*>(x);
+    a.x_ld = 2 * x_ld;
+    a.base = x_dtype == EXL3_F16 ? scale_base : 0;
+    return x_dtype == EXL3_F16 ? launch_rows<kRowF16>("mx4_linear", a, (hipStream_t)stream)
+                               : launch_rows<kRowBF16>("mx4_linear", a, (hipStream_t)stream);
+}
+
+int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,
+                  const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, void* stream) {
+    Mx4Args a{};
+    const int rc = mx4_setup("exl3_mx4_gemm", m, n, k, b_codes, b_scales, bias, C, c_ld, c_dtype, a);
+    if (rc || m == 0) return rc;
+    EXL3_CHECK_ARG(a_codes && a_scales && aligned(a_codes, 16), "exl3_mx4_gemm: row codes must be 16-byte aligned");
+    a.x = a_codes;
+    a.xs = a_scales;
+    a.x_ld = k / 2;
+    return launch_rows<kRowMX4>("mx4_gemm", a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -19,10 +19,9 @@ import ctypes
 import torch
 
 from ._lib import (ACT_GELU_TANH, ACT_SILU, EXL3_F16, EXL3_F32, EXL3_WORDS_PLANAR4, EXL3_WORDS_TILE_ORDER, Exl3Error,
-                   check, lib, ptr, require_device, stream_of)
+                   check, lib, on_device, ptr, require_device, require_same_device, stream_of)
 from .linear import BC_LinearEXL3
-
-ACTS = {"silu": ACT_SILU, "gelu_tanh": ACT_GELU_TANH, ACT_SILU: ACT_SILU, ACT_GELU_TANH: ACT_GELU_TANH}
+from .mx4 import ACTS, MX4Experts, mx4_moe_forward
 
 
 class MixedEXL3:
@@ -404,6 +403,70 @@ def route_fused(x, w0, w1, bias0, bias1, res0, ids0, w0o, want0, ids1, w1o, logi
         rt(lv[:, E0:], bias1, None, mul1, scaling1, ids1, w1o, None)
 
 
+def _balance_args(what, logits, mask, score):
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise Exl3Error(f"{what}: logits must be fp32 [M, E] with contiguous rows")
+    if score not in SCORES:
+        raise NotImplementedError(f"{what}: scoring {score!r}")
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (logits.shape[0],):
+            raise Exl3Error(f"{what}: mask must be bool or uint8 [M]")
+        mask = mask.contiguous()
+    # one row has no stride of its own (torch may give any)
+    return mask, logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
+
+
+def route_balance(logits: torch.Tensor, topk_ids: torch.Tensor, score: str = "softmax",
+                  mask: torch.Tensor | None = None, coef: float = 1.0):
+    """How evenly a routing loads its experts (exl3_route_balance): with the shares p = score(logits) / row sum (score as in
+    route_topk), over the N live rows (mask bool [M], None: all), counts[e] the picks of e in topk_ids and prob[e] the
+    mean of p[:, e]: loss = coef * sum_e E * counts[e] / (k * N) * prob[e] (coef for an even load). logits fp32 [M, E],
+    topk_ids int32 [M, k] (entries outside [0, E) count nowhere). Returns (loss fp32 [1], counts int32 [E], prob fp32
+    [E], rows int32 [1] = N). The picks' own bias or residency terms do not enter."""
+    require_same_device("route_balance", logits, topk_ids, mask)
+    mask, ld = _balance_args("route_balance", logits, mask, score)
+    M, E = logits.shape
+    if topk_ids.dtype != torch.int32 or topk_ids.dim() != 2 or topk_ids.shape[0] != M:
+        raise Exl3Error("route_balance: topk_ids must be int32 [M, k]")
+    topk_ids = topk_ids.contiguous()
+    dev = logits.device
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    prob = torch.empty(E, dtype=torch.float32, device=dev)
+    rows = torch.empty(1, dtype=torch.int32, device=dev)
+    with on_device(logits):
+        check(lib().exl3_route_balance(ptr(logits), ld, M, E, ptr(topk_ids), topk_ids.shape[1], ptr(mask), SCORES[score],
+                                       float(coef), ptr(loss), ptr(counts), ptr(prob), ptr(rows), stream_of(logits)),
+              "route_balance")
+    return loss, counts, prob, rows
+
+
+def route_balance_grad(logits: torch.Tensor, counts: torch.Tensor, rows: torch.Tensor, k: int, score: str = "softmax",
+                       mask: torch.Tensor | None = None, coef: float = 1.0, grad: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of route_balance's loss with respect to the logits (exl3_route_balance_grad), times grad (fp32, one
+    element, on the GPU; None: 1): fp32 [M, E], zero in rows that are not live. counts and rows as route_balance returned
+    them (summed over the processes that share the batch, if several do), constants to the gradient; k picks per row.
+    out may be logits."""
+    require_same_device("route_balance_grad", logits, counts, rows, mask, grad, out)
+    mask, ld = _balance_args("route_balance_grad", logits, mask, score)
+    M, E = logits.shape
+    if counts.dtype != torch.int32 or counts.numel() != E or rows.dtype != torch.int32 or rows.numel() != 1:
+        raise Exl3Error("route_balance_grad: counts must be int32 [E] and rows int32 [1]")
+    if grad is not None and (grad.dtype != torch.float32 or grad.numel() != 1):
+        raise Exl3Error("route_balance_grad: grad must be one fp32 value")
+    if out is None:
+        out = torch.empty(M, E, dtype=torch.float32, device=logits.device)
+    if out.dtype != torch.float32 or tuple(out.shape) != (M, E) or out.stride(1) != 1:
+        raise Exl3Error("route_balance_grad: out must be fp32 [M, E] with contiguous rows")
+    counts = counts.contiguous()
+    with on_device(logits):
+        check(lib().exl3_route_balance_grad(ptr(logits), ld, M, E, int(k), ptr(mask), SCORES[score], float(coef),
+                                            ptr(counts), ptr(rows), ptr(grad), ptr(out), out.stride(0) if M > 1 else E,
+                                            stream_of(logits)), "route_balance_grad")
+    return out
+
+
 def router_logits(x: torch.Tensor, weight: torch.Tensor, E: int | None = None, layout: str = "he",
                   round_fp16: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Router logits fp32 [M, E] = x @ W on the router GEMV (exl3_router_logits). layout "he": weight fp16 [H, >= E]
@@ -525,7 +588,7 @@ class BlockSparseMLP:
     "he", the reference's gate_tensor) or [E, H] ("eh"), optionally rounded to fp16 like a half matmul. Scoring:
     "softmax" (default; the bias ranks and, unless bias_select_only, shifts the softmax), "sigmoid" or
     "sqrt_softplus" (rank by score + bias, weights from the score), renormalised (+1e-20) and scaled by
-    routed_scaling."""
+    routed_scaling. `experts` may be MX4Experts: bf16 rows then reach the experts as they are (the router takes fp16)."""
 
     def __init__(self, experts: ExpertTables, num_experts_per_tok: int, has_shared: bool = False, act="silu",
                  act_limit: float = 0.0, router_weight: torch.Tensor | None = None,
@@ -550,6 +613,8 @@ class BlockSparseMLP:
         self.router_round_fp16 = router_round_fp16
 
     def _fused_router(self) -> bool:
+        if isinstance(self.experts, MX4Experts):
+            return False
         # the one-call path covers softmax ranked and weighted with the bias, renormalised, unscaled
         return (self.scoring == "softmax" and self.renormalize and self.routed_scaling == 1.0 and
                 not (self.bias_select_only and self.selection_bias is not None))
@@ -568,10 +633,16 @@ class BlockSparseMLP:
 
     def forward(self, x: torch.Tensor, params=None, out_dtype=None) -> torch.Tensor:
         x2 = x.reshape(-1, x.shape[-1])
+        mx4 = isinstance(self.experts, MX4Experts)
+        xe = x2 if mx4 and x2.dtype == torch.bfloat16 else None
         if x2.dtype != torch.float16:
             x2 = x2.half()
         x2 = x2.contiguous()
-        if self._fused_router():
+        if mx4:
+            ids, w = self.route(x2, params)
+            out = mx4_moe_forward(x2 if xe is None else xe, ids, w, self.experts, self.act, self.act_limit, self.shared,
+                                  out_dtype=torch.float32)
+        elif self._fused_router():
             out = moe_forward_logits(x2, self.router_logits(x2, params), self.num_experts_per_tok, self.experts,
                                      self.act, self.act_limit, self.shared, self.selection_bias,
                                      out_dtype=torch.float32)

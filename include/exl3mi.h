@@ -30,7 +30,7 @@ enum exl3_status {
     EXL3_ERR_HIP = 3          /* HIP runtime error */
 };
 
-enum exl3_dtype { EXL3_F16 = 0, EXL3_F32 = 1 };
+enum exl3_dtype { EXL3_F16 = 0, EXL3_F32 = 1, EXL3_BF16 = 2 }; /* bf16: the mx4 entry points only */
 enum exl3_act { EXL3_ACT_SILU = 0, EXL3_ACT_GELU_TANH = 1 };
 enum exl3_score { EXL3_SCORE_SOFTMAX = 0, EXL3_SCORE_SIGMOID = 1, EXL3_SCORE_SQRT_SOFTPLUS = 2 };
 enum exl3_route_flags { EXL3_ROUTE_RENORM = 1, EXL3_ROUTE_BIAS_SELECT_ONLY = 2 };
@@ -287,6 +287,70 @@ int exl3_route_block(const float* logits, int64_t ld, int64_t M, int64_t E, cons
  * router GEMV of route_fused / gemv_h (dsv41/xpu/csrc/dsv_moe_glue.sycl:442-470, 520-530). */
 int exl3_router_logits(const uint16_t* x, int64_t x_ld, int64_t M, int64_t H, const uint16_t* W, int64_t w_ld,
                        int64_t E, int w_layout, int round_fp16, float* logits, int64_t logits_ld, void* stream);
+
+/* ---------------------------------------------------------------------------------- microscaled 4-bit values (MX4)
+ * 32 consecutive values of a row share a scale 2^(s - 127) held in a byte s (255: not a number). A value is a 4-bit code:
+ * sign, two exponent bits, one mantissa bit (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), two codes to a byte, the even
+ * one in the low half. A matrix of `rows` x k values is codes uint8 [rows, k / 2] and scales uint8 [rows, k / 32], both
+ * contiguous; k % 32 == 0. No reference counterpart (the reference's weights are EXL3 only). */
+
+/* codes, scales = MX4 of x (fp16, bf16 or fp32 [rows, k], row stride x_ld): the scale of a block is
+ * 2^(floor(log2 max|x|) - 2), at least 2^-127; each x / scale is rounded to the nearest value (ties to the even code,
+ * magnitudes above 6 to 6). A block that holds an infinity or a NaN gets scale byte 255 and codes 0. x and its rows 16-byte
+ * aligned, codes 4-byte. */
+int exl3_mx4_quantize(const void* x, int64_t x_ld, int64_t rows, int64_t k, int x_dtype, uint8_t* codes, uint8_t* scales,
+                      void* stream);
+
+/* out (fp16, bf16 or fp32 [rows, k], row stride out_ld, rows 16-byte aligned) = the values of codes and scales, rounded once
+ * (exact in bf16 and fp32; in fp16 for scales 2^-23 .. 2^13). Scale byte 255: NaN. */
+int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t out_ld,
+                        int out_dtype, void* stream);
+
+/* Linear with MX4 weights: C[m, n] = x @ W^T (+ bias) for x fp16 or bf16 [m, k] (row stride x_ld, rows 16-byte aligned),
+ * W [n, k] as codes (16-byte aligned) and scales, bias fp32 [n] or NULL, C fp16, bf16 or fp32 (row stride c_ld). The
+ * weights are exact in x's type, the sums fp32, one rounding. fp16 x: every block that is not all zeros must have
+ * 104 <= s - scale_base <= 140 (its values times 2^-scale_base are then exact in fp16; the result is scaled back); any
+ * other block's values round, overflow or vanish as fp16 does. bf16 x: scale_base is not used. k and n need not be
+ * multiples of anything but k of 32. */
+int exl3_mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
+                    const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
+                    int c_dtype, void* stream);
+
+/* Product of two MX4 matrices: C[m, n] = A @ B^T (+ bias fp32 [n] or NULL), A [m, k], B [n, k] as codes (16-byte aligned)
+ * and scales, fp32 sums, C fp16, bf16 or fp32 (row stride c_ld). Rows of A are quantised by exl3_mx4_quantize. */
+int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,
+                  const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, void* stream);
+
+/* Routed MoE layer over experts with MX4 weights: as exl3_moe_forward (same routing arguments, inactive slots, shared
+ * expert, activations and order of sums), for x fp16 or bf16 and out fp16, bf16 or fp32. tables: device int64 [9][E], row
+ * 3p + {0, 1, 2} = (address of codes, address of scales, scale_base) of projection p = 0 gate [I, H], 1 up [I, H], 2 down
+ * [H, I], addresses of codes 16-byte aligned, scale_base as in exl3_mx4_linear. act(gate, up) is computed in fp32 and
+ * rounded to x's type for the down product; expert outputs are summed in fp32 in slot order. H % 32 == 0, I % 32 == 0.
+ * x and its rows 16-byte aligned. */
+int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
+                         const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
+                         int64_t shared, void* out, int64_t out_ld, int out_dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ router balance
+ * How evenly a router loads its experts, as a loss. Row t has scores s(t, e) of its logits (EXL3_SCORE_SOFTMAX: exp;
+ * EXL3_SCORE_SIGMOID: sigmoid; EXL3_SCORE_SQRT_SOFTPLUS) and shares p(t, e) = s(t, e) / sum over e; a row whose scores are all
+ * zero in fp32 (every logit -inf) has p = 0. Over the live rows t (mask uint8 [M], non-zero = live; NULL: all), N of them:
+ *   counts[e] = picks of e in ids (int32 [M, topk]; entries outside [0, E) count nowhere)
+ *   prob[e]   = sum p(t, e) / N
+ *   loss      = coef * sum over e of E * counts[e] / (topk * N) * prob[e]
+ * (all 0 for N = 0). logits fp32 [M, E] (row stride ld), E <= 8192; loss fp32 [1], counts int32 [E], prob fp32 [E], rows
+ * int32 [1] = N. Sums in fp32 in an order fixed by the shape. No reference counterpart (the reference counts picks
+ * offline). */
+int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk,
+                       const uint8_t* mask, int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows,
+                       void* stream);
+
+/* Gradient of that loss: dlogits[t, j] = grad * d loss / d logits[t, j] (fp32 [M, E], row stride d_ld; zero in rows that are
+ * not live), counts and rows as exl3_route_balance wrote them (or summed over several processes) and taken as constants,
+ * grad fp32 [1] (device) or NULL for 1. dlogits may be logits. */
+int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t E, int64_t topk, const uint8_t* mask,
+                            int score, float coef, const int32_t* counts, const int32_t* rows, const float* grad,
+                            float* dlogits, int64_t d_ld, void* stream);
 
 #ifdef __cplusplus
 }
