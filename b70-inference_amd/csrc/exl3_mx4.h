@@ -17,6 +17,7 @@
 namespace exl3 {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef int i8_t __attribute__((ext_vector_type(8)));
@@ -62,6 +63,26 @@ __device__ __forceinline__ f4_t mfma16_mx4(u32x4_t a, int sa, u32x4_t b, int sb,
     const i8_t av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
     const i8_t bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, sa, 0, sb);
+}
+
+// 32 x 32 x 64 product of MX4 codes; byte OP of each lane's scale words.
+template <int OP>
+__device__ __forceinline__ f16_t mfma32_mx4(u32x4_t a, int sa, u32x4_t b, int sb, f16_t c) {
+    const i8_t av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i8_t bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, OP, sa, OP, sb);
+}
+
+// This workgroup's tile of nmt x nnt (rows x columns). Ids go round robin over the 8 XCDs; an XCD takes a contiguous run of
+// tiles, eight rows of tiles after one another for each column, so that the workgroups that run together on it share
+// their columns' and rows' operands in its L2. The grid is the tile count rounded up to 8; false past the tiles.
+__device__ __forceinline__ bool mx4_tile_of(unsigned nmt, unsigned nnt, unsigned& mt, unsigned& nt) {
+    const unsigned tiles = nmt * nnt, per = gridDim.x >> 3, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (t >= tiles) return false;
+    const unsigned band = t / (8 * nnt), in = t - band * 8 * nnt, h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
+    nt = in / h;
+    mt = 8 * band + in - nt * h;
+    return true;
 }
 
 __device__ __forceinline__ uint16_t f2bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }

@@ -219,6 +219,179 @@ static int launch_rows(const char* name, const Mx4Args& a, hipStream_t st) {
     return EXL3_OK;
 }
 
+// ------------------------------------------------------------------------------------------------ many MX4 rows
+// Tile of a product of two MX4 matrices on 32 x 32 x 64 scaled MFMAs, for many rows: WM x WN waves of TM x TN products each.
+// Steps of 128 k: 64 bytes of codes per row of either operand, staged through registers into one of two LDS buffers while
+// the other is multiplied; the scales of four steps (16 bytes per row) likewise. Lane l of a fragment takes blocks
+// 2 (l >> 5) and 2 (l >> 5) + 1 of its row's four, one per MFMA, so that both scales are neighbouring bytes of one word.
+// In LDS a row's four 16-byte units are permuted by its row number: eight lanes reading eight rows, or writing two, touch
+// every bank once.
+template <int TM, int TN, int WM, int WN>
+struct Mx4Tile {
+    static constexpr int kThreads = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, R = BM + BN;
+    static constexpr int kUnits = R * 4 / kThreads, kScaleRows = (R + kThreads - 1) / kThreads;
+    static constexpr int kLds = 2 * R * 64 + 2 * R * 16;
+    static_assert(R * 4 % kThreads == 0 && BM % (kThreads / 4) == 0, "staging");
+};
+
+__device__ __forceinline__ int mx4_unit(int row, int unit) { return row * 4 + (unit ^ (row >> 1 & 3)); }
+
+// Scale bytes [at, at + 16) of a matrix of `total` (>= 16) scale bytes; those past the end are 0 (beside codes that are 0).
+__device__ __forceinline__ u32x4_t load_scales16(const uint8_t* p, int64_t at, int64_t total) {
+    typedef u32x4_t any_t __attribute__((aligned(1)));         // (rows of scales have any alignment)
+    const int64_t over = at + 16 - total;
+    const int d = over > 0 ? (int)over : 0;                    // read d bytes earlier, shift them out
+    u32x4_t v = *(const __attribute__((address_space(1))) any_t*)(p + at - d);
+    if (d) {
+        uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+        if (d >= 8) {
+            lo = hi >> (8 * (d - 8));
+            hi = 0;
+        } else {
+            lo = lo >> (8 * d) | hi << (64 - 8 * d);
+            hi >>= 8 * d;
+        }
+        v = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    }
+    return v;
+}
+
+constexpr uint32_t kMx4Out = 0xF0000000u;                      // an offset past every buffer
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx4_rsrc(const uint8_t* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)(bytes < 0xE0000000LL ? bytes : 0xE0000000LL), 0x00020000);
+}
+__device__ __forceinline__ u32x4_t mx4_buffer16(__amdgpu_buffer_rsrc_t r, uint32_t at, int base) {
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, base, 0));
+}
+
+template <int TM, int TN, int WM, int WN, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) {
+    typedef Mx4Tile<TM, TN, WM, WN> T;
+    __shared__ u32x4_t codes[2][T::R * 4];
+    __shared__ uint32_t scales[2][4][T::R];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const unsigned nmt = (unsigned)((a.m + T::BM - 1) / T::BM), nnt = (unsigned)((a.n + T::BN - 1) / T::BN);
+    unsigned mt, nt;
+    if (!mx4_tile_of(nmt, nnt, mt, nt)) return;
+    const int64_t m0 = (int64_t)mt * T::BM, n0 = (int64_t)nt * T::BN;
+    const int kb = a.k / 32, nch = (kb + 3) / 4;
+
+    // staging: this thread's unit t & 3 of rows (t >> 2) + i kThreads / 4, the x rows first, at 32-bit offsets from the
+    // tile's first rows; buffer loads return 0 past the matrix, and x units past their row's end are moved there
+    const __amdgpu_buffer_rsrc_t xr = mx4_rsrc(a.x + m0 * a.x_ld, (a.m - m0) * a.x_ld),
+                                 wr = mx4_rsrc(a.w + n0 * (a.k / 2), (a.n - n0) * (a.k / 2));
+    constexpr int kStep = T::kThreads / 4;
+    uint32_t src[T::kUnits];
+#pragma unroll
+    for (int i = 0; i < T::kUnits; ++i) {
+        const int r = (t >> 2) + i * kStep;
+        src[i] = (uint32_t)(r < T::BM ? r : r - T::BM) * (uint32_t)(a.k / 2) + 16 * (t & 3);
+    }
+    u32x4_t st[T::kUnits], ss[T::kScaleRows];
+    const auto load_codes = [&](int c) {
+        const bool in = 4 * c + (t & 3) < kb;
+#pragma unroll
+        for (int i = 0; i < T::kUnits; ++i)
+            st[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] : kMx4Out, 64 * c) : mx4_buffer16(wr, src[i], 64 * c);
+    };
+    const auto load_scales = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < T::kScaleRows; ++i) {
+            const int r = t + i * T::kThreads;
+            if (T::R % T::kThreads != 0 && r >= T::R) break;
+            const int64_t m = m0 + r, n = n0 + r - T::BM;
+            const bool ix = r < T::BM;
+            const int64_t row = ix ? (m < a.m ? m : a.m - 1) : (n < a.n ? n : a.n - 1);
+            ss[i] = load_scales16(ix ? a.xs : a.ws, row * kb + 16 * s, (ix ? a.m : a.n) * kb);
+        }
+    };
+    const auto store_codes = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < T::kUnits; ++i) codes[buf][mx4_unit((t >> 2) + i * kStep, t & 3)] = st[i];
+    };
+    const auto store_scales = [&](int s) {                     // bytes past a row's end are the next row's: 0 (255 times 0 is NaN)
+#pragma unroll
+        for (int i = 0; i < T::kScaleRows; ++i) {
+            const int r = t + i * T::kThreads;
+            if (T::R % T::kThreads != 0 && r >= T::R) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int left = kb - 16 * s - 4 * q;
+                scales[s & 1][q][r] = ss[i][q] & (left >= 4 ? ~0u : left > 0 ? (1u << (8 * left)) - 1 : 0u);
+            }
+        }
+    };
+
+    const int r = lane & 31, g = lane >> 5, rm = (wave / WN) * 32 * TM + r, rn = T::BM + (wave % WN) * 32 * TN + r;
+    f16_t acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = f16_t{};
+
+    load_codes(0);
+    load_scales(0);
+    store_codes(0);
+    store_scales(0);
+    __syncthreads();
+    const int nsup = (nch + 3) / 4;
+    for (int sp = 0; sp < nsup; ++sp) {
+        load_scales(sp + 1 < nsup ? sp + 1 : sp);
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+            const int c = 4 * sp + cc;
+            if (c >= nch) break;                               // uniform
+            load_codes(c + 1);                                 // (past the last: not used)
+            __builtin_amdgcn_sched_barrier(0);                 // on their way before the products
+            const u32x4_t* cb = codes[cc & 1];
+            const uint32_t* sb = scales[sp & 1][cc];
+            int sx[TM], sw[TN];
+#pragma unroll
+            for (int j = 0; j < TM; ++j) sx[j] = (int)(sb[rm + 32 * j] >> (16 * g));
+#pragma unroll
+            for (int i = 0; i < TN; ++i) sw[i] = (int)(sb[rn + 32 * i] >> (16 * g));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                u32x4_t x[TM], w[TN];
+#pragma unroll
+                for (int j = 0; j < TM; ++j) x[j] = cb[mx4_unit(rm + 32 * j, 2 * g + s)];
+#pragma unroll
+                for (int i = 0; i < TN; ++i) w[i] = cb[mx4_unit(rn + 32 * i, 2 * g + s)];
+#pragma unroll
+                for (int i = 0; i < TN; ++i)
+#pragma unroll
+                    for (int j = 0; j < TM; ++j)
+                        acc[i][j] = s == 0 ? mfma32_mx4<0>(w[i], sw[i], x[j], sx[j], acc[i][j])
+                                           : mfma32_mx4<1>(w[i], sw[i], x[j], sx[j], acc[i][j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);                 // the loads are waited for here, behind the products
+            store_codes(~cc & 1);
+            if (cc == 3) store_scales(sp + 1);
+            __syncthreads();
+        }
+    }
+    // lane l holds column l & 31 (a row of x), rows 8 q + 4 (l >> 5) + 0 .. 3 (neighbouring outputs)
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                mx4_store(a, m0 + rm + 32 * j, n0 + rn - T::BM + 32 * i - r + 8 * q + 4 * g,
+                          f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+}
+
+template <int TM, int TN, int WM, int WN, int OCC>
+static int launch_tile(const Mx4Args& a, hipStream_t st) {
+    typedef Mx4Tile<TM, TN, WM, WN> T;
+    const int64_t tiles = (a.m + T::BM - 1) / T::BM * ((a.n + T::BN - 1) / T::BN);
+    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0, "exl3_mx4_gemm: grid too large");
+    EXL3_LAUNCH("mx4_gemm_tile", (mx4_tile_kernel<TM, TN, WM, WN, OCC>), dim3((unsigned)((tiles + 7) & ~7)), dim3(T::kThreads), 0,
+                st, a);
+    return EXL3_OK;
+}
+
 static bool mx4_dtype(int t) { return t == EXL3_F16 || t == EXL3_F32 || t == EXL3_BF16; }
 static int elem_size(int t) { return t == EXL3_F32 ? 4 : 2; }
 
@@ -326,6 +499,7 @@ int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, in
     a.x = a_codes;
     a.xs = a_scales;
     a.x_ld = k / 2;
+    if (m > 128 && k < 1 << 24 && m * (k / 32) >= 16 && n * (k / 32) >= 16) return launch_tile<4, 2, 2, 2, 2>(a, (hipStream_t)stream);
     return launch_rows<kRowMX4>("mx4_gemm", a, (hipStream_t)stream);
 }
 
