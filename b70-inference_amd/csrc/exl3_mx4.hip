@@ -2,6 +2,7 @@
 // and MX4 rows (exl3_mx4_gemm).
 #include "exl3_mx4.h"
 #include "exl3_mx4_rows.h"
+#include "exl3_mx4_wide.h"
 
 namespace exl3 {
 
@@ -217,6 +218,60 @@ static int launch_rows(const char* name, const Mx4Args& a, hipStream_t st) {
     const int waves = mx4_rows_waves((a.k / 32 + 3) / 4);
     EXL3_LAUNCH(name, fn, dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * nt * mt * 1024, st, a);
     return EXL3_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ many 16-bit rows
+template <int XT, int RG>
+__global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args a) {
+    typedef Mx4Wide<XT, RG> L;
+    __shared__ u32x4_t lds[2 * L::kBuf];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
+    unsigned mt, nt;
+    if (!mx4_tile_of((unsigned)((a.m + 32 * RG - 1) / (32 * RG)), (unsigned)((a.n + 255) / 256), mt, nt)) return;
+    const int64_t m0 = (int64_t)mt * (32 * RG), n0 = (int64_t)nt * 256 + 64 * wave;
+    L p;
+    p.kb = a.k / 32;
+    p.lds = lds;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+        const int64_t m = m0 + (t >> 3) + 32 * i;
+        p.xp[i] = a.x + (m < a.m ? m : a.m - 1) * a.x_ld;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t n = n0 + 32 * i + r, nc = n < a.n ? n : a.n - 1;
+        p.wq[i] = a.w + nc * (a.k / 2);
+        p.wsc[i] = a.ws + nc * p.kb;
+        p.base[i] = XT == kRowF16 ? a.base : 0;
+    }
+    f16_t acc[RG][2];
+#pragma unroll
+    for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
+    p.run(t, acc);
+    // lane l holds column l & 31 (a row of x), rows 8 q + 4 (l >> 5) + 0 .. 3 (neighbouring outputs)
+#pragma unroll
+    for (int j = 0; j < RG; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                mx4_store(a, m0 + 32 * j + r, n0 + 32 * i + 8 * q + 4 * g,
+                          f4_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]});
+}
+
+template <int XT, int RG>
+static int launch_wide(const Mx4Args& a, hipStream_t st) {
+    const int64_t tiles = (a.m + 32 * RG - 1) / (32 * RG) * ((a.n + 255) / 256);
+    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0, "exl3_mx4_linear: grid too large");
+    EXL3_LAUNCH("mx4_linear_wide", (mx4_wide_kernel<XT, RG>), dim3((unsigned)((tiles + 7) & ~7)), dim3(256), 0, st, a);
+    return EXL3_OK;
+}
+
+template <int XT>
+static int linear_run(const Mx4Args& a, hipStream_t st) {
+    if (a.m <= 64) return launch_rows<XT>("mx4_linear", a, st);
+    const int rg = env_int("MX4_RG", a.m <= 96 ? 2 : 4);
+    return rg == 4 ? launch_wide<XT, 4>(a, st) : rg == 2 ? launch_wide<XT, 2>(a, st) : launch_wide<XT, 1>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------------ many MX4 rows
@@ -486,8 +541,7 @@ int exl3_mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t
     a.x = reinterpret_cast<const uint8_t*>(x);
     a.x_ld = 2 * x_ld;
     a.base = x_dtype == EXL3_F16 ? scale_base : 0;
-    return x_dtype == EXL3_F16 ? launch_rows<kRowF16>("mx4_linear", a, (hipStream_t)stream)
-                               : launch_rows<kRowBF16>("mx4_linear", a, (hipStream_t)stream);
+    return x_dtype == EXL3_F16 ? linear_run<kRowF16>(a, (hipStream_t)stream) : linear_run<kRowBF16>(a, (hipStream_t)stream);
 }
 
 int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,

@@ -9,6 +9,8 @@
 #include "exl3_moe_dev.h"
 #include "exl3_mx4.h"
 #include "exl3_mx4_rows.h"
+#include "exl3_mx4_wide.h"
+#include "exl3_mx4_plan.h"
 #include "exl3_plan.h"
 
 namespace exl3 {
@@ -119,6 +121,106 @@ __global__ __launch_bounds__(512) void mx4_down_rows_kernel(Mx4MoeArgs a) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------ blocks of many rows
+// Waves 0 and 1 take 64 gate columns each, waves 2 and 3 the up columns; they meet in LDS, 32 rows at a time.
+constexpr int kMx4CS = 264;            // floats per row there: gate columns at 0, up columns at 132
+
+template <int XT, int RG>
+__global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(Mx4MoeArgs a) {
+    typedef Mx4Wide<XT, RG> L;
+    constexpr int kC = 32 * kMx4CS * 4 / 16;
+    __shared__ u32x4_t lds[2 * L::kBuf > kC ? 2 * L::kBuf : kC];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
+    const unsigned nc = ((unsigned)a.I + 127) / 128;
+    const ItemDesc* d = a.blocks + blockIdx.x / nc;
+    const int cnt = d->cnt, p0 = d->p0, i0 = (int)(blockIdx.x % nc) * 128, pj = wave >> 1;
+    if (cnt == 0) return;
+    L p;
+    p.kb = a.H / 32;
+    p.lds = lds;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+        const int m = (t >> 3) + 32 * i;
+        p.xp[i] = a.x + (int64_t)ldg(a.pair_tok + p0 + (m < cnt ? m : cnt - 1)) * a.x_ld;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mx4_expert_row<XT>(d, pj, i0 + 64 * (wave & 1) + 32 * i + r, a.I, a.H, p.wq[i], p.wsc[i], p.base[i]);
+    f16_t acc[RG][2];
+#pragma unroll
+    for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
+    p.run(t, acc);
+    const int bg = XT == kRowF16 ? (int)d->tab[2] : 0, bu = XT == kRowF16 ? (int)d->tab[5] : 0;
+    float* C = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int j = 0; j < RG; ++j) {
+        if (32 * j >= cnt) break;                              // uniform
+        if (j > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f4_t*>(C + r * kMx4CS + 132 * pj + 64 * (wave & 1) + 32 * i + 8 * q + 4 * g) =
+                    f4_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+        __syncthreads();
+        const int m = 32 * j + (t >> 3);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int col = 32 * q + 4 * (t & 7);
+            const f4_t gv = *reinterpret_cast<const f4_t*>(C + (t >> 3) * kMx4CS + col);
+            const f4_t uv = *reinterpret_cast<const f4_t*>(C + (t >> 3) * kMx4CS + 132 + col);
+            f4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[e] = act_mul_dev(__builtin_ldexpf(gv[e], bg), __builtin_ldexpf(uv[e], bu), a.act, a.limit);
+            if (m < cnt && i0 + col < a.I)
+                store4_as(a.mid, (int64_t)(p0 + m) * a.I + i0 + col, v, XT == kRowF16 ? EXL3_F16 : EXL3_BF16);
+        }
+    }
+}
+
+template <int XT, int RG>
+__global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx4MoeArgs a) {
+    typedef Mx4Wide<XT, RG> L;
+    __shared__ u32x4_t lds[2 * L::kBuf];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
+    const unsigned nc = ((unsigned)a.H + 255) / 256;
+    const ItemDesc* d = a.blocks + blockIdx.x / nc;
+    const int cnt = d->cnt, p0 = d->p0, h0 = (int)(blockIdx.x % nc) * 256 + 64 * wave;
+    if (cnt == 0) return;
+    L p;
+    p.kb = a.I / 32;
+    p.lds = lds;
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+        const int m = (t >> 3) + 32 * i;
+        p.xp[i] = reinterpret_cast<const uint8_t*>(a.mid + (int64_t)(p0 + (m < cnt ? m : cnt - 1)) * a.I);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mx4_expert_row<XT>(d, 2, h0 + 32 * i + r, a.H, a.I, p.wq[i], p.wsc[i], p.base[i]);
+    f16_t acc[RG][2];
+#pragma unroll
+    for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
+    p.run(t, acc);
+    const int bd = XT == kRowF16 ? (int)d->tab[8] : 0;
+#pragma unroll
+    for (int j = 0; j < RG; ++j) {
+        const int m = 32 * j + r;
+        if (m >= cnt) break;
+        const float w = ldg(a.pair_w + p0 + m);
+        float* y = a.y + (int64_t)(p0 + m) * a.H;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int h = h0 + 32 * i + 8 * q + 4 * g;
+                f4_t v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = w * __builtin_ldexpf(acc[j][i][4 * q + e], bd);
+                if (h < a.H) *reinterpret_cast<f4_t*>(y + h) = v;
+            }
+    }
+}
+
 // out[t] = sum of token t's y rows in slot order, four columns per thread.
 __global__ __launch_bounds__(256) void mx4_combine_kernel(Mx4MoeArgs a, int ncb, int vec) {
     const int t = blockIdx.x / (unsigned)ncb, c = 4 * ((blockIdx.x % (unsigned)ncb) * 256 + threadIdx.x);
@@ -150,8 +252,26 @@ __global__ __launch_bounds__(256) void mx4_combine_kernel(Mx4MoeArgs a, int ncb,
 
 typedef void (*mx4_moe_fn)(Mx4MoeArgs);
 
+static int mx4_moe_rows(int64_t npairs, int64_t E) {
+    const int e = env_int("MX4_MOE_ROWS", 0);
+    if (e) return e;
+    return npairs <= 16 * E ? 16 : npairs <= 48 * E ? 32 : npairs <= 96 * E ? 64 : 128;
+}
+
+template <int XT, int RG>
+static int mx4_moe_wide(const Mx4MoeArgs& a, hipStream_t st) {
+    EXL3_LAUNCH("mx4_moe_gateup_wide", (mx4_gateup_wide_kernel<XT, RG>), dim3((unsigned)(a.max_blocks * ((a.I + 127) / 128))),
+                dim3(256), 0, st, a);
+    EXL3_LAUNCH("mx4_moe_down_wide", (mx4_down_wide_kernel<XT, RG>), dim3((unsigned)(a.max_blocks * ((a.H + 255) / 256))),
+                dim3(256), 0, st, a);
+    return EXL3_OK;
+}
+
 template <int XT>
-static int mx4_moe_launch(const Mx4MoeArgs& a, hipStream_t st) {
+static int mx4_moe_launch(const Mx4MoeArgs& a, int rows, hipStream_t st) {
+    if (rows == 32) return mx4_moe_wide<XT, 1>(a, st);
+    if (rows == 64) return mx4_moe_wide<XT, 2>(a, st);
+    if (rows == 128) return mx4_moe_wide<XT, 4>(a, st);
     const int wg = mx4_rows_waves((a.H / 32 + 3) / 4), wd = mx4_rows_waves((a.I / 32 + 3) / 4);
     const mx4_moe_fn gu = mx4_gateup_rows_kernel<XT, 1, 1, 4>, dn = mx4_down_rows_kernel<XT, 2, 1, 4>;
     EXL3_LAUNCH("mx4_moe_gateup", gu, dim3((unsigned)(a.max_blocks * (a.I / 16))), dim3(64 * wg), (size_t)wg * 2048, st, a);
@@ -200,8 +320,8 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
     a.out = out;
     a.out_ld = out_ld;
     a.out_dtype = out_dtype;
-    const int rows = 16;
-    a.max_blocks = (int)(npairs / rows + (E < npairs ? E : npairs) + 1);
+    const int rows = mx4_moe_rows(npairs, E);
+    a.max_blocks = (int)mx4_max_blocks(npairs, E, rows);
     EXL3_CHECK_ARG((int64_t)a.max_blocks * ((H > I ? H : I) / 16) <= 0x7FFFFFFF, "exl3_mx4_moe_forward: grid too large");
     ItemDesc* blocks = nullptr;
     int* pairs = nullptr;
@@ -235,7 +355,7 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
         r.items = blocks;              // (none: max_items is 0)
         r.tables = tables;
         r.use_mfma = 1;
-        r.cut = {rows, 0, 0};
+        r.cut = mx4_cut(rows);
         r.blocks = blocks;
         r.max_blocks = a.max_blocks;
         r.pair_tok = pairs;
@@ -243,7 +363,7 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
         r.pair_of = pairs + np;
         int rc2 = launch_align(r, st);
         if (rc2) return rc2;
-        rc2 = x_dtype == EXL3_F16 ? mx4_moe_launch<kRowF16>(a, st) : mx4_moe_launch<kRowBF16>(a, st);
+        rc2 = x_dtype == EXL3_F16 ? mx4_moe_launch<kRowF16>(a, rows, st) : mx4_moe_launch<kRowBF16>(a, rows, st);
         if (rc2) return rc2;
     }
     const int64_t ncb = (H + 1023) / 1024;
