@@ -73,6 +73,28 @@ __device__ __forceinline__ f16_t mfma32_mx4(u32x4_t a, int sa, u32x4_t b, int sb
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, 4, 4, OP, sa, OP, sb);
 }
 
+// Scale bytes [at, at + 16) from p, `left` bytes before the end of the matrix's scales (which are 16 or more, from any row on or
+// before p); those past the end are 0. Rows of scales have any alignment.
+__device__ __forceinline__ u32x4_t mx4_scales16(const uint8_t* p, int at, int64_t left) {
+    typedef u32x4_t any_t __attribute__((aligned(1)));
+    const int64_t over = at + 16 - left;
+    if (over >= 16) return u32x4_t{};
+    const int d = over > 0 ? (int)over : 0;                    // read d bytes earlier, shift them out
+    u32x4_t v = *(const __attribute__((address_space(1))) any_t*)(p + at - d);
+    if (d) {
+        uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+        if (d >= 8) {
+            lo = hi >> (8 * (d - 8));
+            hi = 0;
+        } else {
+            lo = lo >> (8 * d) | hi << (64 - 8 * d);
+            hi >>= 8 * d;
+        }
+        v = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    }
+    return v;
+}
+
 // This workgroup's tile of nmt x nnt (rows x columns). Ids go round robin over the 8 XCDs; an XCD takes a contiguous run of
 // tiles, eight rows of tiles after one another for each column, so that the workgroups that run together on it share
 // their columns' and rows' operands in its L2. The grid is the tile count rounded up to 8; false past the tiles.

@@ -224,7 +224,7 @@ static int launch_rows(const char* name, const Mx4Args& a, hipStream_t st) {
 template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args a) {
     typedef Mx4Wide<XT, RG> L;
-    __shared__ u32x4_t lds[2 * L::kBuf];
+    __shared__ u32x4_t lds[L::kLds];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
     unsigned mt, nt;
     if (!mx4_tile_of((unsigned)((a.m + 32 * RG - 1) / (32 * RG)), (unsigned)((a.n + 255) / 256), mt, nt)) return;
@@ -241,9 +241,11 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args
     for (int i = 0; i < 2; ++i) {
         const int64_t n = n0 + 32 * i + r, nc = n < a.n ? n : a.n - 1;
         p.wq[i] = a.w + nc * (a.k / 2);
-        p.wsc[i] = a.ws + nc * p.kb;
         p.base[i] = XT == kRowF16 ? a.base : 0;
     }
+    const int64_t ns = n0 + lane < a.n ? n0 + lane : a.n - 1;
+    p.wsc = a.ws + ns * p.kb;
+    p.sleft = (a.n - ns) * p.kb;
     f16_t acc[RG][2];
 #pragma unroll
     for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
@@ -269,7 +271,7 @@ static int launch_wide(const Mx4Args& a, hipStream_t st) {
 
 template <int XT>
 static int linear_run(const Mx4Args& a, hipStream_t st) {
-    if (a.m <= 64) return launch_rows<XT>("mx4_linear", a, st);
+    if (a.m <= 64 || a.n * (a.k / 32) < 16) return launch_rows<XT>("mx4_linear", a, st);
     const int rg = env_int("MX4_RG", a.m <= 96 ? 2 : 4);
     return rg == 4 ? launch_wide<XT, 4>(a, st) : rg == 2 ? launch_wide<XT, 2>(a, st) : launch_wide<XT, 1>(a, st);
 }
@@ -290,26 +292,6 @@ struct Mx4Tile {
 };
 
 __device__ __forceinline__ int mx4_unit(int row, int unit) { return row * 4 + (unit ^ (row >> 1 & 3)); }
-
-// Scale bytes [at, at + 16) of a matrix of `total` (>= 16) scale bytes; those past the end are 0 (beside codes that are 0).
-__device__ __forceinline__ u32x4_t load_scales16(const uint8_t* p, int64_t at, int64_t total) {
-    typedef u32x4_t any_t __attribute__((aligned(1)));         // (rows of scales have any alignment)
-    const int64_t over = at + 16 - total;
-    const int d = over > 0 ? (int)over : 0;                    // read d bytes earlier, shift them out
-    u32x4_t v = *(const __attribute__((address_space(1))) any_t*)(p + at - d);
-    if (d) {
-        uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
-        if (d >= 8) {
-            lo = hi >> (8 * (d - 8));
-            hi = 0;
-        } else {
-            lo = lo >> (8 * d) | hi << (64 - 8 * d);
-            hi >>= 8 * d;
-        }
-        v = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
-    }
-    return v;
-}
 
 constexpr uint32_t kMx4Out = 0xF0000000u;                      // an offset past every buffer
 
@@ -358,7 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
             const int64_t m = m0 + r, n = n0 + r - T::BM;
             const bool ix = r < T::BM;
             const int64_t row = ix ? (m < a.m ? m : a.m - 1) : (n < a.n ? n : a.n - 1);
-            ss[i] = load_scales16(ix ? a.xs : a.ws, row * kb + 16 * s, (ix ? a.m : a.n) * kb);
+            ss[i] = mx4_scales16((ix ? a.xs : a.ws) + row * kb, 16 * s, ((ix ? a.m : a.n) - row) * kb);
         }
     };
     const auto store_codes = [&](int buf) {

@@ -125,11 +125,19 @@ __global__ __launch_bounds__(512) void mx4_down_rows_kernel(Mx4MoeArgs a) {
 // Waves 0 and 1 take 64 gate columns each, waves 2 and 3 the up columns; they meet in LDS, 32 rows at a time.
 constexpr int kMx4CS = 264;            // floats per row there: gate columns at 0, up columns at 132
 
+// Scales of weight row `row` (of `rows`, `k` wide) of projection p of block d.
+template <typename L>
+__device__ __forceinline__ void mx4_expert_scales(const ItemDesc* d, int p, int row, int rows, int k, L& o) {
+    const int64_t r = row < rows ? row : rows - 1;
+    o.wsc = reinterpret_cast<const uint8_t*>(d->tab[3 * p + 1]) + r * (k / 32);
+    o.sleft = (rows - r) * (k / 32);
+}
+
 template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(Mx4MoeArgs a) {
     typedef Mx4Wide<XT, RG> L;
     constexpr int kC = 32 * kMx4CS * 4 / 16;
-    __shared__ u32x4_t lds[2 * L::kBuf > kC ? 2 * L::kBuf : kC];
+    __shared__ u32x4_t lds[L::kLds > kC ? L::kLds : kC];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
     const unsigned nc = ((unsigned)a.I + 127) / 128;
     const ItemDesc* d = a.blocks + blockIdx.x / nc;
@@ -144,7 +152,9 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(
         p.xp[i] = a.x + (int64_t)ldg(a.pair_tok + p0 + (m < cnt ? m : cnt - 1)) * a.x_ld;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mx4_expert_row<XT>(d, pj, i0 + 64 * (wave & 1) + 32 * i + r, a.I, a.H, p.wq[i], p.wsc[i], p.base[i]);
+    for (int i = 0; i < 2; ++i)
+        mx4_expert_row<XT>(d, pj, i0 + 64 * (wave & 1) + 32 * i + r, a.I, a.H, p.wq[i], p.wsc, p.base[i]);
+    mx4_expert_scales(d, pj, i0 + 64 * (wave & 1) + lane, a.I, a.H, p);
     f16_t acc[RG][2];
 #pragma unroll
     for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
@@ -181,7 +191,7 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(
 template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx4MoeArgs a) {
     typedef Mx4Wide<XT, RG> L;
-    __shared__ u32x4_t lds[2 * L::kBuf];
+    __shared__ u32x4_t lds[L::kLds];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
     const unsigned nc = ((unsigned)a.H + 255) / 256;
     const ItemDesc* d = a.blocks + blockIdx.x / nc;
@@ -196,7 +206,8 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx
         p.xp[i] = reinterpret_cast<const uint8_t*>(a.mid + (int64_t)(p0 + (m < cnt ? m : cnt - 1)) * a.I);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mx4_expert_row<XT>(d, 2, h0 + 32 * i + r, a.H, a.I, p.wq[i], p.wsc[i], p.base[i]);
+    for (int i = 0; i < 2; ++i) mx4_expert_row<XT>(d, 2, h0 + 32 * i + r, a.H, a.I, p.wq[i], p.wsc, p.base[i]);
+    mx4_expert_scales(d, 2, h0 + lane, a.H, a.I, p);
     f16_t acc[RG][2];
 #pragma unroll
     for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
