@@ -95,6 +95,16 @@ __device__ __forceinline__ u32x4_t mx4_scales16(const uint8_t* p, int at, int64_
     return v;
 }
 
+// Buffer loads of 16 bytes: 0 past the `bytes` from p (which one of fewer than 2^32 - 2^29 may not reach).
+constexpr uint32_t kMx4Out = 0xF0000000u;  // an offset past every buffer
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx4_rsrc(const uint8_t* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)(bytes < 0xE0000000LL ? bytes : 0xE0000000LL), 0x00020000);
+}
+__device__ __forceinline__ u32x4_t mx4_buffer16(__amdgpu_buffer_rsrc_t r, uint32_t at, int base) {
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, base, 0));
+}
+
 // This workgroup's tile of nmt x nnt (rows x columns). Ids go round robin over the 8 XCDs; an XCD takes a contiguous run of
 // tiles, eight rows of tiles after one another for each column, so that the workgroups that run together on it share
 // their columns' and rows' operands in its L2. The grid is the tile count rounded up to 8; false past the tiles.

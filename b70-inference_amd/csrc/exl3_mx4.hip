@@ -225,40 +225,26 @@ template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args a) {
     typedef Mx4Wide<XT, RG> L;
     __shared__ u32x4_t lds[L::kLds];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     unsigned mt, nt;
     if (!mx4_tile_of((unsigned)((a.m + 32 * RG - 1) / (32 * RG)), (unsigned)((a.n + 255) / 256), mt, nt)) return;
     const int64_t m0 = (int64_t)mt * (32 * RG), n0 = (int64_t)nt * 256 + 64 * wave;
     L p;
     p.kb = a.k / 32;
     p.lds = lds;
+    p.base = XT == kRowF16 ? a.base : 0;
 #pragma unroll
     for (int i = 0; i < RG; ++i) {
         const int64_t m = m0 + (t >> 3) + 32 * i;
         p.xp[i] = a.x + (m < a.m ? m : a.m - 1) * a.x_ld;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t n = n0 + 32 * i + r, nc = n < a.n ? n : a.n - 1;
-        p.wq[i] = a.w + nc * (a.k / 2);
-        p.base[i] = XT == kRowF16 ? a.base : 0;
-    }
-    const int64_t ns = n0 + lane < a.n ? n0 + lane : a.n - 1;
-    p.wsc = a.ws + ns * p.kb;
-    p.sleft = (a.n - ns) * p.kb;
-    f16_t acc[RG][2];
-#pragma unroll
-    for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
+    p.weights(a.w, a.ws, n0, a.n, lane);
+    typename L::Acc acc;
+    L::zero(acc);
     p.run(t, acc);
-    // lane l holds column l & 31 (a row of x), rows 8 q + 4 (l >> 5) + 0 .. 3 (neighbouring outputs)
 #pragma unroll
     for (int j = 0; j < RG; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                mx4_store(a, m0 + 32 * j + r, n0 + 32 * i + 8 * q + 4 * g,
-                          f4_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]});
+        L::each(acc, j, lane, [&](int row, int n, f4_t v) { mx4_store(a, m0 + 32 * j + row, n0 + n, v); });
 }
 
 template <int XT, int RG>
@@ -271,7 +257,7 @@ static int launch_wide(const Mx4Args& a, hipStream_t st) {
 
 template <int XT>
 static int linear_run(const Mx4Args& a, hipStream_t st) {
-    if (a.m <= 64 || a.n * (a.k / 32) < 16) return launch_rows<XT>("mx4_linear", a, st);
+    if (a.m <= 64 || a.n * (a.k / 32) < 16 || a.k > 1 << 24) return launch_rows<XT>("mx4_linear", a, st);
     const int rg = env_int("MX4_RG", a.m <= 96 ? 2 : 4);
     return rg == 4 ? launch_wide<XT, 4>(a, st) : rg == 2 ? launch_wide<XT, 2>(a, st) : launch_wide<XT, 1>(a, st);
 }
@@ -292,15 +278,6 @@ struct Mx4Tile {
 };
 
 __device__ __forceinline__ int mx4_unit(int row, int unit) { return row * 4 + (unit ^ (row >> 1 & 3)); }
-
-constexpr uint32_t kMx4Out = 0xF0000000u;                      // an offset past every buffer
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx4_rsrc(const uint8_t* p, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)(bytes < 0xE0000000LL ? bytes : 0xE0000000LL), 0x00020000);
-}
-__device__ __forceinline__ u32x4_t mx4_buffer16(__amdgpu_buffer_rsrc_t r, uint32_t at, int base) {
-    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, base, 0));
-}
 
 template <int TM, int TN, int WM, int WN, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) {

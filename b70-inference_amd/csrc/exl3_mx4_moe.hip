@@ -125,20 +125,12 @@ __global__ __launch_bounds__(512) void mx4_down_rows_kernel(Mx4MoeArgs a) {
 // Waves 0 and 1 take 64 gate columns each, waves 2 and 3 the up columns; they meet in LDS, 32 rows at a time.
 constexpr int kMx4CS = 264;            // floats per row there: gate columns at 0, up columns at 132
 
-// Scales of weight row `row` (of `rows`, `k` wide) of projection p of block d.
-template <typename L>
-__device__ __forceinline__ void mx4_expert_scales(const ItemDesc* d, int p, int row, int rows, int k, L& o) {
-    const int64_t r = row < rows ? row : rows - 1;
-    o.wsc = reinterpret_cast<const uint8_t*>(d->tab[3 * p + 1]) + r * (k / 32);
-    o.sleft = (rows - r) * (k / 32);
-}
-
 template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(Mx4MoeArgs a) {
     typedef Mx4Wide<XT, RG> L;
     constexpr int kC = 32 * kMx4CS * 4 / 16;
     __shared__ u32x4_t lds[L::kLds > kC ? L::kLds : kC];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned nc = ((unsigned)a.I + 127) / 128;
     const ItemDesc* d = a.blocks + blockIdx.x / nc;
     const int cnt = d->cnt, p0 = d->p0, i0 = (int)(blockIdx.x % nc) * 128, pj = wave >> 1;
@@ -151,13 +143,11 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(
         const int m = (t >> 3) + 32 * i;
         p.xp[i] = a.x + (int64_t)ldg(a.pair_tok + p0 + (m < cnt ? m : cnt - 1)) * a.x_ld;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        mx4_expert_row<XT>(d, pj, i0 + 64 * (wave & 1) + 32 * i + r, a.I, a.H, p.wq[i], p.wsc, p.base[i]);
-    mx4_expert_scales(d, pj, i0 + 64 * (wave & 1) + lane, a.I, a.H, p);
-    f16_t acc[RG][2];
-#pragma unroll
-    for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
+    p.base = XT == kRowF16 ? (int)d->tab[3 * pj + 2] : 0;
+    p.weights(reinterpret_cast<const uint8_t*>(d->tab[3 * pj]), reinterpret_cast<const uint8_t*>(d->tab[3 * pj + 1]),
+              i0 + 64 * (wave & 1), a.I, lane);
+    typename L::Acc acc;
+    L::zero(acc);
     p.run(t, acc);
     const int bg = XT == kRowF16 ? (int)d->tab[2] : 0, bu = XT == kRowF16 ? (int)d->tab[5] : 0;
     float* C = reinterpret_cast<float*>(lds);
@@ -165,12 +155,9 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(
     for (int j = 0; j < RG; ++j) {
         if (32 * j >= cnt) break;                              // uniform
         if (j > 0) __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<f4_t*>(C + r * kMx4CS + 132 * pj + 64 * (wave & 1) + 32 * i + 8 * q + 4 * g) =
-                    f4_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+        L::each(acc, j, lane, [&](int row, int n, f4_t v) {
+            *reinterpret_cast<f4_t*>(C + row * kMx4CS + 132 * pj + 64 * (wave & 1) + n) = v;
+        });
         __syncthreads();
         const int m = 32 * j + (t >> 3);
 #pragma unroll
@@ -192,7 +179,7 @@ template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx4MoeArgs a) {
     typedef Mx4Wide<XT, RG> L;
     __shared__ u32x4_t lds[L::kLds];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 31, g = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned nc = ((unsigned)a.H + 255) / 256;
     const ItemDesc* d = a.blocks + blockIdx.x / nc;
     const int cnt = d->cnt, p0 = d->p0, h0 = (int)(blockIdx.x % nc) * 256 + 64 * wave;
@@ -205,31 +192,21 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx
         const int m = (t >> 3) + 32 * i;
         p.xp[i] = reinterpret_cast<const uint8_t*>(a.mid + (int64_t)(p0 + (m < cnt ? m : cnt - 1)) * a.I);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) mx4_expert_row<XT>(d, 2, h0 + 32 * i + r, a.H, a.I, p.wq[i], p.wsc, p.base[i]);
-    mx4_expert_scales(d, 2, h0 + lane, a.H, a.I, p);
-    f16_t acc[RG][2];
-#pragma unroll
-    for (int j = 0; j < RG; ++j) acc[j][0] = acc[j][1] = f16_t{};
+    p.base = XT == kRowF16 ? (int)d->tab[8] : 0;
+    p.weights(reinterpret_cast<const uint8_t*>(d->tab[6]), reinterpret_cast<const uint8_t*>(d->tab[7]), h0, a.H, lane);
+    typename L::Acc acc;
+    L::zero(acc);
     p.run(t, acc);
-    const int bd = XT == kRowF16 ? (int)d->tab[8] : 0;
 #pragma unroll
-    for (int j = 0; j < RG; ++j) {
-        const int m = 32 * j + r;
-        if (m >= cnt) break;
-        const float w = ldg(a.pair_w + p0 + m);
-        float* y = a.y + (int64_t)(p0 + m) * a.H;
+    for (int j = 0; j < RG; ++j)
+        L::each(acc, j, lane, [&](int row, int n, f4_t v) {
+            const int m = 32 * j + row;
+            if (m >= cnt || h0 + n >= a.H) return;
+            const float w = ldg(a.pair_w + p0 + m);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int h = h0 + 32 * i + 8 * q + 4 * g;
-                f4_t v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = w * __builtin_ldexpf(acc[j][i][4 * q + e], bd);
-                if (h < a.H) *reinterpret_cast<f4_t*>(y + h) = v;
-            }
-    }
+            for (int e = 0; e < 4; ++e) v[e] = w * __builtin_ldexpf(v[e], p.base);
+            *reinterpret_cast<f4_t*>(a.y + (int64_t)(p0 + m) * a.H + h0 + n) = v;
+        });
 }
 
 // out[t] = sum of token t's y rows in slot order, four columns per thread.

@@ -1,13 +1,19 @@
-// Products of many 16-bit rows with MX4 weights on 32 x 32 x 16 MFMAs: a workgroup of four waves takes 32 RG rows of x and
-// 64 weight rows (outputs) per wave. Bound by the MFMAs from about 64 rows (RG 4: 64 MFMAs of 32 cycles per wave and step
-// against 64 conversions and 32 LDS reads), below by the conversions and the weights' bytes.
+// Products of many 16-bit rows with MX4 weights: a workgroup of four waves takes 32 RG rows of x and 64 weight rows (outputs)
+// per wave, in steps of 128 k (four blocks). Bound by the MFMAs at 128 rows (RG 4: 2048 cycles of them per wave and step
+// against 64 conversions and 32 LDS reads), by the weights' bytes at 32.
 //
-// Steps of 128 k (four blocks). Lane l holds weight row l & 31 and blocks 2 g and 2 g + 1, g = l >> 5, of the step: 32
-// neighbouring bytes of codes, read straight from memory (each weight is read and converted by one wave of the workgroup
-// only); every word of a block, converted with the block's scale, is one fragment. x goes through one of two LDS buffers,
-// staged through registers while the step before is multiplied (RG 4: in halves of 64 k, for want of registers); a block
-// of weights is on its way for a whole step before its products.
+// x goes through one of two LDS buffers, staged through registers while the step before is multiplied. Weights are read
+// straight into the lanes that convert them, each by one wave of the workgroup only; every word of a block, converted with
+// the block's scale, is one fragment.
+//   RG 1, 2: 16 x 16 x 32 MFMAs, four tiles per wave. Lane l holds weight row l & 15 of each and block l >> 4 of the step, so a
+//     load takes 64 neighbouring bytes of 16 rows: whole sectors, each asked for once (with 32 x 32 tiles 32 bytes of 32
+//     rows, and the rest of the sector has left the L1 when its turn comes: 1.2 times the time for 20 rows per expert).
+//     Weights and x are on their way for a whole step.
+//   RG 4: 32 x 32 x 16 MFMAs, two tiles per wave, half the fragments in registers (the 16 x 16 form spills). Lane l holds row
+//     l & 31 and blocks 2 (l >> 5) and 2 (l >> 5) + 1; weights and x are on their way for half a step.
 #pragma once
+
+#include <type_traits>
 
 #include "exl3_mx4.h"
 
@@ -32,18 +38,53 @@ struct Mx4Wide {
     static constexpr int kScaleRow = kScaleSteps + 1;              // words per row (odd: 32 rows at one word touch every bank once)
     static constexpr int kScales = 4 * 64 * kScaleRow / 4;         // units of the four waves' scales
     static constexpr int kLds = 2 * kBuf + kScales;
+    static constexpr int kTiles = RG == 4 ? 2 : 4, kRowTiles = RG == 4 ? RG : 2 * RG;
+    typedef std::conditional_t<RG == 4, f16_t, f4_t> Tile;
+    typedef Tile Acc[kRowTiles][kTiles];
     const uint8_t* xp[RG];             // this thread's staged rows (t >> 3) + 32 i
-    const uint8_t* wq[2];              // codes of this lane's weight rows, l & 31 of the wave's two tiles
+    __amdgpu_buffer_rsrc_t wr;         // codes of the wave's 64 weight rows, 0 past the matrix
     const uint8_t* wsc;                // scales of weight row l of the wave's 64
     int64_t sleft;                     // bytes from there to the end of the matrix's scales
-    int base[2];
+    int base;
     int kb;
     u32x4_t* lds;                      // two x buffers, the waves' scales
+
+    // The wave's weight rows n0 .. n0 + 63 of `rows` (n0 below it or not), 32 kb wide.
+    __device__ __forceinline__ void weights(const uint8_t* codes, const uint8_t* scales, int64_t n0, int64_t rows, int lane) {
+        const int64_t left = rows - n0 < 64 ? (rows > n0 ? rows - n0 : 0) : 64, n = n0 + lane < rows ? n0 + lane : rows - 1;
+        wr = mx4_rsrc(codes + (left > 0 ? n0 * kb * 16 : 0), left * kb * 16);
+        wsc = scales + n * kb;
+        sleft = (rows - n) * kb;
+    }
+    __device__ __forceinline__ static void zero(Acc& acc) {
+#pragma unroll
+        for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) acc[j][i] = Tile{};
+    }
+    // fn(row of the 32, weight row of the wave's 64, its four neighbouring outputs' values) over the row group j of acc
+    template <typename F>
+    __device__ __forceinline__ static void each(const Acc& acc, int j, int lane, F fn) {
+        if constexpr (RG == 4) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    fn(lane & 31, 32 * i + 8 * q + 4 * (lane >> 5),
+                       f4_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]});
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) fn(16 * q + (lane & 15), 16 * i + 4 * (lane >> 4), acc[2 * j + q][i]);
+        }
+    }
 
     // unit u (eight k) of row r of a buffer; the row number permutes its sixteen units, so that eight lanes reading eight
     // rows or writing half of one touch every bank once
     __device__ __forceinline__ static int unit(int r, int u) { return r * 16 + (u ^ (r & 15)); }
 
+    // blocks 2 h and 2 h + 1 of step c
     __device__ __forceinline__ void load_x(int c, int h, int t, u32x4_t (&st)[RG]) const {
         const int b = 4 * c + 2 * h + ((t & 7) >> 2), bc = b < kb ? b : kb - 1;
 #pragma unroll
@@ -61,10 +102,10 @@ struct Mx4Wide {
 #pragma unroll
         for (int i = 0; i < RG; ++i) o[unit((t >> 3) + 32 * i, 8 * h + (t & 7))] = st[i];
     }
-    __device__ __forceinline__ void load_w(int c, int j, int g, u32x4_t (&w)[2]) const {
-        const int b = 4 * c + 2 * g + j, bc = b < kb ? b : kb - 1;
+    // this lane's block of step c of the tiles (RG 4: block j of its two); past the row's end the next row's, beside x that is 0
+    __device__ __forceinline__ void load_w(int c, int j, uint32_t off, u32x4_t (&w)[kTiles]) const {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = ldg(reinterpret_cast<const u32x4_t*>(wq[i] + (int64_t)bc * 16));
+        for (int i = 0; i < kTiles; ++i) w[i] = mx4_buffer16(wr, off, (64 / kTiles) * i * kb * 16 + 64 * c + 16 * j);
     }
     __device__ __forceinline__ uint32_t* scale_words(int t) const {
         return reinterpret_cast<uint32_t*>(lds + 2 * kBuf) + (t >> 6) * (64 * kScaleRow);
@@ -82,66 +123,72 @@ struct Mx4Wide {
             }
         }
     }
-    // products of one block: acc += W rows (lane l & 31) x rows of x
-    __device__ __forceinline__ void block(int c, int j, int r, int g, const u32x4_t (&w)[2], const uint32_t (&s)[2],
-                                          f16_t (&acc)[RG][2]) const {
+    // the scales of block b (of a step's four) of this lane's weight rows, from the step's words
+    __device__ __forceinline__ void tile_scales(const uint32_t* sw, int b, float (&sc)[kTiles]) const {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) sc[i] = mx4_scale(sw[64 / kTiles * i * kScaleRow] >> (8 * b) & 255, base);
+    }
+    // products of words v0 .. v1 - 1 of the lane's block b of step c: acc += W rows x rows of x
+    __device__ __forceinline__ void part(int c, int b, int v0, int v1, int r, const u32x4_t (&w)[kTiles], const float (&sc)[kTiles],
+                                         Acc& acc) const {
         const u32x4_t* x = lds + (c & 1) * kBuf;
-        const float s0 = mx4_scale(s[0] >> (16 * g + 8 * j) & 255, base[0]), s1 = mx4_scale(s[1] >> (16 * g + 8 * j) & 255, base[1]);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const u32x4_t f0 = mx4_frag<XT>(w[0][v], s0), f1 = mx4_frag<XT>(w[1][v], s1);
+        for (int v = v0; v < v1; ++v) {
+            u32x4_t f[kTiles];
 #pragma unroll
-            for (int i = 0; i < RG; ++i) {
-                const u32x4_t xv = x[unit(r + 32 * i, 4 * (2 * g + j) + v)];
-                acc[i][0] = mfma32<XT>(f0, xv, acc[i][0]);
-                acc[i][1] = mfma32<XT>(f1, xv, acc[i][1]);
+            for (int i = 0; i < kTiles; ++i) f[i] = mx4_frag<XT>(w[i][v], sc[i]);
+#pragma unroll
+            for (int j = 0; j < kRowTiles; ++j) {
+                const u32x4_t xv = x[unit(r + 32 * RG / kRowTiles * j, 4 * b + v)];
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    if constexpr (RG == 4) acc[j][i] = mfma32<XT>(f[i], xv, acc[j][i]);
+                    else acc[j][i] = mfma16<XT>(f[i], xv, acc[j][i]);
+                }
             }
         }
     }
-    __device__ __forceinline__ void run(int t, f16_t (&acc)[RG][2]) const {
-        const int lane = t & 63, r = lane & 31, g = lane >> 5, nch = (kb + 3) / 4;
-        u32x4_t st[RG], su[RG], w0[2], w1[2], n0[2], n1[2];
+    __device__ __forceinline__ void run(int t, Acc& acc) const {
+        const int lane = t & 63, r = RG == 4 ? lane & 31 : lane & 15, g = RG == 4 ? lane >> 5 : lane >> 4, nch = (kb + 3) / 4;
+        const uint32_t off = (uint32_t)r * (uint32_t)(kb * 16) + (RG == 4 ? 32 : 16) * g;
+        u32x4_t st[RG], su[RG], w[kTiles], n[kTiles];
         load_x(0, 0, t, st);
         load_x(0, 1, t, su);
-        load_w(0, 0, g, w0);
-        load_w(0, 1, g, w1);
+        load_w(0, 0, off, w);
         store_x(0, 0, t, st);
         store_x(0, 1, t, su);
         __syncthreads();
         for (int c = 0; c < nch; ++c) {
             const int cn = c + 1 < nch ? c + 1 : c;            // (past the last: read again, stored into the idle buffer)
+            const uint32_t* sw = scale_words(t) + r * kScaleRow + c % kScaleSteps;
+            float sc[kTiles];
             if (c % kScaleSteps == 0) fetch_scales(c, t);
             load_x(cn, 0, t, st);
-            if constexpr (RG < 4) {
-                load_x(cn, 1, t, su);
-                load_w(cn, 0, g, n0);
-                load_w(cn, 1, g, n1);
-            } else if (c > 0) {
-                load_w(c, 1, g, w1);
-            }
-            const uint32_t* sw = scale_words(t) + r * kScaleRow + c % kScaleSteps;
-            const uint32_t s[2] = {sw[0], sw[32 * kScaleRow]};
-            __builtin_amdgcn_sched_barrier(0);
-            block(c, 0, r, g, w0, s, acc);
-            __builtin_amdgcn_sched_barrier(0);
             if constexpr (RG == 4) {
+                load_w(c, 1, off, n);
+                tile_scales(sw, 2 * g, sc);
+                __builtin_amdgcn_sched_barrier(0);
+                part(c, 2 * g, 0, 4, r, w, sc, acc);
+                __builtin_amdgcn_sched_barrier(0);
                 store_x(c + 1, 0, t, st);
                 load_x(cn, 1, t, st);
-                load_w(cn, 0, g, w0);
+                load_w(cn, 0, off, w);
+                tile_scales(sw, 2 * g + 1, sc);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            block(c, 1, r, g, w1, s, acc);
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (RG < 4) {
+                part(c, 2 * g + 1, 0, 4, r, n, sc, acc);
+                __builtin_amdgcn_sched_barrier(0);
+                store_x(c + 1, 1, t, st);
+            } else {
+                load_x(cn, 1, t, su);
+                load_w(cn, 0, off, n);
+                tile_scales(sw, g, sc);
+                __builtin_amdgcn_sched_barrier(0);
+                part(c, g, 0, 4, r, w, sc, acc);
+                __builtin_amdgcn_sched_barrier(0);
                 store_x(c + 1, 0, t, st);
                 store_x(c + 1, 1, t, su);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    w0[i] = n0[i];
-                    w1[i] = n1[i];
-                }
-            } else {
-                store_x(c + 1, 1, t, st);
+                for (int i = 0; i < kTiles; ++i) w[i] = n[i];
             }
             __syncthreads();
         }
