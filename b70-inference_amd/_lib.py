@@ -148,20 +148,19 @@ def release_workspace():
 
 
 _same_device = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def on_device(t: torch.Tensor):
-    """Context in which t's device is the current one (the library launches on, and takes its workspace from, the current
-    device)."""
-    return _same_device if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def require_same_device(what: str, *ts):
-    """GPU tensors, all on one device."""
-    require_device(*ts)
-    devs = {t.get_device() for t in ts if t is not None}
-    if len(devs) > 1:
-        raise Exl3Error(f"{what}: tensors on several devices {sorted(devs)}")
+def on_device(what: str, t: torch.Tensor, *ts):
+    """Context in which the device of t, a GPU tensor that every other tensor must share, is the current one (the library
+    launches on, and takes its workspace from, the current device)."""
+    d = t.get_device()
+    if d < 0:
+        raise Exl3Error(f"{what}: tensors must be on a GPU, got {t.device}")
+    for o in ts:
+        if o is not None and o.get_device() != d:
+            raise Exl3Error(f"{what}: tensors must be on one GPU, got {o.device} and {t.device}")
+    return _same_device if d == _current_device() else torch.cuda.device(d)
 
 
 def require_device(*ts):

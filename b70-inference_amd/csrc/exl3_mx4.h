@@ -105,12 +105,15 @@ __device__ __forceinline__ u32x4_t mx4_buffer16(__amdgpu_buffer_rsrc_t r, uint32
     return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, base, 0));
 }
 
-// This workgroup's tile of nmt x nnt (rows x columns). Ids go round robin over the 8 XCDs; an XCD takes a contiguous run of
-// tiles, eight rows of tiles after one another for each column, so that the workgroups that run together on it share
-// their columns' and rows' operands in its L2. The grid is the tile count rounded up to 8; false past the tiles.
-__device__ __forceinline__ bool mx4_tile_of(unsigned nmt, unsigned nnt, unsigned& mt, unsigned& nt) {
-    const unsigned tiles = nmt * nnt, per = gridDim.x >> 3, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (t >= tiles) return false;
+// This workgroup's tile of nmt x nnt (rows x columns) and its split of k. Ids go round robin over the 8 XCDs; an XCD takes a
+// contiguous run of tiles, a tile's splits and then eight rows of tiles after one another for each column, so that the
+// workgroups that run together on it share their columns' and rows' operands in its L2. The grid is the tiles times the
+// splits, rounded up to 8; false past them.
+__device__ __forceinline__ bool mx4_tile_of(unsigned nmt, unsigned nnt, int splits, unsigned& mt, unsigned& nt, unsigned& sp) {
+    const unsigned all = nmt * nnt * splits, per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (id >= all) return false;
+    const unsigned t = id / (unsigned)splits;
+    sp = id - t * splits;
     const unsigned band = t / (8 * nnt), in = t - band * 8 * nnt, h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
     nt = in / h;
     mt = 8 * band + in - nt * h;

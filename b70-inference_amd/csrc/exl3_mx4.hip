@@ -1,7 +1,8 @@
 // MX4 (microscaled 4-bit) quantisation, its inverse, and the dense products with MX4 weights: 16-bit rows (exl3_mx4_linear)
 // and MX4 rows (exl3_mx4_gemm).
 #include "exl3_mx4.h"
-#include "exl3_mx4_rows.h"
+#include "exl3_mx4_decode.h"
+#include "exl3_mx4_plan.h"
 #include "exl3_mx4_wide.h"
 
 namespace exl3 {
@@ -152,6 +153,10 @@ struct Mx4Args {
     int64_t out_ld;
     int64_t m, n;
     int k, base, out_dtype, vec;       // vec: four neighbouring outputs may be stored together
+    // k split over workgroups: `splits` of `bps` steps of 128 k each, their sums in part [splits][m][n4]
+    float* part;
+    int splits, bps;
+    int64_t n4;                        // n rounded up to 4
 };
 
 // A dense output's four neighbours n, n + 1, ... of row m: 2^base of the sum, the bias, one rounding.
@@ -171,52 +176,157 @@ __device__ __forceinline__ void mx4_store(const Mx4Args& a, int64_t m, int64_t n
         if (n + q < a.n) store_as(a.out, m * a.out_ld + n + q, v[q], a.out_dtype);
 }
 
-template <int XT, int NT, int MT, int U>
-__global__ __launch_bounds__(512) void mx4_rows_kernel(Mx4Args a) {
-    extern __shared__ f4_t red[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const unsigned nt = (unsigned)((a.n + 16 * NT - 1) / (16 * NT));
-    const int64_t n0 = (int64_t)(blockIdx.x % nt) * (16 * NT), m0 = (int64_t)(blockIdx.x / nt) * (16 * MT);
-    const int r = lane & 15, kb = a.k / 32;
-    const uint8_t *wq[NT], *wsc[NT], *xq[MT], *xsc[MT];
-    int base[NT];
-    f4_t acc[NT][MT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int64_t n = n0 + 16 * i + r, nc = n < a.n ? n : a.n - 1;
-        wq[i] = a.w + nc * (a.k / 2);
-        wsc[i] = a.ws + nc * kb;
-        base[i] = a.base;
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f4_t{};
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int64_t m = m0 + 16 * j + r, mc = m < a.m ? m : a.m - 1;
-        xq[j] = a.x + mc * a.x_ld;
-        xsc[j] = XT == kRowMX4 ? a.xs + mc * kb : nullptr;
-    }
-    mx4_rows_loop<XT, NT, MT, U>(wq, wsc, base, xq, xsc, kb, wave, waves, (kb + 3) / 4, lane >> 4, acc);
-    mx4_rows_put(red, wave, lane, acc);
-    for (int t = threadIdx.x; t < NT * MT * 64; t += blockDim.x) {
-        const int l = t & 63, j = (t >> 6) % MT, i = (t >> 6) / MT;
-        mx4_store(a, m0 + 16 * j + (l & 15), n0 + 16 * i + 4 * (l >> 4), mx4_rows_sum<NT, MT>(red, waves, i, j, l));
+// Four neighbouring sums of row m of split `sp`.
+__device__ __forceinline__ void mx4_put(const Mx4Args& a, int sp, int64_t m, int64_t n, f4_t v) {
+    if (!a.part) {
+        mx4_store(a, m, n, v);
+    } else if (m < a.m && n < a.n4) {
+        *reinterpret_cast<f4_t*>(a.part + ((int64_t)sp * a.m + m) * a.n4 + n) = v;
     }
 }
 
-typedef void (*mx4_fn)(Mx4Args);
+// The splits' sums in order, 2^base, the bias, one rounding.
+__global__ __launch_bounds__(256) void mx4_reduce_kernel(Mx4Args a) {
+    const int64_t q4 = a.n4 / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / q4, n = 4 * (i - m * q4);
+    if (m >= a.m) return;
+    const float* p = a.part + m * a.n4 + n;
+    f4_t v = {};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        f4_t t[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            t[s] = ldg(reinterpret_cast<const f4_t*>(p + (int64_t)(s0 + s < a.splits ? s0 + s : s0) * a.m * a.n4));
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s0 + s < a.splits)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += t[s][e];
+    }
+    mx4_store(a, m, n, v);
+}
+
+// The plan's splits, with the partials' buffer from the workspace. One split: the kernel writes the output itself.
+static int mx4_split(Mx4Args& a, const Mx4Plan& plan, hipStream_t st) {
+    a.splits = plan.P;
+    a.bps = plan.bps;
+    a.n4 = (a.n + 3) & ~(int64_t)3;
+    a.part = nullptr;
+    if (a.splits == 1) return EXL3_OK;
+    Workspace ws;
+    const int rc = workspace((size_t)a.splits * a.m * a.n4 * 4, 0, st, &ws);
+    a.part = reinterpret_cast<float*>(ws.scratch);
+    return rc;
+}
+
+static int launch_reduce(const Mx4Args& a, hipStream_t st) {
+    if (a.splits == 1) return EXL3_OK;
+    const int64_t wgs = (a.m * (a.n4 / 4) + 255) / 256;
+    EXL3_CHECK_ARG(wgs <= 0x7FFFFFFF, "mx4: grid too large");
+    EXL3_LAUNCH("mx4_reduce", mx4_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a);
+    return EXL3_OK;
+}
+
+// One output per thread: matrices of fewer than 16 scale bytes, which the other kernels' 16-byte loads of scales do not fit.
+template <int XT>
+__global__ __launch_bounds__(256) void mx4_tiny_kernel(Mx4Args a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / a.n, n = i - m * a.n;
+    if (m >= a.m) return;
+    const int kb = a.k / 32;
+    float sum = 0.f;
+    for (int b = 0; b < kb; ++b) {
+        const float ws = mx4_scale(a.ws[n * kb + b], a.base), xs = XT == kRowMX4 ? mx4_scale(a.xs[m * kb + b], 0) : 1.f;
+        float part = 0.f;
+        for (int e = 0; e < 16; ++e) {
+            const auto w = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.w[n * (a.k / 2) + 16 * b + e], ws, 0);
+            float x0, x1;
+            if constexpr (XT == kRowMX4) {
+                const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.x[m * a.x_ld + 16 * b + e], 1.f, 0);
+                x0 = x[0];
+                x1 = x[1];
+            } else {
+                const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x + m * a.x_ld) + 32 * b + 2 * e;
+                x0 = XT == kRowF16 ? h2f(x[0]) : bf2f(x[0]);
+                x1 = XT == kRowF16 ? h2f(x[1]) : bf2f(x[1]);
+            }
+            part += x0 * w[0] + x1 * w[1];
+        }
+        sum += part * xs;
+    }
+    if (a.base) sum = __builtin_ldexpf(sum, a.base);
+    if (a.bias) sum += ldg(a.bias + n);
+    store_as(a.out, m * a.out_ld + n, sum, a.out_dtype);
+}
 
 template <int XT>
-static int launch_rows(const char* name, const Mx4Args& a, hipStream_t st) {
-    const int mt = a.m <= 16 ? 1 : a.m <= 32 ? 2 : a.m <= 48 ? 3 : 4, nt = mt == 1 ? 1 : 2;
-    constexpr bool q = XT == kRowMX4;
-    const mx4_fn fn = mt == 1 ? mx4_rows_kernel<XT, 1, 1, 4>
-                    : mt == 2 ? mx4_rows_kernel<XT, 2, 2, q ? 4 : 2>
-                    : mt == 3 ? mx4_rows_kernel<XT, 2, 3, q ? 4 : 1> : mx4_rows_kernel<XT, 2, 4, q ? 4 : 1>;
-    const int64_t grid = (a.n + 16 * nt - 1) / (16 * nt) * ((a.m + 16 * mt - 1) / (16 * mt));
-    EXL3_CHECK_ARG(grid <= 0x7FFFFFFF, "%s: grid too large", name);
-    const int waves = mx4_rows_waves((a.k / 32 + 3) / 4);
-    EXL3_LAUNCH(name, fn, dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * nt * mt * 1024, st, a);
+static int launch_tiny(const char* name, const Mx4Args& a, hipStream_t st) {
+    EXL3_CHECK_ARG(a.m <= (int64_t)0x7FFFFFFF * 256 / a.n - 256, "%s: grid too large", name);
+    EXL3_LAUNCH(name, mx4_tiny_kernel<XT>, dim3((unsigned)((a.m * a.n + 255) / 256)), dim3(256), 0, st, a);
+    return EXL3_OK;
+}
+
+// Up to 16 rows, x in LDS. A workgroup takes every gridDim-th tile of 16 outputs, so x is staged once per resident workgroup.
+template <int XT>
+__global__ __launch_bounds__(1024) void mx4_decode_kernel(Mx4Args a, int xbytes) {
+    extern __shared__ f4_t red[];
+    char* lds = reinterpret_cast<char*>(red);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int rows = (int)a.m, kb = a.k / 32, ng = (kb + 4 * kMx4Group - 1) / (4 * kMx4Group);
+    const unsigned tiles = (unsigned)((a.n + 15) / 16);
+    Mx4Decode<XT> p;
+    p.kb = kb;
+    p.tile.set(a.w, a.ws, (int64_t)blockIdx.x * 16, a.n, kb, lane);
+    typename Mx4Decode<XT>::Group q, nx;
+    p.load(wave, lane, q);
+    const Mx4X x = mx4_stage_x<XT>(lds, rows, kb, [&](int i) { return a.x + i * a.x_ld; }, [&](int i) { return a.xs + (int64_t)i * kb; });
+    __syncthreads();
+    f4_t* const out = reinterpret_cast<f4_t*>(lds + xbytes);
+    unsigned tile = blockIdx.x;
+    for (int buf = 0;; buf ^= 1) {                             // (waves <= ng: every wave has a group of every tile)
+        f4_t acc = {};
+        const unsigned next = tile + gridDim.x;
+        for (int gi = wave; gi < ng; gi += waves) {
+            const bool last = gi + waves >= ng;                // (uniform) then on to the next tile
+            if (!last) {
+                p.load(gi + waves, lane, nx);
+            } else if (next < tiles) {
+                p.tile.set(a.w, a.ws, (int64_t)next * 16, a.n, kb, lane);
+                p.load(wave, lane, nx);
+            }
+            p.mul(gi, lane, x, rows, a.base, q, acc);
+            q = nx;
+        }
+        f4_t* o = out + buf * waves * 64;                      // two, so that one barrier a tile is enough
+        o[wave * 64 + lane] = acc;
+        __syncthreads();
+        if (wave == 0) mx4_store(a, lane & 15, (int64_t)tile * 16 + 4 * (lane >> 4), mx4_decode_sum(o, waves, 0, lane));
+        if (next >= tiles) break;
+        tile = next;
+    }
+}
+
+// LDS of a CU, all of which one workgroup may take.
+constexpr int kMx4Lds = 163840;
+
+// Waves and LDS bytes of a decode call: eight waves, sixteen where x leaves room for one workgroup per CU only (eight rows of
+// 5376 -> 21504: 25.1 us with eight, 21.4 with sixteen). False if x does not fit.
+template <int XT>
+static bool decode_shape(const Mx4Args& a, int& waves, int& xb, int& lds) {
+    if (a.m > 16 || a.k > 1 << 20) return false;
+    const int kb = a.k / 32, ng = (kb + 4 * kMx4Group - 1) / (4 * kMx4Group);
+    xb = mx4_x_bytes<XT>((int)a.m, kb);
+    waves = mx4_decode_waves(ng, 8);
+    if (2 * (xb + 2 * waves * 1024) > kMx4Lds && xb + 2 * 16 * 1024 <= kMx4Lds) waves = mx4_decode_waves(ng, 16);
+    lds = xb + 2 * waves * 1024;
+    return lds <= kMx4Lds;
+}
+
+template <int XT>
+static int launch_decode(const char* name, const Mx4Args& a, int waves, int xb, int lds, hipStream_t st) {
+    // resident workgroups: LDS, and registers for 16 waves per CU
+    const int occ = kMx4Lds / lds < 16 / waves ? kMx4Lds / lds : 16 / waves;
+    const int64_t tiles = (a.n + 15) / 16, grid = tiles < 256 * occ ? tiles : 256 * occ;
+    EXL3_CHECK_ARG(tiles <= 0x3FFFFFFF, "%s: grid too large", name);
+    EXL3_LAUNCH(name, mx4_decode_kernel<XT>, dim3((unsigned)grid), dim3(64 * waves), (size_t)lds, st, a, xb);
     return EXL3_OK;
 }
 
@@ -226,8 +336,8 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args
     typedef Mx4Wide<XT, RG> L;
     __shared__ u32x4_t lds[L::kLds];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    unsigned mt, nt;
-    if (!mx4_tile_of((unsigned)((a.m + 32 * RG - 1) / (32 * RG)), (unsigned)((a.n + 255) / 256), mt, nt)) return;
+    unsigned mt, nt, sp;
+    if (!mx4_tile_of((unsigned)((a.m + 32 * RG - 1) / (32 * RG)), (unsigned)((a.n + 255) / 256), a.splits, mt, nt, sp)) return;
     const int64_t m0 = (int64_t)mt * (32 * RG), n0 = (int64_t)nt * 256 + 64 * wave;
     L p;
     p.kb = a.k / 32;
@@ -241,25 +351,29 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args
     p.weights(a.w, a.ws, n0, a.n, lane);
     typename L::Acc acc;
     L::zero(acc);
-    p.run(t, acc);
+    p.run(t, sp * a.bps, a.bps, acc);
 #pragma unroll
     for (int j = 0; j < RG; ++j)
-        L::each(acc, j, lane, [&](int row, int n, f4_t v) { mx4_store(a, m0 + 32 * j + row, n0 + n, v); });
+        L::each(acc, j, lane, [&](int row, int n, f4_t v) { mx4_put(a, sp, m0 + 32 * j + row, n0 + n, v); });
 }
 
 template <int XT, int RG>
-static int launch_wide(const Mx4Args& a, hipStream_t st) {
+static int launch_wide(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
     const int64_t tiles = (a.m + 32 * RG - 1) / (32 * RG) * ((a.n + 255) / 256);
-    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0, "exl3_mx4_linear: grid too large");
-    EXL3_LAUNCH("mx4_linear_wide", (mx4_wide_kernel<XT, RG>), dim3((unsigned)((tiles + 7) & ~7)), dim3(256), 0, st, a);
-    return EXL3_OK;
+    const int rc = mx4_split(a, plan, st);
+    if (rc) return rc;
+    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0 / a.splits, "exl3_mx4_linear: grid too large");
+    EXL3_LAUNCH("mx4_linear_wide", (mx4_wide_kernel<XT, RG>), dim3((unsigned)((tiles * a.splits + 7) & ~7)), dim3(256), 0, st, a);
+    return launch_reduce(a, st);
 }
 
 template <int XT>
 static int linear_run(const Mx4Args& a, hipStream_t st) {
-    if (a.m <= 64 || a.n * (a.k / 32) < 16 || a.k > 1 << 24) return launch_rows<XT>("mx4_linear", a, st);
-    const int rg = env_int("MX4_RG", a.m <= 96 ? 2 : 4);
-    return rg == 4 ? launch_wide<XT, 4>(a, st) : rg == 2 ? launch_wide<XT, 2>(a, st) : launch_wide<XT, 1>(a, st);
+    if (a.n * (a.k / 32) < 16 || a.k > 1 << 24) return launch_tiny<XT>("mx4_linear_tiny", a, st);
+    int waves, xb, lds;
+    if (decode_shape<XT>(a, waves, xb, lds)) return launch_decode<XT>("mx4_linear", a, waves, xb, lds, st);
+    const Mx4Plan p = mx4_linear_plan(a.m, a.n, a.k, 256);
+    return p.tile == 0 ? launch_wide<XT, 1>(a, p, st) : p.tile == 1 ? launch_wide<XT, 2>(a, p, st) : launch_wide<XT, 4>(a, p, st);
 }
 
 // ------------------------------------------------------------------------------------------------ many MX4 rows
@@ -286,10 +400,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
     __shared__ uint32_t scales[2][4][T::R];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned nmt = (unsigned)((a.m + T::BM - 1) / T::BM), nnt = (unsigned)((a.n + T::BN - 1) / T::BN);
-    unsigned mt, nt;
-    if (!mx4_tile_of(nmt, nnt, mt, nt)) return;
+    unsigned mt, nt, sp;
+    if (!mx4_tile_of(nmt, nnt, a.splits, mt, nt, sp)) return;
     const int64_t m0 = (int64_t)mt * T::BM, n0 = (int64_t)nt * T::BN;
-    const int kb = a.k / 32, nch = (kb + 3) / 4;
+    const int kb = a.k / 32, c0 = sp * a.bps, nch = (kb + 3) / 4 - c0 < a.bps ? (kb + 3) / 4 - c0 : a.bps;
 
     // staging: this thread's unit t & 3 of rows (t >> 2) + i kThreads / 4, the x rows first, at 32-bit offsets from the
     // tile's first rows; buffer loads return 0 past the matrix, and x units past their row's end are moved there
@@ -304,10 +418,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
     }
     u32x4_t st[T::kUnits], ss[T::kScaleRows];
     const auto load_codes = [&](int c) {
-        const bool in = 4 * c + (t & 3) < kb;
+        const bool in = 4 * (c0 + c) + (t & 3) < kb;
 #pragma unroll
         for (int i = 0; i < T::kUnits; ++i)
-            st[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] : kMx4Out, 64 * c) : mx4_buffer16(wr, src[i], 64 * c);
+            st[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] : kMx4Out, 64 * (c0 + c)) : mx4_buffer16(wr, src[i], 64 * (c0 + c));
     };
     const auto load_scales = [&](int s) {
 #pragma unroll
@@ -317,7 +431,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
             const int64_t m = m0 + r, n = n0 + r - T::BM;
             const bool ix = r < T::BM;
             const int64_t row = ix ? (m < a.m ? m : a.m - 1) : (n < a.n ? n : a.n - 1);
-            ss[i] = mx4_scales16((ix ? a.xs : a.ws) + row * kb, 16 * s, ((ix ? a.m : a.n) - row) * kb);
+            ss[i] = mx4_scales16((ix ? a.xs : a.ws) + row * kb, 4 * c0 + 16 * s, ((ix ? a.m : a.n) - row) * kb);
         }
     };
     const auto store_codes = [&](int buf) {
@@ -331,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
             if (T::R % T::kThreads != 0 && r >= T::R) break;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int left = kb - 16 * s - 4 * q;
+                const int left = kb - 4 * c0 - 16 * s - 4 * q;
                 scales[s & 1][q][r] = ss[i][q] & (left >= 4 ? ~0u : left > 0 ? (1u << (8 * left)) - 1 : 0u);
             }
         }
@@ -392,18 +506,20 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
         for (int i = 0; i < TN; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                mx4_store(a, m0 + rm + 32 * j, n0 + rn - T::BM + 32 * i - r + 8 * q + 4 * g,
+                mx4_put(a, sp, m0 + rm + 32 * j, n0 + rn - T::BM + 32 * i - r + 8 * q + 4 * g,
                           f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
 }
 
 template <int TM, int TN, int WM, int WN, int OCC>
-static int launch_tile(const Mx4Args& a, hipStream_t st) {
+static int launch_tile(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
     typedef Mx4Tile<TM, TN, WM, WN> T;
     const int64_t tiles = (a.m + T::BM - 1) / T::BM * ((a.n + T::BN - 1) / T::BN);
-    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0, "exl3_mx4_gemm: grid too large");
-    EXL3_LAUNCH("mx4_gemm_tile", (mx4_tile_kernel<TM, TN, WM, WN, OCC>), dim3((unsigned)((tiles + 7) & ~7)), dim3(T::kThreads), 0,
-                st, a);
-    return EXL3_OK;
+    const int rc = mx4_split(a, plan, st);
+    if (rc) return rc;
+    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0 / a.splits, "exl3_mx4_gemm: grid too large");
+    EXL3_LAUNCH("mx4_gemm_tile", (mx4_tile_kernel<TM, TN, WM, WN, OCC>), dim3((unsigned)((tiles * a.splits + 7) & ~7)),
+                dim3(T::kThreads), 0, st, a);
+    return launch_reduce(a, st);
 }
 
 static bool mx4_dtype(int t) { return t == EXL3_F16 || t == EXL3_F32 || t == EXL3_BF16; }
@@ -418,6 +534,7 @@ static int mx4_setup(const char* what, int64_t m, int64_t n, int64_t k, const ui
     EXL3_CHECK_ARG(c_ld >= n, "%s: output row stride %lld < n", what, (long long)c_ld);
     EXL3_CHECK_ARG(m <= ((int64_t)1 << 40) / k && n <= ((int64_t)1 << 40) / k, "%s: operand too large", what);
     if (m == 0) return EXL3_OK;
+    a.splits = 1;
     EXL3_CHECK_ARG(w && ws && C, "%s: null pointer", what);
     EXL3_CHECK_ARG(aligned(w, 16), "%s: weight codes must be 16-byte aligned", what);
     EXL3_CHECK_ARG(aligned(C, elem_size(c_dtype)) && (!bias || aligned(bias, 4)), "%s: misaligned output or bias", what);
@@ -512,8 +629,15 @@ int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, in
     a.x = a_codes;
     a.xs = a_scales;
     a.x_ld = k / 2;
-    if (m > 128 && k < 1 << 24 && m * (k / 32) >= 16 && n * (k / 32) >= 16) return launch_tile<4, 2, 2, 2, 2>(a, (hipStream_t)stream);
-    return launch_rows<kRowMX4>("mx4_gemm", a, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (m * (k / 32) < 16 || n * (k / 32) < 16 || k > 1 << 24) return launch_tiny<kRowMX4>("mx4_gemm_tiny", a, st);
+    // few rows: the decode kernel up to eight (16 rows, decode / tiles: 4096 x 4096 10.2 / 9.9 us, 5376 -> 21504 23.0 / 19.8;
+    // 4 rows: 6.0 / 9.0, 16.5 / 19.0)
+    int waves, xb, lds;
+    if (m <= 8 && decode_shape<kRowMX4>(a, waves, xb, lds)) return launch_decode<kRowMX4>("mx4_gemm", a, waves, xb, lds, st);
+    const Mx4Plan p = mx4_gemm_plan(m, n, k, 256);
+    return p.tile == 0 ? launch_tile<2, 1, 1, 4, 4>(a, p, st) : p.tile == 1 ? launch_tile<2, 2, 2, 2, 3>(a, p, st)
+                                                              : launch_tile<4, 2, 2, 2, 2>(a, p, st);
 }
 
 }  // extern "C"

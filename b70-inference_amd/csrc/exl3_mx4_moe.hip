@@ -1,14 +1,16 @@
 // Routed MoE layer over experts with MX4 weights. Per call, on the caller's stream:
 //   align    pairs (token, slot) grouped by expert and cut into blocks of rows (exl3_moe.hip, shared with the EXL3 layer;
 //            the tables' entries are (codes, scales, base) instead of (trellis, suh, svh))
-//   gateup   workgroup per (block, 16 columns of I): both projections over H, act(gate, up) in fp32, rounded to x's type
+//   gateup   workgroup per (block, 128 columns of I): both projections over H, act(gate, up) in fp32, rounded to x's type
 //            (the down product's operand: fp32 rows would double its MFMAs; its rounding is that of the 16-bit output)
-//   down     workgroup per (block, columns of H) over I: y[pair] = routing weight * sum, fp32
+//   down     workgroup per (block, 256 columns of H) over I: y[pair] = routing weight * sum, fp32
 //   combine  out[t] = sum of the token's y rows in slot order
+// Few pairs take two launches instead: gateup per (pair, 16 columns of I), down per (token, 16 columns of H) over all of the
+// token's slots.
 #include "exl3_moe.h"
 #include "exl3_moe_dev.h"
 #include "exl3_mx4.h"
-#include "exl3_mx4_rows.h"
+#include "exl3_mx4_decode.h"
 #include "exl3_mx4_wide.h"
 #include "exl3_mx4_plan.h"
 #include "exl3_plan.h"
@@ -35,90 +37,160 @@ struct Mx4MoeArgs {
     int out_dtype;
 };
 
-// The weight row `row` (of `rows`, `k` wide) of projection p of block d: its codes, scales and base (fp16 rows only).
+// ------------------------------------------------------------------------------------------------ few pairs
+// Without the align step: a workgroup takes a pair (token, slot) as it stands. An expert that several tokens picked is read
+// once for each (from the L2).
+struct Mx4PairArgs {
+    const uint8_t* x;
+    int64_t x_ld;                      // bytes
+    int M, H, I, topk, slots, E, shared;
+    const int32_t* ids;
+    const float* tw;
+    const int64_t* tables;             // [9][E]
+    uint16_t* mid;                     // [M * slots][I]
+    int act;
+    float limit;
+    void* out;
+    int64_t out_ld;
+    int out_dtype, vec;
+    // expert of slot j of token t, -1: none
+    __device__ __forceinline__ int expert(int t, int j) const {
+        const int e = j < topk ? ldg(ids + (int64_t)t * topk + j) : shared;
+        return e >= 0 && e < E ? e : -1;
+    }
+    __device__ __forceinline__ int64_t entry(int row, int e) const { return ldg(tables + (int64_t)row * E + e); }
+};
+
+// Workgroup per (pair, 16 columns of I): the gate and the up tile.
 template <int XT>
-__device__ __forceinline__ void mx4_expert_row(const ItemDesc* d, int p, int row, int rows, int k, const uint8_t*& wq,
-                                               const uint8_t*& wsc, int& base) {
-    const int64_t r = row < rows ? row : rows - 1;
-    wq = reinterpret_cast<const uint8_t*>(d->tab[3 * p]) + r * (k / 2);
-    wsc = reinterpret_cast<const uint8_t*>(d->tab[3 * p + 1]) + r * (k / 32);
-    base = XT == kRowF16 ? (int)d->tab[3 * p + 2] : 0;
+__global__ __launch_bounds__(512) void mx4_gateup_pair_kernel(Mx4PairArgs a, int xbytes) {
+    extern __shared__ f4_t red[];
+    char* lds = reinterpret_cast<char*>(red);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const unsigned nc = (unsigned)a.I / 16, pair = blockIdx.x / nc;
+    const int t = pair / (unsigned)a.slots, e = __builtin_amdgcn_readfirstlane(a.expert(t, pair - t * a.slots)), i0 = (blockIdx.x % nc) * 16;
+    if (e < 0) return;
+    const int kb = a.H / 32, ng = (kb + 4 * kMx4Group - 1) / (4 * kMx4Group);
+    Mx4Decode<XT> p[2];
+    typename Mx4Decode<XT>::Group q[2], nx[2];
+    int base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        p[i].kb = kb;
+        base[i] = XT == kRowF16 ? (int)a.entry(3 * i + 2, e) : 0;
+        p[i].tile.set(reinterpret_cast<const uint8_t*>(a.entry(3 * i, e)), reinterpret_cast<const uint8_t*>(a.entry(3 * i + 1, e)), i0,
+                      a.I, kb, lane);
+        p[i].load(wave, lane, q[i]);
+    }
+    const Mx4X x = mx4_stage_x<XT>(lds, 1, kb, [&](int) { return a.x + (int64_t)t * a.x_ld; }, [](int) { return (const uint8_t*)nullptr; });
+    __syncthreads();
+    f4_t acc[2] = {f4_t{}, f4_t{}};
+    for (int gi = wave; gi < ng; gi += waves) {
+        const bool more = gi + waves < ng;                     // uniform
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (more) p[i].load(gi + waves, lane, nx[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            p[i].mul(gi, lane, x, 1, base[i], q[i], acc[i]);
+            q[i] = nx[i];
+        }
+    }
+    f4_t* out = reinterpret_cast<f4_t*>(lds + xbytes);
+    out[wave * 64 + lane] = acc[0];
+    out[(waves + wave) * 64 + lane] = acc[1];
+    __syncthreads();
+    if (wave != 0 || (lane & 15) != 0) return;                 // column 0 of the products is the row
+    const f4_t g = mx4_decode_sum(out, waves, 0, lane), u = mx4_decode_sum(out, waves, 1, lane);
+    f4_t v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        v[j] = act_mul_dev(__builtin_ldexpf(g[j], base[0]), __builtin_ldexpf(u[j], base[1]), a.act, a.limit);
+    store4_as(a.mid, (int64_t)pair * a.I + i0 + 4 * (lane >> 4), v, XT == kRowF16 ? EXL3_F16 : EXL3_BF16);
 }
 
-// Gate and up tiles of CT x 16 columns, blocks of up to 16 MT rows. I and H are multiples of 32, so 16 CT columns (CT 1, 2) are whole.
-template <int XT, int CT, int MT, int U>
-__global__ __launch_bounds__(512) void mx4_gateup_rows_kernel(Mx4MoeArgs a) {
+// Workgroup per (token, 16 columns of H): the token's slots after one another, their groups of 512 rows of I over the waves; a
+// wave adds a slot's sum, times its routing weight, when it goes on to another.
+template <int XT>
+__global__ __launch_bounds__(1024) void mx4_down_pair_kernel(Mx4PairArgs a, int xbytes) {
     extern __shared__ f4_t red[];
+    char* lds = reinterpret_cast<char*>(red);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const unsigned nc = (unsigned)a.I / (16 * CT);
-    const ItemDesc* d = a.blocks + blockIdx.x / nc;
-    const int cnt = d->cnt, p0 = d->p0, i0 = (int)(blockIdx.x % nc) * (16 * CT), r = lane & 15;
-    if (cnt == 0) return;                                      // past the call's blocks
-    const uint8_t *wq[2 * CT], *wsc[2 * CT], *xq[MT], *xsc[MT];
-    int base[2 * CT];
-    f4_t acc[2 * CT][MT];
+    const unsigned nc = (unsigned)a.H / 16;
+    const int t = blockIdx.x / nc, h0 = (blockIdx.x % nc) * 16;
+    const int kb = a.I / 32, ng = (kb + 4 * kMx4Group - 1) / (4 * kMx4Group), all = a.slots * ng;
+    Mx4Decode<XT> p;
+    p.kb = kb;
+    typename Mx4Decode<XT>::Group q, nx;
+    int base = 0, nbase = 0, e = -1, ne = -1;                  // of q's and nx's slots
+    const auto fetch = [&](int gi, int& ex, int& bs, typename Mx4Decode<XT>::Group& o) {
+        const int j = gi / ng;
+        ex = __builtin_amdgcn_readfirstlane(a.expert(t, j));
+        if (ex < 0) return;                                    // uniform
+        bs = XT == kRowF16 ? (int)a.entry(8, ex) : 0;
+        p.tile.set(reinterpret_cast<const uint8_t*>(a.entry(6, ex)), reinterpret_cast<const uint8_t*>(a.entry(7, ex)), h0, a.H, kb, lane);
+        p.load(gi - j * ng, lane, o);
+    };
+    fetch(wave, e, base, q);
+    // (slots without an expert have no middle row: their pair's, which nobody reads)
+    const Mx4X x = mx4_stage_x<XT>(lds, a.slots, kb, [&](int j) {
+        return reinterpret_cast<const uint8_t*>(a.mid + ((int64_t)t * a.slots + j) * a.I); }, [](int) { return (const uint8_t*)nullptr; });
+    __syncthreads();
+    f4_t tot = {}, acc = {};
+    for (int gi = wave; gi < all; gi += waves) {
+        const int j = gi / ng;
+        const bool more = gi + waves < all;
+        if (more) fetch(gi + waves, ne, nbase, nx);
+        if (e >= 0) {
+            const Mx4X xj = {x.p + j * x.stride, x.stride, x.sstride, x.scales};
+            p.mul(gi - j * ng, lane, xj, 1, base, q, acc);
+        }
+        if (!more || (gi + waves) / ng != j) {
+            if (e >= 0) {
+                const float w = j < a.topk ? ldg(a.tw + (int64_t)t * a.topk + j) : 1.f;
 #pragma unroll
-    for (int i = 0; i < 2 * CT; ++i) {
-        mx4_expert_row<XT>(d, i & 1, i0 + 16 * (i >> 1) + r, a.I, a.H, wq[i], wsc[i], base[i]);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f4_t{};
+                for (int i = 0; i < 4; ++i) tot[i] += w * __builtin_ldexpf(acc[i], base);
+            }
+            acc = f4_t{};
+        }
+        q = nx;
+        e = ne;
+        base = nbase;
     }
+    f4_t* out = reinterpret_cast<f4_t*>(lds + xbytes);
+    out[wave * 64 + lane] = tot;
+    __syncthreads();
+    if (wave != 0 || (lane & 15) != 0) return;
+    const f4_t v = mx4_decode_sum(out, waves, 0, lane);
+    const int64_t o = (int64_t)t * a.out_ld + h0 + 4 * (lane >> 4);
+    if (a.vec) {
+        store4_as(a.out, o, v, a.out_dtype);
+    } else {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int m = 16 * j + r;
-        xq[j] = a.x + (int64_t)ldg(a.pair_tok + p0 + (m < cnt ? m : cnt - 1)) * a.x_ld;
-        xsc[j] = nullptr;
-    }
-    const int kb = a.H / 32;
-    mx4_rows_loop<XT, 2 * CT, MT, U>(wq, wsc, base, xq, xsc, kb, wave, waves, (kb + 3) / 4, lane >> 4, acc);
-    mx4_rows_put(red, wave, lane, acc);
-    for (int t = threadIdx.x; t < CT * MT * 64; t += blockDim.x) {
-        const int l = t & 63, j = (t >> 6) % MT, i = (t >> 6) / MT, m = 16 * j + (l & 15);
-        if (m >= cnt) continue;
-        const f4_t g = mx4_rows_sum<2 * CT, MT>(red, waves, 2 * i, j, l), u = mx4_rows_sum<2 * CT, MT>(red, waves, 2 * i + 1, j, l);
-        f4_t v;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            v[q] = act_mul_dev(__builtin_ldexpf(g[q], base[0]), __builtin_ldexpf(u[q], base[1]), a.act, a.limit);
-        store4_as(a.mid, (int64_t)(p0 + m) * a.I + i0 + 16 * i + 4 * (l >> 4), v, XT == kRowF16 ? EXL3_F16 : EXL3_BF16);
+        for (int i = 0; i < 4; ++i) store_as(a.out, o + i, v[i], a.out_dtype);
     }
 }
 
-template <int XT, int NT, int MT, int U>
-__global__ __launch_bounds__(512) void mx4_down_rows_kernel(Mx4MoeArgs a) {
-    extern __shared__ f4_t red[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const unsigned nc = (unsigned)a.H / (16 * NT);
-    const ItemDesc* d = a.blocks + blockIdx.x / nc;
-    const int cnt = d->cnt, p0 = d->p0, h0 = (int)(blockIdx.x % nc) * (16 * NT), r = lane & 15;
-    if (cnt == 0) return;
-    const uint8_t *wq[NT], *wsc[NT], *xq[MT], *xsc[MT];
-    int base[NT];
-    f4_t acc[NT][MT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        mx4_expert_row<XT>(d, 2, h0 + 16 * i + r, a.H, a.I, wq[i], wsc[i], base[i]);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f4_t{};
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-        const int m = 16 * j + r;
-        xq[j] = reinterpret_cast<const uint8_t*>(a.mid + (int64_t)(p0 + (m < cnt ? m : cnt - 1)) * a.I);
-        xsc[j] = nullptr;
-    }
-    const int kb = a.I / 32;
-    mx4_rows_loop<XT, NT, MT, U>(wq, wsc, base, xq, xsc, kb, wave, waves, (kb + 3) / 4, lane >> 4, acc);
-    mx4_rows_put(red, wave, lane, acc);
-    for (int t = threadIdx.x; t < NT * MT * 64; t += blockDim.x) {
-        const int l = t & 63, j = (t >> 6) % MT, i = (t >> 6) / MT, m = 16 * j + (l & 15);
-        if (m >= cnt) continue;
-        const float w = a.pair_w[p0 + m];
-        f4_t v = mx4_rows_sum<NT, MT>(red, waves, i, j, l);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = w * __builtin_ldexpf(v[q], base[0]);
-        *reinterpret_cast<f4_t*>(a.y + (int64_t)(p0 + m) * a.H + h0 + 16 * i + 4 * (l >> 4)) = v;
-    }
+// LDS of the two kernels; the pair path is taken where both are at most 64 KB.
+struct Mx4PairShape {
+    int wg, xg, wd, xd;
+};
+static bool pair_shape(int H, int I, int slots, Mx4PairShape& s) {
+    const int kh = H / 32, ki = I / 32, gh = (kh + 4 * kMx4Group - 1) / (4 * kMx4Group), gi = (ki + 4 * kMx4Group - 1) / (4 * kMx4Group);
+    s.wg = mx4_decode_waves(gh, 8);
+    s.wd = mx4_decode_waves(gi * slots, 16);
+    s.xg = mx4_x_bytes<kRowF16>(1, kh);
+    s.xd = mx4_x_bytes<kRowF16>(slots, ki);
+    return s.xg + s.wg * 2048 <= 65536 && s.xd + s.wd * 1024 <= 65536;
+}
+
+template <int XT>
+static int launch_pairs(const Mx4PairArgs& a, const Mx4PairShape& s, hipStream_t st) {
+    EXL3_LAUNCH("mx4_moe_gateup_pair", mx4_gateup_pair_kernel<XT>, dim3((unsigned)(a.M * a.slots * (a.I / 16))), dim3(64 * s.wg),
+                (size_t)s.xg + s.wg * 2048, st, a, s.xg);
+    EXL3_LAUNCH("mx4_moe_down_pair", mx4_down_pair_kernel<XT>, dim3((unsigned)(a.M * (a.H / 16))), dim3(64 * s.wd),
+                (size_t)s.xd + s.wd * 1024, st, a, s.xd);
+    return EXL3_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ blocks of many rows
@@ -148,7 +220,7 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(
               i0 + 64 * (wave & 1), a.I, lane);
     typename L::Acc acc;
     L::zero(acc);
-    p.run(t, acc);
+    p.run(t, 0, 1 << 30, acc);
     const int bg = XT == kRowF16 ? (int)d->tab[2] : 0, bu = XT == kRowF16 ? (int)d->tab[5] : 0;
     float* C = reinterpret_cast<float*>(lds);
 #pragma unroll
@@ -196,7 +268,7 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx
     p.weights(reinterpret_cast<const uint8_t*>(d->tab[6]), reinterpret_cast<const uint8_t*>(d->tab[7]), h0, a.H, lane);
     typename L::Acc acc;
     L::zero(acc);
-    p.run(t, acc);
+    p.run(t, 0, 1 << 30, acc);
 #pragma unroll
     for (int j = 0; j < RG; ++j)
         L::each(acc, j, lane, [&](int row, int n, f4_t v) {
@@ -238,14 +310,6 @@ __global__ __launch_bounds__(256) void mx4_combine_kernel(Mx4MoeArgs a, int ncb,
     }
 }
 
-typedef void (*mx4_moe_fn)(Mx4MoeArgs);
-
-static int mx4_moe_rows(int64_t npairs, int64_t E) {
-    const int e = env_int("MX4_MOE_ROWS", 0);
-    if (e) return e;
-    return npairs <= 16 * E ? 16 : npairs <= 48 * E ? 32 : npairs <= 96 * E ? 64 : 128;
-}
-
 template <int XT, int RG>
 static int mx4_moe_wide(const Mx4MoeArgs& a, hipStream_t st) {
     EXL3_LAUNCH("mx4_moe_gateup_wide", (mx4_gateup_wide_kernel<XT, RG>), dim3((unsigned)(a.max_blocks * ((a.I + 127) / 128))),
@@ -259,12 +323,7 @@ template <int XT>
 static int mx4_moe_launch(const Mx4MoeArgs& a, int rows, hipStream_t st) {
     if (rows == 32) return mx4_moe_wide<XT, 1>(a, st);
     if (rows == 64) return mx4_moe_wide<XT, 2>(a, st);
-    if (rows == 128) return mx4_moe_wide<XT, 4>(a, st);
-    const int wg = mx4_rows_waves((a.H / 32 + 3) / 4), wd = mx4_rows_waves((a.I / 32 + 3) / 4);
-    const mx4_moe_fn gu = mx4_gateup_rows_kernel<XT, 1, 1, 4>, dn = mx4_down_rows_kernel<XT, 2, 1, 4>;
-    EXL3_LAUNCH("mx4_moe_gateup", gu, dim3((unsigned)(a.max_blocks * (a.I / 16))), dim3(64 * wg), (size_t)wg * 2048, st, a);
-    EXL3_LAUNCH("mx4_moe_down", dn, dim3((unsigned)(a.max_blocks * (a.H / 32))), dim3(64 * wd), (size_t)wd * 2048, st, a);
-    return EXL3_OK;
+    return mx4_moe_wide<XT, 4>(a, st);
 }
 
 }  // namespace exl3
@@ -295,6 +354,21 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
     // pairs index 32-bit tables; the grids hold a workgroup per block and 16 columns
     EXL3_CHECK_ARG(M <= (1 << 24) && npairs <= (1 << 24) && M <= ((int64_t)1 << 45) / x_ld && M <= ((int64_t)1 << 45) / out_ld,
                    "exl3_mx4_moe_forward: too many tokens");
+
+    const int vec = out_ld % 4 == 0 && aligned(out, out_dtype == EXL3_F32 ? 16 : 8);
+    // Pairs as they stand while the weights they ask for, repeated experts and all, are few: pairs / blocks, us: 512 experts of
+    // 2048 -> 512 at 80 and 160 pairs 42 / 57, 71 / 90; of 2560 -> 640 at 80 and 160 69 / 74, 129 / 117; 64 of 4096 -> 1408 at 48
+    // 94.8 / 93.6; 32 of 7168 -> 2048 at 16 and 32 93 / 103, 173 / 150; 8 of 4096 -> 4096 at 8 and 12 54 / 73, 75 / 75.
+    Mx4PairShape ps;
+    if (npairs > 0 && npairs * H * I <= 210000000 && pair_shape((int)H, (int)I, (int)slots, ps)) {
+        Workspace ws;
+        const int rc = workspace((size_t)npairs * I * 2, 0, st, &ws);
+        if (rc) return rc;
+        const Mx4PairArgs p{reinterpret_cast<const uint8_t*>(x), 2 * x_ld, (int)M, (int)H, (int)I, (int)topk, (int)slots, (int)E,
+                            (int)shared, topk_ids, topk_w, tables, reinterpret_cast<uint16_t*>(ws.scratch), act, act_limit, out,
+                            out_ld, out_dtype, vec};
+        return x_dtype == EXL3_F16 ? launch_pairs<kRowF16>(p, ps, st) : launch_pairs<kRowBF16>(p, ps, st);
+    }
 
     Mx4MoeArgs a{};
     a.x = reinterpret_cast<const uint8_t*>(x);
@@ -356,7 +430,6 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
     }
     const int64_t ncb = (H + 1023) / 1024;
     EXL3_CHECK_ARG(M * ncb <= 0x7FFFFFFF, "exl3_mx4_moe_forward: grid too large");
-    const int vec = out_ld % 4 == 0 && aligned(out, out_dtype == EXL3_F32 ? 16 : 8);
     EXL3_LAUNCH("mx4_moe_combine", mx4_combine_kernel, dim3((unsigned)(M * ncb)), dim3(256), 0, st, a, (int)ncb, vec);
     return EXL3_OK;
 }

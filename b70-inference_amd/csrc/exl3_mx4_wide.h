@@ -148,21 +148,23 @@ struct Mx4Wide {
             }
         }
     }
-    __device__ __forceinline__ void run(int t, Acc& acc) const {
-        const int lane = t & 63, r = RG == 4 ? lane & 31 : lane & 15, g = RG == 4 ? lane >> 5 : lane >> 4, nch = (kb + 3) / 4;
+    // acc += the products of steps c0 .. c0 + steps - 1 (those there are)
+    __device__ __forceinline__ void run(int t, int c0, int steps, Acc& acc) const {
+        const int lane = t & 63, r = RG == 4 ? lane & 31 : lane & 15, g = RG == 4 ? lane >> 5 : lane >> 4;
+        const int end = (kb + 3) / 4 - c0 < steps ? (kb + 3) / 4 : c0 + steps;
         const uint32_t off = (uint32_t)r * (uint32_t)(kb * 16) + (RG == 4 ? 32 : 16) * g;
         u32x4_t st[RG], su[RG], w[kTiles], n[kTiles];
-        load_x(0, 0, t, st);
-        load_x(0, 1, t, su);
-        load_w(0, 0, off, w);
-        store_x(0, 0, t, st);
-        store_x(0, 1, t, su);
+        load_x(c0, 0, t, st);
+        load_x(c0, 1, t, su);
+        load_w(c0, 0, off, w);
+        store_x(c0, 0, t, st);
+        store_x(c0, 1, t, su);
         __syncthreads();
-        for (int c = 0; c < nch; ++c) {
-            const int cn = c + 1 < nch ? c + 1 : c;            // (past the last: read again, stored into the idle buffer)
-            const uint32_t* sw = scale_words(t) + r * kScaleRow + c % kScaleSteps;
+        for (int c = c0; c < end; ++c) {
+            const int cn = c + 1 < end ? c + 1 : c;            // (past the last: read again, stored into the idle buffer)
+            const uint32_t* sw = scale_words(t) + r * kScaleRow + (c - c0) % kScaleSteps;
             float sc[kTiles];
-            if (c % kScaleSteps == 0) fetch_scales(c, t);
+            if ((c - c0) % kScaleSteps == 0) fetch_scales(c, t);
             load_x(cn, 0, t, st);
             if constexpr (RG == 4) {
                 load_w(c, 1, off, n);

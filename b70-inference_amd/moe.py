@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from ._lib import (ACT_GELU_TANH, ACT_SILU, EXL3_F16, EXL3_F32, EXL3_WORDS_PLANAR4, EXL3_WORDS_TILE_ORDER, Exl3Error,
-                   check, lib, on_device, ptr, require_device, require_same_device, stream_of)
+                   check, lib, on_device, ptr, require_device, stream_of)
 from .linear import BC_LinearEXL3
 from .mx4 import ACTS, MX4Experts, mx4_moe_forward
 
@@ -423,21 +423,20 @@ def route_balance(logits: torch.Tensor, topk_ids: torch.Tensor, score: str = "so
     mean of p[:, e]: loss = coef * sum_e E * counts[e] / (k * N) * prob[e] (coef for an even load). logits fp32 [M, E],
     topk_ids int32 [M, k] (entries outside [0, E) count nowhere). Returns (loss fp32 [1], counts int32 [E], prob fp32
     [E], rows int32 [1] = N). The picks' own bias or residency terms do not enter."""
-    require_same_device("route_balance", logits, topk_ids, mask)
+    where = on_device("route_balance", logits, topk_ids, mask)
     mask, ld = _balance_args("route_balance", logits, mask, score)
     M, E = logits.shape
     if topk_ids.dtype != torch.int32 or topk_ids.dim() != 2 or topk_ids.shape[0] != M:
         raise Exl3Error("route_balance: topk_ids must be int32 [M, k]")
     topk_ids = topk_ids.contiguous()
-    dev = logits.device
-    loss = torch.empty(1, dtype=torch.float32, device=dev)
-    counts = torch.empty(E, dtype=torch.int32, device=dev)
-    prob = torch.empty(E, dtype=torch.float32, device=dev)
-    rows = torch.empty(1, dtype=torch.int32, device=dev)
-    with on_device(logits):
-        check(lib().exl3_route_balance(ptr(logits), ld, M, E, ptr(topk_ids), topk_ids.shape[1], ptr(mask), SCORES[score],
-                                       float(coef), ptr(loss), ptr(counts), ptr(prob), ptr(rows), stream_of(logits)),
-              "route_balance")
+    loss, prob = logits.new_empty(1), logits.new_empty(E)
+    counts, rows = topk_ids.new_empty(E), topk_ids.new_empty(1)
+    with where:
+        rc = lib().exl3_route_balance(logits.data_ptr(), ld, M, E, topk_ids.data_ptr(), topk_ids.shape[1], ptr(mask),
+                                      SCORES[score], coef, loss.data_ptr(), counts.data_ptr(), prob.data_ptr(),
+                                      rows.data_ptr(), stream_of(logits))
+    if rc:
+        check(rc, "route_balance")
     return loss, counts, prob, rows
 
 
@@ -448,7 +447,7 @@ def route_balance_grad(logits: torch.Tensor, counts: torch.Tensor, rows: torch.T
     element, on the GPU; None: 1): fp32 [M, E], zero in rows that are not live. counts and rows as route_balance returned
     them (summed over the processes that share the batch, if several do), constants to the gradient; k picks per row.
     out may be logits."""
-    require_same_device("route_balance_grad", logits, counts, rows, mask, grad, out)
+    where = on_device("route_balance_grad", logits, counts, rows, mask, grad, out)
     mask, ld = _balance_args("route_balance_grad", logits, mask, score)
     M, E = logits.shape
     if counts.dtype != torch.int32 or counts.numel() != E or rows.dtype != torch.int32 or rows.numel() != 1:
@@ -456,14 +455,16 @@ def route_balance_grad(logits: torch.Tensor, counts: torch.Tensor, rows: torch.T
     if grad is not None and (grad.dtype != torch.float32 or grad.numel() != 1):
         raise Exl3Error("route_balance_grad: grad must be one fp32 value")
     if out is None:
-        out = torch.empty(M, E, dtype=torch.float32, device=logits.device)
-    if out.dtype != torch.float32 or tuple(out.shape) != (M, E) or out.stride(1) != 1:
+        out = logits.new_empty((M, E))
+    elif out.dtype != torch.float32 or tuple(out.shape) != (M, E) or out.stride(1) != 1:
         raise Exl3Error("route_balance_grad: out must be fp32 [M, E] with contiguous rows")
     counts = counts.contiguous()
-    with on_device(logits):
-        check(lib().exl3_route_balance_grad(ptr(logits), ld, M, E, int(k), ptr(mask), SCORES[score], float(coef),
-                                            ptr(counts), ptr(rows), ptr(grad), ptr(out), out.stride(0) if M > 1 else E,
-                                            stream_of(logits)), "route_balance_grad")
+    with where:
+        rc = lib().exl3_route_balance_grad(logits.data_ptr(), ld, M, E, k, ptr(mask), SCORES[score], coef, counts.data_ptr(),
+                                           rows.data_ptr(), ptr(grad), out.data_ptr(), out.stride(0) if M > 1 else E,
+                                           stream_of(logits))
+    if rc:
+        check(rc, "route_balance_grad")
     return out
 
 

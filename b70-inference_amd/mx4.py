@@ -16,8 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import (ACT_GELU_TANH, ACT_SILU, EXL3_BF16, EXL3_F16, EXL3_F32, Exl3Error, check, lib, on_device, ptr,
-                   require_same_device, stream_of)
+from ._lib import ACT_GELU_TANH, ACT_SILU, EXL3_BF16, EXL3_F16, EXL3_F32, Exl3Error, check, lib, on_device, ptr, stream_of
 
 ACTS = {"silu": ACT_SILU, "gelu_tanh": ACT_GELU_TANH, ACT_SILU: ACT_SILU, ACT_GELU_TANH: ACT_GELU_TANH}
 DTYPES = {torch.float16: EXL3_F16, torch.float32: EXL3_F32, torch.bfloat16: EXL3_BF16}
@@ -42,6 +41,15 @@ class MX4Tensor:
             raise Exl3Error("MX4Tensor: codes must be 16-byte aligned")
         self.codes, self.scales = codes, scales
 
+    @classmethod
+    def empty(cls, shape, like: torch.Tensor) -> MX4Tensor:
+        """Uninitialised values of `shape` (the last dimension a multiple of 32) on like's device."""
+        t = cls.__new__(cls)
+        lead, k = tuple(shape[:-1]), shape[-1]
+        t.codes = like.new_empty(lead + (k // 2,), dtype=torch.uint8)
+        t.scales = like.new_empty(lead + (k // 32,), dtype=torch.uint8)
+        return t
+
     @property
     def k(self) -> int:
         return 32 * self.scales.shape[-1]
@@ -58,22 +66,29 @@ class MX4Tensor:
         return MX4Tensor(self.codes.to(dev), self.scales.to(dev))
 
 
+# One row of 4096 x 4096 takes 4.7 us on the GPU and quantising four of them 2: the host path is the bound, so few calls and no views
+# beyond those the shapes need.
 def _rows(x: torch.Tensor, k: int):
-    """x as [M, k] with 16-byte aligned, contiguous, non-overlapping rows (a copy where it is not), and its row stride."""
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    m, ld = x2.shape[0], x2.stride(0)
-    if m <= 1:
-        ld = k
-    if x2.stride(1) != 1 or ld < k or ld * x2.element_size() % 16 or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-        ld = k
-    return x2, ld
+    """x as [M, k] with 16-byte aligned, contiguous, non-overlapping rows (a copy where it is not), M and its row stride."""
+    if x.is_contiguous():
+        if x.data_ptr() % 16 == 0:
+            return x, x.numel() // k, k
+        x2 = x
+    else:
+        x2 = x if x.dim() == 2 else x.reshape(-1, k)
+        m, ld = x2.shape[0], x2.stride(0) if x2.shape[0] > 1 else k
+        if x2.stride(1) == 1 and ld >= k and ld * x2.element_size() % 16 == 0 and x2.data_ptr() % 16 == 0:
+            return x2, m, ld
+    x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2, x2.numel() // k, k
 
 
 def _out2(what: str, out: torch.Tensor, m: int, n: int):
     """Output rows [m, n] of `out` [..., n], and their stride."""
-    if out.dtype not in DTYPES or out.shape[-1] != n or out.numel() != m * n:
+    if out.dtype not in DTYPES or out.dim() < 1 or out.shape[-1] != n or out.numel() != m * n:
         raise Exl3Error(f"{what}: out must be fp16, bf16 or fp32 [..., {n}] with {m} rows")
+    if out.is_contiguous():
+        return out, n
     o2 = out if out.dim() == 2 else out.view(-1, n)
     ld = o2.stride(0) if m > 1 else n
     if (n > 1 and o2.stride(1) != 1) or ld < n:
@@ -85,45 +100,47 @@ def mx4_quantize(x: torch.Tensor, out: MX4Tensor | None = None) -> MX4Tensor:
     """MX4 of x (fp16, bf16 or fp32 [..., k], k a multiple of 32): per 32 values a scale 2^(floor(log2 max|x|) - 2), each
     value rounded to the nearest (ties to the even code, magnitudes above 6 scales to 6). A block with an infinity or a
     NaN becomes NaN."""
-    if x.dtype not in DTYPES:
+    dt = DTYPES.get(x.dtype)
+    if dt is None:
         raise Exl3Error(f"mx4_quantize: x must be fp16, bf16 or fp32, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
-        raise Exl3Error(f"mx4_quantize: the last dimension of {tuple(x.shape)} must be a multiple of 32")
-    require_same_device("mx4_quantize", x, *(() if out is None else (out.codes, out.scales)))
-    k = x.shape[-1]
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] == 0 or shape[-1] % 32:
+        raise Exl3Error(f"mx4_quantize: the last dimension of {tuple(shape)} must be a multiple of 32")
     if out is None:
-        out = MX4Tensor(torch.empty(x.shape[:-1] + (k // 2,), dtype=torch.uint8, device=x.device),
-                        torch.empty(x.shape[:-1] + (k // 32,), dtype=torch.uint8, device=x.device))
-    elif out.shape != x.shape:
-        raise Exl3Error(f"mx4_quantize: out is {tuple(out.shape)}, x {tuple(x.shape)}")
-    if x.numel() == 0:
-        return out
-    x2, ld = _rows(x, k)
-    with on_device(x):
-        check(lib().exl3_mx4_quantize(x2.data_ptr(), ld, x2.shape[0], k, DTYPES[x.dtype], out.codes.data_ptr(),
-                                      out.scales.data_ptr(), stream_of(x)), "mx4_quantize")
+        where = on_device("mx4_quantize", x)
+        out = MX4Tensor.empty(shape, x)
+    else:
+        where = on_device("mx4_quantize", x, out.codes, out.scales)
+        if out.shape != shape:
+            raise Exl3Error(f"mx4_quantize: out is {tuple(out.shape)}, x {tuple(shape)}")
+    k = shape[-1]
+    x2, m, ld = _rows(x, k)
+    with where:
+        rc = lib().exl3_mx4_quantize(x2.data_ptr(), ld, m, k, dt, out.codes.data_ptr(), out.scales.data_ptr(), stream_of(x))
+    if rc:
+        check(rc, "mx4_quantize")
     return out
 
 
 def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float16, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values of t [..., k] (exact in bf16 and fp32; in fp16 for scales 2^-23 .. 2^13, else rounded once)."""
+    codes, scales = t.codes, t.scales
+    shape = t.shape
+    k = shape[-1]
     if out is None:
         if dtype not in DTYPES:
             raise Exl3Error(f"mx4_dequantize: fp16, bf16 or fp32, got {dtype}")
-        out = torch.empty(t.shape, dtype=dtype, device=t.device)
-    require_same_device("mx4_dequantize", t.codes, t.scales, out)
-    if out.shape != t.shape:
-        raise Exl3Error(f"mx4_dequantize: out is {tuple(out.shape)}, the values {tuple(t.shape)}")
-    k = t.k
-    m = t.scales.numel() * 32 // k
+        out = codes.new_empty(shape, dtype=dtype)
+    elif out.shape != shape:
+        raise Exl3Error(f"mx4_dequantize: out is {tuple(out.shape)}, the values {tuple(shape)}")
+    where = on_device("mx4_dequantize", codes, scales, out)
+    m = scales.numel() * 32 // k
     o2, ld = _out2("mx4_dequantize", out, m, k)
-    if m == 0:
-        return out
-    if o2.data_ptr() % 16 or ld * out.element_size() % 16:
-        raise Exl3Error("mx4_dequantize: rows of out must be 16-byte aligned")
-    with on_device(out):
-        check(lib().exl3_mx4_dequantize(t.codes.data_ptr(), t.scales.data_ptr(), m, k, o2.data_ptr(), ld,
-                                        DTYPES[out.dtype], stream_of(out)), "mx4_dequantize")
+    with where:
+        rc = lib().exl3_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), m, k, o2.data_ptr(), ld, DTYPES[out.dtype],
+                                       stream_of(out))
+    if rc:
+        check(rc, "mx4_dequantize")
     return out
 
 
@@ -145,15 +162,17 @@ def mx4_gemm(A: MX4Tensor, B: MX4Tensor, bias: torch.Tensor | None = None, out: 
     if out is None:
         if out_dtype not in DTYPES:
             raise Exl3Error(f"mx4_gemm: out_dtype fp16, bf16 or fp32, got {out_dtype}")
-        out = torch.empty(A.shape[:-1] + (n,), dtype=out_dtype, device=A.device)
-    require_same_device("mx4_gemm", A.codes, A.scales, B.codes, B.scales, bias, out)
+        out = A.codes.new_empty(A.codes.shape[:-1] + (n,), dtype=out_dtype)
+    where = on_device("mx4_gemm", A.codes, A.scales, B.codes, B.scales, bias, out)
     m = A.scales.numel() * 32 // k
     o2, ld = _out2("mx4_gemm", out, m, n)
-    if m == 0 or n == 0:
+    if n == 0:
         return out
-    with on_device(out):
-        check(lib().exl3_mx4_gemm(A.codes.data_ptr(), A.scales.data_ptr(), m, k, B.codes.data_ptr(), B.scales.data_ptr(), n,
-                                  ptr(bias), o2.data_ptr(), ld, DTYPES[out.dtype], stream_of(out)), "mx4_gemm")
+    with where:
+        rc = lib().exl3_mx4_gemm(A.codes.data_ptr(), A.scales.data_ptr(), m, k, B.codes.data_ptr(), B.scales.data_ptr(), n,
+                                 ptr(bias), o2.data_ptr(), ld, DTYPES[out.dtype], stream_of(out))
+    if rc:
+        check(rc, "mx4_gemm")
     return out
 
 
@@ -188,20 +207,18 @@ class MX4Linear:
         k, n, w = self.in_features, self.out_features, self.weight
         if x.dim() < 1 or x.shape[-1] != k:
             raise Exl3Error(f"MX4Linear: x must be [..., {k}], got {tuple(x.shape)}")
-        require_same_device("MX4Linear", x, y, w.codes, self.bias)
+        where = on_device("MX4Linear", x, y, w.codes, self.bias)
         if x.dtype != torch.float16 and x.dtype != torch.bfloat16:
             x = x.half()
         if x.dtype == torch.float16 and not self.fp16_rows:
             raise NotImplementedError("MX4Linear: the weight's scales span more than fp16 holds; use bf16 rows")
-        x2, ld = _rows(x, k)
-        m = x2.shape[0]
+        x2, m, ld = _rows(x, k)
         y2, y_ld = _out2("MX4Linear", y, m, n)
-        if m == 0:
-            return
-        with on_device(x):
-            check(lib().exl3_mx4_linear(x2.data_ptr(), ld, DTYPES[x2.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(), n,
-                                        self.scale_base, ptr(self.bias), y2.data_ptr(), y_ld, DTYPES[y.dtype],
-                                        stream_of(x)), "mx4_linear")
+        with where:
+            rc = lib().exl3_mx4_linear(x2.data_ptr(), ld, DTYPES[x.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(), n,
+                                       self.scale_base, ptr(self.bias), y2.data_ptr(), y_ld, DTYPES[y.dtype], stream_of(x))
+        if rc:
+            check(rc, "mx4_linear")
 
     def run_alloc(self, x: torch.Tensor, out_features: int, output_fp32: bool) -> torch.Tensor:
         dt = torch.float32 if output_fp32 else x.dtype if x.dtype == torch.bfloat16 else torch.float16
@@ -289,17 +306,18 @@ def mx4_moe_forward(x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tenso
     if out is None:
         if out_dtype not in DTYPES:
             raise Exl3Error(f"mx4_moe_forward: out_dtype fp16, bf16 or fp32, got {out_dtype}")
-        out = torch.empty(M, H, dtype=out_dtype, device=x.device)
-    require_same_device("mx4_moe_forward", x, topk_ids, topk_w, experts.tables, out)
+        out = x.new_empty((M, H), dtype=out_dtype)
+    where = on_device("mx4_moe_forward", x, topk_ids, topk_w, experts.tables, out)
     o2, o_ld = _out2("mx4_moe_forward", out, M, H)
     a = ACTS.get(act)
     if a is None:
         raise NotImplementedError(f"mx4_moe_forward: activation {act!r}")
     topk_ids, topk_w = topk_ids.contiguous(), topk_w.contiguous()
-    x2, ld = _rows(x, H)
-    with on_device(x):
-        check(lib().exl3_mx4_moe_forward(x2.data_ptr(), ld, DTYPES[x.dtype], M, H, experts.I, ptr(topk_ids), ptr(topk_w),
-                                         topk_ids.shape[1], experts.E, ptr(experts.tables), a, float(act_limit),
-                                         int(shared), o2.data_ptr(), o_ld, DTYPES[out.dtype], stream_of(x)),
-              "mx4_moe_forward")
+    x2, _, ld = _rows(x, H)
+    with where:
+        rc = lib().exl3_mx4_moe_forward(x2.data_ptr(), ld, DTYPES[x.dtype], M, H, experts.I, topk_ids.data_ptr(),
+                                        topk_w.data_ptr(), topk_ids.shape[1], experts.E, experts.tables.data_ptr(), a,
+                                        act_limit, shared, o2.data_ptr(), o_ld, DTYPES[out.dtype], stream_of(x))
+    if rc:
+        check(rc, "mx4_moe_forward")
     return out
