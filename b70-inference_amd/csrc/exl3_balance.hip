@@ -64,6 +64,22 @@ __device__ __forceinline__ float row_max(float v, float* tmp) {
     return key_float(k);
 }
 
+// Rows first, first + step, .. of a workgroup's or wave's share: fn(row, the next live one or -1, whether it is the first) for
+// the live ones of 64 rows at a time, whose mask bytes are one load; dead(row) for the others.
+template <typename F, typename G>
+__device__ __forceinline__ void each_row(const uint8_t* mask, int M, int first, int step, F fn, G dead) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r0 = first; r0 < M; r0 += 64 * (int64_t)step) {
+        const int64_t r = r0 + lane * (int64_t)step;
+        const uint64_t in = __ballot(r < M), live = mask ? __ballot(r < M && ldg(mask + (r < M ? r : 0)) != 0) : in;
+        for (uint64_t b = live; b; b &= b - 1) {
+            const uint64_t rest = b & (b - 1);
+            fn((int)(r0 + __builtin_ctzll(b) * (int64_t)step), rest ? (int)(r0 + __builtin_ctzll(rest) * (int64_t)step) : -1, b == live);
+        }
+        for (uint64_t b = in & ~live; b; b &= b - 1) dead((int)(r0 + __builtin_ctzll(b) * (int64_t)step));
+    }
+}
+
 template <int V, int W>
 __device__ __forceinline__ void load_row(const float* z, int E, float (&f)[V]) {
     const int l = W > 1 ? threadIdx.x : threadIdx.x & 63;
@@ -139,11 +155,13 @@ __global__ __launch_bounds__(512) void balance_kernel(BalanceArgs a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.f;
     int live = 0;
-    for (int r = first; r < a.M; r += step) {
-        if (a.mask && !a.mask[r]) continue;                    // uniform in the lanes of a row
+    float f[V], nx[V];
+    each_row(a.mask, a.M, first, step, [&](int r, int next, bool start) {
         ++live;
-        float f[V];
-        load_row<V, W>(a.z + (int64_t)r * a.ld, a.E, f);
+        if (start) load_row<V, W>(a.z + (int64_t)r * a.ld, a.E, nx);
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[v] = nx[v];
+        if (next >= 0) load_row<V, W>(a.z + (int64_t)next * a.ld, a.E, nx);
         for (int j = l; j < a.topk; j += 64 * W) {
             const int e = ldg(a.ids + (int64_t)r * a.topk + j);
             if (e >= 0 && e < a.E) atomicAdd(&sc[e], 1);
@@ -151,7 +169,7 @@ __global__ __launch_bounds__(512) void balance_kernel(BalanceArgs a) {
         row_shares<V, W, SC, false>(f, d, a.E, tmp);
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] += f[v];
-    }
+    }, [](int) {});
     if (l == 0) atomicAdd(&s_live, live);
     if constexpr (W == 1) {
         for (int w = 0; w < waves; ++w) {
@@ -215,9 +233,20 @@ __global__ __launch_bounds__(256) void balance_reduce_kernel(BalanceArgs a) {
     if ((t & 63) == 0) s_n[t >> 6] = n;
     float p = 0.f;
     int c = 0;
-    for (int i = g; i < a.G; i += 16) {
-        p += ldg(a.part_p + (int64_t)i * a.E + ec);
-        c += ldg(a.part_c + (int64_t)i * a.E + ec);
+    for (int i0 = g; i0 < a.G; i0 += 128) {                    // eight loads of each kind under way
+        float pv[8];
+        int cv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = i0 + 16 * i < a.G ? i0 + 16 * i : i0;
+            pv[i] = ldg(a.part_p + (int64_t)at * a.E + ec);
+            cv[i] = ldg(a.part_c + (int64_t)at * a.E + ec);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p += i0 + 16 * i < a.G ? pv[i] : 0.f;
+            c += i0 + 16 * i < a.G ? cv[i] : 0;
+        }
     }
     s_p[g][q] = p;
     s_c[g][q] = c;
@@ -271,27 +300,29 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
         w[v] = n > 0 && e < a.E ? g * balance_fraction(ldg(a.counts + e), a.E, a.topk, n) / (float)n : 0.f;
     }
     const int nrow = W > 1 ? 1 : 4;
-    for (int r = W > 1 ? blockIdx.x : blockIdx.x * nrow + wave; r < a.M; r += gridDim.x * nrow) {
-        float* o = a.dz + (int64_t)r * a.d_ld;
-        if (a.mask && !a.mask[r]) {
+    float f[V], nx[V], d[V];
+    each_row(a.mask, a.M, W > 1 ? blockIdx.x : blockIdx.x * nrow + wave, gridDim.x * nrow, [&](int r, int next, bool start) {
+        if (start) load_row<V, W>(a.z + (int64_t)r * a.ld, a.E, nx);
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (l + 64 * W * v < a.E) o[l + 64 * W * v] = 0.f;
-            continue;
-        }
-        float f[V], d[V];
-        load_row<V, W>(a.z + (int64_t)r * a.ld, a.E, f);
+        for (int v = 0; v < V; ++v) f[v] = nx[v];
+        if (next >= 0) load_row<V, W>(a.z + (int64_t)next * a.ld, a.E, nx);
         row_shares<V, W, SC, true>(f, d, a.E, tmp);
         float m = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) m += f[v] * w[v];
         m = row_sum<W>(m, tmp);
+        float* o = a.dz + (int64_t)r * a.d_ld;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const float s = SC == EXL3_SCORE_SOFTMAX ? f[v] : f[v] * d[v];
             if (l + 64 * W * v < a.E) o[l + 64 * W * v] = s * (w[v] - m);
         }
-    }
+    }, [&](int r) {
+        float* o = a.dz + (int64_t)r * a.d_ld;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (l + 64 * W * v < a.E) o[l + 64 * W * v] = 0.f;
+    });
 }
 
 typedef void (*balance_fn)(BalanceArgs);

@@ -416,12 +416,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
         const int r = (t >> 2) + i * kStep;
         src[i] = (uint32_t)(r < T::BM ? r : r - T::BM) * (uint32_t)(a.k / 2) + 16 * (t & 3);
     }
-    u32x4_t st[T::kUnits], ss[T::kScaleRows];
-    const auto load_codes = [&](int c) {
+    u32x4_t st[2][T::kUnits], ss[T::kScaleRows];             // codes of steps c + 1 and c + 2 under way
+    const auto load_codes = [&](int c, u32x4_t (&d)[T::kUnits]) {
         const bool in = 4 * (c0 + c) + (t & 3) < kb;
 #pragma unroll
         for (int i = 0; i < T::kUnits; ++i)
-            st[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] : kMx4Out, 64 * (c0 + c)) : mx4_buffer16(wr, src[i], 64 * (c0 + c));
+            d[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] : kMx4Out, 64 * (c0 + c)) : mx4_buffer16(wr, src[i], 64 * (c0 + c));
     };
     const auto load_scales = [&](int s) {
 #pragma unroll
@@ -434,9 +434,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
             ss[i] = mx4_scales16((ix ? a.xs : a.ws) + row * kb, 4 * c0 + 16 * s, ((ix ? a.m : a.n) - row) * kb);
         }
     };
-    const auto store_codes = [&](int buf) {
+    const auto store_codes = [&](int buf, const u32x4_t (&d)[T::kUnits]) {
 #pragma unroll
-        for (int i = 0; i < T::kUnits; ++i) codes[buf][mx4_unit((t >> 2) + i * kStep, t & 3)] = st[i];
+        for (int i = 0; i < T::kUnits; ++i) codes[buf][mx4_unit((t >> 2) + i * kStep, t & 3)] = d[i];
     };
     const auto store_scales = [&](int s) {                     // bytes past a row's end are the next row's: 0 (255 times 0 is NaN)
 #pragma unroll
@@ -458,9 +458,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = f16_t{};
 
-    load_codes(0);
+    load_codes(0, st[0]);
     load_scales(0);
-    store_codes(0);
+    load_codes(1, st[1]);
+    store_codes(0, st[0]);
     store_scales(0);
     __syncthreads();
     const int nsup = (nch + 3) / 4;
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
         for (int cc = 0; cc < 4; ++cc) {
             const int c = 4 * sp + cc;
             if (c >= nch) break;                               // uniform
-            load_codes(c + 1);                                 // (past the last: not used)
+            load_codes(c + 2, st[cc & 1]);                     // (past the last: not used)
             __builtin_amdgcn_sched_barrier(0);                 // on their way before the products
             const u32x4_t* cb = codes[cc & 1];
             const uint32_t* sb = scales[sp & 1][cc];
@@ -494,7 +495,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
                                            : mfma32_mx4<1>(w[i], sw[i], x[j], sx[j], acc[i][j]);
             }
             __builtin_amdgcn_sched_barrier(0);                 // the loads are waited for here, behind the products
-            store_codes(~cc & 1);
+            store_codes(~cc & 1, st[~cc & 1]);
             if (cc == 3) store_scales(sp + 1);
             __syncthreads();
         }
@@ -637,7 +638,7 @@ int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, in
     if (m <= 8 && decode_shape<kRowMX4>(a, waves, xb, lds)) return launch_decode<kRowMX4>("mx4_gemm", a, waves, xb, lds, st);
     const Mx4Plan p = mx4_gemm_plan(m, n, k, 256);
     return p.tile == 0 ? launch_tile<2, 1, 1, 4, 4>(a, p, st) : p.tile == 1 ? launch_tile<2, 2, 2, 2, 3>(a, p, st)
-                                                              : launch_tile<4, 2, 2, 2, 2>(a, p, st);
+                                                              : launch_tile<4, 2, 2, 4, 2>(a, p, st);
 }
 
 }  // extern "C"

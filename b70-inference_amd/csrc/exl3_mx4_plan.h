@@ -33,7 +33,7 @@ struct Mx4Cand {
 
 // The workgroups spread over the CUs in rounds of occ each; several splits add their partials and the reduce kernel (`red`
 // us). Fitted to measured points (4096 x 1024 .. 21504 x 5376, 8 .. 2048 rows, 1 .. 16 splits): 16-bit rows 578 points, the one
-// picked within 2.3 % of the best on average, 18 % at worst; MX4 rows 693 points, 1.5 % and 12 %.
+// picked within 2.3 % of the best on average, 18 % at worst; MX4 rows 350 points, 0.8 % and 11 %.
 inline Mx4Plan mx4_plan(const Mx4Cand* cand, int ncand, float red, int64_t m, int64_t n, int64_t k, int cus) {
     const int nst = (int)((k + 127) / 128);
     Mx4Plan best = {0, 1, nst};
@@ -64,12 +64,12 @@ inline Mx4Plan mx4_linear_plan(int64_t m, int64_t n, int64_t k, int cus) {
     return mx4_plan(kCand, 3, 5.9f, m, n, k, cus);
 }
 
-// MX4 rows: tiles of 64 x 128, 128 x 128, 256 x 128
+// MX4 rows: tiles of 64 x 128, 128 x 128, 256 x 256
 inline Mx4Plan mx4_gemm_plan(int64_t m, int64_t n, int64_t k, int cus) {
-    static const Mx4Cand kCand[3] = {{64, 128, 4, {0.47f, 0.67f, 0.86f, 0.91f}, 2.9f, 0.39f},
-                                     {128, 128, 3, {0.57f, 0.78f, 1.10f, 0.f}, 3.0f, 0.34f},
-                                     {256, 128, 2, {0.85f, 1.31f, 0.f, 0.f}, 4.8f, 0.30f}};
-    return mx4_plan(kCand, 3, 4.5f, m, n, k, cus);
+    static const Mx4Cand kCand[3] = {{64, 128, 4, {0.39f, 0.56f, 0.75f, 0.76f}, 5.7f, 0.36f},
+                                     {128, 128, 3, {0.47f, 0.70f, 1.09f, 0.f}, 6.0f, 0.29f},
+                                     {256, 256, 1, {1.00f, 0.f, 0.f, 0.f}, 11.7f, 0.25f}};
+    return mx4_plan(kCand, 3, 2.8f, m, n, k, cus);
 }
 
 }  // namespace exl3
