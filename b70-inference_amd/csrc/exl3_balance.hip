@@ -379,10 +379,11 @@ int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, co
     a.counts = counts;
     a.prob = prob;
     a.rows = rows;
-    // eight rows at a time in a workgroup (one of more than 2048 experts): one workgroup up to four rounds, else up to 512
+    // eight rows at a time in a workgroup (one of more than 2048 experts): one workgroup up to four rounds, else up to 480. Not a
+    // power of two: a wave's rows would all lie at one place of padded sequences, all live or all dead.
     const int per = E > 2048 ? 1 : 8;
     const int64_t rounds = (M + per - 1) / per;
-    a.G = (int)(rounds <= 4 ? 1 : rounds / 4 < 512 ? rounds / 4 : 512);
+    a.G = (int)(rounds <= 4 ? 1 : rounds / 4 < 480 ? rounds / 4 : 480);
     if (a.G > 1) {
         Workspace ws;
         const size_t ge = (size_t)a.G * E;
@@ -417,7 +418,7 @@ int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t 
     a.dz = dlogits;
     a.d_ld = d_ld;
     const int64_t wgs = E > 2048 ? M : (M + 3) / 4;
-    EXL3_LAUNCH("route_balance_grad", balance_pick(score, a.E, true), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(256), 0,
+    EXL3_LAUNCH("route_balance_grad", balance_pick(score, a.E, true), dim3((unsigned)(wgs < 1920 ? wgs : 1920)), dim3(256), 0,
                 (hipStream_t)stream, a);
     return EXL3_OK;
 }
