@@ -356,11 +356,11 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
                    "exl3_mx4_moe_forward: too many tokens");
 
     const int vec = out_ld % 4 == 0 && aligned(out, out_dtype == EXL3_F32 ? 16 : 8);
-    // Pairs as they stand while the weights they ask for, repeated experts and all, are few: pairs / blocks, us: 512 experts of
+    // Pairs as they stand while they, and the weights they ask for, repeated experts and all, are few: pairs / blocks, us: 512 experts of
     // 2048 -> 512 at 80 and 160 pairs 42 / 57, 71 / 90; of 2560 -> 640 at 80 and 160 69 / 74, 129 / 117; 64 of 4096 -> 1408 at 48
     // 94.8 / 93.6; 32 of 7168 -> 2048 at 16 and 32 93 / 103, 173 / 150; 8 of 4096 -> 4096 at 8 and 12 54 / 73, 75 / 75.
     Mx4PairShape ps;
-    if (npairs > 0 && npairs * H * I <= 210000000 && pair_shape((int)H, (int)I, (int)slots, ps)) {
+    if (npairs > 0 && npairs <= 160 && npairs * H * I <= 210000000 && pair_shape((int)H, (int)I, (int)slots, ps)) {
         Workspace ws;
         const int rc = workspace((size_t)npairs * I * 2, 0, st, &ws);
         if (rc) return rc;

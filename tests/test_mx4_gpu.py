@@ -56,6 +56,18 @@ def test_quantize_ties_and_extremes(exl3, dtype):
     assert np.array_equal(t.codes.cpu().numpy(), c)
 
 
+def test_dequantize_rounds_once_to_fp16(exl3):
+    """Scales beyond fp16's exact range: the value rounded as numpy rounds it, infinite above the largest."""
+    codes = np.tile(np.arange(256, dtype=np.uint8)[:, None], (1, 16))
+    scales = np.arange(0, 256, dtype=np.uint8)[:, None]
+    for roll in (0, 3, 8, 100):
+        s = np.roll(scales, roll, 0)
+        t = exl3.MX4Tensor(torch.from_numpy(codes).to(DEV), torch.from_numpy(s.copy()).to(DEV))
+        with np.errstate(over="ignore"):
+            want = U.values(codes, s).astype(np.float16)
+        assert np.array_equal(exl3.mx4_dequantize(t, torch.float16).cpu().numpy(), want, equal_nan=True)
+
+
 @pytest.mark.parametrize("dtype", T3)
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
 def test_quantize_not_finite(exl3, dtype, bad):
@@ -96,7 +108,7 @@ def test_quantize_strides_shapes_and_out(exl3):
 
 # ------------------------------------------------------------------------------------------------ dense products
 SHAPES = [(1, 32, 1), (1, 64, 17), (2, 96, 33), (3, 160, 130), (16, 128, 64), (17, 544, 100), (31, 4096, 48), (33, 1056, 96),
-          (48, 512, 31), (64, 2080, 160), (65, 1024, 257), (100, 4096, 128), (129, 288, 384), (257, 640, 300), (520, 1024, 520)]
+          (48, 512, 31), (64, 2080, 160), (65, 1024, 257), (100, 4096, 128), (129, 288, 384), (257, 640, 300), (520, 1024, 520), (4, 8192, 50), (8, 8192, 50), (16, 4096, 48), (7, 21504, 40)]
 
 
 @pytest.mark.parametrize("dtype", T16)
@@ -127,6 +139,32 @@ def test_gemm(exl3, m, k, n):
     b = rows((n,), torch.bfloat16, 4)
     y = exl3.mx4_gemm(a, w, bias=b.to(DEV), out_dtype=torch.float32)
     U.check(y, ref + b.double().numpy(), mag + np.abs(b.double().numpy()), k, torch.float32)
+
+
+# One shape for every tile of the two plans, without and with k-splits (test_mx4_plan.py pins which they take), ragged in every
+# dimension. The reference covers the first, last and some other columns.
+TILES = [("linear", 3000, 160, 2601), ("linear", 2001, 8224, 70), ("linear", 1001, 160, 12301), ("linear", 1501, 4128, 2602),
+         ("gemm", 97, 544, 16401), ("gemm", 1501, 8224, 70), ("gemm", 1001, 160, 12301), ("gemm", 201, 8224, 16402)]
+
+
+@pytest.mark.parametrize("kind,m,k,n", TILES)
+def test_every_tile(exl3, kind, m, k, n):
+    w, wv = mx(exl3, (n, k), m + n)
+    cols = np.unique(np.r_[:40, n - 40:n, np.random.default_rng(m).integers(0, n, 40)] % n)
+    wv = wv[cols]
+    b = rows((n,), torch.float32, m).to(DEV)
+    bv = b.cpu().double().numpy()[cols]
+    for dtype in T16 if kind == "linear" else (torch.bfloat16,):
+        x = rows((m, k), dtype, m).to(DEV)
+        if kind == "linear":
+            xv = x.cpu().double().numpy()
+            y = exl3.MX4Linear(w, b).run_alloc(x, n, True)
+        else:
+            q = exl3.mx4_quantize(x)
+            xv = U.values(q.codes.cpu().numpy(), q.scales.cpu().numpy())
+            y = exl3.mx4_gemm(q, w, bias=b, out_dtype=torch.float32)
+        U.check(y[:, torch.from_numpy(cols).to(DEV)], xv @ wv.T + bv, np.abs(xv) @ np.abs(wv).T + np.abs(bv), k, torch.float32)
+        assert torch.isfinite(y).all()
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 200])
@@ -219,7 +257,7 @@ def test_offsets_past_32_bits(exl3):
     c, s = U.random_mx4((64, k), 51)
     w.codes[-64:] = torch.from_numpy(c).to(DEV)
     w.scales[-64:] = torch.from_numpy(s).to(DEV)
-    for m in (1, 100):
+    for m in (1, 20, 200):
         x = rows((m, k), torch.bfloat16, 52)
         a = exl3.mx4_quantize(x.to(DEV))
         xv, wv = x.double().numpy(), U.values(c, s)
@@ -292,7 +330,8 @@ def routing(M, k, E, seed, distinct=True):
 
 
 MOE = [(1, 64, 32, 4, 2), (1, 512, 160, 16, 4), (3, 96, 64, 8, 3), (8, 256, 128, 32, 4), (17, 160, 96, 3, 2), (40, 128, 256, 2, 2),
-       (70, 288, 160, 5, 1), (200, 256, 96, 4, 2), (150, 1056, 32, 64, 4)]
+       (70, 288, 160, 5, 1), (200, 256, 96, 4, 2), (150, 1056, 32, 64, 4), (300, 288, 160, 5, 1), (130, 128, 256, 2, 2),
+       (97, 96, 64, 30, 2), (4, 7168, 2048, 3, 2)]
 
 
 @pytest.mark.parametrize("dtype", T16)
@@ -384,7 +423,7 @@ def test_moe_repeatable_and_rows_independent(exl3):
 
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("dtype", T16)
-@pytest.mark.parametrize("M", [2, 40])
+@pytest.mark.parametrize("M", [2, 40, 100])
 def test_block_sparse_mlp_over_mx4_experts(exl3, dtype, M):
     E, H, I, k = 8, 256, 96, 2
     ex, _, _ = layer(exl3, E + 1, H, I, 100)

@@ -15,6 +15,13 @@ SHIM = """
 #define _Float16 short
 #include "exl3_mx4_plan.h"
 using namespace exl3;
+extern "C" void plan(int64_t m, int64_t n, int64_t k, int both, int cus, int* out) {
+    const Mx4Plan p = both ? mx4_gemm_plan(m, n, k, cus) : mx4_linear_plan(m, n, k, cus);
+    out[0] = p.tile;
+    out[1] = p.P;
+    out[2] = p.bps;
+}
+extern "C" int moe_rows(int64_t npairs, int64_t E) { return mx4_moe_rows(npairs, E); }
 extern "C" int64_t max_blocks(int64_t npairs, int64_t E, int rows) { return mx4_max_blocks(npairs, E, rows); }
 // blocks of an expert with c rows by count(), by walking locate() over every row as the align kernels do; largest block
 extern "C" void cut(int rows, int c, int* out) {
@@ -50,6 +57,9 @@ def lib(tmp_path_factory):
     L = ctypes.CDLL(str(d / "plan.so"))
     L.max_blocks.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]
     L.max_blocks.restype = ctypes.c_int64
+    L.plan.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
+    L.plan.restype = None
+    L.moe_rows.argtypes = [ctypes.c_int64] * 2
     return L
 
 
@@ -75,3 +85,35 @@ def test_blocks_of_a_call_fit_their_table(lib, rows):
             lone = min(E, npairs) - 1
             worst = lone + cut(lib, rows, npairs - lone)[0]
             assert worst <= lib.max_blocks(npairs, E, rows)
+
+
+def plan(lib, m, n, k, both, cus=256):
+    out = (ctypes.c_int * 3)()
+    lib.plan(m, n, k, both, cus, out)
+    return tuple(out)
+
+
+def test_plans_cover_k_and_stay_within_bounds(lib):
+    rng = random.Random(3)
+    for _ in range(3000):
+        m, n, k = rng.randrange(1, 5000), rng.randrange(1, 30000), 32 * rng.randrange(1, 700)
+        for both in (0, 1):
+            tile, P, bps = plan(lib, m, n, k, both, rng.choice((64, 256, 304)))
+            nst = -(-k // 128)
+            assert 0 <= tile < 3 and 1 <= P <= 16
+            assert (P - 1) * bps < nst <= P * bps        # every split has work, together they cover k
+
+
+def test_shapes_of_the_tile_tests(lib):
+    """The shapes that the GPU tests take for every tile, without and with splits."""
+    want = {(0, 3000, 160, 2601): (1, False), (0, 2001, 8224, 70): (1, True), (0, 1001, 160, 12301): (2, False),
+            (0, 1501, 4128, 2602): (2, True), (1, 97, 544, 16401): (1, False), (1, 1501, 8224, 70): (1, True),
+            (1, 1001, 160, 12301): (2, False), (1, 201, 8224, 16402): (2, True), (0, 520, 1024, 520): (0, False),
+            (0, 31, 4096, 48): (0, True), (1, 520, 1024, 520): (0, False), (1, 100, 4096, 128): (0, True)}
+    for (both, m, k, n), (tile, split) in want.items():
+        p = plan(lib, m, n, k, both)
+        assert (p[0], p[1] > 1) == (tile, split), (both, m, k, n, p)
+
+
+def test_rows_per_block(lib):
+    assert [lib.moe_rows(p, 4) for p in (1, 104, 105, 384, 385, 100000)] == [32, 32, 64, 64, 128, 128]
