@@ -152,7 +152,7 @@ struct Mx4Args {
     void* out;
     int64_t out_ld;
     int64_t m, n;
-    int k, base, out_dtype, vec;       // vec: four neighbouring outputs may be stored together
+    int k, base, out_dtype, vec;       // vec: four neighbouring outputs may be stored together; 2: eight 16-bit ones
     // k split over workgroups: `splits` of `bps` steps of 128 k each, their sums in part [splits][m][n4]
     float* part;
     int splits, bps;
@@ -183,6 +183,40 @@ __device__ __forceinline__ void mx4_put(const Mx4Args& a, int sp, int64_t m, int
     } else if (m < a.m && n < a.n4) {
         *reinterpret_cast<f4_t*>(a.part + ((int64_t)sp * a.m + m) * a.n4 + n) = v;
     }
+}
+
+// Outputs of a 32 x 32 product: of row m, sixteen from n on; lane group g (lane >> 5) holds those at 4 g in v and at 8 + 4 g in w.
+// 16-bit outputs change hands between the groups, so that a lane stores eight neighbours (16 bytes) instead of twice four: the
+// stores of 16-byte pieces of 32 rows bound the epilogue.
+__device__ __forceinline__ void mx4_put16(const Mx4Args& a, int sp, int64_t m, int64_t n, int g, f4_t v, f4_t w) {
+    if (a.part || a.vec != 2) {                                // uniform
+        mx4_put(a, sp, m, n + 4 * g, v);
+        mx4_put(a, sp, m, n + 8 + 4 * g, w);
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (a.base) {
+            v[q] = __builtin_ldexpf(v[q], a.base);
+            w[q] = __builtin_ldexpf(w[q], a.base);
+        }
+        if (a.bias) {
+            v[q] += ldg(a.bias + (n + 4 * g + q < a.n ? n + 4 * g + q : 0));
+            w[q] += ldg(a.bias + (n + 8 + 4 * g + q < a.n ? n + 8 + 4 * g + q : 0));
+        }
+    }
+    uint32_t p[2], r[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const bool h = a.out_dtype == EXL3_F16;
+        p[q] = h ? f2h(v[2 * q]) | (uint32_t)f2h(v[2 * q + 1]) << 16 : f2bf(v[2 * q]) | (uint32_t)f2bf(v[2 * q + 1]) << 16;
+        r[q] = h ? f2h(w[2 * q]) | (uint32_t)f2h(w[2 * q + 1]) << 16 : f2bf(w[2 * q]) | (uint32_t)f2bf(w[2 * q + 1]) << 16;
+        const auto x = __builtin_amdgcn_permlane32_swap(p[q], r[q], false, false);
+        p[q] = x[0];
+        r[q] = x[1];
+    }
+    if (m < a.m && n + 8 * g < a.n)
+        *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(a.out) + m * a.out_ld + n + 8 * g) = u32x4_t{p[0], p[1], r[0], r[1]};
 }
 
 // The splits' sums in order, 2^base, the bias, one rounding.
@@ -353,8 +387,12 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args
     L::zero(acc);
     p.run(t, sp * a.bps, a.bps, acc);
 #pragma unroll
-    for (int j = 0; j < RG; ++j)
-        L::each(acc, j, lane, [&](int row, int n, f4_t v) { mx4_put(a, sp, m0 + 32 * j + row, n0 + n, v); });
+    for (int j = 0; j < RG; ++j) {
+        if constexpr (RG == 4)
+            L::each16(acc, j, lane, [&](int row, int n, f4_t v, f4_t w) { mx4_put16(a, sp, m0 + 32 * j + row, n0 + n, lane >> 5, v, w); });
+        else
+            L::each(acc, j, lane, [&](int row, int n, f4_t v) { mx4_put(a, sp, m0 + 32 * j + row, n0 + n, v); });
+    }
 }
 
 template <int XT, int RG>
@@ -506,9 +544,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                mx4_put(a, sp, m0 + rm + 32 * j, n0 + rn - T::BM + 32 * i - r + 8 * q + 4 * g,
-                          f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+            for (int q = 0; q < 4; q += 2)
+                mx4_put16(a, sp, m0 + rm + 32 * j, n0 + rn - T::BM + 32 * i - r + 8 * q, g,
+                          f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]},
+                          f4_t{acc[i][j][4 * q + 4], acc[i][j][4 * q + 5], acc[i][j][4 * q + 6], acc[i][j][4 * q + 7]});
 }
 
 template <int TM, int TN, int WM, int WN, int OCC>
@@ -549,6 +588,7 @@ static int mx4_setup(const char* what, int64_t m, int64_t n, int64_t k, const ui
     a.k = (int)k;
     a.out_dtype = c_dtype;
     a.vec = n % 4 == 0 && c_ld % 4 == 0 && aligned(C, 4 * elem_size(c_dtype));
+    if (c_dtype != EXL3_F32 && n % 8 == 0 && c_ld % 8 == 0 && aligned(C, 16)) a.vec = 2;
     return EXL3_OK;
 }
 

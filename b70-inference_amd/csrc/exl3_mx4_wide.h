@@ -80,6 +80,18 @@ struct Mx4Wide {
         }
     }
 
+    // RG 4: fn(row of the 32, first of sixteen weight rows, this lane's four at 4 (lane >> 5) of them, those at 8 + 4 (lane >> 5))
+    template <typename F>
+    __device__ __forceinline__ static void each16(const Acc& acc, int j, int lane, F fn) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; q += 2)
+                fn(lane & 31, 32 * i + 8 * q,
+                   f4_t{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]},
+                   f4_t{acc[j][i][4 * q + 4], acc[j][i][4 * q + 5], acc[j][i][4 * q + 6], acc[j][i][4 * q + 7]});
+    }
+
     // unit u (eight k) of row r of a buffer; the row number permutes its sixteen units, so that eight lanes reading eight
     // rows or writing half of one touch every bank once
     __device__ __forceinline__ static int unit(int r, int u) { return r * 16 + (u ^ (r & 15)); }

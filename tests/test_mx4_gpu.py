@@ -165,6 +165,16 @@ def test_every_tile(exl3, kind, m, k, n):
             y = exl3.mx4_gemm(q, w, bias=b, out_dtype=torch.float32)
         U.check(y[:, torch.from_numpy(cols).to(DEV)], xv @ wv.T + bv, np.abs(xv) @ np.abs(wv).T + np.abs(bv), k, torch.float32)
         assert torch.isfinite(y).all()
+        # 16-bit outputs, rows of a multiple of eight of them: the same sums, rounded
+        n8 = n // 8 * 8
+        w8 = exl3.MX4Tensor(w.codes[:n8], w.scales[:n8])
+        for out in T16:
+            buf = torch.full((m, n8 + 8), 3.0, dtype=out, device=DEV)
+            if kind == "linear":
+                exl3.MX4Linear(w8, b[:n8]).run(x, buf[:, :n8])
+            else:
+                exl3.mx4_gemm(q, w8, bias=b[:n8], out=buf[:, :n8])
+            assert torch.equal(buf[:, :n8], y[:, :n8].to(out)) and (buf[:, n8:] == 3).all()
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 200])
