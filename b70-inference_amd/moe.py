@@ -433,7 +433,7 @@ def route_balance(logits: torch.Tensor, topk_ids: torch.Tensor, score: str = "so
     counts, rows = topk_ids.new_empty(E), topk_ids.new_empty(1)
     with where:
         rc = lib().exl3_route_balance(logits.data_ptr(), ld, M, E, topk_ids.data_ptr(), topk_ids.shape[1], ptr(mask),
-                                      SCORES[score], coef, loss.data_ptr(), counts.data_ptr(), prob.data_ptr(),
+                                      SCORES[score], float(coef), loss.data_ptr(), counts.data_ptr(), prob.data_ptr(),
                                       rows.data_ptr(), stream_of(logits))
     if rc:
         check(rc, "route_balance")
@@ -460,8 +460,8 @@ def route_balance_grad(logits: torch.Tensor, counts: torch.Tensor, rows: torch.T
         raise Exl3Error("route_balance_grad: out must be fp32 [M, E] with contiguous rows")
     counts = counts.contiguous()
     with where:
-        rc = lib().exl3_route_balance_grad(logits.data_ptr(), ld, M, E, k, ptr(mask), SCORES[score], coef, counts.data_ptr(),
-                                           rows.data_ptr(), ptr(grad), out.data_ptr(), out.stride(0) if M > 1 else E,
+        rc = lib().exl3_route_balance_grad(logits.data_ptr(), ld, M, E, int(k), ptr(mask), SCORES[score], float(coef),
+                                           counts.data_ptr(), rows.data_ptr(), ptr(grad), out.data_ptr(), out.stride(0) if M > 1 else E,
                                            stream_of(logits))
     if rc:
         check(rc, "route_balance_grad")

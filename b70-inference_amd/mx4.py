@@ -317,7 +317,8 @@ def mx4_moe_forward(x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tenso
     with where:
         rc = lib().exl3_mx4_moe_forward(x2.data_ptr(), ld, DTYPES[x.dtype], M, H, experts.I, topk_ids.data_ptr(),
                                         topk_w.data_ptr(), topk_ids.shape[1], experts.E, experts.tables.data_ptr(), a,
-                                        act_limit, shared, o2.data_ptr(), o_ld, DTYPES[out.dtype], stream_of(x))
+                                        float(act_limit), int(shared), o2.data_ptr(), o_ld, DTYPES[out.dtype],
+                                        stream_of(x))
     if rc:
         check(rc, "mx4_moe_forward")
     return out
