@@ -26,10 +26,10 @@ typedef int i8_t __attribute__((ext_vector_type(8)));
 enum { kRowF16 = 0, kRowBF16 = 1, kRowMX4 = 2 };
 
 // Scale byte s less the power of two taken out of the matrix (fp16 rows), as the float whose exponent the conversions
-// read. A block that needs a smaller scale than 2^-127 holds zeros only (the host checks the range); 255 stays 255.
+// read. A block whose scale leaves 2^-127 .. 2^127 so holds zeros only (the host checks the range); 255 stays 255.
 __device__ __forceinline__ float mx4_scale(int s, int base) {
     const int e = s - base;
-    return __builtin_bit_cast(float, (s == 255 ? 255 : e > 0 ? e : 0) << 23);
+    return __builtin_bit_cast(float, (s == 255 ? 255 : e < 0 ? 0 : e > 254 ? 254 : e) << 23);
 }
 
 // Eight codes (one word) times the scale, as fp16 or bf16.

@@ -199,6 +199,23 @@ def test_scales_over_the_whole_range(exl3, m):
     U.check(exl3.mx4_gemm(a, w, out_dtype=torch.float32), av @ wv.T, np.abs(av) @ np.abs(wv).T, k, torch.float32)
 
 
+@pytest.mark.parametrize("m", [1, 40, 200])
+@pytest.mark.parametrize("lo", [20, 85, 130, 190])
+def test_blocks_of_zeros_take_any_scale(exl3, m, lo):
+    k, n = 256, 255
+    w, _ = mx(exl3, (n, k), 15, lo, lo + 15)                              # fp16 rows take a power of two out of these
+    w.codes[:, 32:48] = torch.tensor([0, 8, 128, 136], dtype=torch.uint8, device=DEV).repeat(4)
+    w.scales[:, 2] = torch.arange(n, device=DEV).to(torch.uint8)          # 0 .. 254 beside zeros of either sign
+    lin = exl3.MX4Linear(w)
+    assert lin.fp16_rows
+    wv = U.values(w.codes.cpu().numpy(), w.scales.cpu().numpy())
+    for dt in T16:
+        x = rows((m, k), dt, 16)
+        y = lin.run_alloc(x.to(DEV), n, True)
+        xv = x.double().numpy()
+        U.check(y, xv @ wv.T, np.abs(xv) @ np.abs(wv).T, k, torch.float32, extra=k * 2.0 ** -149)
+
+
 @pytest.mark.parametrize("m", [1, 3, 20, 200])
 @pytest.mark.parametrize("k", [96, 512])
 def test_not_finite_stays_in_its_row(exl3, m, k):
