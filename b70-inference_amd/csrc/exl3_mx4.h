@@ -95,14 +95,15 @@ __device__ __forceinline__ u32x4_t mx4_scales16(const uint8_t* p, int at, int64_
     return v;
 }
 
-// Buffer loads of 16 bytes: 0 past the `bytes` from p (which one of fewer than 2^32 - 2^29 may not reach).
+// Buffer loads of 16 bytes: 0 past the `bytes` from p (which one of fewer than 2^32 - 2^29 may not reach). The whole offset is
+// in the vector register: the hardware does not check a scalar one.
 constexpr uint32_t kMx4Out = 0xF0000000u;  // an offset past every buffer
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx4_rsrc(const uint8_t* p, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)(bytes < 0xE0000000LL ? bytes : 0xE0000000LL), 0x00020000);
 }
-__device__ __forceinline__ u32x4_t mx4_buffer16(__amdgpu_buffer_rsrc_t r, uint32_t at, int base) {
-    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, base, 0));
+__device__ __forceinline__ u32x4_t mx4_buffer16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0));
 }
 
 // This workgroup's tile of nmt x nnt (rows x columns) and its split of k. Ids go round robin over the 8 XCDs; an XCD takes a

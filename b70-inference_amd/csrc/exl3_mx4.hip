@@ -407,7 +407,7 @@ static int launch_wide(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
 
 template <int XT>
 static int linear_run(const Mx4Args& a, hipStream_t st) {
-    if (a.n * (a.k / 32) < 16 || a.k > 1 << 24) return launch_tiny<XT>("mx4_linear_tiny", a, st);
+    if (a.n * (a.k / 32) < 16) return launch_tiny<XT>("mx4_linear_tiny", a, st);
     int waves, xb, lds;
     if (decode_shape<XT>(a, waves, xb, lds)) return launch_decode<XT>("mx4_linear", a, waves, xb, lds, st);
     const Mx4Plan p = mx4_linear_plan(a.m, a.n, a.k, 256);
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
         const bool in = 4 * (c0 + c) + (t & 3) < kb;
 #pragma unroll
         for (int i = 0; i < T::kUnits; ++i)
-            d[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] : kMx4Out, 64 * (c0 + c)) : mx4_buffer16(wr, src[i], 64 * (c0 + c));
+            d[i] = i * kStep < T::BM ? mx4_buffer16(xr, in ? src[i] + 64 * (c0 + c) : kMx4Out) : mx4_buffer16(wr, src[i] + 64 * (c0 + c));
     };
     const auto load_scales = [&](int s) {
 #pragma unroll
@@ -568,8 +568,8 @@ static int elem_size(int t) { return t == EXL3_F32 ? 4 : 2; }
 // What both products check of their weights and output; sets those of the kernel's arguments.
 static int mx4_setup(const char* what, int64_t m, int64_t n, int64_t k, const uint8_t* w, const uint8_t* ws,
                      const float* bias, void* C, int64_t c_ld, int c_dtype, Mx4Args& a) {
-    EXL3_CHECK_ARG(m >= 0 && n > 0 && k > 0 && k % 32 == 0 && k <= (1 << 30), "%s: bad sizes (m %lld, n %lld, k %lld; k a "
-                   "multiple of 32)", what, (long long)m, (long long)n, (long long)k);
+    EXL3_CHECK_ARG(m >= 0 && n > 0 && k > 0 && k % 32 == 0 && k <= (1 << 24), "%s: bad sizes (m %lld, n %lld, k %lld; k a "
+                   "multiple of 32, at most 2^24)", what, (long long)m, (long long)n, (long long)k);
     EXL3_CHECK_ARG(mx4_dtype(c_dtype), "%s: the output must be fp16, bf16 or fp32", what);
     EXL3_CHECK_ARG(c_ld >= n, "%s: output row stride %lld < n", what, (long long)c_ld);
     EXL3_CHECK_ARG(m <= ((int64_t)1 << 40) / k && n <= ((int64_t)1 << 40) / k, "%s: operand too large", what);
@@ -671,7 +671,7 @@ int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, in
     a.xs = a_scales;
     a.x_ld = k / 2;
     hipStream_t st = (hipStream_t)stream;
-    if (m * (k / 32) < 16 || n * (k / 32) < 16 || k > 1 << 24) return launch_tiny<kRowMX4>("mx4_gemm_tiny", a, st);
+    if (m * (k / 32) < 16 || n * (k / 32) < 16) return launch_tiny<kRowMX4>("mx4_gemm_tiny", a, st);
     // few rows: the decode kernel up to eight (16 rows, decode / tiles: 4096 x 4096 10.2 / 9.9 us, 5376 -> 21504 23.0 / 19.8;
     // 4 rows: 6.0 / 9.0, 16.5 / 19.0)
     int waves, xb, lds;

@@ -77,7 +77,7 @@ struct Mx4Decode {
     __device__ __forceinline__ void load(int gi, int lane, Group& q) const {
         const uint32_t off = (uint32_t)(lane & 15) * (uint32_t)(kb * 16) + 16 * (lane >> 4);
 #pragma unroll
-        for (int u = 0; u < kMx4Group; ++u) q.w[u] = mx4_buffer16(tile.w, off, 64 * (kMx4Group * gi + u));
+        for (int u = 0; u < kMx4Group; ++u) q.w[u] = mx4_buffer16(tile.w, off + 64 * (kMx4Group * gi + u));
         q.s = mx4_scales16(tile.sc, 4 * kMx4Group * gi, tile.sleft);
     }
     // acc += the group's products, the weights times 2^-base; rows: of x (columns past them repeat the last)

@@ -117,7 +117,7 @@ struct Mx4Wide {
     // this lane's block of step c of the tiles (RG 4: block j of its two); past the row's end the next row's, beside x that is 0
     __device__ __forceinline__ void load_w(int c, int j, uint32_t off, u32x4_t (&w)[kTiles]) const {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) w[i] = mx4_buffer16(wr, off, (64 / kTiles) * i * kb * 16 + 64 * c + 16 * j);
+        for (int i = 0; i < kTiles; ++i) w[i] = mx4_buffer16(wr, off + ((64 / kTiles) * i * kb * 16 + 64 * c + 16 * j));
     }
     __device__ __forceinline__ uint32_t* scale_words(int t) const {
         return reinterpret_cast<uint32_t*>(lds + 2 * kBuf) + (t >> 6) * (64 * kScaleRow);

@@ -310,8 +310,8 @@ int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t row
  * W [n, k] as codes (16-byte aligned) and scales, bias fp32 [n] or NULL, C fp16, bf16 or fp32 (row stride c_ld). The
  * weights are exact in x's type, the sums fp32, one rounding. fp16 x: every block that is not all zeros must have
  * 104 <= s - scale_base <= 140 (its values times 2^-scale_base are then exact in fp16; the result is scaled back); any
- * other block's values round, overflow or vanish as fp16 does. bf16 x: scale_base is not used. k and n need not be
- * multiples of anything but k of 32. */
+ * other block's values round, overflow or vanish as fp16 does. bf16 x: scale_base is not used. k is a multiple of 32 up to
+ * 2^24, n any number. */
 int exl3_mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
                     const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
                     int c_dtype, void* stream);
@@ -322,10 +322,11 @@ int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, in
                   const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, void* stream);
 
 /* Routed MoE layer over experts with MX4 weights: as exl3_moe_forward (same routing arguments, inactive slots, shared
- * expert, activations and order of sums), for x fp16 or bf16 and out fp16, bf16 or fp32. tables: device int64 [9][E], row
+ * expert and activations), for x fp16 or bf16 and out fp16, bf16 or fp32. tables: device int64 [9][E], row
  * 3p + {0, 1, 2} = (address of codes, address of scales, scale_base) of projection p = 0 gate [I, H], 1 up [I, H], 2 down
  * [H, I], addresses of codes 16-byte aligned, scale_base as in exl3_mx4_linear. act(gate, up) is computed in fp32 and
- * rounded to x's type for the down product; expert outputs are summed in fp32 in slot order. H % 32 == 0, I % 32 == 0.
+ * rounded to x's type for the down product; expert outputs are summed in fp32, in an order fixed by the sizes and a row's
+ * picks. H % 32 == 0, I % 32 == 0.
  * x and its rows 16-byte aligned. */
 int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
                          const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
@@ -347,7 +348,7 @@ int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, co
 
 /* Gradient of that loss: dlogits[t, j] = grad * d loss / d logits[t, j] (fp32 [M, E], row stride d_ld; zero in rows that are
  * not live), counts and rows as exl3_route_balance wrote them (or summed over several processes) and taken as constants,
- * grad fp32 [1] (device) or NULL for 1. dlogits may be logits. */
+ * grad fp32 [1] (device) or NULL for 1. dlogits may be logits (with d_ld = ld). */
 int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t E, int64_t topk, const uint8_t* mask,
                             int score, float coef, const int32_t* counts, const int32_t* rows, const float* grad,
                             float* dlogits, int64_t d_ld, void* stream);

@@ -56,7 +56,10 @@ def test_c_refusals(exl3):
     assert ln(P, 64, 0, 1, 64, P, P, 0, 0, None, P, 16, 0, None) == 1
     assert ln(P, 64, 0, 0, 64, P, P, 16, 0, None, P, 16, 0, None) == 0
     assert ln(P, 64, 0, 1, 64, P, None, 16, 0, None, P, 16, 0, None) == 1
+    wide = (1 << 24) + 32                                                   # longer sums than fp32 is good for
+    assert ln(P, wide, 0, 1, wide, P, P, 16, 0, None, P, 16, 0, None) == 1
     g = L.exl3_mx4_gemm
+    assert g(P, P, 1, wide, P, P, 16, None, P, 16, 0, None) == 1
     assert g(P, P, 1, 48, P, P, 16, None, P, 16, 0, None) == 1
     assert g(ODD, P, 1, 64, P, P, 16, None, P, 16, 0, None) == 1
     assert g(P, None, 1, 64, P, P, 16, None, P, 16, 0, None) == 1
