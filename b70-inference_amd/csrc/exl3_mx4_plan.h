@@ -1,5 +1,5 @@
-// Host-side choices of the MX4 kernels: tiles, k-splits, row blocks and their number. Plain C++ without device code. They follow from the shape
-// alone: a call gives the same bits eager and captured.
+// Host-side choices of the MX4 kernels: tiles, k-splits, row blocks and their number. Plain C++ without device code. They follow
+// from the shape alone: a call gives the same bits eager and captured.
 #pragma once
 
 #include <stdint.h>

@@ -1,6 +1,8 @@
 // Products of many 16-bit rows with MX4 weights: a workgroup of four waves takes 32 RG rows of x and 64 weight rows (outputs)
 // per wave, in steps of 128 k (four blocks). Bound by the MFMAs at 128 rows (RG 4: 2048 cycles of them per wave and step
-// against 64 conversions and 32 LDS reads), by the weights' bytes at 32.
+// against 64 conversions and 32 LDS reads), by the weights' bytes at 32. 1021 rows of 5376 -> 21504 (RG 4) 238 us, 0.99
+// PFLOP/s, MFMAs busy 55 % of the time (672 tiles over 512 slots are half of what is missing); 512 experts of 2560 -> 640
+// with 20 rows each (RG 1) gate and up 239 us, 3.7 TB/s of weights, down 135 us, 3.3 beside 0.8 of outputs.
 //
 // x goes through one of two LDS buffers, staged through registers while the step before is multiplied. Weights are read
 // straight into the lanes that convert them, each by one wave of the workgroup only; every word of a block, converted with
@@ -11,6 +13,9 @@
 //     Weights and x are on their way for a whole step.
 //   RG 4: 32 x 32 x 16 MFMAs, two tiles per wave, half the fragments in registers (the 16 x 16 form spills). Lane l holds row
 //     l & 31 and blocks 2 (l >> 5) and 2 (l >> 5) + 1; weights and x are on their way for half a step.
+// Scales: a step needs four bytes of a row, a cache line holds those of 32 steps, and the lines of all the rows under way do
+// not stay in the L2; so a wave takes the words of 16 steps (RG 4: 8, for want of LDS) of each of its 64 rows at a time
+// into LDS of its own.
 #pragma once
 
 #include <type_traits>
@@ -26,10 +31,6 @@ __device__ __forceinline__ f16_t mfma32(u32x4_t a, u32x4_t b, f16_t c) {
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
 }
-
-// Scales: a step needs four bytes of a row, a cache line holds those of 32 steps, and the lines of all the rows under way do
-// not stay in the L2; so a wave takes the words of 16 steps (RG 4: 8, for want of LDS) of each of its 64 rows at a time
-// into LDS of its own.
 
 template <int XT, int RG>
 struct Mx4Wide {

@@ -461,8 +461,8 @@ def route_balance_grad(logits: torch.Tensor, counts: torch.Tensor, rows: torch.T
     counts = counts.contiguous()
     with where:
         rc = lib().exl3_route_balance_grad(logits.data_ptr(), ld, M, E, int(k), ptr(mask), SCORES[score], float(coef),
-                                           counts.data_ptr(), rows.data_ptr(), ptr(grad), out.data_ptr(), out.stride(0) if M > 1 else E,
-                                           stream_of(logits))
+                                           counts.data_ptr(), rows.data_ptr(), ptr(grad), out.data_ptr(),
+                                           out.stride(0) if M > 1 else E, stream_of(logits))
     if rc:
         check(rc, "route_balance_grad")
     return out
