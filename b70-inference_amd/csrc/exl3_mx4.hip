@@ -300,8 +300,8 @@ static int launch_tiny(const char* name, const Mx4Args& a, hipStream_t st) {
 }
 
 // Up to 16 rows, x in LDS. A workgroup takes every gridDim-th tile of 16 outputs, so x is staged once per resident workgroup.
-// Six rows of 5376 -> 21504 18 us (62 MB: 3.4 TB/s; a tile is two groups of a wave, whose start and sum over the waves are
-// what keeps it from the copy's rate), one of 4096 -> 4096 under 5 (a chain of the first load, the sum and the store).
+// Six rows of 5376 -> 21504 18.4 us replayed (62 MB: 3.4 TB/s; the same with 6, 8 or 10 waves, so the memory's rate behind the
+// launch and the first loads), one of 4096 -> 4096 4.7 (a chain of the first load, the sum and the store).
 template <int XT>
 __global__ __launch_bounds__(1024) void mx4_decode_kernel(Mx4Args a, int xbytes) {
     extern __shared__ f4_t red[];
@@ -361,7 +361,8 @@ template <int XT>
 static int launch_decode(const char* name, const Mx4Args& a, int waves, int xb, int lds, hipStream_t st) {
     // resident workgroups: LDS, and registers for 16 waves per CU
     const int occ = kMx4Lds / lds < 16 / waves ? kMx4Lds / lds : 16 / waves;
-    const int64_t tiles = (a.n + 15) / 16, grid = tiles < 256 * occ ? tiles : 256 * occ;
+    // the fewest that need no more rounds (six rows of 5376 -> 21504: 448 of 512 workgroups, 18.7 -> 18.4 us)
+    const int64_t tiles = (a.n + 15) / 16, rounds = (tiles + 256 * occ - 1) / (256 * occ), grid = (tiles + rounds - 1) / rounds;
     EXL3_CHECK_ARG(tiles <= 0x3FFFFFFF, "%s: grid too large", name);
     EXL3_LAUNCH(name, mx4_decode_kernel<XT>, dim3((unsigned)grid), dim3(64 * waves), (size_t)lds, st, a, xb);
     return EXL3_OK;

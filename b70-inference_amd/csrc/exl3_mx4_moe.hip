@@ -9,7 +9,7 @@
 // token's slots.
 // Bound by the weights' bytes: 1024 tokens, top-10 of 512 experts 2560 -> 640, 421 us for 1.35 GB (align 31, gateup 239, down 135,
 // combine 18); 260 tokens, top-2 of 32 experts 7168 -> 2048 and a shared one, 253 us for 0.78 GB (14, 158, 89, 6); one token,
-// top-10 of 512 experts 2048 -> 512, 15.9 us for 17 MB, two chains of load, sum and store.
+// top-10 of 512 experts 2048 -> 512, 12.0 us replayed for 17 MB, two chains of load, sum and store.
 #include "exl3_moe.h"
 #include "exl3_moe_dev.h"
 #include "exl3_mx4.h"
