@@ -209,9 +209,13 @@ __device__ __forceinline__ void mx4_put16(const Mx4Args& a, int sp, int64_t m, i
     uint32_t p[2], r[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        const bool h = a.out_dtype == EXL3_F16;
-        p[q] = h ? f2h(v[2 * q]) | (uint32_t)f2h(v[2 * q + 1]) << 16 : f2bf(v[2 * q]) | (uint32_t)f2bf(v[2 * q + 1]) << 16;
-        r[q] = h ? f2h(w[2 * q]) | (uint32_t)f2h(w[2 * q + 1]) << 16 : f2bf(w[2 * q]) | (uint32_t)f2bf(w[2 * q + 1]) << 16;
+        if (a.out_dtype == EXL3_F16) {                         // uniform
+            p[q] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)v[2 * q], (_Float16)v[2 * q + 1]});
+            r[q] = __builtin_bit_cast(uint32_t, h2_t{(_Float16)w[2 * q], (_Float16)w[2 * q + 1]});
+        } else {
+            p[q] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)v[2 * q], (__bf16)v[2 * q + 1]});
+            r[q] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)w[2 * q], (__bf16)w[2 * q + 1]});
+        }
         const auto x = __builtin_amdgcn_permlane32_swap(p[q], r[q], false, false);
         p[q] = x[0];
         r[q] = x[1];
@@ -426,7 +430,7 @@ static int linear_run(const Mx4Args& a, hipStream_t st) {
 // 2 (l >> 5) and 2 (l >> 5) + 1 of its row's four, one per MFMA, so that both scales are neighbouring bytes of one word.
 // In LDS a row's four 16-byte units are permuted by its row number: eight lanes reading eight rows, or writing two, touch
 // every bank once.
-// 2048 rows of 5376 -> 21504 (256 x 256) 167 us, 2.8 PFLOP/s: a step takes 2500 cycles for 1024 of MFMAs; the LDS is busy for
+// 2048 rows of 5376 -> 21504 (256 x 256) 165 us, 2.9 PFLOP/s: a step takes 2500 cycles for 1024 of MFMAs; the LDS is busy for
 // 1500, mostly with the stores of the staged codes, and the barrier keeps the waves in step, so that little of either hides
 // behind the other; and 672 tiles take three rounds of the CUs for 2.6 rounds' work.
 template <int TM, int TN, int WM, int WN>
