@@ -142,4 +142,31 @@ __device__ __forceinline__ void store4_as(void* p, int64_t i, f4_t v, int dtype)
     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
+// fp16 intermediates with a power of two per group of a row's columns, which is held as v 2^-e. A group whose largest magnitude
+// (`top`, float bits) lies in [2^-8, 2^15) stands as it is, e = 0: what falls below fp16's normal range is then off by 2^-17 of the
+// largest at most. Any other has its largest value in [2^14, 2^15), zeros the least e. A group with an infinity or a NaN keeps
+// them.
+__device__ __forceinline__ int mid_exponent(uint32_t top) {
+    const int f = (int)(top >> 23) - 127;
+    return f >= -8 && f < 15 ? 0 : f - 14 < -126 ? -126 : f - 14;
+}
+// v 2^d (d <= 0), eight fp16 values: what brings a group to its row's largest exponent (d: its own less that one). fp16 has no
+// factor below 2^-24, but the group's largest values stay above its least step down to d = -39.
+__device__ __forceinline__ u32x4_t half_times(u32x4_t v, int d) {
+    const uint32_t h = d >= -14 ? (uint32_t)(15 + d) << 10 : d >= -24 ? 1u << (24 + d) : 0u, p = h | h << 16;
+    u32x4_t r;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        r[q] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, (uint32_t)v[q]) * __builtin_bit_cast(h2_t, p));
+    return r;
+}
+__device__ __forceinline__ u32x4_t half_shift(u32x4_t v, int d) {
+    if (d < -24) {
+        v = half_times(v, -24);
+        d += 24;
+    }
+    return half_times(v, d);
+}
+__device__ __forceinline__ uint32_t magnitude_bits(float f) { return __builtin_bit_cast(uint32_t, f) & 0x7FFFFFFFu; }
+
 }  // namespace exl3

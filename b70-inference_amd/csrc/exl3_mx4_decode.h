@@ -131,8 +131,13 @@ struct Mx4Decode {
         for (int u = 0; u < kMx4Group; ++u) q.w[u] = mx4_buffer16(tile.w, off + 64 * (kMx4Group * gi + u));
         q.s = mx4_scales16(tile.sc, 4 * kMx4Group * gi, tile.sleft);
     }
-    // acc += the group's products, the weights times 2^-base; rows: of x (columns past them repeat the last)
+    // acc += the group's products, the weights times 2^-base; rows: of x (columns past them repeat the last); fx(u, v, word): the
+    // eight values of x beside word v of chunk u, as they are multiplied
     __device__ __forceinline__ void mul(int gi, int lane, const Mx4X& x, int rows, int base, Group& q, f4_t& acc) const {
+        mul(gi, lane, x, rows, base, q, acc, [](int, int, u32x4_t v) { return v; });
+    }
+    template <typename F>
+    __device__ __forceinline__ void mul(int gi, int lane, const Mx4X& x, int rows, int base, Group& q, f4_t& acc, F fx) const {
         const int g = lane >> 4, r = (lane & 15) < rows ? lane & 15 : rows - 1, left = kb - 4 * kMx4Group * gi;
         if (left < 4 * kMx4Group) {                            // uniform: scale bytes past the row's end are the next row's
 #pragma unroll
@@ -152,7 +157,7 @@ struct Mx4Decode {
                 const u32x4_t* xp = reinterpret_cast<const u32x4_t*>(x.p + r * x.stride + 256 * c + 64 * g);
                 const float s = mx4_scale(sb, base);
 #pragma unroll
-                for (int v = 0; v < 4; ++v) acc = mfma16<XT>(mx4_frag<XT>(q.w[u][v], s), xp[v], acc);
+                for (int v = 0; v < 4; ++v) acc = mfma16<XT>(mx4_frag<XT>(q.w[u][v], s), fx(u, v, xp[v]), acc);
             }
         }
     }

@@ -2,7 +2,11 @@
 //   align    pairs (token, slot) grouped by expert and cut into blocks of rows (exl3_moe.hip, shared with the EXL3 layer;
 //            the tables' entries are (codes, scales, base) instead of (trellis, suh, svh))
 //   gateup   workgroup per (block, 128 columns of I): both projections over H, act(gate, up) in fp32, rounded to x's type
-//            (the down product's operand: fp32 rows would double its MFMAs; its rounding is that of the 16-bit output)
+//            (the down product's operand: one of more bits, in two parts, would double its MFMAs, its LDS and its reads of rows;
+//            this rounding adds to the output's: 1.4 times the error of a 16-bit output, and an fp32 output has no more than
+//            x's type's 8 or 11 bits of the middle). fp16 does not hold every magnitude that a product of two sums has, so fp16
+//            middles carry a power of two per workgroup's columns (mid_exponent in exl3_mx4.h; all of it costs one token, top-10 of 512
+//            experts 2048 -> 512, 0.3 of 13.5 us, and 1024 of them 2 of 422)
 //   down     workgroup per (block, 256 columns of H) over I: y[pair] = routing weight * sum, fp32
 //   combine  out[t] = sum of the token's y rows in slot order
 // Few pairs take two launches instead: gateup per (pair, 16 columns of I), down per (token, 16 columns of H) over all of the
@@ -32,6 +36,7 @@ struct Mx4MoeArgs {
     const float* pair_w;
     const int* pair_of;
     uint16_t* mid;                     // [pairs][I] in x's type
+    int8_t* mexp;                      // fp16: exponents of mid's groups of 128 columns, [pairs][ceil(I / 128)]
     float* y;                          // [pairs][H]
     int act;
     float limit;
@@ -51,6 +56,7 @@ struct Mx4PairArgs {
     const float* tw;
     const int64_t* tables;             // [9][E]
     uint16_t* mid;                     // [M * slots][I]
+    int8_t* mexp;                      // fp16: exponents of mid's groups of 16 columns, [M * slots][I / 16]
     int act;
     float limit;
     void* out;
@@ -109,11 +115,24 @@ __global__ __launch_bounds__(512) void mx4_gateup_pair_kernel(Mx4PairArgs a, int
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         v[j] = act_mul_dev(__builtin_ldexpf(g[j], base[0]), __builtin_ldexpf(u[j], base[1]), a.act, a.limit);
+    if constexpr (XT == kRowF16) {                             // (the four lanes here are all of them)
+        uint32_t m = 0, top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, magnitude_bits(v[j]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, (uint32_t)__builtin_amdgcn_readlane((int)m, 16 * j));
+        const int ex = mid_exponent(top);
+        if (ex != 0)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __builtin_ldexpf(v[j], -ex);
+        if (lane == 0) a.mexp[(int64_t)pair * nc + blockIdx.x % nc] = (int8_t)ex;
+    }
     store4_as(a.mid, (int64_t)pair * a.I + i0 + 4 * (lane >> 4), v, XT == kRowF16 ? EXL3_F16 : EXL3_BF16);
 }
 
 // Workgroup per (token, 16 columns of H): the token's slots after one another, their groups of 512 rows of I over the waves; a
-// wave adds a slot's sum, times its routing weight, when it goes on to another.
+// wave adds a slot's sum, times its routing weight, when it goes on to another. fp16: the sum is held at the largest exponent of the
+// middle's groups so far.
 template <int XT>
 __global__ __launch_bounds__(1024) void mx4_down_pair_kernel(Mx4PairArgs a, int xbytes) {
     extern __shared__ f4_t red[];
@@ -125,16 +144,29 @@ __global__ __launch_bounds__(1024) void mx4_down_pair_kernel(Mx4PairArgs a, int 
     Mx4Decode<XT> p;
     p.kb = kb;
     typename Mx4Decode<XT>::Group q, nx;
+    constexpr int kNone = -1000;
     int base = 0, nbase = 0, e = -1, ne = -1;                  // of q's and nx's slots
-    const auto fetch = [&](int gi, int& ex, int& bs, typename Mx4Decode<XT>::Group& o) {
+    int held = XT == kRowF16 ? kNone : 0;                      // exponent of acc
+    struct Exps {
+        uint32_t b[kMx4Group];                                 // of this lane's block of each chunk, two bytes
+    } qe, nqe;
+    const auto fetch = [&](int gi, int& ex, int& bs, typename Mx4Decode<XT>::Group& o, Exps& oe) {
         const int j = gi / ng;
         ex = __builtin_amdgcn_readfirstlane(a.expert(t, j));
         if (ex < 0) return;                                    // uniform
         bs = XT == kRowF16 ? (int)a.entry(8, ex) : 0;
         p.tile.set(reinterpret_cast<const uint8_t*>(a.entry(6, ex)), reinterpret_cast<const uint8_t*>(a.entry(7, ex)), h0, a.H, kb, lane);
         p.load(gi - j * ng, lane, o);
+        if constexpr (XT == kRowF16) {
+            const uint16_t* ep = reinterpret_cast<const uint16_t*>(a.mexp + ((int64_t)t * a.slots + j) * (a.I / 16));
+#pragma unroll
+            for (int u = 0; u < kMx4Group; ++u) {
+                const int b = 4 * (kMx4Group * (gi - j * ng) + u) + (lane >> 4);
+                oe.b[u] = ldg(ep + (b < kb ? b : kb - 1));     // (past the row's end, beside x that is 0: the last block's)
+            }
+        }
     };
-    fetch(wave, e, base, q);
+    fetch(wave, e, base, q, qe);
     // (slots without an expert have no middle row: their pair's, which nobody reads)
     const Mx4X x = mx4_stage_x<XT>(lds, a.slots, kb, [&](int j) {
         return reinterpret_cast<const uint8_t*>(a.mid + ((int64_t)t * a.slots + j) * a.I); }, [](int) { return (const uint8_t*)nullptr; });
@@ -143,20 +175,44 @@ __global__ __launch_bounds__(1024) void mx4_down_pair_kernel(Mx4PairArgs a, int 
     for (int gi = wave; gi < all; gi += waves) {
         const int j = gi / ng;
         const bool more = gi + waves < all;
-        if (more) fetch(gi + waves, ne, nbase, nx);
+        if (more) fetch(gi + waves, ne, nbase, nx, nqe);
         if (e >= 0) {
             const Mx4X xj = {x.p + j * x.stride, x.stride, x.sstride, x.scales};
-            p.mul(gi - j * ng, lane, xj, 1, base, q, acc);
+            bool plain = true;
+            if constexpr (XT == kRowF16) {
+                int top = 0;
+                plain = __ballot((qe.b[0] | qe.b[1] | qe.b[2] | qe.b[3]) != 0) == 0;
+                if (!plain) {
+                    top = -126;
+#pragma unroll
+                    for (int u = 0; u < kMx4Group; ++u) top = max(top, max((int)(int8_t)qe.b[u], (int)(int8_t)(qe.b[u] >> 8)));
+                    top = max(top, __shfl_xor(top, 16));
+                    top = __builtin_amdgcn_readfirstlane(max(top, __shfl_xor(top, 32)));
+                }
+                if (top > held) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i] = __builtin_ldexpf(acc[i], held - top);
+                    held = top;
+                }
+                plain = plain && held == 0;
+                if (!plain)
+                    p.mul(gi - j * ng, lane, xj, 1, base, q, acc, [&](int u, int v, u32x4_t f) {
+                        return half_shift(f, (int)(int8_t)(qe.b[u] >> (v < 2 ? 0 : 8)) - held);
+                    });
+            }
+            if (plain) p.mul(gi - j * ng, lane, xj, 1, base, q, acc);
         }
         if (!more || (gi + waves) / ng != j) {
             if (e >= 0) {
                 const float w = j < a.topk ? ldg(a.tw + (int64_t)t * a.topk + j) : 1.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tot[i] += w * __builtin_ldexpf(acc[i], base);
+                for (int i = 0; i < 4; ++i) tot[i] += w * __builtin_ldexpf(acc[i], base + held);
             }
             acc = f4_t{};
+            if (XT == kRowF16) held = kNone;
         }
         q = nx;
+        qe = nqe;
         e = ne;
         base = nbase;
     }
@@ -235,25 +291,45 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_gateup_wide_kernel(
         });
         __syncthreads();
         const int m = 32 * j + (t >> 3);
+        f4_t v[4];
+        uint32_t top = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int col = 32 * q + 4 * (t & 7);
             const f4_t gv = *reinterpret_cast<const f4_t*>(C + (t >> 3) * kMx4CS + col);
             const f4_t uv = *reinterpret_cast<const f4_t*>(C + (t >> 3) * kMx4CS + 132 + col);
-            f4_t v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = act_mul_dev(__builtin_ldexpf(gv[e], bg), __builtin_ldexpf(uv[e], bu), a.act, a.limit);
+            for (int e = 0; e < 4; ++e) {
+                v[q][e] = act_mul_dev(__builtin_ldexpf(gv[e], bg), __builtin_ldexpf(uv[e], bu), a.act, a.limit);
+                if (i0 + col < a.I) top = max(top, magnitude_bits(v[q][e]));
+            }
+        }
+        if constexpr (XT == kRowF16) {                         // eight lanes hold a row's 128 columns
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+            const int ex = mid_exponent(top);
+            if (__ballot(ex != 0))                             // uniform
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[q][e] = __builtin_ldexpf(v[q][e], -ex);
+            if (m < cnt && (t & 7) == 0) a.mexp[(int64_t)(p0 + m) * nc + blockIdx.x % nc] = (int8_t)ex;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int col = 32 * q + 4 * (t & 7);
             if (m < cnt && i0 + col < a.I)
-                store4_as(a.mid, (int64_t)(p0 + m) * a.I + i0 + col, v, XT == kRowF16 ? EXL3_F16 : EXL3_BF16);
+                store4_as(a.mid, (int64_t)(p0 + m) * a.I + i0 + col, v[q], XT == kRowF16 ? EXL3_F16 : EXL3_BF16);
         }
     }
 }
 
 template <int XT, int RG>
 __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx4MoeArgs a) {
-    typedef Mx4Wide<XT, RG> L;
+    constexpr bool kMid = XT == kRowF16;
+    typedef Mx4Wide<XT, RG, kMid> L;
     __shared__ u32x4_t lds[L::kLds];
+    __shared__ int s_er[kMid ? 64 * RG : 1];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned nc = ((unsigned)a.H + 255) / 256;
     const ItemDesc* d = a.blocks + blockIdx.x / nc;
@@ -266,7 +342,10 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx
     for (int i = 0; i < RG; ++i) {
         const int m = (t >> 3) + 32 * i;
         p.xp[i] = reinterpret_cast<const uint8_t*>(a.mid + (int64_t)(p0 + (m < cnt ? m : cnt - 1)) * a.I);
+        if constexpr (kMid) s_er[32 * RG + m] = (m < cnt ? m : cnt - 1) * ((a.I + 127) / 128);   // (the wave's own rows: no barrier)
     }
+    p.xe = kMid ? a.mexp + (int64_t)p0 * ((a.I + 127) / 128) : nullptr;
+    p.er = s_er;
     p.base = XT == kRowF16 ? (int)d->tab[8] : 0;
     p.weights(reinterpret_cast<const uint8_t*>(d->tab[6]), reinterpret_cast<const uint8_t*>(d->tab[7]), h0, a.H, lane);
     typename L::Acc acc;
@@ -278,8 +357,9 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx
             const int m = 32 * j + row;
             if (m >= cnt || h0 + n >= a.H) return;
             const float w = ldg(a.pair_w + p0 + m);
+            const int ex = p.base + (kMid ? s_er[m] : 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = w * __builtin_ldexpf(v[e], p.base);
+            for (int e = 0; e < 4; ++e) v[e] = w * __builtin_ldexpf(v[e], ex);
             *reinterpret_cast<f4_t*>(a.y + (int64_t)(p0 + m) * a.H + h0 + n) = v;
         });
 }
@@ -365,10 +445,15 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
     Mx4PairShape ps;
     if (npairs > 0 && npairs <= 160 && npairs * H * I <= 210000000 && pair_shape((int)H, (int)I, (int)slots, ps)) {
         Workspace ws;
-        const int rc = workspace((size_t)npairs * I * 2, 0, st, &ws);
+        const size_t np = (size_t)npairs;
+        const int rc = workspace(carve_size(np * I, 2) + carve_size(np * I / 16, 1), 0, st, &ws);
         if (rc) return rc;
+        Carve c{ws.scratch, ws.scratch_bytes};
+        uint16_t* mid = c.take<uint16_t>(np * I);
+        int8_t* mexp = c.take<int8_t>(np * I / 16);
+        if (!mexp) return fail(EXL3_ERR_INVALID, "exl3_mx4_moe_forward: workspace carve failed");
         const Mx4PairArgs p{reinterpret_cast<const uint8_t*>(x), 2 * x_ld, (int)M, (int)H, (int)I, (int)topk, (int)slots, (int)E,
-                            (int)shared, topk_ids, topk_w, tables, reinterpret_cast<uint16_t*>(ws.scratch), act, act_limit, out,
+                            (int)shared, topk_ids, topk_w, tables, mid, mexp, act, act_limit, out,
                             out_ld, out_dtype, vec};
         return x_dtype == EXL3_F16 ? launch_pairs<kRowF16>(p, ps, st) : launch_pairs<kRowBF16>(p, ps, st);
     }
@@ -394,7 +479,7 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
         Workspace ws;
         const size_t np = (size_t)npairs;
         const int rc = workspace(carve_size(a.max_blocks, sizeof(ItemDesc)) + carve_size(2 * np, 4) + carve_size(np, 4) +
-                                     carve_size(np * I, 2) + carve_size(np * H, 4), 0, st, &ws);
+                                     carve_size(np * I, 2) + carve_size(np * ((I + 127) / 128), 1) + carve_size(np * H, 4), 0, st, &ws);
         if (rc) return rc;
         Carve c{ws.scratch, ws.scratch_bytes};
         blocks = c.take<ItemDesc>(a.max_blocks);
@@ -405,6 +490,7 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
         a.pair_of = pairs + np;
         a.pair_w = pw;
         a.mid = c.take<uint16_t>(np * I);
+        a.mexp = c.take<int8_t>(np * ((I + 127) / 128));
         a.y = c.take<float>(np * H);
         if (!a.y) return fail(EXL3_ERR_INVALID, "exl3_mx4_moe_forward: workspace carve failed");
 

@@ -32,7 +32,9 @@ __device__ __forceinline__ f16_t mfma32(u32x4_t a, u32x4_t b, f16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
 }
 
-template <int XT, int RG>
+// MID: x rows are fp16 intermediates with an exponent per step of 128 (mid_exponent); staging brings a row's steps to the largest
+// of them (er), by which the caller scales the sums.
+template <int XT, int RG, bool MID = false>
 struct Mx4Wide {
     static constexpr int kBuf = 32 * RG * 16;                      // units of 16 bytes of an x buffer
     static constexpr int kScaleSteps = RG == 4 ? 8 : 16;
@@ -49,6 +51,29 @@ struct Mx4Wide {
     int base;
     int kb;
     u32x4_t* lds;                      // two x buffers, the waves' scales
+    const int8_t* xe;                  // MID: exponents of the block's rows
+    int ev[RG];                        // those of the staged rows' step on its way
+    int* er;                           // LDS: a row's largest [32 RG], where its exponents begin [32 RG]
+
+    // The staged rows' largest exponents: the eight lanes that stage a row share its steps.
+    __device__ __forceinline__ void row_exponents(int t) const {
+        const int n = (kb + 3) / 4;
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+            const int8_t* p = xe + (unsigned)er[32 * RG + (t >> 3) + 32 * i];
+            int top = -126;
+            for (int c = t & 7; c < n; c += 8) {
+                const int e = ldg(p + c);
+                top = top > e ? top : e;
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                const int e = __shfl_xor(top, o);
+                top = top > e ? top : e;
+            }
+            er[(t >> 3) + 32 * i] = top;                       // (the wave's own rows: no barrier)
+        }
+    }
 
     // The wave's weight rows n0 .. n0 + 63 of `rows` (n0 below it or not), 32 kb wide.
     __device__ __forceinline__ void weights(const uint8_t* codes, const uint8_t* scales, int64_t n0, int64_t rows, int lane) {
@@ -98,12 +123,24 @@ struct Mx4Wide {
     __device__ __forceinline__ static int unit(int r, int u) { return r * 16 + (u ^ (r & 15)); }
 
     // blocks 2 h and 2 h + 1 of step c
-    __device__ __forceinline__ void load_x(int c, int h, int t, u32x4_t (&st)[RG]) const {
+    __device__ __forceinline__ void load_x(int c, int h, int t, u32x4_t (&st)[RG]) {
+        if constexpr (MID) {
+            if (h == 0)
+#pragma unroll
+                for (int i = 0; i < RG; ++i) ev[i] = ldg(xe + (unsigned)er[32 * RG + (t >> 3) + 32 * i] + c);
+        }
         const int b = 4 * c + 2 * h + ((t & 7) >> 2), bc = b < kb ? b : kb - 1;
 #pragma unroll
         for (int i = 0; i < RG; ++i) st[i] = ldg(reinterpret_cast<const u32x4_t*>(xp[i] + (int64_t)bc * 64) + (t & 3));
     }
     __device__ __forceinline__ void store_x(int c, int h, int t, u32x4_t (&st)[RG]) const {
+        if constexpr (MID) {
+#pragma unroll
+            for (int i = 0; i < RG; ++i) {
+                const int d = ev[i] - er[(t >> 3) + 32 * i];
+                if (__ballot(d != 0)) st[i] = half_shift(st[i], d);   // uniform
+            }
+        }
         if (4 * c + 4 > kb) {                                  // uniform: blocks past the row are 0
             const uint32_t keep = 4 * c + 2 * h + ((t & 7) >> 2) < kb ? ~0u : 0u;
 #pragma unroll
@@ -162,7 +199,7 @@ struct Mx4Wide {
         }
     }
     // acc += the products of steps c0 .. c0 + steps - 1 (those there are)
-    __device__ __forceinline__ void run(int t, int c0, int steps, Acc& acc) const {
+    __device__ __forceinline__ void run(int t, int c0, int steps, Acc& acc) {
         const int lane = t & 63, r = RG == 4 ? lane & 31 : lane & 15, g = RG == 4 ? lane >> 5 : lane >> 4;
         const int end = (kb + 3) / 4 - c0 < steps ? (kb + 3) / 4 : c0 + steps;
         const uint32_t off = (uint32_t)r * (uint32_t)(kb * 16) + (RG == 4 ? 32 : 16) * g;
@@ -170,6 +207,7 @@ struct Mx4Wide {
         load_x(c0, 0, t, st);
         load_x(c0, 1, t, su);
         load_w(c0, 0, off, w);
+        if constexpr (MID) row_exponents(t);
         store_x(c0, 0, t, st);
         store_x(c0, 1, t, su);
         __syncthreads();

@@ -291,7 +291,7 @@ def mx4_moe_forward(x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tenso
                     act_limit: float = 0.0, shared: int = -1, out: torch.Tensor | None = None,
                     out_dtype=torch.float32) -> torch.Tensor:
     """out[t] = sum_j topk_w[t, j] * expert_{topk_ids[t, j]}(x[t]) (+ expert `shared` with weight 1), fp32 sums, expert(x) =
-    down(act(gate(x), up(x))) with act(gate, up) rounded to x's type. x fp16 or bf16 [M, H]; topk_ids int32 [M, k] (outside
+    down(act(gate(x), up(x))) with act(gate, up) rounded to x's type (its magnitude may leave fp16's range). x fp16 or bf16 [M, H]; topk_ids int32 [M, k] (outside
     [0, E): inactive); topk_w fp32 [M, k]; out fp16, bf16 or fp32. The arguments are moe_forward's."""
     H = experts.H
     if x.dim() != 2 or x.dtype not in (torch.float16, torch.bfloat16) or x.shape[1] != H:

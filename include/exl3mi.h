@@ -325,8 +325,9 @@ int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, in
  * expert and activations), for x fp16 or bf16 and out fp16, bf16 or fp32. tables: device int64 [9][E], row
  * 3p + {0, 1, 2} = (address of codes, address of scales, scale_base) of projection p = 0 gate [I, H], 1 up [I, H], 2 down
  * [H, I], addresses of codes 16-byte aligned, scale_base as in exl3_mx4_linear. act(gate, up) is computed in fp32 and
- * rounded to x's type for the down product; expert outputs are summed in fp32, in an order fixed by the sizes and a row's
- * picks. H % 32 == 0, I % 32 == 0. x and its rows 16-byte aligned. */
+ * rounded to x's type for the down product. fp16 of any magnitude: groups of up to 128 columns whose largest value leaves
+ * [2^-8, 2^15) are held with a power of two of their own; a value is off by half a step of fp16 or by 2^-17 of its row's largest
+ * value, whichever is more. Expert outputs are summed in fp32, in an order fixed by the sizes and a row's picks. H % 32 == 0, I % 32 == 0. x and its rows 16-byte aligned. */
 int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
                          const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
                          int64_t shared, void* out, int64_t out_ld, int out_dtype, void* stream);
