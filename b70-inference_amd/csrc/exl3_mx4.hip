@@ -265,7 +265,8 @@ static int launch_reduce(const Mx4Args& a, hipStream_t st) {
     return EXL3_OK;
 }
 
-// One output per thread: matrices of fewer than 16 scale bytes, which the other kernels' 16-byte loads of scales do not fit.
+// One output per thread: matrices of fewer than 16 scale bytes, which the other kernels' 16-byte loads of scales do not fit. A block's
+// sum is of plain codes, times both scales at once: one of them alone may leave fp32 where the product does not.
 template <int XT>
 __global__ __launch_bounds__(256) void mx4_tiny_kernel(Mx4Args a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / a.n, n = i - m * a.n;
@@ -273,10 +274,10 @@ __global__ __launch_bounds__(256) void mx4_tiny_kernel(Mx4Args a) {
     const int kb = a.k / 32;
     float sum = 0.f;
     for (int b = 0; b < kb; ++b) {
-        const float ws = mx4_scale(a.ws[n * kb + b], a.base), xs = XT == kRowMX4 ? mx4_scale(a.xs[m * kb + b], 0) : 1.f;
+        const int ws = a.ws[n * kb + b], xs = XT == kRowMX4 ? a.xs[m * kb + b] : 127;
         float part = 0.f;
         for (int e = 0; e < 16; ++e) {
-            const auto w = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.w[n * (a.k / 2) + 16 * b + e], ws, 0);
+            const auto w = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.w[n * (a.k / 2) + 16 * b + e], 1.f, 0);
             float x0, x1;
             if constexpr (XT == kRowMX4) {
                 const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.x[m * a.x_ld + 16 * b + e], 1.f, 0);
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(256) void mx4_tiny_kernel(Mx4Args a) {
             }
             part += x0 * w[0] + x1 * w[1];
         }
-        sum += part * xs;
+        sum += ws == 255 || xs == 255 ? __builtin_nanf("") : __builtin_ldexpf(part, ws + xs - 254 - a.base);
     }
     if (a.base) sum = __builtin_ldexpf(sum, a.base);
     if (a.bias) sum += ldg(a.bias + n);
