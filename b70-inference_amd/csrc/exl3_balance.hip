@@ -91,9 +91,12 @@ __device__ __forceinline__ void load_row(const float* z, int E, float (&f)[V]) {
     }
 }
 
-// Shares p of a row's logits f (0 past E); in the gradient also each score's derivative over the score, ds / (s dl).
+// Shares p of a row's logits f (0 past E), which lie at z; in the gradient also each score's derivative over the score, ds / (s dl).
+// Far below 0 sigmoid(l) is e^l and sqrt(softplus(l)) is e^(l / 2), the forms taken where the others' parts leave fp32 (l < -80). A row
+// whose scores add up to so little that all its logits are below -16 takes them relative to its largest logit, as softmax
+// does: its shares stay what they are however low it lies.
 template <int V, int W, int SC, bool GRAD>
-__device__ __forceinline__ void row_shares(float (&f)[V], float (&d)[V], int E, float* tmp) {
+__device__ __forceinline__ void row_shares(float (&f)[V], float (&d)[V], const float* zrow, int E, float* tmp) {
     const int l = W > 1 ? threadIdx.x : threadIdx.x & 63;
     float mx = 0.f;
     if constexpr (SC == EXL3_SCORE_SOFTMAX) {
@@ -112,11 +115,12 @@ __device__ __forceinline__ void row_shares(float (&f)[V], float (&d)[V], int E, 
         if constexpr (SC == EXL3_SCORE_SOFTMAX) {
             s = expf(z - mx);
         } else if constexpr (SC == EXL3_SCORE_SIGMOID) {
-            s = 1.f / (1.f + expf(-z));
+            const float e = expf(z < -80.f ? z : -z);
+            s = z < -80.f ? e : 1.f / (1.f + e);
             if constexpr (GRAD) d[v] = 1.f / (1.f + expf(z));
         } else {
-            const float sp = z > 20.f ? z : log1pf(expf(z));
-            s = sqrtf(sp);
+            const float e = expf(z < -80.f ? 0.5f * z : z), sp = z > 20.f ? z : log1pf(e);
+            s = z < -80.f ? e : sqrtf(sp);
             // sigma / softplus tends to 1 below; past e^-17 it is 1 to fp32 (and softplus may be 0)
             if constexpr (GRAD) d[v] = z < -17.f ? 0.5f : 0.5f / ((1.f + expf(-z)) * sp);
         }
@@ -124,6 +128,25 @@ __device__ __forceinline__ void row_shares(float (&f)[V], float (&d)[V], int E, 
         sum += f[v];
     }
     sum = row_sum<W>(sum, tmp);
+    if constexpr (SC != EXL3_SCORE_SOFTMAX) {
+        // e^l < 2^-24 for every l (a wave's, or with W > 1 the workgroup's, common value)
+        if (__builtin_amdgcn_readfirstlane(sum < (SC == EXL3_SCORE_SIGMOID ? 0x1p-24f : 0x1p-12f))) {
+            load_row<V, W>(zrow, E, f);
+            mx = -__builtin_inff();
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (l + 64 * W * v < E) mx = fmaxf(mx, f[v]);
+            mx = row_max<W>(mx, tmp);
+            if (mx == -__builtin_inff()) mx = 0.f;             // every logit -inf: scores 0
+            sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                f[v] = l + 64 * W * v < E ? expf((SC == EXL3_SCORE_SIGMOID ? 1.f : 0.5f) * (f[v] - mx)) : 0.f;
+                sum += f[v];
+            }
+            sum = row_sum<W>(sum, tmp);
+        }
+    }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int v = 0; v < V; ++v) f[v] *= inv;
@@ -167,7 +190,7 @@ __global__ __launch_bounds__(512) void balance_kernel(BalanceArgs a) {
             const int e = ldg(a.ids + (int64_t)r * a.topk + j);
             if (e >= 0 && e < a.E) atomicAdd(&sc[e], 1);
         }
-        row_shares<V, W, SC, false>(f, d, a.E, tmp);
+        row_shares<V, W, SC, false>(f, d, a.z + (int64_t)r * a.ld, a.E, tmp);
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] += f[v];
     }, [](int) {});
@@ -307,7 +330,7 @@ __global__ __launch_bounds__(256) void balance_grad_kernel(BalanceArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) f[v] = nx[v];
         if (next >= 0) load_row<V, W>(a.z + (int64_t)next * a.ld, a.E, nx);
-        row_shares<V, W, SC, true>(f, d, a.E, tmp);
+        row_shares<V, W, SC, true>(f, d, a.z + (int64_t)r * a.ld, a.E, tmp);
         float m = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) m += f[v] * w[v];

@@ -334,8 +334,8 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
 
 /* ------------------------------------------------------------------------------------------------ router balance
  * How evenly a router loads its experts, as a loss. Row t has scores s(t, e) of its logits (EXL3_SCORE_SOFTMAX: exp;
- * EXL3_SCORE_SIGMOID: sigmoid; EXL3_SCORE_SQRT_SOFTPLUS) and shares p(t, e) = s(t, e) / sum over e; a row whose scores are all
- * zero in fp32 (every logit -inf) has p = 0. Over the live rows t (mask uint8 [M], non-zero = live; NULL: all), N of them:
+ * EXL3_SCORE_SIGMOID: sigmoid; EXL3_SCORE_SQRT_SOFTPLUS) and shares p(t, e) = s(t, e) / sum over e, of logits however
+ * low; a row of which every logit is -inf has p = 0. Over the live rows t (mask uint8 [M], non-zero = live; NULL: all), N of them:
  *   counts[e] = picks of e in ids (int32 [M, topk]; entries outside [0, E) count nowhere)
  *   prob[e]   = sum p(t, e) / N
  *   loss      = coef * sum over e of E * counts[e] / (topk * N) * prob[e]
