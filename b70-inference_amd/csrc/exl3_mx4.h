@@ -1,7 +1,7 @@
 // Microscaled 4-bit values (MX4): 32 consecutive values of a row share a scale 2^(s - 127) held in a byte (255: not a
 // number); a value is sign, two exponent bits and one mantissa bit (0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the even
 // one in the low half. A matrix is codes uint8 [rows][k / 2] and scales uint8 [rows][k / 32], both row-major. Every value
-// times its scale is exact in bf16 and fp32, and in fp16 for scales 2^-23 .. 2^13.
+// times its scale is exact in bf16 and fp32 for scales to 2^125 (above, 4 2^126 and 2 2^127 are 2^128), and in fp16 for 2^-23 .. 2^13.
 //
 // The gfx950 conversions take the scale's exponent bits as that byte (the mantissa is not read, exponent 0 is 2^-127),
 // round to nearest even and saturate; the scaled MFMAs take the codes as they lie in memory: lane l of a 16 x 16 x 128

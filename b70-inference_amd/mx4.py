@@ -23,6 +23,7 @@ DTYPES = {torch.float16: EXL3_F16, torch.float32: EXL3_F32, torch.bfloat16: EXL3
 
 # Scale bytes whose blocks are exact in fp16: 0.5 * 2^-23 is its smallest magnitude, 6 * 2^13 below its largest.
 _F16_LO, _F16_HI = 104, 140
+_BF16_HI = 252                         # 6 * 2^125 is below bf16's largest magnitude (and fp32's)
 
 
 class MX4Tensor:
@@ -123,7 +124,8 @@ def mx4_quantize(x: torch.Tensor, out: MX4Tensor | None = None) -> MX4Tensor:
 
 
 def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float16, out: torch.Tensor | None = None) -> torch.Tensor:
-    """The values of t [..., k] (exact in bf16 and fp32; in fp16 for scales 2^-23 .. 2^13, else rounded once)."""
+    """The values of t [..., k], exact in bf16 and fp32 up to their largest magnitude (scales to 2^125; infinite from 2^128 on),
+    in fp16 for scales 2^-23 .. 2^13, else rounded once."""
     codes, scales = t.codes, t.scales
     shape = t.shape
     k = shape[-1]
@@ -178,7 +180,8 @@ def mx4_gemm(A: MX4Tensor, B: MX4Tensor, bias: torch.Tensor | None = None, out: 
 
 def _scale_bases(w: MX4Tensor):
     """Per leading matrix of w [..., n, k]: the power of two to take out of its scales so that every block that is not all
-    zeros is exact in fp16 (0 where none is needed), and whether there is one. Reads the weights once, on the host's time."""
+    zeros is exact in fp16 (0 where none is needed), whether there is one, and whether every value fits bf16 (of magnitudes
+    2^128 and more, which the two largest scales have, none does). Reads the weights once, on the host's time."""
     s = w.scales.flatten(-2).to(torch.int16)
     blk = (w.codes.view(torch.int64) & 0x7777777777777777).unflatten(-1, (-1, 2)).ne(0).any(-1).flatten(-2)
     live = blk & (s < 255)                                     # (NaN blocks stay NaN under any base)
@@ -186,13 +189,22 @@ def _scale_bases(w: MX4Tensor):
     hi = torch.where(live, s, torch.full_like(s, -1)).amax(-1).reshape(-1).tolist()
     base = [0 if b < 0 or (a >= _F16_LO and b <= _F16_HI) else b - _F16_HI for a, b in zip(lo, hi)]
     ok = [b < 0 or a - e >= _F16_LO for a, b, e in zip(lo, hi, base)]
-    return base, ok
+    fits = [True] * len(hi)
+    if max(hi) > _BF16_HI:
+        c = w.codes.unflatten(-1, (-1, 16))
+        top = torch.maximum(c & 7, c >> 4 & 7).amax(-1).flatten(-2)
+        past = ((s == 253) & (top >= 6)) | ((s == 254) & (top >= 4))           # from 4 2^126 and 2 2^127 on
+        fits = past.any(-1).logical_not().reshape(-1).tolist()
+    return base, ok, fits
 
 
 class MX4Linear:
     """y = x @ W^T (+ bias) with W [n, k] in MX4 and 16-bit rows x. The weights are exact in the rows' type; fp16 rows need
     the matrix's scales (of blocks that are not all zeros) to span at most 2^36: MX4Linear finds the power of two to take
-    out once, here, and refuses fp16 rows of a wider matrix (bf16 rows take any)."""
+    out once, here, and refuses fp16 rows of a wider matrix (bf16 rows take any) and bf16 rows of one with values of 2^128 and
+    more."""
+
+    bf16_rows = True
 
     def __init__(self, weight: MX4Tensor, bias: torch.Tensor | None = None):
         if len(weight.shape) != 2 or weight.shape[0] == 0:
@@ -200,7 +212,7 @@ class MX4Linear:
         self.weight = weight
         self.out_features, self.in_features = weight.shape
         self.bias = _bias("MX4Linear", bias, self.out_features)
-        (self.scale_base,), (self.fp16_rows,) = _scale_bases(weight)
+        (self.scale_base,), (self.fp16_rows,), (self.bf16_rows,) = _scale_bases(weight)
 
     def run(self, x: torch.Tensor, y: torch.Tensor) -> None:
         """x [..., k] fp16 or bf16 (other types become fp16) -> y (fp16, bf16 or fp32, preallocated) [..., n]."""
@@ -212,6 +224,8 @@ class MX4Linear:
             x = x.half()
         if x.dtype == torch.float16 and not self.fp16_rows:
             raise NotImplementedError("MX4Linear: the weight's scales span more than fp16 holds; use bf16 rows")
+        if x.dtype == torch.bfloat16 and not self.bf16_rows:
+            raise NotImplementedError("MX4Linear: the weight has values of 2^128 and more, which bf16 does not hold")
         x2, m, ld = _rows(x, k)
         y2, y_ld = _out2("MX4Linear", y, m, n)
         with where:
@@ -255,16 +269,17 @@ class MX4Experts:
             if any(tuple(t.shape) != want for t in ts):
                 raise Exl3Error(f"MX4Experts: every gate and up must be {shapes[0]}, every down {shapes[2]}")
             rows += [[t.codes.data_ptr() for t in ts], [t.scales.data_ptr() for t in ts], [b[0][0] for b in bs]]
-        self._finish([t for ts in projs for t in ts], rows, shapes[0], all(b[1][0] for bs in bases for b in bs))
+        self._finish([t for ts in projs for t in ts], rows, shapes[0], all(b[1][0] for bs in bases for b in bs),
+                     all(b[2][0] for bs in bases for b in bs))
 
-    def _finish(self, tensors, rows, shape, fp16_rows):
+    def _finish(self, tensors, rows, shape, fp16_rows, bf16_rows):
         self.tensors = tensors
         if len({t.device for t in tensors}) > 1:
             raise Exl3Error("MX4Experts: weights on several devices")
         self.E, (self.I, self.H) = len(rows[0]), shape
         if self.I % 32:
             raise Exl3Error(f"MX4Experts: {self.I} intermediate columns are not a multiple of 32")
-        self.fp16_rows = fp16_rows
+        self.fp16_rows, self.bf16_rows = fp16_rows, bf16_rows
         self.tables = torch.tensor(rows, dtype=torch.int64).to(tensors[0].device)
 
     @classmethod
@@ -273,17 +288,17 @@ class MX4Experts:
         if len(gate.shape) != 3 or gate.shape[0] == 0 or up.shape != gate.shape \
                 or tuple(down.shape) != (gate.shape[0], gate.shape[2], gate.shape[1]):
             raise Exl3Error("MX4Experts.stacked: gate and up [E, I, H] and down [E, H, I] expected")
-        rows, fine = [], True
+        rows, fine, fits = [], True, True
         for t in (gate, up, down):
             base, ok = [], True
             for e0 in range(0, t.shape[0], 16):                # a few experts at a time: the check's scratch stays small
-                b, o = _scale_bases(MX4Tensor(t.codes[e0:e0 + 16], t.scales[e0:e0 + 16]))
-                base, ok = base + b, ok and all(o)
+                b, o, f = _scale_bases(MX4Tensor(t.codes[e0:e0 + 16], t.scales[e0:e0 + 16]))
+                base, ok, fits = base + b, ok and all(o), fits and all(f)
             n, c, s = t.shape[0], t.codes[0].numel(), t.scales[0].numel()
             rows += [[t.codes.data_ptr() + e * c for e in range(n)], [t.scales.data_ptr() + e * s for e in range(n)], base]
             fine = fine and ok
         self = cls.__new__(cls)
-        self._finish([gate, up, down], rows, gate.shape[1:], fine)
+        self._finish([gate, up, down], rows, gate.shape[1:], fine, fits)
         return self
 
 
@@ -298,6 +313,8 @@ def mx4_moe_forward(x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tenso
         raise Exl3Error(f"mx4_moe_forward: x must be fp16 or bf16 [M, {H}]")
     if x.dtype == torch.float16 and not experts.fp16_rows:
         raise NotImplementedError("mx4_moe_forward: an expert's scales span more than fp16 holds; use bf16 rows")
+    if x.dtype == torch.bfloat16 and not experts.bf16_rows:
+        raise NotImplementedError("mx4_moe_forward: an expert has values of 2^128 and more, which bf16 does not hold")
     M = x.shape[0]
     if topk_ids.dtype != torch.int32 or topk_w.dtype != torch.float32:
         raise Exl3Error("mx4_moe_forward: topk_ids int32 and topk_w fp32 expected")

@@ -302,7 +302,8 @@ int exl3_mx4_quantize(const void* x, int64_t x_ld, int64_t rows, int64_t k, int 
                       void* stream);
 
 /* out (fp16, bf16 or fp32 [rows, k], row stride out_ld, rows 16-byte aligned) = the values of codes and scales, rounded once
- * (exact in bf16 and fp32; in fp16 for scales 2^-23 .. 2^13). Scale byte 255: NaN. */
+ * (exact in bf16 and fp32 for scales to 2^125, above them the codes 2 or 4 and more are infinite; exact in fp16 for scales
+ * 2^-23 .. 2^13). Scale byte 255: NaN. */
 int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t out_ld,
                         int out_dtype, void* stream);
 
@@ -310,7 +311,8 @@ int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t row
  * W [n, k] as codes (16-byte aligned) and scales, bias fp32 [n] or NULL, C fp16, bf16 or fp32 (row stride c_ld). The
  * weights are exact in x's type, the sums fp32, one rounding. fp16 x: every block that is not all zeros must have
  * 104 <= s - scale_base <= 140 (its values times 2^-scale_base are then exact in fp16; the result is scaled back); any
- * other block's values round, overflow or vanish as fp16 does. bf16 x: scale_base is not used. k is a multiple of 32 up to
+ * other block's values round, overflow or vanish as fp16 does. bf16 x: scale_base is not used, and a weight of 2^128 or more
+ * (4 and 6 at scale byte 253, 2 to 6 at 254) is infinite. k is a multiple of 32 up to
  * 2^24, n any number. */
 int exl3_mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
                     const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
