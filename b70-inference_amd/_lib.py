@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 
 import torch
@@ -54,14 +55,24 @@ SIGNATURES = {
     "exl3_mx4_quantize": [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp],
     "exl3_mx4_dequantize": [_vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp],
     "exl3_mx4_linear": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp],
+    "exl3_mx4_linear_in": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _i64, _vp],
+    "exl3_mx4_linear_scratch": [_i64, _i64, _i64],
     "exl3_mx4_gemm": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _vp],
+    "exl3_mx4_gemm_in": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp],
+    "exl3_mx4_gemm_scratch": [_i64, _i64, _i64],
     "exl3_mx4_moe_forward": [_vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _f32, _i64, _vp, _i64,
                              _i32, _vp],
+    "exl3_mx4_moe_forward_in": [_vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _f32, _i64, _vp, _i64,
+                                _i32, _vp, _i64, _vp],
+    "exl3_mx4_moe_scratch": [_i64, _i64, _i64, _i64, _i64, _i64],
+    "exl3_route_balance_in": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "exl3_route_balance_scratch": [_i64, _i64],
     "exl3_route_balance": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp],
     "exl3_route_balance_grad": [_vp, _i64, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp],
     "exl3_router_logits": [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
 }
-_RESTYPE = {"exl3_last_error": ctypes.c_char_p}
+_RESTYPE = {"exl3_last_error": ctypes.c_char_p, "exl3_mx4_linear_scratch": _i64, "exl3_mx4_gemm_scratch": _i64,
+            "exl3_mx4_moe_scratch": _i64, "exl3_route_balance_scratch": _i64}
 
 _lib = None
 
@@ -145,6 +156,19 @@ def reserve_workspace(nbytes: int, ncounters: int = 0):
 def release_workspace():
     """Free outgrown workspace buffers (synchronises; no graph captured before may be replayed afterwards)."""
     check(lib().exl3_release_workspace(), "exl3_release_workspace")
+
+
+# Scratch of the calls that take it from the caller: torch's allocator gives every call memory of its own until the stream that it
+# runs on is done with it (a graph's calls, the graph's), so they may overlap on any streams and threads. The sizes follow from the
+# shapes alone.
+@functools.lru_cache(maxsize=4096)
+def scratch_bytes(what: str, *sizes: int) -> int:
+    return getattr(lib(), what)(*sizes)
+
+
+def scratch(n: int, like: torch.Tensor):
+    """n bytes on like's device for a call on its current stream; the tensor must live until the call has been made."""
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 _same_device = contextlib.nullcontext()

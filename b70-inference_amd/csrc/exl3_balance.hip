@@ -222,6 +222,7 @@ __global__ __launch_bounds__(512) void balance_kernel(BalanceArgs a) {
             a.part_c[(int64_t)blockIdx.x * a.E + e] = sc[e];
         });
         if (t == 0) a.part_n[blockIdx.x] = s_live;
+        if (t == 0 && blockIdx.x == 0) *a.arrived = 0;         // (counted by the reduction, a launch later)
         return;
     }
     const int n = s_live;
@@ -384,15 +385,21 @@ static int balance_setup(const char* what, const float* logits, int64_t ld, int6
     return EXL3_OK;
 }
 
-}  // namespace exl3
+// Workgroups of a forward pass, eight rows at a time in each (one of more than 2048 experts): one up to seven rounds of rows, then one
+// for every four rounds, up to 480. Not a power of two: a wave's rows would all lie at one place of padded sequences, all
+// live or all dead.
+static int balance_groups(int64_t M, int64_t E) {
+    const int per = E > 2048 ? 1 : 8;
+    const int64_t rounds = (M + per - 1) / per;
+    return (int)(rounds < 8 ? 1 : rounds / 4 < 480 ? rounds / 4 : 480);
+}
+static size_t balance_bytes(int G, int64_t E) {
+    return carve_size((size_t)G * E, 4) * 2 + carve_size(G, 4) + carve_size((size_t)(E + 15) / 16, 4) + carve_size(1, 4);
+}
 
-extern "C" {
-
-using namespace exl3;
-
-int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk,
-                       const uint8_t* mask, int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows,
-                       void* stream) {
+static int balance(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk, const uint8_t* mask,
+                   int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows, const CallScratch& s,
+                   void* stream) {
     hipStream_t st = (hipStream_t)stream;
     BalanceArgs a{};
     int rc = balance_setup("exl3_route_balance", logits, ld, M, E, topk, score, mask, coef, a);
@@ -403,30 +410,50 @@ int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, co
     a.counts = counts;
     a.prob = prob;
     a.rows = rows;
-    // eight rows at a time in a workgroup (one of more than 2048 experts): one workgroup up to four rounds, else up to 480. Not a
-    // power of two: a wave's rows would all lie at one place of padded sequences, all live or all dead.
-    const int per = E > 2048 ? 1 : 8;
-    const int64_t rounds = (M + per - 1) / per;
-    a.G = (int)(rounds <= 4 ? 1 : rounds / 4 < 480 ? rounds / 4 : 480);
+    a.G = balance_groups(M, E);
     if (a.G > 1) {
-        Workspace ws;
         const size_t ge = (size_t)a.G * E;
         const int ncb = (int)((E + 15) / 16);
-        rc = workspace(carve_size(ge, 4) * 2 + carve_size(a.G, 4) + carve_size(ncb, 4), 1, st, &ws);
+        Carve c{};
+        rc = call_scratch("exl3_route_balance", balance_bytes(a.G, E), s, st, &c);
         if (rc) return rc;
-        Carve c{ws.scratch, ws.scratch_bytes};
         a.part_p = c.take<float>(ge);
         a.part_c = c.take<int32_t>(ge);
         a.part_n = c.take<int32_t>(a.G);
         a.part_l = c.take<float>(ncb);
-        a.arrived = ws.counters;
-        if (!a.part_l) return fail(EXL3_ERR_INVALID, "exl3_route_balance: workspace carve failed");
+        a.arrived = c.take<int>(1);
+        if (!a.arrived) return fail(EXL3_ERR_INVALID, "exl3_route_balance: workspace carve failed");
     }
     EXL3_LAUNCH("route_balance", balance_pick(score, a.E, false), dim3((unsigned)a.G), dim3(E > 2048 ? 256 : 512),
                 (size_t)E * (E > 2048 ? 4 : 8), st, a);
     if (a.G > 1)
         EXL3_LAUNCH("route_balance_reduce", balance_reduce_kernel, dim3((unsigned)((E + 15) / 16)), dim3(256), 0, st, a);
     return EXL3_OK;
+}
+
+}  // namespace exl3
+
+extern "C" {
+
+using namespace exl3;
+
+int64_t exl3_route_balance_scratch(int64_t M, int64_t E) {
+    if (M < 0 || M > 0x3FFFFFFF || E < 1 || E > 8192) return 0;
+    const int G = balance_groups(M, E);
+    return G > 1 ? (int64_t)balance_bytes(G, E) : 0;
+}
+
+int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk,
+                       const uint8_t* mask, int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows,
+                       void* stream) {
+    return balance(logits, ld, M, E, ids, topk, mask, score, coef, loss, counts, prob, rows, kLibScratch, stream);
+}
+
+int exl3_route_balance_in(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk,
+                          const uint8_t* mask, int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows,
+                          void* scratch, int64_t scratch_bytes, void* stream) {
+    return balance(logits, ld, M, E, ids, topk, mask, score, coef, loss, counts, prob, rows, CallScratch{scratch, scratch_bytes, false},
+                   stream);
 }
 
 int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t E, int64_t topk, const uint8_t* mask,

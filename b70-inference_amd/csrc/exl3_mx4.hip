@@ -244,16 +244,23 @@ __global__ __launch_bounds__(256) void mx4_reduce_kernel(Mx4Args a) {
     mx4_store(a, m, n, v);
 }
 
-// The plan's splits, with the partials' buffer from the workspace. One split: the kernel writes the output itself.
-static int mx4_split(Mx4Args& a, const Mx4Plan& plan, hipStream_t st) {
+static int64_t mx4_n4(int64_t n) { return (n + 3) & ~(int64_t)3; }
+
+// Bytes of a plan's partials.
+static int64_t mx4_part_bytes(const Mx4Plan& plan, int64_t m, int64_t n) {
+    return plan.P == 1 ? 0 : (int64_t)plan.P * m * mx4_n4(n) * 4;
+}
+
+// The plan's splits, with the partials in the call's scratch. One split: the kernel writes the output itself.
+static int mx4_split(const char* what, Mx4Args& a, const Mx4Plan& plan, const CallScratch& s, hipStream_t st) {
     a.splits = plan.P;
     a.bps = plan.bps;
-    a.n4 = (a.n + 3) & ~(int64_t)3;
+    a.n4 = mx4_n4(a.n);
     a.part = nullptr;
     if (a.splits == 1) return EXL3_OK;
-    Workspace ws;
-    const int rc = workspace((size_t)a.splits * a.m * a.n4 * 4, 0, st, &ws);
-    a.part = reinterpret_cast<float*>(ws.scratch);
+    Carve c{};
+    const int rc = call_scratch(what, (size_t)mx4_part_bytes(plan, a.m, a.n), s, st, &c);
+    a.part = reinterpret_cast<float*>(c.p);
     return rc;
 }
 
@@ -349,13 +356,14 @@ __global__ __launch_bounds__(1024) void mx4_decode_kernel(Mx4Args a, int xbytes)
 // LDS of a CU, all of which one workgroup may take.
 constexpr int kMx4Lds = 163840;
 
-// Waves and LDS bytes of a decode call: eight waves, sixteen where x leaves room for one workgroup per CU only (eight rows of
+// Rows that the decode kernel takes: up to 16 with 16-bit rows, with MX4 rows up to eight (16 rows, decode / tiles: 4096 x 4096 10.2 /
+// 9.9 us, 5376 -> 21504 23.0 / 19.8; 4 rows: 6.0 / 9.0, 16.5 / 19.0). Waves and LDS bytes of a call: eight waves, sixteen where x leaves room for one workgroup per CU only (eight rows of
 // 5376 -> 21504: 25.1 us with eight, 21.4 with sixteen). False if x does not fit.
 template <int XT>
-static bool decode_shape(const Mx4Args& a, int& waves, int& xb, int& lds) {
-    if (a.m > 16 || a.k > 1 << 20) return false;
-    const int kb = a.k / 32, ng = (kb + 4 * kMx4Group - 1) / (4 * kMx4Group);
-    xb = mx4_x_bytes<XT>((int)a.m, kb);
+static bool decode_shape(int64_t m, int64_t k, int& waves, int& xb, int& lds) {
+    if (m > (XT == kRowMX4 ? 8 : 16) || k > 1 << 20) return false;
+    const int kb = (int)k / 32, ng = (kb + 4 * kMx4Group - 1) / (4 * kMx4Group);
+    xb = mx4_x_bytes<XT>((int)m, kb);
     waves = mx4_decode_waves(ng, 8);
     if (2 * (xb + 2 * waves * 1024) > kMx4Lds && xb + 2 * 16 * 1024 <= kMx4Lds) waves = mx4_decode_waves(ng, 16);
     lds = xb + 2 * waves * 1024;
@@ -405,9 +413,9 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args
 }
 
 template <int XT, int RG>
-static int launch_wide(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
+static int launch_wide(Mx4Args a, const Mx4Plan& plan, const CallScratch& s, hipStream_t st) {
     const int64_t tiles = (a.m + 32 * RG - 1) / (32 * RG) * ((a.n + 255) / 256);
-    const int rc = mx4_split(a, plan, st);
+    const int rc = mx4_split("exl3_mx4_linear", a, plan, s, st);
     if (rc) return rc;
     EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0 / a.splits, "exl3_mx4_linear: grid too large");
     EXL3_LAUNCH("mx4_linear_wide", (mx4_wide_kernel<XT, RG>), dim3((unsigned)((tiles * a.splits + 7) & ~7)), dim3(256), 0, st, a);
@@ -415,12 +423,13 @@ static int launch_wide(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
 }
 
 template <int XT>
-static int linear_run(const Mx4Args& a, hipStream_t st) {
+static int linear_run(const Mx4Args& a, const CallScratch& s, hipStream_t st) {
     if (a.n * (a.k / 32) < 16) return launch_tiny<XT>("mx4_linear_tiny", a, st);
     int waves, xb, lds;
-    if (decode_shape<XT>(a, waves, xb, lds)) return launch_decode<XT>("mx4_linear", a, waves, xb, lds, st);
+    if (decode_shape<XT>(a.m, a.k, waves, xb, lds)) return launch_decode<XT>("mx4_linear", a, waves, xb, lds, st);
     const Mx4Plan p = mx4_linear_plan(a.m, a.n, a.k, 256);
-    return p.tile == 0 ? launch_wide<XT, 1>(a, p, st) : p.tile == 1 ? launch_wide<XT, 2>(a, p, st) : launch_wide<XT, 4>(a, p, st);
+    return p.tile == 0 ? launch_wide<XT, 1>(a, p, s, st) : p.tile == 1 ? launch_wide<XT, 2>(a, p, s, st)
+                                                                       : launch_wide<XT, 4>(a, p, s, st);
 }
 
 // ------------------------------------------------------------------------------------------------ many MX4 rows
@@ -564,10 +573,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_tile_kernel(Mx4Args a) 
 }
 
 template <int TM, int TN, int WM, int WN, int OCC>
-static int launch_tile(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
+static int launch_tile(Mx4Args a, const Mx4Plan& plan, const CallScratch& s, hipStream_t st) {
     typedef Mx4Tile<TM, TN, WM, WN> T;
     const int64_t tiles = (a.m + T::BM - 1) / T::BM * ((a.n + T::BN - 1) / T::BN);
-    const int rc = mx4_split(a, plan, st);
+    const int rc = mx4_split("exl3_mx4_gemm", a, plan, s, st);
     if (rc) return rc;
     EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0 / a.splits, "exl3_mx4_gemm: grid too large");
     EXL3_LAUNCH("mx4_gemm_tile", (mx4_tile_kernel<TM, TN, WM, WN, OCC>), dim3((unsigned)((tiles * a.splits + 7) & ~7)),
@@ -577,6 +586,11 @@ static int launch_tile(Mx4Args a, const Mx4Plan& plan, hipStream_t st) {
 
 static bool mx4_dtype(int t) { return t == EXL3_F16 || t == EXL3_F32 || t == EXL3_BF16; }
 static int elem_size(int t) { return t == EXL3_F32 ? 4 : 2; }
+
+// Sizes that both products take.
+static bool mx4_sizes(int64_t m, int64_t n, int64_t k) {
+    return m >= 0 && n > 0 && k > 0 && k % 32 == 0 && k <= (1 << 24) && m <= ((int64_t)1 << 40) / k && n <= ((int64_t)1 << 40) / k;
+}
 
 // What both products check of their weights and output; sets those of the kernel's arguments.
 static int mx4_setup(const char* what, int64_t m, int64_t n, int64_t k, const uint8_t* w, const uint8_t* ws,
@@ -603,6 +617,42 @@ static int mx4_setup(const char* what, int64_t m, int64_t n, int64_t k, const ui
     a.vec = n % 4 == 0 && c_ld % 4 == 0 && aligned(C, 4 * elem_size(c_dtype));
     if (c_dtype != EXL3_F32 && n % 8 == 0 && c_ld % 8 == 0 && aligned(C, 16)) a.vec = 2;
     return EXL3_OK;
+}
+
+static int mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const uint8_t* scales,
+                      int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld, int c_dtype, const CallScratch& s,
+                      void* stream) {
+    EXL3_CHECK_ARG(x_dtype == EXL3_F16 || x_dtype == EXL3_BF16, "exl3_mx4_linear: x must be fp16 or bf16");
+    EXL3_CHECK_ARG(x_ld >= k, "exl3_mx4_linear: x row stride %lld < k", (long long)x_ld);
+    EXL3_CHECK_ARG(scale_base >= -140 && scale_base <= 140, "exl3_mx4_linear: scale_base %d out of range", scale_base);
+    Mx4Args a{};
+    const int rc = mx4_setup("exl3_mx4_linear", m, n, k, codes, scales, bias, C, c_ld, c_dtype, a);
+    if (rc || m == 0) return rc;
+    EXL3_CHECK_ARG(x && aligned(x, 16) && (m == 1 || x_ld % 8 == 0), "exl3_mx4_linear: x rows must be 16-byte aligned");
+    EXL3_CHECK_ARG(m <= ((int64_t)1 << 45) / x_ld, "exl3_mx4_linear: operand too large");
+    a.x = reinterpret_cast<const uint8_t*>(x);
+    a.x_ld = 2 * x_ld;
+    a.base = x_dtype == EXL3_F16 ? scale_base : 0;
+    return x_dtype == EXL3_F16 ? linear_run<kRowF16>(a, s, (hipStream_t)stream) : linear_run<kRowBF16>(a, s, (hipStream_t)stream);
+}
+
+static int mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,
+                    const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, const CallScratch& s,
+                    void* stream) {
+    Mx4Args a{};
+    const int rc = mx4_setup("exl3_mx4_gemm", m, n, k, b_codes, b_scales, bias, C, c_ld, c_dtype, a);
+    if (rc || m == 0) return rc;
+    EXL3_CHECK_ARG(a_codes && a_scales && aligned(a_codes, 16), "exl3_mx4_gemm: row codes must be 16-byte aligned");
+    a.x = a_codes;
+    a.xs = a_scales;
+    a.x_ld = k / 2;
+    hipStream_t st = (hipStream_t)stream;
+    if (m * (k / 32) < 16 || n * (k / 32) < 16) return launch_tiny<kRowMX4>("mx4_gemm_tiny", a, st);
+    int waves, xb, lds;
+    if (decode_shape<kRowMX4>(m, k, waves, xb, lds)) return launch_decode<kRowMX4>("mx4_gemm", a, waves, xb, lds, st);
+    const Mx4Plan p = mx4_gemm_plan(m, n, k, 256);
+    return p.tile == 0 ? launch_tile<2, 1, 1, 4, 4>(a, p, s, st) : p.tile == 1 ? launch_tile<2, 2, 2, 2, 3>(a, p, s, st)
+                                                              : launch_tile<4, 2, 2, 4, 2>(a, p, s, st);
 }
 
 }  // namespace exl3
@@ -657,41 +707,41 @@ int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t row
     return EXL3_OK;
 }
 
+int64_t exl3_mx4_linear_scratch(int64_t m, int64_t k, int64_t n) {
+    int waves, xb, lds;
+    if (!mx4_sizes(m, n, k) || m == 0 || n * (k / 32) < 16 || decode_shape<kRowF16>(m, k, waves, xb, lds)) return 0;
+    return mx4_part_bytes(mx4_linear_plan(m, n, k, 256), m, n);
+}
+
+int64_t exl3_mx4_gemm_scratch(int64_t m, int64_t k, int64_t n) {
+    int waves, xb, lds;
+    if (!mx4_sizes(m, n, k) || m == 0 || m * (k / 32) < 16 || n * (k / 32) < 16 || decode_shape<kRowMX4>(m, k, waves, xb, lds)) return 0;
+    return mx4_part_bytes(mx4_gemm_plan(m, n, k, 256), m, n);
+}
+
 int exl3_mx4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
                     const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
                     int c_dtype, void* stream) {
-    EXL3_CHECK_ARG(x_dtype == EXL3_F16 || x_dtype == EXL3_BF16, "exl3_mx4_linear: x must be fp16 or bf16");
-    EXL3_CHECK_ARG(x_ld >= k, "exl3_mx4_linear: x row stride %lld < k", (long long)x_ld);
-    EXL3_CHECK_ARG(scale_base >= -140 && scale_base <= 140, "exl3_mx4_linear: scale_base %d out of range", scale_base);
-    Mx4Args a{};
-    const int rc = mx4_setup("exl3_mx4_linear", m, n, k, codes, scales, bias, C, c_ld, c_dtype, a);
-    if (rc || m == 0) return rc;
-    EXL3_CHECK_ARG(x && aligned(x, 16) && (m == 1 || x_ld % 8 == 0), "exl3_mx4_linear: x rows must be 16-byte aligned");
-    EXL3_CHECK_ARG(m <= ((int64_t)1 << 45) / x_ld, "exl3_mx4_linear: operand too large");
-    a.x = reinterpret_cast<const uint8_t*>(x);
-    a.x_ld = 2 * x_ld;
-    a.base = x_dtype == EXL3_F16 ? scale_base : 0;
-    return x_dtype == EXL3_F16 ? linear_run<kRowF16>(a, (hipStream_t)stream) : linear_run<kRowBF16>(a, (hipStream_t)stream);
+    return mx4_linear(x, x_ld, x_dtype, m, k, codes, scales, n, scale_base, bias, C, c_ld, c_dtype, kLibScratch, stream);
+}
+
+int exl3_mx4_linear_in(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
+                       const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
+                       int c_dtype, void* scratch, int64_t scratch_bytes, void* stream) {
+    return mx4_linear(x, x_ld, x_dtype, m, k, codes, scales, n, scale_base, bias, C, c_ld, c_dtype,
+                      CallScratch{scratch, scratch_bytes, false}, stream);
 }
 
 int exl3_mx4_gemm(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,
                   const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, void* stream) {
-    Mx4Args a{};
-    const int rc = mx4_setup("exl3_mx4_gemm", m, n, k, b_codes, b_scales, bias, C, c_ld, c_dtype, a);
-    if (rc || m == 0) return rc;
-    EXL3_CHECK_ARG(a_codes && a_scales && aligned(a_codes, 16), "exl3_mx4_gemm: row codes must be 16-byte aligned");
-    a.x = a_codes;
-    a.xs = a_scales;
-    a.x_ld = k / 2;
-    hipStream_t st = (hipStream_t)stream;
-    if (m * (k / 32) < 16 || n * (k / 32) < 16) return launch_tiny<kRowMX4>("mx4_gemm_tiny", a, st);
-    // few rows: the decode kernel up to eight (16 rows, decode / tiles: 4096 x 4096 10.2 / 9.9 us, 5376 -> 21504 23.0 / 19.8;
-    // 4 rows: 6.0 / 9.0, 16.5 / 19.0)
-    int waves, xb, lds;
-    if (m <= 8 && decode_shape<kRowMX4>(a, waves, xb, lds)) return launch_decode<kRowMX4>("mx4_gemm", a, waves, xb, lds, st);
-    const Mx4Plan p = mx4_gemm_plan(m, n, k, 256);
-    return p.tile == 0 ? launch_tile<2, 1, 1, 4, 4>(a, p, st) : p.tile == 1 ? launch_tile<2, 2, 2, 2, 3>(a, p, st)
-                                                              : launch_tile<4, 2, 2, 4, 2>(a, p, st);
+    return mx4_gemm(a_codes, a_scales, m, k, b_codes, b_scales, n, bias, C, c_ld, c_dtype, kLibScratch, stream);
+}
+
+int exl3_mx4_gemm_in(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,
+                     const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, void* scratch,
+                     int64_t scratch_bytes, void* stream) {
+    return mx4_gemm(a_codes, a_scales, m, k, b_codes, b_scales, n, bias, C, c_ld, c_dtype, CallScratch{scratch, scratch_bytes, false},
+                    stream);
 }
 
 }  // extern "C"

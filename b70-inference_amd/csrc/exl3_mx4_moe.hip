@@ -409,15 +409,41 @@ static int mx4_moe_launch(const Mx4MoeArgs& a, int rows, hipStream_t st) {
     return mx4_moe_wide<XT, 4>(a, st);
 }
 
-}  // namespace exl3
+// Sizes that a call takes.
+static bool moe_sizes(int64_t M, int64_t H, int64_t I, int64_t topk, int64_t E) {
+    return M >= 0 && M <= (1 << 24) && topk >= 0 && topk <= 64 && E > 0 && E <= kMoeMaxExperts && H > 0 && I > 0 && H % 32 == 0 &&
+           I % 32 == 0 && H <= (1 << 20) && I <= (1 << 20);
+}
 
-extern "C" {
+// The path of a call of npairs pairs and its scratch.
+struct Mx4MoeShape {
+    bool pairs;
+    Mx4PairShape ps;
+    int rows;                          // of a block
+    int64_t max_blocks;
+    size_t bytes;
+};
+// Pairs as they stand while they, and the weights they ask for, repeated experts and all, are few: pairs / blocks, us: 512 experts of
+// 2048 -> 512 at 80 and 160 pairs 42 / 57, 71 / 90; of 2560 -> 640 at 80 and 160 69 / 74, 129 / 117; 64 of 4096 -> 1408 at 48
+// 94.8 / 93.6; 32 of 7168 -> 2048 at 16 and 32 93 / 103, 173 / 150; 8 of 4096 -> 4096 at 8 and 12 54 / 73, 75 / 75.
+static Mx4MoeShape moe_shape(int64_t npairs, int64_t H, int64_t I, int64_t slots, int64_t E) {
+    Mx4MoeShape s{};
+    const size_t np = (size_t)npairs;
+    s.pairs = npairs > 0 && npairs <= 160 && npairs * H * I <= 210000000 && pair_shape((int)H, (int)I, (int)slots, s.ps);
+    if (s.pairs) {
+        s.bytes = carve_size(np * I, 2) + carve_size(np * I / 16, 1);
+        return s;
+    }
+    s.rows = mx4_moe_rows(npairs, E);
+    s.max_blocks = mx4_max_blocks(npairs, E, s.rows);
+    s.bytes = carve_size((size_t)s.max_blocks, sizeof(ItemDesc)) + carve_size(2 * np, 4) + carve_size(np, 4) + carve_size(np * I, 2) +
+              carve_size(np * ((I + 127) / 128), 1) + carve_size(np * H, 4);
+    return s;
+}
 
-using namespace exl3;
-
-int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
-                         const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
-                         int64_t shared, void* out, int64_t out_ld, int out_dtype, void* stream) {
+static int mx4_moe(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
+                   const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit, int64_t shared,
+                   void* out, int64_t out_ld, int out_dtype, const CallScratch& s, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     EXL3_CHECK_ARG(x_dtype == EXL3_F16 || x_dtype == EXL3_BF16, "exl3_mx4_moe_forward: x must be fp16 or bf16");
     EXL3_CHECK_ARG(out_dtype == EXL3_F16 || out_dtype == EXL3_F32 || out_dtype == EXL3_BF16,
@@ -439,23 +465,19 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
                    "exl3_mx4_moe_forward: too many tokens");
 
     const int vec = out_ld % 4 == 0 && aligned(out, out_dtype == EXL3_F32 ? 16 : 8);
-    // Pairs as they stand while they, and the weights they ask for, repeated experts and all, are few: pairs / blocks, us: 512 experts of
-    // 2048 -> 512 at 80 and 160 pairs 42 / 57, 71 / 90; of 2560 -> 640 at 80 and 160 69 / 74, 129 / 117; 64 of 4096 -> 1408 at 48
-    // 94.8 / 93.6; 32 of 7168 -> 2048 at 16 and 32 93 / 103, 173 / 150; 8 of 4096 -> 4096 at 8 and 12 54 / 73, 75 / 75.
-    Mx4PairShape ps;
-    if (npairs > 0 && npairs <= 160 && npairs * H * I <= 210000000 && pair_shape((int)H, (int)I, (int)slots, ps)) {
-        Workspace ws;
+    const Mx4MoeShape sh = moe_shape(npairs, H, I, slots, E);
+    if (sh.pairs) {
         const size_t np = (size_t)npairs;
-        const int rc = workspace(carve_size(np * I, 2) + carve_size(np * I / 16, 1), 0, st, &ws);
+        Carve c{};
+        const int rc = call_scratch("exl3_mx4_moe_forward", sh.bytes, s, st, &c);
         if (rc) return rc;
-        Carve c{ws.scratch, ws.scratch_bytes};
         uint16_t* mid = c.take<uint16_t>(np * I);
         int8_t* mexp = c.take<int8_t>(np * I / 16);
         if (!mexp) return fail(EXL3_ERR_INVALID, "exl3_mx4_moe_forward: workspace carve failed");
         const Mx4PairArgs p{reinterpret_cast<const uint8_t*>(x), 2 * x_ld, (int)M, (int)H, (int)I, (int)topk, (int)slots, (int)E,
                             (int)shared, topk_ids, topk_w, tables, mid, mexp, act, act_limit, out,
                             out_ld, out_dtype, vec};
-        return x_dtype == EXL3_F16 ? launch_pairs<kRowF16>(p, ps, st) : launch_pairs<kRowBF16>(p, ps, st);
+        return x_dtype == EXL3_F16 ? launch_pairs<kRowF16>(p, sh.ps, st) : launch_pairs<kRowBF16>(p, sh.ps, st);
     }
 
     Mx4MoeArgs a{};
@@ -470,18 +492,16 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
     a.out = out;
     a.out_ld = out_ld;
     a.out_dtype = out_dtype;
-    const int rows = mx4_moe_rows(npairs, E);
-    a.max_blocks = (int)mx4_max_blocks(npairs, E, rows);
+    const int rows = sh.rows;
+    a.max_blocks = (int)sh.max_blocks;
     EXL3_CHECK_ARG((int64_t)a.max_blocks * ((H > I ? H : I) / 16) <= 0x7FFFFFFF, "exl3_mx4_moe_forward: grid too large");
     ItemDesc* blocks = nullptr;
     int* pairs = nullptr;
     if (npairs > 0) {
-        Workspace ws;
         const size_t np = (size_t)npairs;
-        const int rc = workspace(carve_size(a.max_blocks, sizeof(ItemDesc)) + carve_size(2 * np, 4) + carve_size(np, 4) +
-                                     carve_size(np * I, 2) + carve_size(np * ((I + 127) / 128), 1) + carve_size(np * H, 4), 0, st, &ws);
+        Carve c{};
+        const int rc = call_scratch("exl3_mx4_moe_forward", sh.bytes, s, st, &c);
         if (rc) return rc;
-        Carve c{ws.scratch, ws.scratch_bytes};
         blocks = c.take<ItemDesc>(a.max_blocks);
         pairs = c.take<int>(2 * np);
         float* pw = c.take<float>(np);
@@ -521,6 +541,34 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
     EXL3_CHECK_ARG(M * ncb <= 0x7FFFFFFF, "exl3_mx4_moe_forward: grid too large");
     EXL3_LAUNCH("mx4_moe_combine", mx4_combine_kernel, dim3((unsigned)(M * ncb)), dim3(256), 0, st, a, (int)ncb, vec);
     return EXL3_OK;
+}
+
+}  // namespace exl3
+
+extern "C" {
+
+using namespace exl3;
+
+int64_t exl3_mx4_moe_scratch(int64_t M, int64_t H, int64_t I, int64_t topk, int64_t E, int64_t shared) {
+    if (!moe_sizes(M, H, I, topk, E) || M == 0) return 0;
+    const int64_t slots = topk + (shared >= 0 ? 1 : 0);
+    if (slots == 0 || M * slots > (1 << 24)) return 0;
+    return (int64_t)moe_shape(M * slots, H, I, slots, E).bytes;
+}
+
+int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
+                         const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
+                         int64_t shared, void* out, int64_t out_ld, int out_dtype, void* stream) {
+    return mx4_moe(x, x_ld, x_dtype, M, H, I, topk_ids, topk_w, topk, E, tables, act, act_limit, shared, out, out_ld, out_dtype,
+                   kLibScratch, stream);
+}
+
+int exl3_mx4_moe_forward_in(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
+                            const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
+                            int64_t shared, void* out, int64_t out_ld, int out_dtype, void* scratch, int64_t scratch_bytes,
+                            void* stream) {
+    return mx4_moe(x, x_ld, x_dtype, M, H, I, topk_ids, topk_w, topk, E, tables, act, act_limit, shared, out, out_ld, out_dtype,
+                   CallScratch{scratch, scratch_bytes, false}, stream);
 }
 
 }  // extern "C"

@@ -172,6 +172,19 @@ int workspace(size_t bytes, size_t ncounters, hipStream_t st, Workspace* out) {
     return EXL3_OK;
 }
 
+int call_scratch(const char* what, size_t bytes, const CallScratch& s, hipStream_t st, Carve* out) {
+    if (s.lib) {
+        Workspace ws;
+        const int rc = workspace(bytes, 0, st, &ws);
+        *out = Carve{ws.scratch, ws.scratch_bytes};
+        return rc;
+    }
+    EXL3_CHECK_ARG(s.bytes >= 0 && (size_t)s.bytes >= bytes && (s.p || !bytes) && aligned(s.p, 256),
+                   "%s: %zu bytes of 256-byte aligned scratch needed, got %lld at %p", what, bytes, (long long)s.bytes, s.p);
+    *out = Carve{reinterpret_cast<char*>(s.p), (size_t)s.bytes};
+    return EXL3_OK;
+}
+
 size_t workspace_room(hipStream_t st) {
     if (!capturing(st)) return SIZE_MAX;
     int dev = 0;

@@ -91,6 +91,15 @@ struct Carve {
     }
 };
 
+// Scratch of one call: the caller's buffer (256-byte aligned), or with `lib` the device's workspace. `bytes` of it for carving.
+struct CallScratch {
+    void* p;
+    int64_t bytes;
+    bool lib;
+};
+constexpr CallScratch kLibScratch = {nullptr, 0, true};
+int call_scratch(const char* what, size_t bytes, const CallScratch& s, hipStream_t stream, Carve* out);
+
 inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 // Opt-in kernel timing (exl3_profile_enable): every library launch gets a HIP event pair that the runtime records

@@ -9,14 +9,16 @@ bits and one mantissa bit (0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the even o
   * mx4_gemm(A, B)                                  A @ B^T of two MX4Tensors on the scaled matrix instructions
   * MX4Experts, mx4_moe_forward(x, ids, w, experts) the routed layer of moe_forward over MX4 experts (BlockSparseMLP takes
     MX4Experts too)
-Tensors live on the GPU; every op is asynchronous on the current stream of its tensors' device. The reference has no
+Tensors live on the GPU; every op is asynchronous on the current stream of its tensors' device and has scratch of its own (calls may
+overlap on several streams, and with replays of graphs that hold some). The reference has no
 counterpart: its weights are EXL3 only.
 """
 from __future__ import annotations
 
 import torch
 
-from ._lib import ACT_GELU_TANH, ACT_SILU, EXL3_BF16, EXL3_F16, EXL3_F32, Exl3Error, check, lib, on_device, ptr, stream_of
+from ._lib import ACT_GELU_TANH, ACT_SILU, EXL3_BF16, EXL3_F16, EXL3_F32, Exl3Error, check, lib, on_device, ptr, scratch, \
+    scratch_bytes, stream_of
 
 ACTS = {"silu": ACT_SILU, "gelu_tanh": ACT_GELU_TANH, ACT_SILU: ACT_SILU, ACT_GELU_TANH: ACT_GELU_TANH}
 DTYPES = {torch.float16: EXL3_F16, torch.float32: EXL3_F32, torch.bfloat16: EXL3_BF16}
@@ -170,9 +172,11 @@ def mx4_gemm(A: MX4Tensor, B: MX4Tensor, bias: torch.Tensor | None = None, out: 
     o2, ld = _out2("mx4_gemm", out, m, n)
     if n == 0:
         return out
+    need = scratch_bytes("exl3_mx4_gemm_scratch", m, k, n)
+    ws = scratch(need, out)
     with where:
-        rc = lib().exl3_mx4_gemm(A.codes.data_ptr(), A.scales.data_ptr(), m, k, B.codes.data_ptr(), B.scales.data_ptr(), n,
-                                 ptr(bias), o2.data_ptr(), ld, DTYPES[out.dtype], stream_of(out))
+        rc = lib().exl3_mx4_gemm_in(A.codes.data_ptr(), A.scales.data_ptr(), m, k, B.codes.data_ptr(), B.scales.data_ptr(), n,
+                                    ptr(bias), o2.data_ptr(), ld, DTYPES[out.dtype], ptr(ws), need, stream_of(out))
     if rc:
         check(rc, "mx4_gemm")
     return out
@@ -228,9 +232,12 @@ class MX4Linear:
             raise NotImplementedError("MX4Linear: the weight has values of 2^128 and more, which bf16 does not hold")
         x2, m, ld = _rows(x, k)
         y2, y_ld = _out2("MX4Linear", y, m, n)
+        need = scratch_bytes("exl3_mx4_linear_scratch", m, k, n)
+        ws = scratch(need, x)
         with where:
-            rc = lib().exl3_mx4_linear(x2.data_ptr(), ld, DTYPES[x.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(), n,
-                                       self.scale_base, ptr(self.bias), y2.data_ptr(), y_ld, DTYPES[y.dtype], stream_of(x))
+            rc = lib().exl3_mx4_linear_in(x2.data_ptr(), ld, DTYPES[x.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(), n,
+                                          self.scale_base, ptr(self.bias), y2.data_ptr(), y_ld, DTYPES[y.dtype], ptr(ws), need,
+                                          stream_of(x))
         if rc:
             check(rc, "mx4_linear")
 
@@ -331,11 +338,13 @@ def mx4_moe_forward(x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tenso
         raise NotImplementedError(f"mx4_moe_forward: activation {act!r}")
     topk_ids, topk_w = topk_ids.contiguous(), topk_w.contiguous()
     x2, _, ld = _rows(x, H)
+    k, shared = topk_ids.shape[1], int(shared)
+    need = scratch_bytes("exl3_mx4_moe_scratch", M, H, experts.I, k, experts.E, shared)
+    ws = scratch(need, x)
     with where:
-        rc = lib().exl3_mx4_moe_forward(x2.data_ptr(), ld, DTYPES[x.dtype], M, H, experts.I, topk_ids.data_ptr(),
-                                        topk_w.data_ptr(), topk_ids.shape[1], experts.E, experts.tables.data_ptr(), a,
-                                        float(act_limit), int(shared), o2.data_ptr(), o_ld, DTYPES[out.dtype],
-                                        stream_of(x))
+        rc = lib().exl3_mx4_moe_forward_in(x2.data_ptr(), ld, DTYPES[x.dtype], M, H, experts.I, topk_ids.data_ptr(),
+                                           topk_w.data_ptr(), k, experts.E, experts.tables.data_ptr(), a, float(act_limit), shared,
+                                           o2.data_ptr(), o_ld, DTYPES[out.dtype], ptr(ws), need, stream_of(x))
     if rc:
         check(rc, "mx4_moe_forward")
     return out

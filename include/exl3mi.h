@@ -4,7 +4,8 @@
  * (NULL = the default stream), never synchronises the host (the workspace calls below say where they do), and
  * returns an exl3_status. The caller owns every input and output buffer; outputs are written in place.
  * Library-owned scratch is cached per device (grown on demand; see exl3_reserve_workspace). Calls on one device must
- * be ordered on one stream: they share that device's workspace, and two calls that overlap in time race on it.
+ * be ordered on one stream: they share that device's workspace, and two calls that overlap in time race on it. (The _in
+ * entry points take their scratch from the caller instead.)
  *
  * Data formats (identical to exllamav3 / the reference, ext-op-inventory.md:698-777):
  *   trellis  int16 [k/16][n/16][16*K], K = bits per weight (1..8), one 16x16 tile = 8*K little-endian uint32 words
@@ -334,6 +335,24 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
                          const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
                          int64_t shared, void* out, int64_t out_ld, int out_dtype, void* stream);
 
+/* The same calls with scratch from the caller (256-byte aligned device memory, at least as many bytes as *_scratch says for the
+ * sizes, whatever it holds; NULL for 0 bytes) instead of the device's workspace: calls with scratch of their own may overlap
+ * on several streams and threads and with replays of graphs that captured such calls. *_scratch returns bytes, 0 for sizes that
+ * the call refuses. */
+int64_t exl3_mx4_linear_scratch(int64_t m, int64_t k, int64_t n);
+int exl3_mx4_linear_in(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes,
+                       const uint8_t* scales, int64_t n, int scale_base, const float* bias, void* C, int64_t c_ld,
+                       int c_dtype, void* scratch, int64_t scratch_bytes, void* stream);
+int64_t exl3_mx4_gemm_scratch(int64_t m, int64_t k, int64_t n);
+int exl3_mx4_gemm_in(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, int64_t k, const uint8_t* b_codes,
+                     const uint8_t* b_scales, int64_t n, const float* bias, void* C, int64_t c_ld, int c_dtype, void* scratch,
+                     int64_t scratch_bytes, void* stream);
+int64_t exl3_mx4_moe_scratch(int64_t M, int64_t H, int64_t I, int64_t topk, int64_t E, int64_t shared);
+int exl3_mx4_moe_forward_in(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t H, int64_t I, const int32_t* topk_ids,
+                            const float* topk_w, int64_t topk, int64_t E, const int64_t* tables, int act, float act_limit,
+                            int64_t shared, void* out, int64_t out_ld, int out_dtype, void* scratch, int64_t scratch_bytes,
+                            void* stream);
+
 /* ------------------------------------------------------------------------------------------------ router balance
  * How evenly a router loads its experts, as a loss. Row t has scores s(t, e) of its logits (EXL3_SCORE_SOFTMAX: exp;
  * EXL3_SCORE_SIGMOID: sigmoid; EXL3_SCORE_SQRT_SOFTPLUS) and shares p(t, e) = s(t, e) / sum over e, of logits however
@@ -347,6 +366,12 @@ int exl3_mx4_moe_forward(const void* x, int64_t x_ld, int x_dtype, int64_t M, in
 int exl3_route_balance(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk,
                        const uint8_t* mask, int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows,
                        void* stream);
+
+/* With scratch from the caller, as the _in calls above. */
+int64_t exl3_route_balance_scratch(int64_t M, int64_t E);
+int exl3_route_balance_in(const float* logits, int64_t ld, int64_t M, int64_t E, const int32_t* ids, int64_t topk,
+                          const uint8_t* mask, int score, float coef, float* loss, int32_t* counts, float* prob, int32_t* rows,
+                          void* scratch, int64_t scratch_bytes, void* stream);
 
 /* Gradient of that loss: dlogits[t, j] = grad * d loss / d logits[t, j] (fp32 [M, E], row stride d_ld; zero in rows that are
  * not live), counts and rows as exl3_route_balance wrote them (or summed over several processes) and taken as constants,
