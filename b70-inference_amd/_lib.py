@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import functools
 import os
 
 import torch
@@ -161,14 +160,19 @@ def release_workspace():
 # Scratch of the calls that take it from the caller: torch's allocator gives every call memory of its own until the stream that it
 # runs on is done with it (a graph's calls, the graph's), so they may overlap on any streams and threads. The sizes follow from the
 # shapes alone.
-@functools.lru_cache(maxsize=4096)
-def scratch_bytes(what: str, *sizes: int) -> int:
-    return getattr(lib(), what)(*sizes)
+_scratch = {}
 
 
-def scratch(n: int, like: torch.Tensor):
-    """n bytes on like's device for a call on its current stream; the tensor must live until the call has been made."""
-    return like.new_empty(n, dtype=torch.uint8) if n else None
+def scratch(what: str, like: torch.Tensor, *sizes):
+    """Scratch of the call `what` with these sizes on like's device, for its current stream (None: it needs none), and its bytes. The
+    tensor must live until the call has been made."""
+    key = (what, *sizes)
+    n = _scratch.get(key)
+    if n is None:
+        if len(_scratch) >= 65536:
+            _scratch.clear()
+        n = _scratch[key] = getattr(lib(), what + "_scratch")(*sizes)
+    return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
 _same_device = contextlib.nullcontext()

@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from ._lib import (ACT_GELU_TANH, ACT_SILU, EXL3_F16, EXL3_F32, EXL3_WORDS_PLANAR4, EXL3_WORDS_TILE_ORDER, Exl3Error,
-                   check, lib, on_device, ptr, require_device, scratch, scratch_bytes, stream_of)
+                   check, lib, on_device, ptr, require_device, scratch, stream_of)
 from .linear import BC_LinearEXL3
 from .mx4 import ACTS, MX4Experts, mx4_moe_forward
 
@@ -431,8 +431,7 @@ def route_balance(logits: torch.Tensor, topk_ids: torch.Tensor, score: str = "so
     topk_ids = topk_ids.contiguous()
     loss, prob = logits.new_empty(1), logits.new_empty(E)
     counts, rows = topk_ids.new_empty(E), topk_ids.new_empty(1)
-    need = scratch_bytes("exl3_route_balance_scratch", M, E)
-    ws = scratch(need, logits)
+    ws, need = scratch("exl3_route_balance", logits, M, E)
     with where:
         rc = lib().exl3_route_balance_in(logits.data_ptr(), ld, M, E, topk_ids.data_ptr(), topk_ids.shape[1], ptr(mask),
                                          SCORES[score], float(coef), loss.data_ptr(), counts.data_ptr(), prob.data_ptr(),

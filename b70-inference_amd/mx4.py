@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import ACT_GELU_TANH, ACT_SILU, EXL3_BF16, EXL3_F16, EXL3_F32, Exl3Error, check, lib, on_device, ptr, scratch, \
-    scratch_bytes, stream_of
+    stream_of
 
 ACTS = {"silu": ACT_SILU, "gelu_tanh": ACT_GELU_TANH, ACT_SILU: ACT_SILU, ACT_GELU_TANH: ACT_GELU_TANH}
 DTYPES = {torch.float16: EXL3_F16, torch.float32: EXL3_F32, torch.bfloat16: EXL3_BF16}
@@ -159,21 +159,23 @@ def _bias(what: str, bias, n: int):
 def mx4_gemm(A: MX4Tensor, B: MX4Tensor, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
              out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """A [..., k] @ B^T (+ bias [n]) for B [n, k], both MX4: [..., n] with fp32 sums, one rounding."""
-    if len(B.shape) != 2 or A.k != B.k:
+    k = A.k
+    if B.scales.dim() != 2 or B.k != k:
         raise Exl3Error(f"mx4_gemm: A {tuple(A.shape)} and B {tuple(B.shape)} must share k, B [n, k]")
-    n, k = B.shape
-    bias = _bias("mx4_gemm", bias, n)
+    n, m = B.scales.shape[0], A.scales.numel() * 32 // k
+    bias = None if bias is None else _bias("mx4_gemm", bias, n)
     if out is None:
         if out_dtype not in DTYPES:
             raise Exl3Error(f"mx4_gemm: out_dtype fp16, bf16 or fp32, got {out_dtype}")
-        out = A.codes.new_empty(A.codes.shape[:-1] + (n,), dtype=out_dtype)
-    where = on_device("mx4_gemm", A.codes, A.scales, B.codes, B.scales, bias, out)
-    m = A.scales.numel() * 32 // k
-    o2, ld = _out2("mx4_gemm", out, m, n)
+        out = o2 = A.codes.new_empty(A.codes.shape[:-1] + (n,), dtype=out_dtype)
+        ld = n
+        where = on_device("mx4_gemm", A.codes, A.scales, B.codes, B.scales, bias)
+    else:
+        where = on_device("mx4_gemm", A.codes, A.scales, B.codes, B.scales, bias, out)
+        o2, ld = _out2("mx4_gemm", out, m, n)
     if n == 0:
         return out
-    need = scratch_bytes("exl3_mx4_gemm_scratch", m, k, n)
-    ws = scratch(need, out)
+    ws, need = scratch("exl3_mx4_gemm", out, m, k, n)
     with where:
         rc = lib().exl3_mx4_gemm_in(A.codes.data_ptr(), A.scales.data_ptr(), m, k, B.codes.data_ptr(), B.scales.data_ptr(), n,
                                     ptr(bias), o2.data_ptr(), ld, DTYPES[out.dtype], ptr(ws), need, stream_of(out))
@@ -232,8 +234,7 @@ class MX4Linear:
             raise NotImplementedError("MX4Linear: the weight has values of 2^128 and more, which bf16 does not hold")
         x2, m, ld = _rows(x, k)
         y2, y_ld = _out2("MX4Linear", y, m, n)
-        need = scratch_bytes("exl3_mx4_linear_scratch", m, k, n)
-        ws = scratch(need, x)
+        ws, need = scratch("exl3_mx4_linear", x, m, k, n)
         with where:
             rc = lib().exl3_mx4_linear_in(x2.data_ptr(), ld, DTYPES[x.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(), n,
                                           self.scale_base, ptr(self.bias), y2.data_ptr(), y_ld, DTYPES[y.dtype], ptr(ws), need,
@@ -330,17 +331,19 @@ def mx4_moe_forward(x: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tenso
     if out is None:
         if out_dtype not in DTYPES:
             raise Exl3Error(f"mx4_moe_forward: out_dtype fp16, bf16 or fp32, got {out_dtype}")
-        out = x.new_empty((M, H), dtype=out_dtype)
-    where = on_device("mx4_moe_forward", x, topk_ids, topk_w, experts.tables, out)
-    o2, o_ld = _out2("mx4_moe_forward", out, M, H)
+        out = o2 = x.new_empty((M, H), dtype=out_dtype)
+        o_ld = H
+        where = on_device("mx4_moe_forward", x, topk_ids, topk_w, experts.tables)
+    else:
+        where = on_device("mx4_moe_forward", x, topk_ids, topk_w, experts.tables, out)
+        o2, o_ld = _out2("mx4_moe_forward", out, M, H)
     a = ACTS.get(act)
     if a is None:
         raise NotImplementedError(f"mx4_moe_forward: activation {act!r}")
     topk_ids, topk_w = topk_ids.contiguous(), topk_w.contiguous()
     x2, _, ld = _rows(x, H)
     k, shared = topk_ids.shape[1], int(shared)
-    need = scratch_bytes("exl3_mx4_moe_scratch", M, H, experts.I, k, experts.E, shared)
-    ws = scratch(need, x)
+    ws, need = scratch("exl3_mx4_moe", x, M, H, experts.I, k, experts.E, shared)
     with where:
         rc = lib().exl3_mx4_moe_forward_in(x2.data_ptr(), ld, DTYPES[x.dtype], M, H, experts.I, topk_ids.data_ptr(),
                                            topk_w.data_ptr(), k, experts.E, experts.tables.data_ptr(), a, float(act_limit), shared,
