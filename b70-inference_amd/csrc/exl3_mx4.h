@@ -22,6 +22,9 @@ typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef int i8_t __attribute__((ext_vector_type(8)));
 
+// Workgroups of 256 threads that one launch can have: a dimension of the grid has fewer than 2^32 threads.
+constexpr int64_t kMx4Grid = (1 << 24) - 1;
+
 // Type of the rows that a product takes: 16-bit values, or MX4 codes and scales.
 enum { kRowF16 = 0, kRowBF16 = 1, kRowMX4 = 2 };
 

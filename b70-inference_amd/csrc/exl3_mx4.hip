@@ -142,6 +142,24 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
     }
 }
 
+// Units and workgroups of a row, and the rows of a launch. Rows without gaps are one, as long as a launch can hold it.
+struct QuantGrid {
+    int64_t rows, upr, cpr, most;
+};
+static bool quant_grid(int64_t rows, int64_t k, int64_t ld, QuantGrid& g) {
+    constexpr int64_t kWg = 256 * kQuantUnits;
+    if (ld == k && (rows * (k / 8) + kWg - 1) / kWg <= kMx4Grid) {
+        k *= rows;
+        rows = 1;
+    }
+    g.rows = rows;
+    g.upr = k / 8;
+    g.cpr = (g.upr + kWg - 1) / kWg;
+    if (g.cpr > kMx4Grid) return false;
+    g.most = kMx4Grid / g.cpr;
+    return true;
+}
+
 // ================================================================================================ dense products
 struct Mx4Args {
     const uint8_t* x;                  // rows: 16-bit values, or MX4 codes
@@ -267,7 +285,7 @@ static int mx4_split(const char* what, Mx4Args& a, const Mx4Plan& plan, const Ca
 static int launch_reduce(const Mx4Args& a, hipStream_t st) {
     if (a.splits == 1) return EXL3_OK;
     const int64_t wgs = (a.m * (a.n4 / 4) + 255) / 256;
-    EXL3_CHECK_ARG(wgs <= 0x7FFFFFFF, "mx4: grid too large");
+    EXL3_CHECK_ARG(wgs <= kMx4Grid, "mx4: grid too large");
     EXL3_LAUNCH("mx4_reduce", mx4_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a);
     return EXL3_OK;
 }
@@ -306,7 +324,7 @@ __global__ __launch_bounds__(256) void mx4_tiny_kernel(Mx4Args a) {
 
 template <int XT>
 static int launch_tiny(const char* name, const Mx4Args& a, hipStream_t st) {
-    EXL3_CHECK_ARG(a.m <= (int64_t)0x7FFFFFFF * 256 / a.n - 256, "%s: grid too large", name);
+    EXL3_CHECK_ARG(a.m <= kMx4Grid * 256 / a.n, "%s: grid too large", name);
     EXL3_LAUNCH(name, mx4_tiny_kernel<XT>, dim3((unsigned)((a.m * a.n + 255) / 256)), dim3(256), 0, st, a);
     return EXL3_OK;
 }
@@ -415,9 +433,9 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_wide_kernel(Mx4Args
 template <int XT, int RG>
 static int launch_wide(Mx4Args a, const Mx4Plan& plan, const CallScratch& s, hipStream_t st) {
     const int64_t tiles = (a.m + 32 * RG - 1) / (32 * RG) * ((a.n + 255) / 256);
+    EXL3_CHECK_ARG(tiles * plan.P <= kMx4Grid - 7, "exl3_mx4_linear: grid too large");
     const int rc = mx4_split("exl3_mx4_linear", a, plan, s, st);
     if (rc) return rc;
-    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0 / a.splits, "exl3_mx4_linear: grid too large");
     EXL3_LAUNCH("mx4_linear_wide", (mx4_wide_kernel<XT, RG>), dim3((unsigned)((tiles * a.splits + 7) & ~7)), dim3(256), 0, st, a);
     return launch_reduce(a, st);
 }
@@ -576,9 +594,9 @@ template <int TM, int TN, int WM, int WN, int OCC>
 static int launch_tile(Mx4Args a, const Mx4Plan& plan, const CallScratch& s, hipStream_t st) {
     typedef Mx4Tile<TM, TN, WM, WN> T;
     const int64_t tiles = (a.m + T::BM - 1) / T::BM * ((a.n + T::BN - 1) / T::BN);
+    EXL3_CHECK_ARG(tiles * plan.P <= kMx4Grid * 256 / T::kThreads - 7, "exl3_mx4_gemm: grid too large");
     const int rc = mx4_split("exl3_mx4_gemm", a, plan, s, st);
     if (rc) return rc;
-    EXL3_CHECK_ARG(tiles <= 0x7FFFFFF0 / a.splits, "exl3_mx4_gemm: grid too large");
     EXL3_LAUNCH("mx4_gemm_tile", (mx4_tile_kernel<TM, TN, WM, WN, OCC>), dim3((unsigned)((tiles * a.splits + 7) & ~7)),
                 dim3(T::kThreads), 0, st, a);
     return launch_reduce(a, st);
@@ -671,16 +689,17 @@ int exl3_mx4_quantize(const void* x, int64_t x_ld, int64_t rows, int64_t k, int 
     EXL3_CHECK_ARG(aligned(x, 16) && (rows == 1 || x_ld * elem_size(x_dtype) % 16 == 0) && aligned(codes, 4),
                    "exl3_mx4_quantize: rows must be 16-byte aligned and codes 4-byte");
     EXL3_CHECK_ARG(rows <= ((int64_t)1 << 45) / x_ld, "exl3_mx4_quantize: too large");
-    if (x_ld == k) {                                           // one row of all values
-        k *= rows;
-        rows = 1;
-    }
-    const int64_t upr = k / 8, cpr = (upr + 256 * kQuantUnits - 1) / (256 * kQuantUnits);
-    EXL3_CHECK_ARG(cpr <= 0x7FFFFFFF / rows, "exl3_mx4_quantize: too large");
+    const int elem = elem_size(x_dtype);
     const auto fn = x_dtype == EXL3_F16 ? mx4_quantize_kernel<EXL3_F16>
                   : x_dtype == EXL3_BF16 ? mx4_quantize_kernel<EXL3_BF16> : mx4_quantize_kernel<EXL3_F32>;
-    EXL3_LAUNCH("mx4_quantize", fn, dim3((unsigned)(rows * cpr)), dim3(256), 0, (hipStream_t)stream, x, x_ld, upr, (int)cpr,
-                reinterpret_cast<uint32_t*>(codes), scales);
+    QuantGrid g;
+    if (!quant_grid(rows, k, x_ld, g)) return fail(EXL3_ERR_INVALID, "exl3_mx4_quantize: too large");
+    for (int64_t r = 0; r < g.rows; r += g.most) {
+        const int64_t n = g.rows - r < g.most ? g.rows - r : g.most;
+        EXL3_LAUNCH("mx4_quantize", fn, dim3((unsigned)(n * g.cpr)), dim3(256), 0, (hipStream_t)stream,
+                    reinterpret_cast<const char*>(x) + r * x_ld * elem, x_ld, g.upr, (int)g.cpr,
+                    reinterpret_cast<uint32_t*>(codes) + r * g.upr, scales + r * (g.upr / 4));
+    }
     return EXL3_OK;
 }
 
@@ -694,16 +713,17 @@ int exl3_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t row
     EXL3_CHECK_ARG(aligned(out, 16) && (rows == 1 || out_ld * elem_size(out_dtype) % 16 == 0) && aligned(codes, 4),
                    "exl3_mx4_dequantize: rows must be 16-byte aligned and codes 4-byte");
     EXL3_CHECK_ARG(rows <= ((int64_t)1 << 45) / out_ld, "exl3_mx4_dequantize: too large");
-    if (out_ld == k) {
-        k *= rows;
-        rows = 1;
-    }
-    const int64_t upr = k / 8, cpr = (upr + 256 * kQuantUnits - 1) / (256 * kQuantUnits);
-    EXL3_CHECK_ARG(cpr <= 0x7FFFFFFF / rows, "exl3_mx4_dequantize: too large");
+    const int elem = elem_size(out_dtype);
     const auto fn = out_dtype == EXL3_F16 ? mx4_dequantize_kernel<EXL3_F16>
                   : out_dtype == EXL3_BF16 ? mx4_dequantize_kernel<EXL3_BF16> : mx4_dequantize_kernel<EXL3_F32>;
-    EXL3_LAUNCH("mx4_dequantize", fn, dim3((unsigned)(rows * cpr)), dim3(256), 0, (hipStream_t)stream,
-                reinterpret_cast<const uint32_t*>(codes), scales, upr, (int)cpr, out, out_ld);
+    QuantGrid g;
+    if (!quant_grid(rows, k, out_ld, g)) return fail(EXL3_ERR_INVALID, "exl3_mx4_dequantize: too large");
+    for (int64_t r = 0; r < g.rows; r += g.most) {
+        const int64_t n = g.rows - r < g.most ? g.rows - r : g.most;
+        EXL3_LAUNCH("mx4_dequantize", fn, dim3((unsigned)(n * g.cpr)), dim3(256), 0, (hipStream_t)stream,
+                    reinterpret_cast<const uint32_t*>(codes) + r * g.upr, scales + r * (g.upr / 4), g.upr, (int)g.cpr,
+                    reinterpret_cast<char*>(out) + r * out_ld * elem, out_ld);
+    }
     return EXL3_OK;
 }
 

@@ -364,9 +364,9 @@ __global__ __launch_bounds__(256, mx4_wide_occ(RG)) void mx4_down_wide_kernel(Mx
         });
 }
 
-// out[t] = sum of token t's y rows in slot order, four columns per thread.
-__global__ __launch_bounds__(256) void mx4_combine_kernel(Mx4MoeArgs a, int ncb, int vec) {
-    const int t = blockIdx.x / (unsigned)ncb, c = 4 * ((blockIdx.x % (unsigned)ncb) * 256 + threadIdx.x);
+// out[t] = sum of token t's y rows in slot order, four columns per thread; tokens from `first` on.
+__global__ __launch_bounds__(256) void mx4_combine_kernel(Mx4MoeArgs a, int first, int ncb, int vec) {
+    const int t = first + (int)(blockIdx.x / (unsigned)ncb), c = 4 * ((blockIdx.x % (unsigned)ncb) * 256 + threadIdx.x);
     if (c >= a.H) return;
     f4_t v = {};
     const int* po = a.pair_of + (int64_t)t * a.slots;
@@ -494,7 +494,8 @@ static int mx4_moe(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t 
     a.out_dtype = out_dtype;
     const int rows = sh.rows;
     a.max_blocks = (int)sh.max_blocks;
-    EXL3_CHECK_ARG((int64_t)a.max_blocks * ((H > I ? H : I) / 16) <= 0x7FFFFFFF, "exl3_mx4_moe_forward: grid too large");
+    const int64_t nci = (I + 127) / 128, nch = (H + 255) / 256;
+    EXL3_CHECK_ARG(a.max_blocks * (nci > nch ? nci : nch) <= kMx4Grid, "exl3_mx4_moe_forward: grid too large");
     ItemDesc* blocks = nullptr;
     int* pairs = nullptr;
     if (npairs > 0) {
@@ -538,8 +539,10 @@ static int mx4_moe(const void* x, int64_t x_ld, int x_dtype, int64_t M, int64_t 
         if (rc2) return rc2;
     }
     const int64_t ncb = (H + 1023) / 1024;
-    EXL3_CHECK_ARG(M * ncb <= 0x7FFFFFFF, "exl3_mx4_moe_forward: grid too large");
-    EXL3_LAUNCH("mx4_moe_combine", mx4_combine_kernel, dim3((unsigned)(M * ncb)), dim3(256), 0, st, a, (int)ncb, vec);
+    for (int64_t t = 0; t < M; t += kMx4Grid / ncb) {
+        const int64_t n = M - t < kMx4Grid / ncb ? M - t : kMx4Grid / ncb;
+        EXL3_LAUNCH("mx4_moe_combine", mx4_combine_kernel, dim3((unsigned)(n * ncb)), dim3(256), 0, st, a, (int)t, (int)ncb, vec);
+    }
     return EXL3_OK;
 }
 
