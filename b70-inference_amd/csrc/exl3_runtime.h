@@ -114,8 +114,14 @@ struct ProfEvents {
 ProfEvents prof_begin(const char* name);
 int prof_repeat();
 
+// HIP takes a grid of 2^32 threads or more in a dimension without an error and runs a part of it.
+inline bool grid_fits(dim3 grid, dim3 block) {
+    return (uint64_t)grid.x * block.x >> 32 == 0 && (uint64_t)grid.y * block.y >> 32 == 0 && (uint64_t)grid.z * block.z >> 32 == 0;
+}
+
 #define EXL3_LAUNCH(name, kernel, grid, block, lds, stream, ...)                                          \
     do {                                                                                                \
+        EXL3_CHECK_ARG(::exl3::grid_fits(grid, block), "%s: grid too large", name);                     \
         const ::exl3::ProfEvents pe_ = ::exl3::prof_begin(name);                                        \
         if (pe_.a) {                                                                                    \
             const int reps_ = ::exl3::prof_repeat();                                                    \

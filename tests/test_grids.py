@@ -26,6 +26,15 @@ def test_refused_before_a_launch(exl3):
     assert b"grid" in L.exl3_last_error()
 
 
+def test_other_calls_are_refused_too(exl3):
+    """2^32 threads of an activation, a workgroup of 64 for each of 2^27 rows of logits."""
+    L = exl3.lib()
+    for n in (1 << 32, (1 << 32) - 255):
+        assert L.exl3_act_mul(P, P, P, n, 0, 0, F(0.0), None) == 1
+    assert b"grid" in L.exl3_last_error()
+    assert L.exl3_route_topk(P, 8, 1 << 27, 8, None, 2, 0, 1, F(1.0), P, P, None) == 1
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_more_rows_than_a_launch_has_workgroups(exl3, dtype):
