@@ -21,7 +21,7 @@ import torch
 from ._lib import (ACT_GELU_TANH, ACT_SILU, EXL3_F16, EXL3_F32, EXL3_WORDS_PLANAR4, EXL3_WORDS_TILE_ORDER, Exl3Error,
                    check, lib, on_device, ptr, require_device, scratch, stream_of)
 from .linear import BC_LinearEXL3
-from .mx4 import ACTS, MX4Experts, mx4_moe_forward
+from .mx4 import ACTS, MX4Experts, MX4Linear, mx4_moe_forward
 
 
 class MixedEXL3:
@@ -56,6 +56,8 @@ class MixedEXL3:
 
 
 def _proj_K(p) -> int:
+    if isinstance(p, MX4Linear):
+        raise NotImplementedError("ExpertTables: EXL3 projections expected; MX4 ones go into MX4Experts")
     return 0 if isinstance(p, MixedEXL3) else p.Ki
 
 
@@ -590,7 +592,8 @@ class BlockSparseMLP:
     "he", the reference's gate_tensor) or [E, H] ("eh"), optionally rounded to fp16 like a half matmul. Scoring:
     "softmax" (default; the bias ranks and, unless bias_select_only, shifts the softmax), "sigmoid" or
     "sqrt_softplus" (rank by score + bias, weights from the score), renormalised (+1e-20) and scaled by
-    routed_scaling. `experts` may be MX4Experts: bf16 rows then reach the experts as they are (the router takes fp16)."""
+    routed_scaling. `experts` may be MX4Experts: bf16 rows then reach the experts as they are. The router takes fp16: rows with
+    values of 65520 and more need params["router_logits"]."""
 
     def __init__(self, experts: ExpertTables, num_experts_per_tok: int, has_shared: bool = False, act="silu",
                  act_limit: float = 0.0, router_weight: torch.Tensor | None = None,

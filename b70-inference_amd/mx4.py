@@ -4,8 +4,8 @@
 bits and one mantissa bit (0, .5, 1, 1.5, 2, 3, 4, 6), two to a byte, the even one in the low half: 4.25 bits per weight.
 
   * mx4_quantize(x) / mx4_dequantize(t, dtype)     rows of fp16, bf16 or fp32 to MX4Tensor and back
-  * MX4Linear(weight, bias): run(x, y) / run_alloc  y = x @ W^T (+ bias), 16-bit rows, weights exact in the rows' type (the
-    interface of BC_LinearEXL3)
+  * MX4Linear(weight, bias): run(x, y) / run_alloc  y = x @ W^T (+ bias), 16-bit rows, weights exact in the rows' type (run
+    and run_alloc as BC_LinearEXL3's; as a projection it belongs into MX4Experts, not into ExpertTables or BC_GatedMLP)
   * mx4_gemm(A, B)                                  A @ B^T of two MX4Tensors on the scaled matrix instructions
   * MX4Experts, mx4_moe_forward(x, ids, w, experts) the routed layer of moe_forward over MX4 experts (BlockSparseMLP takes
     MX4Experts too)
@@ -208,7 +208,7 @@ class MX4Linear:
     """y = x @ W^T (+ bias) with W [n, k] in MX4 and 16-bit rows x. The weights are exact in the rows' type; fp16 rows need
     the matrix's scales (of blocks that are not all zeros) to span at most 2^36: MX4Linear finds the power of two to take
     out once, here, and refuses fp16 rows of a wider matrix (bf16 rows take any) and bf16 rows of one with values of 2^128 and
-    more."""
+    more. A weight that is changed afterwards needs an MX4Linear of its own."""
 
     bf16_rows = True
 
@@ -252,7 +252,8 @@ class MX4Linear:
 class MX4Experts:
     """Device table of E experts with MX4 weights: int64 [9, E] = (codes address, scales address, scale base) of gate [I, H],
     up [I, H] and down [H, I]. Holds references to every tensor that it points at. Lists of MX4Tensor or MX4Linear (without
-    biases), one per expert; MX4Experts.stacked takes one MX4Tensor [E, rows, k] per projection."""
+    biases), one per expert; MX4Experts.stacked takes one MX4Tensor [E, rows, k] per projection. Weights that are changed afterwards need
+    a table of their own."""
 
     def __init__(self, gates, ups, downs):
         if not (len(gates) == len(ups) == len(downs)) or not gates:
