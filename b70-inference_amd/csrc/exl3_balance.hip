@@ -5,8 +5,9 @@
 //     sigmoid        d/dl_j = p_j (1 - s_j) (a_j - abar)                   (ds/dl = s (1 - s))
 //     sqrt-softplus  d/dl_j = p_j sigma(l_j) / (2 softplus(l_j)) (a_j - abar)   (ds/dl = sigma / (2 s))
 // A wave takes a row (E <= 2048; above, the four waves of a workgroup share one) and holds it in registers, so each pass
-// reads the logits once; both passes are bound by those bytes (32768 padded rows of 512: forward 17.3 us and 6.9 for the
-// partials, gradient 21.0), a decode step's few rows by launch latency.
+// reads the logits once. 32768 padded rows of 512, half of them live: gradient 21.0 us, near its bytes (101 MB); forward 17.3 for 34
+// MB, a wait for memory per live row, since its picks arrive behind the next row's logits, and 6.9 for the partials. A decode
+// step's few rows are bound by launch latency.
 #include "exl3_device.h"
 #include "exl3_runtime.h"
 

@@ -330,8 +330,8 @@ static int launch_tiny(const char* name, const Mx4Args& a, hipStream_t st) {
 }
 
 // Up to 16 rows, x in LDS. A workgroup takes every gridDim-th tile of 16 outputs, so x is staged once per resident workgroup.
-// Six rows of 5376 -> 21504 18.4 us replayed (62 MB: 3.4 TB/s; the same with 6, 8 or 10 waves, so the memory's rate behind the
-// launch and the first loads), one of 4096 -> 4096 4.7 (a chain of the first load, the sum and the store).
+// Six rows of 5376 -> 21504 17.5 us among eager calls, 18.4 as a graph's node (62 MB: 3.5 and 3.4 TB/s; the same with 6, 8 or 10
+// waves), one of 4096 -> 4096 4.8 as a graph's node (a chain of the first load, the sum and the store).
 template <int XT>
 __global__ __launch_bounds__(1024) void mx4_decode_kernel(Mx4Args a, int xbytes) {
     extern __shared__ f4_t red[];
@@ -456,11 +456,11 @@ static int linear_run(const Mx4Args& a, const CallScratch& s, hipStream_t st) {
 // the other is multiplied, two steps' loads under way (one: 205 us instead of 183); the scales of four steps (16 bytes per row)
 // likewise. Lane l of a fragment takes blocks
 // 2 (l >> 5) and 2 (l >> 5) + 1 of its row's four, one per MFMA, so that both scales are neighbouring bytes of one word.
-// In LDS a row's four 16-byte units are permuted by its row number: eight lanes reading eight rows, or writing two, touch
-// every bank once.
-// 2048 rows of 5376 -> 21504 (256 x 256) 165 us, 2.9 PFLOP/s: a step takes 2500 cycles for 1024 of MFMAs; the LDS is busy for
-// 1500, mostly with the stores of the staged codes, and the barrier keeps the waves in step, so that little of either hides
-// behind the other; and 672 tiles take three rounds of the CUs for 2.6 rounds' work.
+// In LDS a row's four 16-byte units are permuted by its row number, so that eight neighbouring lanes reading eight rows, or writing
+// two, touch every bank once (the counters show conflicts for a third of the LDS cycles nevertheless).
+// 2048 rows of 5376 -> 21504 (256 x 256) 165 us, 2.9 PFLOP/s: a step takes 2500 cycles for 1024 of MFMAs and 1050 to 1400 of LDS (42 %,
+// 56 % with the conflicts); the barrier keeps the waves in step, so that little of either hides behind the other; and 672 tiles
+// take three rounds of the CUs for 2.6 rounds' work.
 template <int TM, int TN, int WM, int WN>
 struct Mx4Tile {
     static constexpr int kThreads = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, R = BM + BN;

@@ -174,7 +174,7 @@ __device__ __forceinline__ f4_t mx4_decode_sum(const f4_t* red, int waves, int i
     return s;
 }
 
-// Waves for `groups` groups of work: as few rounds as 16 waves take, with as few waves as do them.
+// Waves for `groups` groups of work: as few rounds as `most` waves take, with as few waves as do them.
 inline int mx4_decode_waves(int groups, int most) {
     const int rounds = (groups + most - 1) / most;
     return rounds > 0 ? (groups + rounds - 1) / rounds : 1;

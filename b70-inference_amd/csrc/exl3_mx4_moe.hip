@@ -5,15 +5,15 @@
 //            (the down product's operand: one of more bits, in two parts, would double its MFMAs, its LDS and its reads of rows;
 //            this rounding adds to the output's: 1.4 times the error of a 16-bit output, and an fp32 output has no more than
 //            x's type's 8 or 11 bits of the middle). fp16 does not hold every magnitude that a product of two sums has, so fp16
-//            middles carry a power of two per workgroup's columns (mid_exponent in exl3_mx4.h; all of it costs one token, top-10 of 512
-//            experts 2048 -> 512, 0.3 of 13.5 us, and 1024 of them 2 of 422)
+//            middles carry a power of two per workgroup's columns (mid_exponent in exl3_mx4.h: 0.3 us of the one token's time
+//            below, 3 of the 1024 tokens')
 //   down     workgroup per (block, 256 columns of H) over I: y[pair] = routing weight * sum, fp32
 //   combine  out[t] = sum of the token's y rows in slot order
 // Few pairs take two launches instead: gateup per (pair, 16 columns of I), down per (token, 16 columns of H) over all of the
 // token's slots.
-// Bound by the weights' bytes: 1024 tokens, top-10 of 512 experts 2560 -> 640, 421 us for 1.35 GB (align 31, gateup 239, down 135,
-// combine 18); 260 tokens, top-2 of 32 experts 7168 -> 2048 and a shared one, 253 us for 0.78 GB (14, 158, 89, 6); one token,
-// top-10 of 512 experts 2048 -> 512, 12.0 us replayed for 17 MB, two chains of load, sum and store.
+// Bound by the weights' bytes: 1024 tokens, top-10 of 512 experts 2560 -> 640, 421 us for 1.35 GB (align 31, gateup 239, down 138,
+// combine 18); 260 tokens, top-2 of 32 experts 7168 -> 2048 and a shared one, 256 us for 0.78 GB (14, 158, 89, 6); one token,
+// top-10 of 512 experts 2048 -> 512, 12.3 us replayed for 17 MB, two chains of load, sum and store.
 #include "exl3_moe.h"
 #include "exl3_moe_dev.h"
 #include "exl3_mx4.h"

@@ -2,7 +2,7 @@
 // per wave, in steps of 128 k (four blocks). Bound by the MFMAs at 128 rows (RG 4: 2048 cycles of them per wave and step
 // against 64 conversions and 32 LDS reads), by the weights' bytes at 32. 1021 rows of 5376 -> 21504 (RG 4) 238 us, 0.99
 // PFLOP/s, MFMAs busy 55 % of the time (672 tiles over 512 slots are half of what is missing); 512 experts of 2560 -> 640
-// with 20 rows each (RG 1) gate and up 239 us, 3.7 TB/s of weights, down 135 us, 3.3 beside 0.8 of outputs.
+// with 20 rows each (RG 1) gate and up 239 us, 3.7 TB/s of weights, down 138 us, 3.2 beside 0.8 of outputs.
 //
 // x goes through one of two LDS buffers, staged through registers while the step before is multiplied. Weights are read
 // straight into the lanes that convert them, each by one wave of the workgroup only; every word of a block, converted with
@@ -119,7 +119,7 @@ struct Mx4Wide {
     }
 
     // unit u (eight k) of row r of a buffer; the row number permutes its sixteen units, so that eight lanes reading eight
-    // rows or writing half of one touch every bank once
+    // rows or writing half of one touch every bank once (with RG 1 the counters show conflicts for a third of the LDS cycles)
     __device__ __forceinline__ static int unit(int r, int u) { return r * 16 + (u ^ (r & 15)); }
 
     // blocks 2 h and 2 h + 1 of step c
