@@ -109,3 +109,23 @@ def test_moe_wide_blocks_of_long_rows(exl3, dtype, M, H, I, E, k):
     ref, err = reference(x.double().numpy(), ids, w, gv, uv, dv, "silu", U.HALF_STEP[dtype], 0 if dtype == torch.bfloat16 else 128)
     y = exl3.mx4_moe_forward(x.to(DEV), torch.from_numpy(ids).to(DEV), torch.from_numpy(w).to(DEV), ex)
     U.check(y, ref, 0.0, H, torch.float32, extra=err)
+
+
+@pytest.mark.parametrize("M,H,I,E,k", [(2, 64, 8224, 2, 1), (3, 32, 8736, 3, 1), (100, 96, 1120, 4, 2), (90, 64, 1312, 8, 2), (260, 64, 2208, 2, 1)])
+def test_moe_middle_whose_groups_change(exl3, M, H, I, E, k):
+    """Pairs: a wave takes two groups of 512 columns of a row, each smaller, larger or like the other; blocks: more steps than lanes
+    that share a row."""
+    def by(b):
+        g = b // 16 if M < 10 else b // 4
+        return (0, 14, -14)[(g % 9) % 3 if g < 9 else (g % 9) // 3]
+
+    g, gv = shifted(exl3, (E, I, H), 7, lambda b: 0, 1)
+    u, uv = shifted(exl3, (E, I, H), 8, by, 1)
+    d, dv = shifted(exl3, (E, H, I), 9, lambda b: -by(b), 2)
+    ex = exl3.MX4Experts.stacked(g, u, d)
+    assert ex.fp16_rows
+    x = rows((M, H), torch.float16, M, 0.3)
+    ids, w = routing(M, k, E, M)
+    ref, err = reference(x.double().numpy(), ids, w, gv, uv, dv, "silu", U.HALF_STEP[torch.float16], 16 if M < 10 else 128)
+    y = exl3.mx4_moe_forward(x.to(DEV), torch.from_numpy(ids).to(DEV), torch.from_numpy(w).to(DEV), ex)
+    U.check(y, ref, 0.0, H, torch.float32, extra=err)
