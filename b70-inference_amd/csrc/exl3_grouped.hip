@@ -1,0 +1,116 @@
+// Products grouped by expert with 16-bit weights and their gradients: entry points, and the products whose weights lie along the
+// contraction.
+#include "exl3_grouped_tile.h"
+
+namespace exl3 {
+
+int grouped_rows_along(const GroupedArgs& g, int dtype, int tile, hipStream_t st) {
+    return dtype == EXL3_F16 ? launch_grouped_rows<kRowF16, false>(g, tile, st) : launch_grouped_rows<kRowBF16, false>(g, tile, st);
+}
+
+static int out_size(int t) { return t == EXL3_F32 ? 4 : 2; }
+static bool out_type(int t) { return t == EXL3_F16 || t == EXL3_F32 || t == EXL3_BF16; }
+
+constexpr int64_t kMostRows = 0x3FFFFFFF, kMostWidth = 1 << 22;
+
+// What the products and the weights' gradient check alike.
+static int grouped_setup(const char* what, int dtype, int64_t T, int64_t n, int64_t k, const int32_t* ends, int64_t E, int out_dtype) {
+    EXL3_CHECK_ARG(T >= 0 && T <= kMostRows && n > 0 && n <= kMostWidth && k > 0 && k <= kMostWidth && E > 0 && E <= 65536,
+                   "%s: bad sizes (%lld rows, %lld and %lld columns, %lld experts)", what, (long long)T, (long long)n, (long long)k,
+                   (long long)E);
+    EXL3_CHECK_ARG(dtype == EXL3_F16 || dtype == EXL3_BF16, "%s: rows and weights must be fp16 or bf16", what);
+    EXL3_CHECK_ARG(out_type(out_dtype), "%s: the output must be fp16, bf16 or fp32", what);
+    EXL3_CHECK_ARG(ends && aligned(ends, 4), "%s: ends must be a 4-byte aligned pointer", what);
+    return EXL3_OK;
+}
+
+static bool units16(const void* p, int64_t ld, int64_t cols) { return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0; }
+
+static bool vec_out(const void* p, int dtype, int64_t ld, int64_t n) {
+    return aligned(p, 16) && n % 8 == 0 && ld * out_size(dtype) % 16 == 0;
+}
+
+}  // namespace exl3
+
+extern "C" {
+
+using namespace exl3;
+
+int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k, const void* w, int64_t w_ld, int64_t w_es,
+                    int w_layout, int64_t n, const int32_t* ends, int64_t E, void* out, int64_t out_ld, int out_dtype, int rest,
+                    void* stream) {
+    const char* what = "exl3_grouped_mm";
+    const int rc = grouped_setup(what, dtype, T, n, k, ends, E, out_dtype);
+    if (rc) return rc;
+    EXL3_CHECK_ARG(w_layout == EXL3_GROUPED_W_NK || w_layout == EXL3_GROUPED_W_KN, "%s: weight layout %d", what, w_layout);
+    EXL3_CHECK_ARG(rest == 0 || rest == 1, "%s: rest %d", what, rest);
+    const bool across = w_layout == EXL3_GROUPED_W_KN;
+    EXL3_CHECK_ARG(w_ld >= (across ? n : k) && w_ld <= kMostWidth && w_es >= 0 && (T <= 1 || (x_ld >= k && out_ld >= n)) &&
+                       x_ld <= kMostWidth && out_ld <= ((int64_t)1 << 40),
+                   "%s: bad strides (rows %lld, weights %lld and %lld, output %lld)", what, (long long)x_ld, (long long)w_ld,
+                   (long long)w_es, (long long)out_ld);
+    if (T == 0) return EXL3_OK;
+    EXL3_CHECK_ARG(x && w && out && aligned(x, 2) && aligned(w, 2) && aligned(out, out_size(out_dtype)),
+                   "%s: null or misaligned pointer", what);
+    GroupedArgs g{};
+    g.a = reinterpret_cast<const uint16_t*>(x);
+    g.b = reinterpret_cast<const uint16_t*>(w);
+    g.out = out;
+    g.a_ld = T == 1 ? k : x_ld;
+    g.b_ld = w_ld;
+    g.b_es = w_es;
+    g.out_ld = T == 1 ? n : out_ld;
+    g.ends = ends;
+    g.E = (int)E;
+    g.T = (int)T;
+    g.c = (int)k;
+    g.n = (int)n;
+    g.out_dtype = out_dtype;
+    g.vec = vec_out(out, out_dtype, g.out_ld, n);
+    g.rest = rest;
+    const bool direct = units16(x, g.a_ld, k) && units16(w, w_ld, across ? n : k) && (E == 1 || w_es % 8 == 0);
+    const int64_t mean = T / E;
+    int tile = !direct ? (mean <= 48 ? kTileAny32 : kTileAny128)
+             : mean <= 24 ? kTile32 : mean <= 64 ? kTile64 : mean <= 160 ? kTile128 : kTile256;
+    const int want = env_int("EXL3MI_GROUPED_TILE", 0);
+    if (direct && want > 0 && want <= 4) tile = want - 1;
+    return (across ? grouped_rows_across : grouped_rows_along)(g, dtype, tile, (hipStream_t)stream);
+}
+
+int exl3_grouped_mm_dw(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
+                       const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
+                       void* stream) {
+    const char* what = "exl3_grouped_mm_dw";
+    const int rc = grouped_setup(what, dtype, T, n, k, ends, E, dw_dtype);
+    if (rc) return rc;
+    EXL3_CHECK_ARG(accumulate == 0 || accumulate == 1, "%s: accumulate %d", what, accumulate);
+    EXL3_CHECK_ARG((T <= 1 || (dy_ld >= n && x_ld >= k)) && dy_ld <= kMostWidth && x_ld <= kMostWidth && (n == 1 || dw_ld >= k) &&
+                       dw_ld <= ((int64_t)1 << 40) && dw_es >= 0 && dw_es <= ((int64_t)1 << 45) && (E == 1 || dw_es >= (n - 1) * dw_ld + k),
+                   "%s: bad strides (gradients %lld, rows %lld, output %lld and %lld)", what, (long long)dy_ld, (long long)x_ld,
+                   (long long)dw_ld, (long long)dw_es);
+    EXL3_CHECK_ARG((T == 0 || (dy && x && aligned(dy, 2) && aligned(x, 2))) && dw && aligned(dw, out_size(dw_dtype)),
+                   "%s: null or misaligned pointer", what);
+    GroupedArgs g{};
+    g.a = reinterpret_cast<const uint16_t*>(dy);
+    g.b = reinterpret_cast<const uint16_t*>(x);
+    g.out = dw;
+    g.a_ld = T <= 1 ? n : dy_ld;
+    g.b_ld = T <= 1 ? k : x_ld;
+    g.out_ld = n == 1 ? k : dw_ld;
+    g.out_es = dw_es;
+    g.ends = ends;
+    g.E = (int)E;
+    g.T = (int)T;
+    g.m = (int)n;
+    g.n = (int)k;
+    g.out_dtype = dw_dtype;
+    g.vec = vec_out(dw, dw_dtype, g.out_ld, k) && (E == 1 || dw_es * out_size(dw_dtype) % 16 == 0);
+    g.accumulate = accumulate;
+    const bool direct = units16(dy, g.a_ld, n) && units16(x, g.b_ld, k);
+    int tile = !direct ? kTileAny128 : (n + 255) / 256 * ((k + 255) / 256) * E >= 512 ? kTile256 : kTile128;
+    const int want = env_int("EXL3MI_GROUPED_TILE", 0);
+    if (direct && want > 0 && want <= 2) tile = want - 1;
+    return grouped_weights(g, dtype, tile, (hipStream_t)stream);
+}
+
+}  // extern "C"

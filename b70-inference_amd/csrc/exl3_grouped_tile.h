@@ -1,0 +1,363 @@
+// Products of 16-bit matrices grouped by expert: tiles of BM x BN outputs on 16 x 16 x 32 MFMAs, contraction in steps of 64.
+//   out[m, n] = sum_c A(m, c) B(n, c)
+// Either operand lies in memory with the contraction along its rows ("along": x and dy rows, weights of the forward product) or
+// across them ("across": row c holds all m or n; weights of the rows' gradient, both operands of the weights' gradient).
+//
+// Both go to LDS by direct loads of 16 bytes a lane, ST steps deep: a barrier per step, behind which the step read last is
+// loaded anew. Along: 64 values (eight 16-byte units) of each of the tile's rows. Across: 64 rows of the tile's width, which the
+// transposing LDS read turns: sixteen lanes read 4 rows of 16 columns and get a column's 4 values each.
+// Units are permuted on their way in (by the address that a lane loads from) so that lanes that read together touch different banks.
+//
+// The MFMAs take n as their rows: a lane then holds four neighbouring n of one m. Two products share 32 columns n, of which the
+// first takes 8 g + 0 .. 3 and the second 8 g + 4 .. 7 (g: lane >> 4), so a lane has eight neighbours and stores 16 bytes (or 32).
+#pragma once
+
+#include "exl3_grouped.h"
+
+namespace exl3 {
+
+struct GroupedArgs {
+    const uint16_t* a;                 // rows (x, dy)
+    const uint16_t* b;                 // weights; of the weights' gradient x
+    void* out;
+    int64_t a_ld, b_ld, b_es, out_ld, out_es;   // elements from row to row, and from expert to expert
+    const int32_t* ends;
+    int E, T;
+    int c;                             // contraction (the weights' gradient: the expert's rows)
+    int m, n;                          // outputs: columns n; the weights' gradient has m rows
+    int out_dtype, vec;                // vec: eight neighbouring outputs may be stored as 16-byte pieces
+    int rest;                          // rows of no expert become 0
+    int accumulate;                    // the weights' gradient is added to what out holds
+};
+
+enum { kGroupRows = 0, kGroupWeights = 1 };
+
+__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t at, void* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)at, 0, 0, 0);
+}
+
+// Four values of a column each, from 4 rows of 16 columns: sixteen lanes give the addresses of four neighbours.
+typedef short s4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 lds_read_tr(const char* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p));
+}
+
+// Row permutations (see above): natural rows 0 .. 15 of lanes 0 .. 15, and rows 8 (r >> 2) + (r & 3) of lane r.
+__device__ __forceinline__ int swz_rows(int r) { return r & 7; }
+__device__ __forceinline__ int swz_pairs(int r) { return (r & 3) | (r >> 1 & 4); }
+
+// A tile of R rows (along: R x 64, across: 64 x R) in LDS.
+//   N: the n side, whose fragments are the pairs above
+template <int R, bool ACROSS, bool N, int THREADS, bool DIRECT>
+struct GroupTile {
+    static constexpr int kUnits = R * 8, kLoads = kUnits / THREADS;
+    static_assert(kUnits % THREADS == 0, "whole loads per thread");
+    const uint16_t* p;                 // first value of the tile's step
+    int64_t step;                      // elements from step to step
+    int64_t ld;
+    int rows, cols;                    // along: rows there are (of R), contraction left; across: contraction left, columns there are
+    uint32_t off[kLoads];              // bytes from p, or kMx4Out for what is not there at any step
+    u32x4_t v[DIRECT ? 1 : kLoads];
+
+    // unit u of a step: its row and the eight values (from 8 * second on) that lie there
+    __device__ __forceinline__ static int2 place(int u) {
+        if constexpr (!ACROSS) {
+            const int r = u >> 3;
+            return make_int2(r, (u & 7) ^ (N ? swz_pairs(r) : swz_rows(r)));
+        } else {
+            constexpr int kRow = R / 8;
+            const int r = u / kRow, q = u % kRow;
+            // 32 columns (64 bytes) move together on the n side, 16 on the m side
+            if constexpr (N) return make_int2(r, (((q >> 2) ^ (r & 3)) << 2) | (q & 3));
+            else return make_int2(r, (((q >> 1) ^ (swz_pairs(r) & (R / 16 - 1))) << 1) | (q & 1));
+        }
+    }
+    // p_ at the tile's first row (along) or column (across); `have` rows or columns of the tile, `left` of the contraction
+    __device__ __forceinline__ void set(const uint16_t* p_, int64_t ld_, int have, int left, int t) {
+        p = p_;
+        ld = ld_;
+        step = ACROSS ? 64 * ld_ : 64;
+        rows = ACROSS ? left : have;
+        cols = ACROSS ? have : left;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int2 at = place(t + i * THREADS);
+            const bool in = ACROSS ? 8 * at.y < have : at.x < have;
+            off[i] = in ? (uint32_t)at.x * (uint32_t)(2 * ld_) + 16 * at.y : kMx4Out;
+        }
+    }
+    // Eight values at p + e of which n are there: unaligned, the rest 0.
+    __device__ __forceinline__ static u32x4_t load_any(const uint16_t* q, int n) {
+        typedef u32x4_t any_t __attribute__((aligned(2)));
+        if (n >= 8) return *(const __attribute__((address_space(1))) any_t*)q;
+        u32x4_t r = {};
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < n) r[i >> 1] |= (uint32_t)ldg(q + i) << (16 * (i & 1));
+        return r;
+    }
+    // the next step's loads, to LDS or (not DIRECT) on their way to registers
+    __device__ __forceinline__ void load(u32x4_t* lds, int t) {
+        const int left = ACROSS ? rows : cols;
+        if constexpr (DIRECT) {
+            const __amdgpu_buffer_rsrc_t r = mx4_rsrc(reinterpret_cast<const uint8_t*>(p), 0xE0000000LL);
+            const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int2 at = place(t + i * THREADS);
+                const bool in = ACROSS ? at.x < left : 8 * at.y < left;
+                lds_load16(r, in ? off[i] : kMx4Out, lds + wave * 64 + i * THREADS);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int2 at = place(t + i * THREADS);
+                const int n = at.x < rows ? cols - 8 * at.y : 0;
+                v[i] = n > 0 ? load_any(p + at.x * ld + 8 * at.y, n) : u32x4_t{};
+            }
+        }
+        p += left > 64 ? step : 0;     // (the last step's place stays inside the matrix)
+        if constexpr (ACROSS) rows -= 64;
+        else cols -= 64;
+    }
+    __device__ __forceinline__ void store(u32x4_t* lds, int t) const {
+        if constexpr (!DIRECT)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) lds[t + i * THREADS] = v[i];
+    }
+    // Fragment of the 16 rows (or columns) of tile i from w0 on, contraction 32 ks + 8 (lane >> 4) ..
+    __device__ __forceinline__ static u32x4_t frag(const u32x4_t* lds, int w0, int i, int ks, int lane) {
+        const int l = lane & 15, g = lane >> 4;
+        if constexpr (!ACROSS) {
+            const int r = N ? w0 + 32 * (i >> 1) + 8 * (l >> 2) + 4 * (i & 1) + (l & 3) : w0 + 16 * i + l;
+            return lds[r * 8 + ((4 * ks + g) ^ (N ? swz_pairs(r) : swz_rows(r)))];
+        } else {
+            const int r = 32 * ks + 8 * g + (l >> 2);          // and r + 4: the permutations take the same value
+            const char* row = reinterpret_cast<const char*>(lds) + r * (2 * R);
+            int at;
+            if constexpr (N) {
+                const int c = w0 + 32 * (i >> 1);
+                at = (((c >> 5) ^ (r & 3)) << 6) + 16 * (l & 3) + 8 * (i & 1);
+            } else {
+                const int c = w0 + 16 * i;
+                at = (((c >> 4) ^ (swz_pairs(r) & (R / 16 - 1))) << 5) + 8 * (l & 3);
+            }
+            const uint2 lo = lds_read_tr(row + at), hi = lds_read_tr(row + 4 * (2 * R) + at);
+            return u32x4_t{lo.x, lo.y, hi.x, hi.y};
+        }
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void wait_step() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
+    if (dtype == EXL3_F32) return ldg(reinterpret_cast<const float*>(p) + i);
+    const uint16_t v = ldg(reinterpret_cast<const uint16_t*>(p) + i);
+    return dtype == EXL3_F16 ? h2f(v) : bf2f(v);
+}
+
+// Eight neighbouring outputs at element i, `left` of which are there.
+template <int OP>
+__device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, int left, f4_t v, f4_t w) {
+    if (!g.vec) {                      // uniform
+#pragma unroll 1
+        for (int q = 0; q < (left < 8 ? left : 8); ++q) {
+            float f = q < 4 ? v[q & 3] : w[q & 3];
+            if (OP == kGroupWeights && g.accumulate) f += load_as(g.out, i + q, g.out_dtype);
+            store_as(g.out, i + q, f, g.out_dtype);
+        }
+        return;
+    }
+    if (g.out_dtype == EXL3_F32) {
+        f4_t* o = reinterpret_cast<f4_t*>(reinterpret_cast<float*>(g.out) + i);
+        if (OP == kGroupWeights && g.accumulate) {
+            const f4_t p = ldg(o), r = ldg(o + 1);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[q] += p[q];
+                w[q] += r[q];
+            }
+        }
+        o[0] = v;
+        o[1] = w;
+        return;
+    }
+    u32x4_t* o = reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(g.out) + i);
+    if (OP == kGroupWeights && g.accumulate) {
+        const u32x4_t p = ldg(o);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const uint16_t h = (uint16_t)(p[q >> 1] >> (16 * (q & 1)));
+            (q < 4 ? v[q & 3] : w[q & 3]) += g.out_dtype == EXL3_F16 ? h2f(h) : bf2f(h);
+        }
+    }
+    u32x4_t r;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        r[q] = g.out_dtype == EXL3_F16 ? __builtin_bit_cast(uint32_t, h2_t{(_Float16)v[2 * q], (_Float16)v[2 * q + 1]})
+                                       : __builtin_bit_cast(uint32_t, b2_t{(__bf16)v[2 * q], (__bf16)v[2 * q + 1]});
+        r[2 + q] = g.out_dtype == EXL3_F16 ? __builtin_bit_cast(uint32_t, h2_t{(_Float16)w[2 * q], (_Float16)w[2 * q + 1]})
+                                           : __builtin_bit_cast(uint32_t, b2_t{(__bf16)w[2 * q], (__bf16)w[2 * q + 1]});
+    }
+    *o = r;
+}
+
+template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs g) {
+    constexpr int kThreads = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+    static_assert(TM > 0 && TN > 1 && TN % 2 == 0, "pairs of tiles");
+    typedef GroupTile<BM, OP == kGroupWeights, false, kThreads, DIRECT> A;
+    typedef GroupTile<BN, BACROSS, true, kThreads, DIRECT> B;
+    constexpr int kStep = A::kUnits + B::kUnits;
+    __shared__ u32x4_t lds[ST * kStep];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const unsigned nnt = (unsigned)((g.n + BN - 1) / BN);
+    unsigned mt, nt, sp;
+    GroupSlot s;
+    int64_t m0 = 0;
+    int have, left;
+    if constexpr (OP == kGroupRows) {
+        if (!mx4_tile_of((unsigned)(g.T / BM + g.E + g.rest), nnt, 1, mt, nt, sp)) return;
+        s = group_slot<BM>(g.ends, g.E, g.T, mt);
+        if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
+        have = s.rows;
+        left = s.e == g.E ? 0 : g.c;
+    } else {
+        const unsigned nmt = (unsigned)((g.m + BM - 1) / BM);
+        // an expert's tiles after one another: the same rows
+        const unsigned per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if (id >= nmt * nnt * g.E) return;
+        s.e = (int)(id / (nmt * nnt));
+        const unsigned tile = id - s.e * (nmt * nnt), band = tile / (8 * nnt), in = tile - band * 8 * nnt,
+                       h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
+        nt = in / h;
+        mt = 8 * band + in - nt * h;
+        const int lo = __builtin_amdgcn_readfirstlane(s.e > 0 ? group_end(g.ends, s.e - 1, g.T) : 0);
+        const int hi = __builtin_amdgcn_readfirstlane(group_end(g.ends, s.e, g.T));
+        s.row = lo;
+        s.rows = hi > lo ? hi - lo : 0;
+        if (g.accumulate && s.rows == 0) return;
+        m0 = (int64_t)mt * BM;
+        have = (int)(g.m - m0 < BM ? g.m - m0 : BM);
+        left = s.rows;
+    }
+    const int64_t n0 = (int64_t)nt * BN;
+    const int cols = (int)(g.n - n0 < BN ? g.n - n0 : BN);
+    A a;
+    B b;
+    if constexpr (OP == kGroupRows) {
+        a.set(g.a + s.row * g.a_ld, g.a_ld, have, left, t);
+        const uint16_t* w = g.b + (s.e < g.E ? s.e : 0) * g.b_es;
+        b.set(w + (BACROSS ? n0 : n0 * g.b_ld), g.b_ld, cols, left, t);
+    } else {
+        a.set(g.a + s.row * g.a_ld + m0, g.a_ld, have, left, t);
+        b.set(g.b + s.row * g.b_ld + n0, g.b_ld, cols, left, t);
+    }
+    const int steps = (left + 63) / 64;
+    const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+    const bool live = wm < have;                               // (uniform) this wave's rows are there
+    f4_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{};
+
+    const auto compute = [&](const u32x4_t* base) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            u32x4_t fa[TM], fb[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[j] = B::frag(base + A::kUnits, wn, j, ks, lane);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[i] = A::frag(base, wm, i, ks, lane);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<XT>(fb[j], fa[i], acc[i][j]);
+        }
+    };
+    if (steps > 0) {
+        if constexpr (DIRECT) {
+            constexpr int kLoads = A::kLoads + B::kLoads;
+#pragma unroll
+            for (int c = 0; c < ST - 1; ++c) {                 // (past the last: zeros)
+                a.load(lds + c * kStep, t);
+                b.load(lds + c * kStep + A::kUnits, t);
+            }
+            int at = 0;
+            for (int c = 0; c < steps; ++c) {
+                wait_step<kLoads * (ST - 2)>();
+                __builtin_amdgcn_s_barrier();
+                const int next = at == 0 ? ST - 1 : at - 1;
+                a.load(lds + next * kStep, t);
+                b.load(lds + next * kStep + A::kUnits, t);
+                if (live) compute(lds + at * kStep);
+                at = at == ST - 1 ? 0 : at + 1;
+            }
+            wait_step<0>();                                    // the LDS is the next workgroup's behind the end
+        } else {
+            a.load(nullptr, t);
+            b.load(nullptr, t);
+            a.store(lds, t);
+            b.store(lds + A::kUnits, t);
+            __syncthreads();
+            for (int c = 0; c < steps; ++c) {
+                a.load(nullptr, t);
+                b.load(nullptr, t);
+                if (live) compute(lds + (c & 1) * kStep);
+                u32x4_t* o = lds + (~c & 1) * kStep;
+                a.store(o, t);
+                b.store(o + A::kUnits, t);
+                __syncthreads();
+            }
+        }
+    }
+    if (!live) return;
+    const int64_t row0 = OP == kGroupRows ? s.row : m0, base = OP == kGroupRows ? 0 : s.e * g.out_es;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = wm + 16 * i + (lane & 15);
+        if (m >= have) continue;
+#pragma unroll
+        for (int j = 0; j < TN; j += 2) {
+            const int n = wn + 16 * j + 8 * (lane >> 4);
+            if (n < cols) grouped_store<OP>(g, base + (row0 + m) * g.out_ld + n0 + n, cols - n, acc[i][j], acc[i][j + 1]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+// Tiles of a call: rows (and of the weights' gradient columns) of a workgroup; unaligned operands go through registers.
+enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTileAny128 = 4, kTileAny32 = 5 };
+
+template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
+static int launch_grouped(const char* name, const GroupedArgs& g, hipStream_t st) {
+    const int64_t nmt = OP == kGroupRows ? group_slots(g.T, g.E, BM, g.rest) : (g.m + BM - 1) / BM * g.E;
+    const int64_t tiles = nmt * ((g.n + BN - 1) / BN);
+    EXL3_CHECK_ARG(tiles <= kMx4Grid * 256 / (64 * WM * WN) - 7, "%s: grid too large", name);
+    EXL3_LAUNCH(name, (grouped_kernel<XT, OP, BACROSS, BM, BN, WM, WN, ST, OCC, DIRECT>), dim3((unsigned)((tiles + 7) & ~7)),
+                dim3(64 * WM * WN), 0, st, g);
+    return EXL3_OK;
+}
+
+template <int XT, bool BACROSS>
+static int launch_grouped_rows(const GroupedArgs& g, int tile, hipStream_t st) {
+    const char* name = "grouped_rows";
+    switch (tile) {
+        case kTile256: return launch_grouped<XT, kGroupRows, BACROSS, 256, 256, 2, 4, 2, 2, true>(name, g, st);
+        case kTile128: return launch_grouped<XT, kGroupRows, BACROSS, 128, 128, 2, 2, 2, 2, true>(name, g, st);
+        case kTile64: return launch_grouped<XT, kGroupRows, BACROSS, 64, 128, 1, 4, 3, 2, true>(name, g, st);
+        case kTile32: return launch_grouped<XT, kGroupRows, BACROSS, 32, 128, 1, 4, 4, 2, true>(name, g, st);
+        case kTileAny128: return launch_grouped<XT, kGroupRows, BACROSS, 128, 128, 2, 2, 2, 2, false>(name, g, st);
+        default: return launch_grouped<XT, kGroupRows, BACROSS, 32, 128, 1, 4, 2, 2, false>(name, g, st);
+    }
+}
+
+int grouped_rows_along(const GroupedArgs& g, int dtype, int tile, hipStream_t st);
+int grouped_rows_across(const GroupedArgs& g, int dtype, int tile, hipStream_t st);
+int grouped_weights(const GroupedArgs& g, int dtype, int tile, hipStream_t st);
+
+}  // namespace exl3

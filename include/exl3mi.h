@@ -31,7 +31,7 @@ enum exl3_status {
     EXL3_ERR_HIP = 3          /* HIP runtime error */
 };
 
-enum exl3_dtype { EXL3_F16 = 0, EXL3_F32 = 1, EXL3_BF16 = 2 }; /* bf16: the mx4 entry points only */
+enum exl3_dtype { EXL3_F16 = 0, EXL3_F32 = 1, EXL3_BF16 = 2 }; /* bf16: the mx4, grouped and g4 entry points only */
 enum exl3_act { EXL3_ACT_SILU = 0, EXL3_ACT_GELU_TANH = 1 };
 enum exl3_score { EXL3_SCORE_SOFTMAX = 0, EXL3_SCORE_SIGMOID = 1, EXL3_SCORE_SQRT_SOFTPLUS = 2 };
 enum exl3_route_flags { EXL3_ROUTE_RENORM = 1, EXL3_ROUTE_BIAS_SELECT_ONLY = 2 };
@@ -379,6 +379,29 @@ int exl3_route_balance_in(const float* logits, int64_t ld, int64_t M, int64_t E,
 int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t E, int64_t topk, const uint8_t* mask,
                             int score, float coef, const int32_t* counts, const int32_t* rows, const float* grad,
                             float* dlogits, int64_t d_ld, void* stream);
+
+/* ------------------------------------------------------------------------------ products grouped by expert
+ * Rows t with ends[e - 1] <= t < ends[e] (0 for ends[-1]) of a matrix of T rows belong to expert e; ends int32 [E] on the device,
+ * ascending, at most T (other values lead to no access out of range, but to rows that belong to no or to several experts). An
+ * expert may have no rows; rows from ends[E - 1] on belong to none. Any sizes (columns at most 2^22, as the row strides);
+ * operands of 16-byte aligned rows of whole multiples of eight values are read fastest. Sums are fp32 in an order fixed by the
+ * sizes, with one rounding. No scratch; calls may overlap. No reference counterpart (the reference's experts are EXL3 only). */
+enum exl3_grouped_w { EXL3_GROUPED_W_NK = 0, EXL3_GROUPED_W_KN = 1 };
+
+/* out[t, n] = sum over k of x[t, k] W_e(n, k) for the rows t of every expert e: x fp16 or bf16 (`dtype`) [T, k] (row stride x_ld), W
+ * of the same type, an expert's matrix w_es elements behind the one before: [n, k] (EXL3_GROUPED_W_NK, row stride w_ld >= k) or
+ * [k, n] (EXL3_GROUPED_W_KN, w_ld >= n). out fp16, bf16 or fp32 [T, n] (row stride out_ld). Rows of no expert: left as they are
+ * (rest 0) or set to 0 (rest 1). The gradient with respect to x is the same product of the output's gradient in the other layout. */
+int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k, const void* w, int64_t w_ld, int64_t w_es,
+                    int w_layout, int64_t n, const int32_t* ends, int64_t E, void* out, int64_t out_ld, int out_dtype, int rest,
+                    void* stream);
+
+/* Gradient with respect to the weights: dw[e, n, k] = sum over the rows t of expert e of dy[t, n] x[t, k], 0 for an expert without
+ * rows; with accumulate 1 added to what dw holds (one rounding of the sum). dy [T, n] and x [T, k] fp16 or bf16 (`dtype`), dw fp16,
+ * bf16 or fp32 [E, n, k] (row stride dw_ld, expert stride dw_es >= (n - 1) dw_ld + k). */
+int exl3_grouped_mm_dw(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
+                       const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
+                       void* stream);
 
 #ifdef __cplusplus
 }
