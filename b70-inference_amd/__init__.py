@@ -4,6 +4,7 @@ Import with importlib (the directory name is not a Python identifier):
     exl3 = importlib.import_module("b70-inference_amd")
 """
 from ._lib import ACT_GELU_TANH, ACT_SILU, Exl3Error, lib  # noqa: F401
+from .g4 import G4Linear, G4Tensor  # noqa: F401
 from .grouped import grouped_mm, grouped_mm_dw, grouped_mm_dx  # noqa: F401
 from .linear import (BC_LinearEXL3, exl3_gemm, exl3_gemm_noalloc, exl3_mgemm, exl3_reconstruct,  # noqa: F401
                      fuse_linears, had_r_128, linear, mgemm_tables, reconstruct, reconstruct_had_slice,

@@ -1,0 +1,112 @@
+// Products with 4-bit weights and group scales: entry points, the choice of kernel, and matrices of fewer than four scales.
+#include "exl3_g4.h"
+
+namespace exl3 {
+
+// One output per thread: tensors of fewer than four scales, which the other kernels' loads of scales do not fit.
+template <int XT>
+__global__ __launch_bounds__(256) void g4_tiny_kernel(G4Args g, int group) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / g.n, n = i - m * g.n;
+    if (m >= g.T) return;
+    int e = 0;
+    if (g.ends)
+        while (e < g.E && group_end(g.ends, e, g.T) <= m) ++e;
+    if (e == g.E) {
+        if (g.rest) store_as(g.out, m * g.out_ld + n, 0.f, g.out_dtype);
+        return;
+    }
+    const int64_t row = (int64_t)e * g.n + n;
+    float sum = 0.f;
+    for (int G = 0; G < g.groups; ++G) {
+        const int z = g.zeros ? ldg(g.zeros + row * g.groups + G) & 15 : 8;
+        float part = 0.f;
+        for (int k = G * group; k < (G + 1) * group; ++k) {
+            const uint16_t v = ldg(g.x + m * g.x_ld + k);
+            part += (XT == kRowF16 ? h2f(v) : bf2f(v)) * (float)((ldg(g.codes + row * (g.k / 2) + k / 2) >> (4 * (k & 1)) & 15) - z);
+        }
+        sum += g4_scale(ldg(g.scales + row * g.groups + G), g.scale_bf16) * part;
+    }
+    store_as(g.out, m * g.out_ld + n, sum + (g.bias ? ldg(g.bias + n) : 0.f), g.out_dtype);
+}
+
+static int out_size(int t) { return t == EXL3_F32 ? 4 : 2; }
+
+static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, int64_t m, int64_t k, const uint8_t* codes,
+                      const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const int32_t* ends,
+                      int64_t E, const float* bias, void* out, int64_t out_ld, int out_dtype, int rest, void* stream) {
+    EXL3_CHECK_ARG(m >= 0 && m <= 0x3FFFFFFF && n > 0 && n <= 0x3FFFFFFF && E > 0 && E <= 65536 && k > 0 && k <= (1 << 22) &&
+                       k % 32 == 0 && n * E <= ((int64_t)1 << 42) / k,
+                   "%s: bad sizes (%lld rows, %lld outputs, %lld inputs, %lld matrices; inputs a multiple of 32)", what,
+                   (long long)m, (long long)n, (long long)k, (long long)E);
+    EXL3_CHECK_ARG(dtype == EXL3_F16 || dtype == EXL3_BF16, "%s: rows must be fp16 or bf16", what);
+    EXL3_CHECK_ARG(scale_dtype == EXL3_F16 || scale_dtype == EXL3_BF16, "%s: scales must be fp16 or bf16", what);
+    EXL3_CHECK_ARG(out_dtype == EXL3_F16 || out_dtype == EXL3_F32 || out_dtype == EXL3_BF16, "%s: the output must be fp16, bf16 or "
+                   "fp32", what);
+    if (group != 32 && group != 64 && (group <= 0 || group % 128))
+        return fail(EXL3_ERR_UNSUPPORTED, "%s: groups of %lld (32, 64 and multiples of 128)", what, (long long)group);
+    EXL3_CHECK_ARG(k % group == 0, "%s: %lld inputs are not whole groups of %lld", what, (long long)k, (long long)group);
+    EXL3_CHECK_ARG(m <= 1 || (x_ld >= k && x_ld <= (1 << 22) && out_ld >= n && out_ld <= ((int64_t)1 << 40)),
+                   "%s: bad strides (rows %lld, output %lld)", what, (long long)x_ld, (long long)out_ld);
+    if (m == 0) return EXL3_OK;
+    EXL3_CHECK_ARG(x && codes && scales && out, "%s: null pointer", what);
+    EXL3_CHECK_ARG(aligned(x, 16) && (m == 1 || x_ld % 8 == 0) && aligned(codes, 16), "%s: rows and codes must be 16-byte aligned", what);
+    EXL3_CHECK_ARG(aligned(scales, 2) && aligned(out, out_size(out_dtype)) && (!bias || aligned(bias, 4)) && (!ends || aligned(ends, 4)),
+                   "%s: misaligned pointer", what);
+    G4Args g{};
+    g.x = reinterpret_cast<const uint16_t*>(x);
+    g.x_ld = m == 1 ? k : x_ld;
+    g.codes = codes;
+    g.scales = reinterpret_cast<const uint16_t*>(scales);
+    g.zeros = zeros;
+    g.bias = bias;
+    g.out = out;
+    g.out_ld = m == 1 ? n : out_ld;
+    g.ends = ends;
+    g.E = (int)E;
+    g.T = (int)m;
+    g.k = (int)k;
+    g.n = (int)n;
+    g.groups = (int)(k / group);
+    g.per = group > 128 ? (int)(group / 128) : 1;
+    g.scale_bf16 = scale_dtype == EXL3_BF16;
+    g.out_dtype = out_dtype;
+    g.vec = n % 4 == 0 && g.out_ld % 4 == 0 && aligned(out, 4 * out_size(out_dtype));
+    g.rest = rest;
+    hipStream_t st = (hipStream_t)stream;
+    if (E * n * g.groups < 4) {
+        EXL3_CHECK_ARG(m <= kMx4Grid * 256 / n, "%s: grid too large", what);
+        const dim3 grid((unsigned)((m * n + 255) / 256));
+        if (dtype == EXL3_F16) EXL3_LAUNCH("g4_tiny", g4_tiny_kernel<kRowF16>, grid, dim3(256), 0, st, g, (int)group);
+        else EXL3_LAUNCH("g4_tiny", g4_tiny_kernel<kRowBF16>, grid, dim3(256), 0, st, g, (int)group);
+        return EXL3_OK;
+    }
+    const int64_t mean = m / E;
+    int tile = mean <= 16 && k <= 8192 ? 0 : mean <= 48 ? 1 : mean <= 96 ? 2 : 3;
+    const int want = env_int("EXL3MI_G4_TILE", 0);
+    if (want > (k <= 8192 ? 0 : 1) && want <= 4) tile = want - 1;
+    return dtype == EXL3_F16 ? g4_run_f16(g, (int)group, tile, st) : g4_run_bf16(g, (int)group, tile, st);
+}
+
+}  // namespace exl3
+
+extern "C" {
+
+using namespace exl3;
+
+int exl3_g4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const void* scales,
+                   int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,
+                   int c_dtype, void* stream) {
+    return g4_product("exl3_g4_linear", x, x_ld, x_dtype, m, k, codes, scales, scale_dtype, zeros, group, n, nullptr, 1, bias, C, c_ld,
+                      c_dtype, 0, stream);
+}
+
+int exl3_grouped_g4(const void* x, int64_t x_ld, int x_dtype, int64_t T, int64_t k, const uint8_t* codes, const void* scales,
+                    int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const int32_t* ends, int64_t E, void* out,
+                    int64_t out_ld, int out_dtype, int rest, void* stream) {
+    EXL3_CHECK_ARG(ends, "exl3_grouped_g4: null pointer");
+    EXL3_CHECK_ARG(rest == 0 || rest == 1, "exl3_grouped_g4: rest %d", rest);
+    return g4_product("exl3_grouped_g4", x, x_ld, x_dtype, T, k, codes, scales, scale_dtype, zeros, group, n, ends, E, nullptr, out,
+                      out_ld, out_dtype, rest, stream);
+}
+
+}  // extern "C"

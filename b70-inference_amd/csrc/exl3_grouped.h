@@ -20,28 +20,38 @@ __device__ __forceinline__ int group_end(const int32_t* ends, int e, int T) {
     return v < 0 ? 0 : v > T ? T : v;
 }
 
-// The same value in every lane (wave-uniform).
+// Slots of T rows over E experts, and with `rest` of the rows of none: of blocks of BM rows, or where that is fewer one for every
+// row, of which a block's first does the block's work (few rows over many experts: an empty slot costs a workgroup's launch).
+inline int64_t group_slots(int64_t T, int64_t E, int64_t BM, bool rest) {
+    const int64_t n = T / BM + E + (rest ? 1 : 0);
+    return T < n ? T : n;
+}
+
+// The same value in every lane (wave-uniform). `slots`: group_slots.
 template <int BM>
-__device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int T, unsigned slot) {
+__device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int T, unsigned slot, int slots) {
     const int lane = threadIdx.x & 63;
+    const bool by_row = slots == T;    // (every block's first row is a slot's then too if T = T / BM + E)
     int e = 0;
     for (int i = 0; i < E; i += 64) {
-        const int at = i + lane;
-        const bool in = at < E && (unsigned)(group_end(ends, at < E ? at : E - 1, T) / BM + at + 1) <= slot;
+        const int at = i + lane, end = group_end(ends, at < E ? at : E - 1, T);
+        const bool in = at < E && (by_row ? (unsigned)end : (unsigned)(end / BM + at + 1)) <= slot;
         e += __popcll(__ballot(in));
     }
     e = __builtin_amdgcn_readfirstlane(e);
     const int lo = __builtin_amdgcn_readfirstlane(e > 0 ? group_end(ends, e - 1, T) : 0);
     const int hi = __builtin_amdgcn_readfirstlane(e < E ? group_end(ends, e, T) : T);
-    const int64_t block = (int64_t)slot - (lo / BM + e), row = lo + block * BM;
     GroupSlot s;
     s.e = e;
-    s.row = row;
-    s.rows = block < 0 || row >= hi ? 0 : hi - row < BM ? (int)(hi - row) : BM;
+    if (by_row) {
+        s.row = slot;
+        s.rows = (int)slot < lo || (int)slot >= hi || ((int)slot - lo) % BM != 0 ? 0 : hi - (int)slot < BM ? hi - (int)slot : BM;
+        return s;
+    }
+    const int64_t block = (int64_t)slot - (lo / BM + e);
+    s.row = lo + block * BM;
+    s.rows = block < 0 || s.row >= hi ? 0 : hi - s.row < BM ? (int)(hi - s.row) : BM;
     return s;
 }
-
-// Slots of T rows over E experts, and of the rows of none.
-inline int64_t group_slots(int64_t T, int64_t E, int64_t BM, bool rest) { return T / BM + E + (rest ? 1 : 0); }
 
 }  // namespace exl3

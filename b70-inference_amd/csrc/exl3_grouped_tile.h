@@ -28,6 +28,7 @@ struct GroupedArgs {
     int out_dtype, vec;                // vec: eight neighbouring outputs may be stored as 16-byte pieces
     int rest;                          // rows of no expert become 0
     int accumulate;                    // the weights' gradient is added to what out holds
+    int slots;                         // row blocks of the grid
 };
 
 enum { kGroupRows = 0, kGroupWeights = 1 };
@@ -191,7 +192,9 @@ __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, i
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             const uint16_t h = (uint16_t)(p[q >> 1] >> (16 * (q & 1)));
-            (q < 4 ? v[q & 3] : w[q & 3]) += g.out_dtype == EXL3_F16 ? h2f(h) : bf2f(h);
+            const float f = g.out_dtype == EXL3_F16 ? h2f(h) : bf2f(h);
+            if (q < 4) v[q & 3] += f;
+            else w[q & 3] += f;
         }
     }
     u32x4_t r;
@@ -220,8 +223,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
     int64_t m0 = 0;
     int have, left;
     if constexpr (OP == kGroupRows) {
-        if (!mx4_tile_of((unsigned)(g.T / BM + g.E + g.rest), nnt, 1, mt, nt, sp)) return;
-        s = group_slot<BM>(g.ends, g.E, g.T, mt);
+        if (!mx4_tile_of((unsigned)g.slots, nnt, 1, mt, nt, sp)) return;
+        s = group_slot<BM>(g.ends, g.E, g.T, mt, g.slots);
         if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
         have = s.rows;
         left = s.e == g.E ? 0 : g.c;
@@ -334,8 +337,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
 enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTileAny128 = 4, kTileAny32 = 5 };
 
 template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
-static int launch_grouped(const char* name, const GroupedArgs& g, hipStream_t st) {
+static int launch_grouped(const char* name, GroupedArgs g, hipStream_t st) {
     const int64_t nmt = OP == kGroupRows ? group_slots(g.T, g.E, BM, g.rest) : (g.m + BM - 1) / BM * g.E;
+    g.slots = (int)nmt;
     const int64_t tiles = nmt * ((g.n + BN - 1) / BN);
     EXL3_CHECK_ARG(tiles <= kMx4Grid * 256 / (64 * WM * WN) - 7, "%s: grid too large", name);
     EXL3_LAUNCH(name, (grouped_kernel<XT, OP, BACROSS, BM, BN, WM, WN, ST, OCC, DIRECT>), dim3((unsigned)((tiles + 7) & ~7)),

@@ -16,8 +16,9 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, stream_of
-from .mx4 import DTYPES
+from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, stream_of
+from .g4 import G4Tensor
+from .mx4 import DTYPES, _rows
 
 _HALF = {torch.float16: EXL3_F16, torch.bfloat16: EXL3_BF16}
 _W_NK, _W_KN = 0, 1                    # exl3_grouped_w
@@ -57,7 +58,24 @@ def _matrices(what: str, w: torch.Tensor):
     return w.contiguous(), _W_NK, k, n * k
 
 
+def _out_rows(what: str, x: torch.Tensor, T: int, n: int, out, out_dtype):
+    """out [T, n] (allocated where it is None), and its row stride."""
+    if out is None:
+        dt = x.dtype if out_dtype is None else out_dtype
+        if dt not in DTYPES:
+            raise Exl3Error(f"{what}: out_dtype fp16, bf16 or fp32, got {dt}")
+        return x.new_empty((T, n), dtype=dt), n
+    if out.dtype not in DTYPES or tuple(out.shape) != (T, n):
+        raise Exl3Error(f"{what}: out must be fp16, bf16 or fp32 [{T}, {n}], got {out.dtype} {tuple(out.shape)}")
+    ld = out.stride(0) if T > 1 else n
+    if (n > 1 and out.stride(1) != 1) or ld < n:
+        raise Exl3Error(f"{what}: rows of out must be contiguous and must not overlap")
+    return out, ld
+
+
 def _mm(what: str, x, w, ends, transpose: bool, out, out_dtype):
+    if isinstance(w, G4Tensor):
+        raise NotImplementedError(f"{what}: 4-bit weights have no gradient of their rows")
     if w.dim() != 3 or w.dtype not in _HALF or 0 in w.shape:
         raise Exl3Error(f"{what}: w must be fp16 or bf16 [E, N, K], got {w.dtype} {tuple(w.shape)}")
     x, ld = _rows2(what, "dy" if transpose else "x", x)
@@ -69,18 +87,7 @@ def _mm(what: str, x, w, ends, transpose: bool, out, out_dtype):
         raise Exl3Error(f"{what}: rows {x.dtype} {tuple(x.shape)} and weights {w.dtype} {tuple(w.shape)} do not belong together")
     ends = _ends(what, ends, E)
     rest = out is None
-    if rest:
-        dt = x.dtype if out_dtype is None else out_dtype
-        if dt not in DTYPES:
-            raise Exl3Error(f"{what}: out_dtype fp16, bf16 or fp32, got {dt}")
-        out = x.new_empty((T, n), dtype=dt)
-        o_ld = n
-    else:
-        if out.dtype not in DTYPES or tuple(out.shape) != (T, n):
-            raise Exl3Error(f"{what}: out must be fp16, bf16 or fp32 [{T}, {n}], got {out.dtype} {tuple(out.shape)}")
-        o_ld = out.stride(0) if T > 1 else n
-        if (n > 1 and out.stride(1) != 1) or o_ld < n:
-            raise Exl3Error(f"{what}: rows of out must be contiguous and must not overlap")
+    out, o_ld = _out_rows(what, x, T, n, out, out_dtype)
     where = on_device(what, x, w, ends, out)
     w, layout, w_ld, w_es = _matrices(what, w)
     if transpose:
@@ -93,11 +100,32 @@ def _mm(what: str, x, w, ends, transpose: bool, out, out_dtype):
     return out
 
 
+def _mm_g4(what: str, x, w: G4Tensor, ends, out, out_dtype):
+    if w.codes.dim() != 3:
+        raise Exl3Error(f"{what}: w must be a G4Tensor [E, N, K], got {tuple(w.shape)}")
+    E, n, k = w.shape
+    if x.dim() != 2 or x.dtype not in _HALF or x.shape[1] != k:
+        raise Exl3Error(f"{what}: x must be fp16 or bf16 [T, {k}], got {x.dtype} {tuple(x.shape)}")
+    ends = _ends(what, ends, E)
+    rest = out is None
+    x2, T, ld = _rows(x, k)
+    out, o_ld = _out_rows(what, x, T, n, out, out_dtype)
+    with on_device(what, x, w.codes, ends, out):
+        rc = lib().exl3_grouped_g4(x2.data_ptr(), ld, _HALF[x.dtype], T, k, w.codes.data_ptr(), w.scales.data_ptr(),
+                                   _HALF[w.scales.dtype], ptr(w.zeros), w.group, n, ends.data_ptr(), E, out.data_ptr(), o_ld,
+                                   DTYPES[out.dtype], int(rest), stream_of(x))
+    if rc:
+        check(rc, what)
+    return out
+
+
 def grouped_mm(x: torch.Tensor, w, ends: torch.Tensor, out: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y[t] = w[e] @ x[t] for the rows t of every expert e: x fp16 or bf16 [T, K], w of x's type [E, N, K] (any strides; matrices
-    whose rows or columns are contiguous are read in place), ends int32 [E]. Returns [T, N] of out_dtype (fp16, bf16 or fp32; None:
+    whose rows or columns are contiguous are read in place) or a G4Tensor [E, N, K], ends int32 [E]. Returns [T, N] of out_dtype (fp16, bf16 or fp32; None:
     x's type), 0 in rows of no expert, or writes out, which keeps such rows as they are."""
+    if isinstance(w, G4Tensor):
+        return _mm_g4("grouped_mm", x, w, ends, out, out_dtype)
     return _mm("grouped_mm", x, w, ends, False, out, out_dtype)
 
 
