@@ -106,7 +106,7 @@ __device__ __forceinline__ uint32_t g4_zeros4(const uint8_t* p, int at, int grou
 // Block of rows, and its expert's first matrix row: slot s of blocks of BM rows.
 template <int BM>
 __device__ __forceinline__ GroupSlot g4_slot(const G4Args& g, unsigned slot) {
-    if (g.ends) return group_slot<BM>(g.ends, g.E, g.T, slot, g.slots);
+    if (g.ends) return group_slot<BM>(g.ends, g.E, g.T, slot);
     GroupSlot s;
     s.e = 0;
     s.row = (int64_t)slot * BM;

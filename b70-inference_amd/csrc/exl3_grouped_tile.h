@@ -8,9 +8,11 @@
 // transposing LDS read turns: sixteen lanes read 4 rows of 16 columns and get a column's 4 values each.
 // Units are permuted on their way in (by the address that a lane loads from) so that lanes that read together touch different banks.
 //
-// The MFMAs take n as their rows: a lane then holds four neighbouring n of one m. Two products share 32 columns n, of which the
-// first takes 8 g + 0 .. 3 and the second 8 g + 4 .. 7 (g: lane >> 4), so a lane has eight neighbours and stores 16 bytes (or 32).
+// The MFMAs take n as their rows: a lane then holds four neighbouring n of one m. The products of two tiles of 16 n change hands at
+// the end, so that a lane has eight neighbours and stores 16 bytes (or 32).
 #pragma once
+
+#include <type_traits>
 
 #include "exl3_grouped.h"
 
@@ -33,8 +35,11 @@ struct GroupedArgs {
 
 enum { kGroupRows = 0, kGroupWeights = 1 };
 
-__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t at, void* lds) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)at, 0, 0, 0);
+// 16 bytes per lane from `at` bytes on to LDS (address `lds` and 16 bytes a lane from there on). Inline assembly: behind the builtin
+// the compiler waits for the load before every transposing read, whatever it reads. What it brings is waited for by wait_step.
+__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t at, const void* lds) {
+    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(r));
 }
 
 // Four values of a column each, from 4 rows of 16 columns: sixteen lanes give the addresses of four neighbours.
@@ -43,13 +48,11 @@ __device__ __forceinline__ uint2 lds_read_tr(const char* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p));
 }
 
-// Row permutations (see above): natural rows 0 .. 15 of lanes 0 .. 15, and rows 8 (r >> 2) + (r & 3) of lane r.
-__device__ __forceinline__ int swz_rows(int r) { return r & 7; }
-__device__ __forceinline__ int swz_pairs(int r) { return (r & 3) | (r >> 1 & 4); }
+// Bits 0, 1 and 3 of a row: what the rows that the transposing read takes together differ in.
+__device__ __forceinline__ int swz_across(int r) { return (r & 3) | (r >> 1 & 4); }
 
 // A tile of R rows (along: R x 64, across: 64 x R) in LDS.
-//   N: the n side, whose fragments are the pairs above
-template <int R, bool ACROSS, bool N, int THREADS, bool DIRECT>
+template <int R, bool ACROSS, int THREADS, bool DIRECT>
 struct GroupTile {
     static constexpr int kUnits = R * 8, kLoads = kUnits / THREADS;
     static_assert(kUnits % THREADS == 0, "whole loads per thread");
@@ -64,13 +67,11 @@ struct GroupTile {
     __device__ __forceinline__ static int2 place(int u) {
         if constexpr (!ACROSS) {
             const int r = u >> 3;
-            return make_int2(r, (u & 7) ^ (N ? swz_pairs(r) : swz_rows(r)));
+            return make_int2(r, (u & 7) ^ (r & 7));
         } else {
             constexpr int kRow = R / 8;
             const int r = u / kRow, q = u % kRow;
-            // 32 columns (64 bytes) move together on the n side, 16 on the m side
-            if constexpr (N) return make_int2(r, (((q >> 2) ^ (r & 3)) << 2) | (q & 3));
-            else return make_int2(r, (((q >> 1) ^ (swz_pairs(r) & (R / 16 - 1))) << 1) | (q & 1));
+            return make_int2(r, (((q >> 1) ^ (swz_across(r) & (R / 16 - 1))) << 1) | (q & 1));   // 16 columns together
         }
     }
     // p_ at the tile's first row (along) or column (across); `have` rows or columns of the tile, `left` of the contraction
@@ -97,29 +98,28 @@ struct GroupTile {
             if (i < n) r[i >> 1] |= (uint32_t)ldg(q + i) << (16 * (i & 1));
         return r;
     }
-    // the next step's loads, to LDS or (not DIRECT) on their way to registers
-    __device__ __forceinline__ void load(u32x4_t* lds, int t) {
-        const int left = ACROSS ? rows : cols;
+    // load i of the next step: to LDS, or (not DIRECT) on its way to registers
+    __device__ __forceinline__ void load_one(int i, u32x4_t* lds, int t) {
+        const int2 at = place(t + i * THREADS);
         if constexpr (DIRECT) {
             const __amdgpu_buffer_rsrc_t r = mx4_rsrc(reinterpret_cast<const uint8_t*>(p), 0xE0000000LL);
-            const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int2 at = place(t + i * THREADS);
-                const bool in = ACROSS ? at.x < left : 8 * at.y < left;
-                lds_load16(r, in ? off[i] : kMx4Out, lds + wave * 64 + i * THREADS);
-            }
+            const bool in = ACROSS ? at.x < rows : 8 * at.y < cols;
+            lds_load16(r, in ? off[i] : kMx4Out, lds + __builtin_amdgcn_readfirstlane(t >> 6) * 64 + i * THREADS);
         } else {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int2 at = place(t + i * THREADS);
-                const int n = at.x < rows ? cols - 8 * at.y : 0;
-                v[i] = n > 0 ? load_any(p + at.x * ld + 8 * at.y, n) : u32x4_t{};
-            }
+            const int n = at.x < rows ? cols - 8 * at.y : 0;
+            v[i] = n > 0 ? load_any(p + at.x * ld + 8 * at.y, n) : u32x4_t{};
         }
-        p += left > 64 ? step : 0;     // (the last step's place stays inside the matrix)
+    }
+    // behind a step's loads
+    __device__ __forceinline__ void next() {
+        p += (ACROSS ? rows : cols) > 64 ? step : 0;           // (the last step's place stays inside the matrix)
         if constexpr (ACROSS) rows -= 64;
         else cols -= 64;
+    }
+    __device__ __forceinline__ void load(u32x4_t* lds, int t) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load_one(i, lds, t);
+        next();
     }
     __device__ __forceinline__ void store(u32x4_t* lds, int t) const {
         if constexpr (!DIRECT)
@@ -130,19 +130,12 @@ struct GroupTile {
     __device__ __forceinline__ static u32x4_t frag(const u32x4_t* lds, int w0, int i, int ks, int lane) {
         const int l = lane & 15, g = lane >> 4;
         if constexpr (!ACROSS) {
-            const int r = N ? w0 + 32 * (i >> 1) + 8 * (l >> 2) + 4 * (i & 1) + (l & 3) : w0 + 16 * i + l;
-            return lds[r * 8 + ((4 * ks + g) ^ (N ? swz_pairs(r) : swz_rows(r)))];
+            const int r = w0 + 16 * i + l;
+            return lds[r * 8 + ((4 * ks + g) ^ (r & 7))];
         } else {
-            const int r = 32 * ks + 8 * g + (l >> 2);          // and r + 4: the permutations take the same value
+            const int r = 32 * ks + 8 * g + (l >> 2);          // and r + 4: the permutation takes the same value
             const char* row = reinterpret_cast<const char*>(lds) + r * (2 * R);
-            int at;
-            if constexpr (N) {
-                const int c = w0 + 32 * (i >> 1);
-                at = (((c >> 5) ^ (r & 3)) << 6) + 16 * (l & 3) + 8 * (i & 1);
-            } else {
-                const int c = w0 + 16 * i;
-                at = (((c >> 4) ^ (swz_pairs(r) & (R / 16 - 1))) << 5) + 8 * (l & 3);
-            }
+            const int at = ((((w0 >> 4) + i) ^ (swz_across(r) & (R / 16 - 1))) << 5) + 8 * (l & 3);
             const uint2 lo = lds_read_tr(row + at), hi = lds_read_tr(row + 4 * (2 * R) + at);
             return u32x4_t{lo.x, lo.y, hi.x, hi.y};
         }
@@ -158,6 +151,18 @@ __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
     if (dtype == EXL3_F32) return ldg(reinterpret_cast<const float*>(p) + i);
     const uint16_t v = ldg(reinterpret_cast<const uint16_t*>(p) + i);
     return dtype == EXL3_F16 ? h2f(v) : bf2f(v);
+}
+
+// The outputs of two tiles of 16 n, four neighbours of each per lane, to eight neighbours: of lane groups 0 and 2 the first tile's n 0 .. 7
+// and 8 .. 15, of 1 and 3 the second's.
+__device__ __forceinline__ void grouped_pair(f4_t& v, f4_t& w) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const auto x = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, (float)v[q]), __builtin_bit_cast(uint32_t, (float)w[q]),
+                                                        false, false);
+        v[q] = __builtin_bit_cast(float, (uint32_t)x[0]);
+        w[q] = __builtin_bit_cast(float, (uint32_t)x[1]);
+    }
 }
 
 // Eight neighbouring outputs at element i, `left` of which are there.
@@ -208,36 +213,47 @@ __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, i
     *o = r;
 }
 
+// This workgroup's place in a grid that takes `chunk` tiles after one another on an XCD, the XCDs in turn (workgroups go round robin over
+// them): what runs together on one shares operands in its L2, and tiles of little work (experts of few rows) spread over all.
+__device__ __forceinline__ unsigned grouped_place(unsigned chunk) {
+    const unsigned j = blockIdx.x >> 3, c = j / chunk;
+    return (c * 8 + (blockIdx.x & 7)) * chunk + j - c * chunk;
+}
+// Tile `in` of nmt x nnt: eight rows of tiles after one another for each column.
+__device__ __forceinline__ void grouped_tile(unsigned in, unsigned nmt, unsigned nnt, unsigned& mt, unsigned& nt) {
+    const unsigned band = in / (8 * nnt), i = in - band * 8 * nnt, h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
+    nt = i / h;
+    mt = 8 * band + i - nt * h;
+}
+constexpr unsigned kChunk = 32;        // the CUs of an XCD
+
 template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs g) {
     constexpr int kThreads = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
     static_assert(TM > 0 && TN > 1 && TN % 2 == 0, "pairs of tiles");
-    typedef GroupTile<BM, OP == kGroupWeights, false, kThreads, DIRECT> A;
-    typedef GroupTile<BN, BACROSS, true, kThreads, DIRECT> B;
+    typedef GroupTile<BM, OP == kGroupWeights, kThreads, DIRECT> A;
+    typedef GroupTile<BN, BACROSS, kThreads, DIRECT> B;
     constexpr int kStep = A::kUnits + B::kUnits;
     __shared__ u32x4_t lds[ST * kStep];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned nnt = (unsigned)((g.n + BN - 1) / BN);
-    unsigned mt, nt, sp;
+    unsigned mt, nt;
+    const unsigned id = grouped_place(kChunk);
     GroupSlot s;
     int64_t m0 = 0;
     int have, left;
     if constexpr (OP == kGroupRows) {
-        if (!mx4_tile_of((unsigned)g.slots, nnt, 1, mt, nt, sp)) return;
-        s = group_slot<BM>(g.ends, g.E, g.T, mt, g.slots);
+        if (id >= g.slots * nnt) return;
+        grouped_tile(id, (unsigned)g.slots, nnt, mt, nt);
+        s = group_slot<BM>(g.ends, g.E, g.T, mt);
         if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
         have = s.rows;
         left = s.e == g.E ? 0 : g.c;
     } else {
         const unsigned nmt = (unsigned)((g.m + BM - 1) / BM);
-        // an expert's tiles after one another: the same rows
-        const unsigned per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
         if (id >= nmt * nnt * g.E) return;
         s.e = (int)(id / (nmt * nnt));
-        const unsigned tile = id - s.e * (nmt * nnt), band = tile / (8 * nnt), in = tile - band * 8 * nnt,
-                       h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
-        nt = in / h;
-        mt = 8 * band + in - nt * h;
+        grouped_tile(id - s.e * (nmt * nnt), nmt, nnt, mt, nt);
         const int lo = __builtin_amdgcn_readfirstlane(s.e > 0 ? group_end(g.ends, s.e - 1, g.T) : 0);
         const int hi = __builtin_amdgcn_readfirstlane(group_end(g.ends, s.e, g.T));
         s.row = lo;
@@ -268,37 +284,74 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{};
 
-    const auto compute = [&](const u32x4_t* base) {
+    constexpr int kLoads = A::kLoads + B::kLoads, kFrags = TM + TN, kMul = TM * TN;
+    // Fragments of half a step (32) from `base`, with `loads` the loads of a step to `to`, and with `products` those of the half step
+    // that ma and mb hold, in turn: reads or loads in a row wait for the LDS's and the caches' ports, and a wave issues in order, so
+    // the MFMAs behind them would wait too. Reads and loads are through after three quarters.
+    const auto half = [&](auto loads, auto products, const u32x4_t* base, int ks, u32x4_t (&fa)[TM], u32x4_t (&fb)[TN], u32x4_t* to,
+                          const u32x4_t (&ma)[TM], const u32x4_t (&mb)[TN]) {
+        constexpr int kLead = kMul * 3 / 4;
+        const auto mul = [&](int m) { acc[m / TN][m % TN] = mfma16<XT>(mb[m % TN], ma[m / TN], acc[m / TN][m % TN]); };
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            u32x4_t fa[TM], fb[TN];
+        for (int f = 0; f < kFrags; ++f) {
+            if constexpr (loads)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j] = B::frag(base + A::kUnits, wn, j, ks, lane);
+                for (int i = f * kLoads / kFrags; i < (f + 1) * kLoads / kFrags; ++i) {
+                    if (i < A::kLoads) a.load_one(i, to, t);
+                    else b.load_one(i - A::kLoads, to + A::kUnits, t);
+                }
+            if (f < TN) fb[f] = B::frag(base + A::kUnits, wn, f, ks, lane);
+            else fa[f - TN] = A::frag(base, wm, f - TN, ks, lane);
+            if constexpr (products) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i) fa[i] = A::frag(base, wm, i, ks, lane);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<XT>(fb[j], fa[i], acc[i][j]);
+                for (int m = f * kLead / kFrags; m < (f + 1) * kLead / kFrags; ++m) mul(m);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-    };
-    if (steps > 0) {
-        if constexpr (DIRECT) {
-            constexpr int kLoads = A::kLoads + B::kLoads;
+        if constexpr (loads) {
+            a.next();
+            b.next();
+        }
+        if constexpr (products)
 #pragma unroll
-            for (int c = 0; c < ST - 1; ++c) {                 // (past the last: zeros)
+            for (int m = kLead; m < kMul; ++m) mul(m);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (steps > 0) {
+        u32x4_t fa[TM], fb[TN], ga[TM], gb[TN];
+        if constexpr (DIRECT) {
+            // Half a step's fragments are read while the half before is multiplied. The barrier is between the halves: behind it the
+            // next step lies in LDS, and the one whose second half is on its way to the MFMAs is loaded anew.
+#pragma unroll
+            for (int c = 0; c < ST; ++c) {                     // (past the last: zeros)
                 a.load(lds + c * kStep, t);
                 b.load(lds + c * kStep + A::kUnits, t);
             }
+            wait_step<kLoads * (ST - 1)>();
+            __builtin_amdgcn_s_barrier();
             int at = 0;
-            for (int c = 0; c < steps; ++c) {
-                wait_step<kLoads * (ST - 2)>();
-                __builtin_amdgcn_s_barrier();
-                const int next = at == 0 ? ST - 1 : at - 1;
-                a.load(lds + next * kStep, t);
-                b.load(lds + next * kStep + A::kUnits, t);
-                if (live) compute(lds + at * kStep);
-                at = at == ST - 1 ? 0 : at + 1;
+            if (live) {
+                half(no, no, lds, 0, fa, fb, nullptr, ga, gb);
+                for (int c = 0; c < steps; ++c) {
+                    const int next = at == ST - 1 ? 0 : at + 1;
+                    __builtin_amdgcn_sched_barrier(0);
+                    half(no, yes, lds + at * kStep, 1, ga, gb, nullptr, fa, fb);
+                    __builtin_amdgcn_sched_barrier(0);
+                    wait_step<kLoads * (ST - 2)>();
+                    __builtin_amdgcn_s_barrier();
+                    __builtin_amdgcn_sched_barrier(0);
+                    half(yes, yes, lds + next * kStep, 0, fa, fb, lds + at * kStep, ga, gb);
+                    at = next;
+                }
+            } else {                                           // loads alone
+                for (int c = 0; c < steps; ++c) {
+                    wait_step<kLoads * (ST - 2)>();
+                    __builtin_amdgcn_s_barrier();
+                    a.load(lds + at * kStep, t);
+                    b.load(lds + at * kStep + A::kUnits, t);
+                    at = at == ST - 1 ? 0 : at + 1;
+                }
             }
             wait_step<0>();                                    // the LDS is the next workgroup's behind the end
         } else {
@@ -310,7 +363,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
             for (int c = 0; c < steps; ++c) {
                 a.load(nullptr, t);
                 b.load(nullptr, t);
-                if (live) compute(lds + (c & 1) * kStep);
+                if (live) {
+                    half(no, no, lds + (c & 1) * kStep, 0, fa, fb, nullptr, ga, gb);
+                    half(no, yes, lds + (c & 1) * kStep, 1, ga, gb, nullptr, fa, fb);
+#pragma unroll
+                    for (int m = 0; m < kMul; ++m) acc[m / TN][m % TN] = mfma16<XT>(gb[m % TN], ga[m / TN], acc[m / TN][m % TN]);
+                }
                 u32x4_t* o = lds + (~c & 1) * kStep;
                 a.store(o, t);
                 b.store(o + A::kUnits, t);
@@ -320,14 +378,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
     }
     if (!live) return;
     const int64_t row0 = OP == kGroupRows ? s.row : m0, base = OP == kGroupRows ? 0 : s.e * g.out_es;
+    const int g4 = lane >> 4;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int m = wm + 16 * i + (lane & 15);
-        if (m >= have) continue;
 #pragma unroll
         for (int j = 0; j < TN; j += 2) {
-            const int n = wn + 16 * j + 8 * (lane >> 4);
-            if (n < cols) grouped_store<OP>(g, base + (row0 + m) * g.out_ld + n0 + n, cols - n, acc[i][j], acc[i][j + 1]);
+            grouped_pair(acc[i][j], acc[i][j + 1]);
+            const int n = wn + 16 * (j + (g4 & 1)) + 8 * (g4 >> 1);
+            if (m < have && n < cols) grouped_store<OP>(g, base + (row0 + m) * g.out_ld + n0 + n, cols - n, acc[i][j], acc[i][j + 1]);
         }
     }
 }
@@ -341,8 +400,9 @@ static int launch_grouped(const char* name, GroupedArgs g, hipStream_t st) {
     const int64_t nmt = OP == kGroupRows ? group_slots(g.T, g.E, BM, g.rest) : (g.m + BM - 1) / BM * g.E;
     g.slots = (int)nmt;
     const int64_t tiles = nmt * ((g.n + BN - 1) / BN);
-    EXL3_CHECK_ARG(tiles <= kMx4Grid * 256 / (64 * WM * WN) - 7, "%s: grid too large", name);
-    EXL3_LAUNCH(name, (grouped_kernel<XT, OP, BACROSS, BM, BN, WM, WN, ST, OCC, DIRECT>), dim3((unsigned)((tiles + 7) & ~7)),
+    constexpr int64_t kRound = 8 * kChunk;
+    EXL3_CHECK_ARG(tiles <= kMx4Grid * 256 / (64 * WM * WN) - kRound, "%s: grid too large", name);
+    EXL3_LAUNCH(name, (grouped_kernel<XT, OP, BACROSS, BM, BN, WM, WN, ST, OCC, DIRECT>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)),
                 dim3(64 * WM * WN), 0, st, g);
     return EXL3_OK;
 }
