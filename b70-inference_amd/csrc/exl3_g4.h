@@ -53,6 +53,17 @@ __device__ __forceinline__ uint32_t g4_zero(int z) {
 template <int XT, bool Z>
 constexpr float kG4Scale = XT == kRowBF16 && !Z ? 16.f : 1.f;
 
+// The signed 4-bit number in the low bits of byte B, as sixteenths of 16 (the compiler shifts the byte down first, mostly).
+template <int B>
+__device__ __forceinline__ float g4_off(uint32_t w) {
+    float f;
+    if constexpr (B == 0) asm("v_cvt_off_f32_i4 %0, %1" : "=v"(f) : "v"(w));
+    if constexpr (B == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+    if constexpr (B == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+    if constexpr (B == 3) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+    return f;
+}
+
 // Eight q - z of a word, exact, in order: fp16 by setting the codes below 1024 and subtracting 1024 + z; bf16 by way of fp32, where
 // a conversion takes signed 4-bit numbers to sixteenths of them (z = 8), or signed bytes.
 template <int XT, bool Z>
@@ -67,10 +78,10 @@ __device__ __forceinline__ u32x4_t g4_frag(uint32_t w, uint32_t zero) {
                                                     __builtin_bit_cast(h2_t, zero));
     } else if constexpr (!Z) {
         const uint32_t e = w ^ 0x88888888u, o = e >> 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            r[i] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)__builtin_amdgcn_cvt_off_f32_i4((int)(e >> (8 * i))),
-                                                     (__bf16)__builtin_amdgcn_cvt_off_f32_i4((int)(o >> (8 * i)))});
+        r[0] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)g4_off<0>(e), (__bf16)g4_off<0>(o)});
+        r[1] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)g4_off<1>(e), (__bf16)g4_off<1>(o)});
+        r[2] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)g4_off<2>(e), (__bf16)g4_off<2>(o)});
+        r[3] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)g4_off<3>(e), (__bf16)g4_off<3>(o)});
     } else {
         const uint32_t e = ((w & 0x0F0F0F0Fu) + zero) ^ 0x80808080u, o = ((w >> 4 & 0x0F0F0F0Fu) + zero) ^ 0x80808080u;
 #pragma unroll
@@ -81,27 +92,6 @@ __device__ __forceinline__ u32x4_t g4_frag(uint32_t w, uint32_t zero) {
 }
 
 __device__ __forceinline__ float g4_scale(uint32_t v, int bf16) { return bf16 ? bf2f((uint16_t)v) : h2f((uint16_t)v); }
-
-// Scales at .. at + 3 of a row of `groups` that lies at p, 0 behind them. `left`: scales from p to the end of the tensor, which has
-// four or more: where a load would pass it, it begins earlier.
-__device__ __forceinline__ uint64_t g4_scales4(const uint16_t* p, int at, int groups, int64_t left) {
-    typedef uint64_t any_t __attribute__((aligned(2)));
-    const int in = groups - at;
-    if (in <= 0) return 0;
-    const int64_t over = at + 4 - left;
-    const int d = over > 0 ? (int)over : 0;
-    uint64_t v = *(const __attribute__((address_space(1))) any_t*)(p + at - d);
-    v >>= 16 * d;
-    return in >= 4 ? v : v & ((1ull << (16 * in)) - 1);
-}
-__device__ __forceinline__ uint32_t g4_zeros4(const uint8_t* p, int at, int groups, int64_t left) {
-    typedef uint32_t any_t __attribute__((aligned(1)));
-    if (at >= groups) return 0;
-    const int64_t over = at + 4 - left;
-    const int d = over > 0 ? (int)over : 0;
-    const uint32_t v = *(const __attribute__((address_space(1))) any_t*)(p + at - d);
-    return v >> (8 * d);
-}
 
 // Block of rows, and its expert's first matrix row: slot s of blocks of BM rows.
 template <int BM>
@@ -129,7 +119,7 @@ __device__ __forceinline__ void g4_store4(const G4Args& g, int64_t m, int64_t n,
         if (n + q < g.n) store_as(g.out, m * g.out_ld + n + q, v[q], g.out_dtype);
 }
 
-// tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows
+// tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows, 4, 5 of 32, 64 rows with split chunks
 int g4_run_f16(const G4Args& g, int group, int tile, hipStream_t st);
 int g4_run_bf16(const G4Args& g, int group, int tile, hipStream_t st);
 

@@ -83,7 +83,7 @@ static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, 
     const int64_t mean = m / E;
     int tile = mean <= 16 && k <= 8192 ? 0 : mean <= 48 ? 1 : mean <= 96 ? 2 : 3;
     const int want = env_int("EXL3MI_G4_TILE", 0);
-    if (want > (k <= 8192 ? 0 : 1) && want <= 4) tile = want - 1;
+    if (want > (k <= 8192 ? 0 : 1) && want <= 6) tile = want - 1;
     return dtype == EXL3_F16 ? g4_run_f16(g, (int)group, tile, st) : g4_run_bf16(g, (int)group, tile, st);
 }
 

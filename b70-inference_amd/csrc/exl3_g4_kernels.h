@@ -6,33 +6,49 @@
 
 namespace exl3 {
 
-// A weight row's scales (and zeros) of chunks that a load brings at once: four scales.
+// Where a wave's scales and zeros begin, and how many lie from there to the tensor's end.
+struct G4Base {
+    const uint16_t* s;
+    const uint8_t* z;
+    int left;
+    __device__ __forceinline__ G4Base(const G4Args& g, int64_t row, int64_t rows)
+        : s(g.scales + row * g.groups), z(g.zeros ? g.zeros + row * g.groups : nullptr) {
+        const int64_t n = (rows - row) * g.groups;
+        left = (int)(n < 0x40000000 ? n : 0x40000000);
+    }
+};
+
+// Four scales (and zeros) of a weight row from a chunk's first on: those of 4 / SG chunks. Kept as the loads bring them, so that nothing
+// waits where they are asked for; where a load would pass the tensor's end (which has four or more) it begins earlier.
 template <int XT, int SG, bool Z>
 struct G4Scales {
-    static constexpr int kChunks = 4 / SG;
     uint64_t s;
     uint32_t z;
-    __device__ __forceinline__ void load(const G4Args& g, int64_t row, int64_t rows, int chunk) {
-        const int64_t at = row * g.groups, left = (rows - row) * g.groups;
-        if (SG > 1 || g.per == 1) {    // uniform
-            s = g4_scales4(g.scales + at, SG * chunk, g.groups, left);
-            if constexpr (Z) z = g4_zeros4(g.zeros + at, SG * chunk, g.groups, left);
-        } else {                       // groups of several chunks: each chunk's own
-            s = 0;
-            z = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int G = (chunk + i) / g.per;
-                if (G < g.groups) {
-                    s |= (uint64_t)ldg(g.scales + at + G) << (16 * i);
-                    if constexpr (Z) z |= (uint32_t)ldg(g.zeros + at + G) << (8 * i);
-                }
-            }
-        }
+    __device__ __forceinline__ static int first(const G4Args& g, int chunk) { return SG > 1 || g.per == 1 ? SG * chunk : chunk / g.per; }
+    // `row`: where the row's begin, from the base
+    __device__ __forceinline__ static int back(const G4Base& b, int at) { return at + 4 > b.left ? at + 4 - b.left : 0; }
+    __device__ __forceinline__ void load(const G4Args& g, const G4Base& b, int row, int chunk) {
+        typedef uint64_t any8_t __attribute__((aligned(2)));
+        typedef uint32_t any4_t __attribute__((aligned(1)));
+        const int f = first(g, chunk), at = row + (f < g.groups ? f : 0), from = at - back(b, at);   // (behind the row: not used)
+        s = *(const __attribute__((address_space(1))) any8_t*)(b.s + from);
+        if constexpr (Z) z = *(const __attribute__((address_space(1))) any4_t*)(b.z + from);
     }
-    // scale i of the four
-    __device__ __forceinline__ float scale(int i, int bf16) const { return g4_scale((uint32_t)(s >> (16 * i)), bf16) * kG4Scale<XT, Z>; }
-    __device__ __forceinline__ uint32_t zero(int i) const { return g4_zero<XT, Z>(Z ? z >> (8 * i) & 255 : 8); }
+    // behind a load with the same arguments, where they are used: the first scale first
+    __device__ __forceinline__ void fix(const G4Args& g, const G4Base& b, int row, int chunk) {
+        const int d = back(b, row + first(g, chunk));
+        s >>= 16 * (d & 3);
+        if constexpr (Z) z >>= 8 * (d & 3);
+    }
+    // which of them is that of place i of chunk c (of 4 / SG from `chunk`)
+    __device__ __forceinline__ static int index(const G4Args& g, int chunk, int c, int i) {
+        return SG > 1 || g.per == 1 ? SG * (c - chunk) + i : c / g.per - chunk / g.per;
+    }
+    // scale i of the four; `in`: 0 for those that are not there, beside x that is 0
+    __device__ __forceinline__ float scale(int i, bool in, int bf16) const {
+        return in ? g4_scale((uint32_t)(s >> (16 * i)), bf16) * kG4Scale<XT, Z> : 0.f;
+    }
+    __device__ __forceinline__ uint32_t zero(int i) const { return g4_zero<XT, Z>(Z ? z >> (8 * i) & 15 : 8); }
 };
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -66,14 +82,15 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
         u32x4_t w[4];
         G4Scales<XT, SG, Z> sc[SG];
     };
+    typedef G4Scales<XT, SG, Z> S;
     const auto load = [&](int tile, Group& d) {
         const int64_t n0 = (int64_t)tile * 16, left = g.n - n0 < 16 ? g.n - n0 : 16;
         const __amdgpu_buffer_rsrc_t r = mx4_rsrc(codes + n0 * kb * 16, left * kb * 16);
 #pragma unroll
         for (int u = 0; u < 4; ++u) d.w[u] = mx4_buffer16(r, 4 * (c0 + u) + q4 < kb ? off + 64 * u : kMx4Out);
-        const int64_t n = n0 + l < g.n ? n0 + l : g.n - 1;
+        const G4Base b(g, row0 + n0, rows);
 #pragma unroll
-        for (int u = 0; u < SG; ++u) d.sc[u].load(g, row0 + n, rows, c0 + u * (4 / SG));
+        for (int u = 0; u < SG; ++u) d.sc[u].load(g, b, (l < left ? l : (int)left - 1) * g.groups, c0 + u * (4 / SG));
     };
     Group q, nx;
     load(first, q);
@@ -91,6 +108,12 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
     for (int tile = first; tile < tiles; tile += split, buf ^= 1) {
         if (tile + split < tiles) load(tile + split, nx);
         f4_t acc = {};
+        {
+            const int64_t n0 = (int64_t)tile * 16, left = g.n - n0 < 16 ? g.n - n0 : 16;
+            const G4Base b(g, row0 + n0, rows);
+#pragma unroll
+            for (int u = 0; u < SG; ++u) q.sc[u].fix(g, b, (l < left ? l : (int)left - 1) * g.groups, c0 + u * (4 / SG));
+        }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             if (4 * (c0 + u) >= kb) break;                     // uniform
@@ -98,13 +121,13 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
             g4_turn(w);
 #pragma unroll
             for (int i = 0; i < SG; ++i) {
-                const int at = u * SG + i;                     // of the sixteen or fewer scales
-                const uint32_t zero = q.sc[at / 4].zero(at & 3);
+                const int set = u * SG / 4, cf = c0 + set * (4 / SG), at = S::index(g, cf, c0 + u, i);
+                const uint32_t zero = q.sc[set].zero(at);
                 f4_t part = {};
 #pragma unroll
                 for (int v = i * (4 / SG); v < (i + 1) * (4 / SG); ++v)
                     part = mfma16<XT>(x[u][v], g4_frag<XT, Z>(w[v], zero), part);
-                const float sc = q.sc[at / 4].scale(at & 3, g.scale_bf16);
+                const float sc = q.sc[set].scale(at, S::first(g, cf) + at < g.groups, g.scale_bf16);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(sc, part[e], acc[e]);
             }
@@ -143,17 +166,158 @@ static int launch_g4_decode(G4Args g, hipStream_t st) {
     return EXL3_OK;
 }
 
+// ------------------------------------------------------------------------------------------------ some rows
+// Tiles of 16 RT rows x 64 outputs whose chunks go round the waves of a workgroup, which are added in order through LDS: more
+// workgroups, and fewer steps for each, than the tiles below have where those leave CUs idle or each wave one step after
+// another to wait for. A wave has its own chunks of x, so x comes straight into registers, half a chunk (64 inputs) ahead; the
+// weights and scales a chunk ahead. Output j of a wave's four is 4 (lane & 15) + j.
+template <int XT, int SG, bool Z, int RT>
+__global__ __launch_bounds__(512, 2) void g4_split_kernel(G4Args g) {
+    extern __shared__ f4_t red[];
+    const int lane = threadIdx.x & 63, l = lane & 15, q4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+              waves = blockDim.x >> 6;
+    const unsigned nnt = (unsigned)((g.n + 63) / 64), id = grouped_place(kChunk);
+    if (id >= g.slots * nnt) return;
+    unsigned mt, nt;
+    grouped_tile(id, (unsigned)g.slots, nnt, mt, nt);
+    const GroupSlot s = g4_slot<16 * RT>(g, mt);
+    if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
+    const int kb = g.k / 32, steps = s.e == g.E ? 0 : (kb + 3) / 4;
+    const int64_t n0 = (int64_t)nt * 64, row0 = (int64_t)(s.e < g.E ? s.e : 0) * g.n, rows = (int64_t)g.E * g.n;
+    const int left = (int)(g.n - n0 < 64 ? g.n - n0 : 64);
+    f4_t acc[RT][4];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[r][j] = f4_t{};
+    if (wave < steps) {
+        const __amdgpu_buffer_rsrc_t wr = mx4_rsrc(g.codes + (row0 + n0) * (kb * 16), (int64_t)left * kb * 16);
+        const uint32_t wo = (uint32_t)(4 * l) * (uint32_t)(kb * 16) + 16 * q4;
+        const auto load_w = [&](int c, u32x4_t (&w)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = mx4_buffer16(wr, 4 * c + q4 < kb ? wo + j * kb * 16 + 64 * c : kMx4Out);
+        };
+        const uint8_t* xp = reinterpret_cast<const uint8_t*>(g.x + s.row * g.x_ld);
+        uint32_t xo[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int m = 16 * r + l;
+            xo[r] = m < s.rows ? (uint32_t)m * (uint32_t)(2 * g.x_ld) + 16 * q4 : kMx4Out;
+        }
+        const auto load_x = [&](int c, int h, u32x4_t (&x)[RT][2]) {
+            const __amdgpu_buffer_rsrc_t xr = mx4_rsrc(xp + (c < steps ? (int64_t)c * 256 : 0), 0xE0000000LL);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+                    x[r][v] = mx4_buffer16(xr, 4 * c + 2 * h + v < kb && xo[r] != kMx4Out ? xo[r] + 128 * h + 64 * v : kMx4Out);
+        };
+        const G4Base sb(g, row0 + n0, rows);
+        typedef G4Scales<XT, SG, Z> S;
+        S sc[4], sn[4];
+        const auto srow = [&](int j) { return (4 * l + j < left ? 4 * l + j : left - 1) * g.groups; };
+        const auto load_s = [&](int c, G4Scales<XT, SG, Z> (&d)[4]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j].load(g, sb, srow(j), c);
+        };
+        u32x4_t w[4], nw[4], x[RT][2], nx[RT][2];
+        load_w(wave, nw);
+        load_s(wave, sn);
+        load_x(wave, 0, nx);
+#pragma unroll 1
+        for (int c = wave; c < steps; c += waves) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = nw[j];
+                sc[j] = sn[j];
+                sc[j].fix(g, sb, srow(j), c);
+            }
+            const int there = g.groups - S::first(g, c);       // scales from the chunk's first on
+            load_w(c + waves, nw);                             // (past the last: zeros)
+            load_s(c + waves, sn);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g4_turn(w[j]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) x[r][v] = nx[r][v];
+                load_x(h == 0 ? c : c + waves, 1 - h, nx);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // with groups of 64 and more one scale and zero for both products
+                    const int i0 = SG == 4 ? 2 * h : SG == 2 ? h : 0, i1 = SG == 4 ? i0 + 1 : i0;
+                    const u32x4_t f0 = g4_frag<XT, Z>(w[j][2 * h], sc[j].zero(i0)), f1 = g4_frag<XT, Z>(w[j][2 * h + 1], sc[j].zero(i1));
+                    const float s0 = sc[j].scale(i0, i0 < there, g.scale_bf16), s1 = SG == 4 ? sc[j].scale(i1, i1 < there, g.scale_bf16) : s0;
+                    f4_t p[RT];
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) p[r] = mfma16<XT>(x[r][0], f0, f4_t{});
+                    if constexpr (SG == 4) {
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[r][j][e] = __builtin_fmaf(s0, p[r][e], acc[r][j][e]);
+                            p[r] = f4_t{};
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) p[r] = mfma16<XT>(x[r][1], f1, p[r]);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[r][j][e] = __builtin_fmaf(s1, p[r][e], acc[r][j][e]);
+                }
+            }
+        }
+    }
+    // row 16 r + 4 q4 + e, outputs 4 l ..: piece 4 r + e of a wave; the pieces go round the waves
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            red[(wave * 4 * RT + 4 * r + e) * 64 + lane] = f4_t{acc[r][0][e], acc[r][1][e], acc[r][2][e], acc[r][3][e]};
+    __syncthreads();
+    for (int p = wave; p < 4 * RT; p += waves) {
+        const int m = 16 * (p >> 2) + 4 * q4 + (p & 3);
+        f4_t v = red[p * 64 + lane];
+        for (int u = 1; u < waves; ++u) {
+            const f4_t o = red[(u * 4 * RT + p) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += o[e];
+        }
+        if (m < s.rows) g4_store4(g, s.row + m, n0 + 4 * l, v);
+    }
+}
+
+template <int XT, int SG, bool Z, int RT>
+static int launch_g4_split(G4Args g, hipStream_t st) {
+    g.slots = (int)(g.ends ? group_slots(g.T, g.E, 16 * RT, g.rest) : (g.T + 16 * RT - 1) / (16 * RT));
+    const int64_t tiles = (int64_t)g.slots * ((g.n + 63) / 64), steps = (g.k + 127) / 128;
+    const int waves = steps < 8 ? (int)steps : 8;
+    constexpr int64_t kRound = 8 * kChunk;
+    EXL3_CHECK_ARG(tiles <= kMx4Grid / 2 - kRound, "g4: grid too large");
+    EXL3_LAUNCH("g4_split", (g4_split_kernel<XT, SG, Z, RT>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)), dim3(64 * waves),
+                (size_t)waves * 4 * RT * 1024, st, g);
+    return EXL3_OK;
+}
+
 // ------------------------------------------------------------------------------------------------ many rows
 // Tiles of BM rows x 256 outputs, 64 of them per wave, in steps of a chunk. x goes to one of two LDS buffers by direct loads (eight
 // values a unit, permuted as in the 16-bit products), the weights straight to the registers of the one wave that converts
-// them, both a step ahead. Tile j of a wave has outputs 4 (lane & 15) + j, so that a lane stores four neighbours.
+// them, both a step ahead, the scales four at a time. Tile j of a wave has outputs 4 (lane & 15) + j, so that a lane stores four
+// neighbours. Two of the four are converted and multiplied at a time, over pairs of 16 rows: four chains of MFMAs, whose sums are
+// scaled behind the next four.
 template <int XT, int SG, bool Z, int BM, int OCC>
 __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
     constexpr int kUnits = BM * 16, kLoads = kUnits / 256, RT = BM / 16;
-    __shared__ u32x4_t lds[2 * kUnits];
+    __shared__ u32x4_t lds[2 * kUnits + 4 * (Z ? 128 : 64)];   // x, and the waves' scales and zeros
     const int t = threadIdx.x, lane = t & 63, l = lane & 15, q4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    unsigned mt, nt, sp;
-    if (!mx4_tile_of((unsigned)g.slots, (unsigned)((g.n + 255) / 256), 1, mt, nt, sp)) return;
+    const unsigned nnt = (unsigned)((g.n + 255) / 256), id = grouped_place(kChunk);
+    if (id >= g.slots * nnt) return;
+    unsigned mt, nt;
+    grouped_tile(id, (unsigned)g.slots, nnt, mt, nt);
     const GroupSlot s = g4_slot<BM>(g, mt);
     if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
     const int kb = g.k / 32, steps = s.e == g.E ? 0 : (kb + 3) / 4;
@@ -165,81 +329,102 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
         for (int j = 0; j < 4; ++j) acc[i][j] = f4_t{};
     if (steps > 0) {
         // x: unit u of a row lies at u ^ (row & 15)
-        const __amdgpu_buffer_rsrc_t xr = mx4_rsrc(reinterpret_cast<const uint8_t*>(g.x + s.row * g.x_ld), 0xE0000000LL);
+        const uint8_t* xp = reinterpret_cast<const uint8_t*>(g.x + s.row * g.x_ld);
         uint32_t xo[kLoads];
-        const int xu = t & 15;
+        const int xu = (t & 15) ^ (t >> 4 & 15);               // this thread's unit, alike in all its rows
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int r = (t >> 4) + 16 * i;
-            xo[i] = r < s.rows ? (uint32_t)r * (uint32_t)(2 * g.x_ld) + 16 * (xu ^ (r & 15)) : kMx4Out;
+            xo[i] = r < s.rows ? (uint32_t)r * (uint32_t)(2 * g.x_ld) + 16 * xu : kMx4Out;
         }
-        const int block = (xu ^ (t >> 4 & 15)) >> 2;           // of the chunk, that this thread's units lie in (alike for all i)
         const auto load_x = [&](int c) {
+            const __amdgpu_buffer_rsrc_t xr = mx4_rsrc(xp + (c < steps ? (int64_t)c * 256 : 0), 0xE0000000LL);
+            const bool in = 4 * c + (xu >> 2) < kb;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(lds + (c & 1) * kUnits + wave * 64 + i * 256),
-                                                         16, (int)(4 * c + block < kb && xo[i] != kMx4Out ? xo[i] + 256 * c : kMx4Out), 0, 0, 0);
+            for (int i = 0; i < kLoads; ++i) lds_load16(xr, in ? xo[i] : kMx4Out, lds + (c & 1) * kUnits + wave * 64 + i * 256);
         };
         const int64_t left = g.n - n0 < 64 ? (g.n > n0 ? g.n - n0 : 0) : 64;
         const __amdgpu_buffer_rsrc_t wr = mx4_rsrc(g.codes + (row0 + (left > 0 ? n0 : 0)) * (kb * 16), left * kb * 16);
         const uint32_t wo = (uint32_t)(4 * l) * (uint32_t)(kb * 16) + 16 * q4;
-        const auto load_w = [&](int c, u32x4_t (&w)[4]) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = mx4_buffer16(wr, 4 * c + q4 < kb ? wo + j * kb * 16 + 64 * c : kMx4Out);
+        const auto next_w = [&](int c, int j) {
+            return mx4_buffer16(wr, 4 * c + q4 < kb ? wo + j * kb * 16 + 64 * c : kMx4Out);
         };
-        G4Scales<XT, SG, Z> sc[4];
-        const auto load_s = [&](int c) {
+        // Scales and zeros: lane r brings four of the wave's row r and lays them out in LDS as they are used, [four][64 rows].
+        const G4Base sb(g, row0 + (left > 0 ? n0 : 0), rows);
+        const int srow = (lane < left ? lane : left > 0 ? (int)left - 1 : 0) * g.groups;
+        typedef G4Scales<XT, SG, Z> S;
+        S raw;
+        float* const ls = reinterpret_cast<float*>(lds + 2 * kUnits) + wave * (Z ? 512 : 256);
+        uint32_t* const lz = reinterpret_cast<uint32_t*>(ls + 256);
+        u32x4_t w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t n = n0 + 4 * l + j;
-                sc[j].load(g, row0 + (n < g.n ? n : g.n - 1), rows, c);
-            }
-        };
-        u32x4_t nx[4];
+        for (int j = 0; j < 4; ++j) w[j] = next_w(0, j);
+        raw.load(g, sb, srow, 0);
         load_x(0);
-        load_w(0, nx);
         for (int c = 0; c < steps; ++c) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0070);                // vmcnt(0) lgkmcnt(0)
+            asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
-            u32x4_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = nx[j];
             const int at = c % (4 / SG) * SG;
-            if (at == 0) load_s(c);
-            load_x(c + 1);                                     // (past the last: zeros)
-            load_w(c + 1, nx);
+            if (SG == 4 || at == 0) {                          // uniform
+                raw.fix(g, sb, srow, c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g4_turn(w[j]);
-            const u32x4_t* xb = lds + (c & 1) * kUnits;
-#pragma unroll
-            for (int i = 0; i < SG; ++i) {
-                constexpr int V = 4 / SG;
-                u32x4_t f[4][V];
-                float scale[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t zero = sc[j].zero(at + i);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) f[j][v] = g4_frag<XT, Z>(w[j][i * V + v], zero);
-                    scale[j] = sc[j].scale(at + i, g.scale_bf16);
+                for (int i = 0; i < 4; ++i) {
+                    const int k = S::index(g, c, c + i / SG, i % SG);
+                    ls[64 * i + lane] = raw.scale(k, S::first(g, c) + k < g.groups, g.scale_bf16);
+                    if constexpr (Z) lz[64 * i + lane] = raw.zero(k);
                 }
+                raw.load(g, sb, srow, c + 4 / SG);             // (past the last: not used)
+            }
+            load_x(c + 1);
+            const u32x4_t* xb = lds + (c & 1) * kUnits;
+            const auto read_x = [&](int r, u32x4_t (&x)[4]) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) x[v] = xb[(16 * r + l) * 16 + ((4 * v + q4) ^ l)];
+            };
+#pragma unroll
+            for (int jp = 0; jp < 4; jp += 2) {
+                u32x4_t f[2][4], x[2][4];
+                read_x(0, x[0]);
+                f2_t scale[SG];
+                uint2 zero[SG];
+#pragma unroll
+                for (int i = 0; i < SG; ++i) {
+                    scale[i] = *reinterpret_cast<const f2_t*>(ls + 64 * (at + i) + 4 * l + jp);
+                    if constexpr (Z) zero[i] = *reinterpret_cast<const uint2*>(lz + 64 * (at + i) + 4 * l + jp);
+                    else zero[i] = make_uint2(g4_zero<XT, Z>(8), g4_zero<XT, Z>(8));
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    g4_turn(w[jp + j]);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) f[j][v] = g4_frag<XT, Z>(w[jp + j][v], j ? zero[v / (4 / SG)].y : zero[v / (4 / SG)].x);
+                    w[jp + j] = next_w(c + 1, jp + j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    f4_t part[4] = {};
+                    if (r + 1 < RT) read_x(r + 1, x[(r + 1) & 1]);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const u32x4_t xv = xb[(16 * r + l) * 16 + ((4 * (i * V + v) + q4) ^ l)];
+                    for (int i = 0; i < SG; ++i) {
+                        constexpr int V = 4 / SG;
+                        f4_t part[2] = {};
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) part[j] = mfma16<XT>(xv, f[j][v], part[j]);
+                        for (int v = i * V; v < (i + 1) * V; ++v)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) part[j] = mfma16<XT>(x[r & 1][v], f[j][v], part[j]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[r][jp + j][e] = __builtin_fmaf(scale[i][j], part[j][e], acc[r][jp + j][e]);
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[r][j][e] = __builtin_fmaf(scale[j], part[j][e], acc[r][j][e]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // the LDS is the next workgroup's behind the end
+        __builtin_amdgcn_s_waitcnt(0x0070);                    // the LDS is the next workgroup's behind the end
+        asm volatile("" ::: "memory");
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -254,18 +439,21 @@ template <int XT, int SG, bool Z, int BM, int OCC>
 static int launch_g4_wide(G4Args g, hipStream_t st) {
     g.slots = (int)(g.ends ? group_slots(g.T, g.E, BM, g.rest) : (g.T + BM - 1) / BM);
     const int64_t tiles = (int64_t)g.slots * ((g.n + 255) / 256);
-    EXL3_CHECK_ARG(tiles <= kMx4Grid - 7, "g4: grid too large");
-    EXL3_LAUNCH("g4_wide", (g4_wide_kernel<XT, SG, Z, BM, OCC>), dim3((unsigned)((tiles + 7) & ~7)), dim3(256), 0, st, g);
+    constexpr int64_t kRound = 8 * kChunk;
+    EXL3_CHECK_ARG(tiles <= kMx4Grid - kRound, "g4: grid too large");
+    EXL3_LAUNCH("g4_wide", (g4_wide_kernel<XT, SG, Z, BM, OCC>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)), dim3(256), 0,
+                st, g);
     return EXL3_OK;
 }
 
 template <int XT, int SG, bool Z>
 static int launch_g4(const G4Args& g, int tile, hipStream_t st) {
-    return tile == 0 ? launch_g4_decode<XT, SG, Z>(g, st) : tile == 1 ? launch_g4_wide<XT, SG, Z, 32, 4>(g, st)
-         : tile == 2 ? launch_g4_wide<XT, SG, Z, 64, 3>(g, st) : launch_g4_wide<XT, SG, Z, 128, 2>(g, st);
+    return tile == 0 ? launch_g4_decode<XT, SG, Z>(g, st) : tile == 1 ? launch_g4_wide<XT, SG, Z, 32, 3>(g, st)
+         : tile == 2 ? launch_g4_wide<XT, SG, Z, 64, 2>(g, st) : tile == 3 ? launch_g4_wide<XT, SG, Z, 128, 2>(g, st)
+         : tile == 4 ? launch_g4_split<XT, SG, Z, 2>(g, st) : launch_g4_split<XT, SG, Z, 4>(g, st);
 }
 
-// tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows
+// tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows, 4, 5 of 32, 64 rows with split chunks
 template <int XT>
 static int launch_g4(const G4Args& g, int group, int tile, hipStream_t st) {
     if (g.zeros)

@@ -64,4 +64,25 @@ __device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int 
     return s;
 }
 
+// This workgroup's place in a grid that takes `chunk` tiles after one another on an XCD, the XCDs in turn (workgroups go round robin over
+// them): what runs together on one shares operands in its L2, and tiles of little work (experts of few rows) spread over all.
+__device__ __forceinline__ unsigned grouped_place(unsigned chunk) {
+    const unsigned j = blockIdx.x >> 3, c = j / chunk;
+    return (c * 8 + (blockIdx.x & 7)) * chunk + j - c * chunk;
+}
+// Tile `in` of nmt x nnt: eight rows of tiles after one another for each column.
+__device__ __forceinline__ void grouped_tile(unsigned in, unsigned nmt, unsigned nnt, unsigned& mt, unsigned& nt) {
+    const unsigned band = in / (8 * nnt), i = in - band * 8 * nnt, h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
+    nt = i / h;
+    mt = 8 * band + i - nt * h;
+}
+constexpr unsigned kChunk = 32;        // the CUs of an XCD
+
+// 16 bytes per lane from `at` bytes on to LDS (address `lds` and 16 bytes a lane from there on). Inline assembly: behind the builtin
+// the compiler waits for the load before every transposing read, whatever it reads. What it brings is waited for by wait_step.
+__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t at, const void* lds) {
+    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(r));
+}
+
 }  // namespace exl3

@@ -35,13 +35,6 @@ struct GroupedArgs {
 
 enum { kGroupRows = 0, kGroupWeights = 1 };
 
-// 16 bytes per lane from `at` bytes on to LDS (address `lds` and 16 bytes a lane from there on). Inline assembly: behind the builtin
-// the compiler waits for the load before every transposing read, whatever it reads. What it brings is waited for by wait_step.
-__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t at, const void* lds) {
-    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(r));
-}
-
 // Four values of a column each, from 4 rows of 16 columns: sixteen lanes give the addresses of four neighbours.
 typedef short s4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint2 lds_read_tr(const char* p) {
@@ -212,20 +205,6 @@ __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, i
     }
     *o = r;
 }
-
-// This workgroup's place in a grid that takes `chunk` tiles after one another on an XCD, the XCDs in turn (workgroups go round robin over
-// them): what runs together on one shares operands in its L2, and tiles of little work (experts of few rows) spread over all.
-__device__ __forceinline__ unsigned grouped_place(unsigned chunk) {
-    const unsigned j = blockIdx.x >> 3, c = j / chunk;
-    return (c * 8 + (blockIdx.x & 7)) * chunk + j - c * chunk;
-}
-// Tile `in` of nmt x nnt: eight rows of tiles after one another for each column.
-__device__ __forceinline__ void grouped_tile(unsigned in, unsigned nmt, unsigned nnt, unsigned& mt, unsigned& nt) {
-    const unsigned band = in / (8 * nnt), i = in - band * 8 * nnt, h = nmt - 8 * band < 8 ? nmt - 8 * band : 8;
-    nt = i / h;
-    mt = 8 * band + i - nt * h;
-}
-constexpr unsigned kChunk = 32;        // the CUs of an XCD
 
 template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs g) {
