@@ -69,13 +69,15 @@ SIGNATURES = {
     "exl3_grouped_mm": [_vp, _i64, _i32, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp],
     "exl3_grouped_mm_dw": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp],
     "exl3_g4_linear": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp],
+    "exl3_g4_linear_in": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp],
+    "exl3_g4_linear_scratch": [_i64, _i64, _i64, _i64],
     "exl3_grouped_g4": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp],
     "exl3_route_balance": [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp],
     "exl3_route_balance_grad": [_vp, _i64, _i64, _i64, _i64, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp],
     "exl3_router_logits": [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
 }
 _RESTYPE = {"exl3_last_error": ctypes.c_char_p, "exl3_mx4_linear_scratch": _i64, "exl3_mx4_gemm_scratch": _i64,
-            "exl3_mx4_moe_scratch": _i64, "exl3_route_balance_scratch": _i64}
+            "exl3_mx4_moe_scratch": _i64, "exl3_g4_linear_scratch": _i64, "exl3_route_balance_scratch": _i64}
 
 _lib = None
 

@@ -32,6 +32,10 @@ struct G4Args {
     int groups, per;                   // scales of a row; chunks of 128 that share one (groups of 32 and 64: 1)
     int scale_bf16, out_dtype, vec, rest;
     int slots;                         // row blocks of the grid
+    // steps of 128 inputs split over workgroups: `splits` of `spc`, their sums in part [splits][T][n4] (n4: n rounded up to 4)
+    int splits, spc;
+    float* part;
+    int64_t n4;
 };
 
 // 4 x 4 words of lane groups and blocks turned.
@@ -91,7 +95,11 @@ __device__ __forceinline__ u32x4_t g4_frag(uint32_t w, uint32_t zero) {
     return r;
 }
 
-__device__ __forceinline__ float g4_scale(uint32_t v, int bf16) { return bf16 ? bf2f((uint16_t)v) : h2f((uint16_t)v); }
+// A scale of either type, or 0 where it is not there (masks: a choice that is alike in all lanes becomes a branch).
+__device__ __forceinline__ float g4_scale(uint32_t v, int bf16, bool in = true) {
+    const uint32_t m = -(uint32_t)bf16, k = -(uint32_t)in;
+    return __builtin_bit_cast(float, ((v << 16 & m) | (__builtin_bit_cast(uint32_t, h2f((uint16_t)v)) & ~m)) & k);
+}
 
 // Block of rows, and its expert's first matrix row: slot s of blocks of BM rows.
 template <int BM>
@@ -119,7 +127,13 @@ __device__ __forceinline__ void g4_store4(const G4Args& g, int64_t m, int64_t n,
         if (n + q < g.n) store_as(g.out, m * g.out_ld + n + q, v[q], g.out_dtype);
 }
 
-// tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows, 4, 5 of 32, 64 rows with split chunks
+// The same of split sp: the output, or its sums.
+__device__ __forceinline__ void g4_put4(const G4Args& g, unsigned sp, int64_t m, int64_t n, f4_t v) {
+    if (!g.part) g4_store4(g, m, n, v);
+    else if (n < g.n4) *reinterpret_cast<f4_t*>(g.part + ((int64_t)sp * g.T + m) * g.n4 + n) = v;
+}
+
+// tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows
 int g4_run_f16(const G4Args& g, int group, int tile, hipStream_t st);
 int g4_run_bf16(const G4Args& g, int group, int tile, hipStream_t st);
 

@@ -29,11 +29,69 @@ __global__ __launch_bounds__(256) void g4_tiny_kernel(G4Args g, int group) {
     store_as(g.out, m * g.out_ld + n, sum + (g.bias ? ldg(g.bias + n) : 0.f), g.out_dtype);
 }
 
+// The splits' sums in order, the bias, one rounding.
+__global__ __launch_bounds__(256) void g4_reduce_kernel(G4Args g) {
+    const int64_t q4 = g.n4 / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / q4, n = 4 * (i - m * q4);
+    if (m >= g.T) return;
+    const float* p = g.part + m * g.n4 + n;
+    f4_t v = {};
+    for (int s0 = 0; s0 < g.splits; s0 += 4) {
+        f4_t t[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            t[s] = ldg(reinterpret_cast<const f4_t*>(p + (int64_t)(s0 + s < g.splits ? s0 + s : s0) * g.T * g.n4));
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s0 + s < g.splits)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += t[s][e];
+    }
+    g4_store4(g, m, n, v);
+}
+
+// Kernel and splits of a call: the least time by an estimate from measurements (4096 -> 4096 and 5376 -> 21504 at 1 to 512 rows), in
+// microseconds for 256 CUs. Splits are the linear's alone (experts have workgroups enough, or few rows).
+struct G4Plan {
+    int tile, splits, spc;
+};
+static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t E) {
+    const int64_t steps = (k + 127) / 128;
+    G4Plan best = {0, 1, (int)steps};
+    double least = 1e30;
+    // blocks of 16 rows: a workgroup's waves hold 512 inputs each; more of them to a CU take longer for each tile
+    const int64_t live = E == 1 ? (m + 15) / 16 : m / 16 + (m < E ? m : E);
+    if (k <= 8192 && (E == 1 || m <= 16 * E)) {
+        const int64_t waves = (k + 511) / 512, per = 16 / waves < 4 ? 16 / waves : 4;
+        least = 7.0 + (double)(live * ((n + 15) / 16)) / (double)(256 * per) * (0.5 + 0.3 * (double)(waves * per));
+    }
+    // blocks of 32, 64, 128 rows: time of a step with one, two, three workgroups to a CU, full rounds and what is left
+    static const double kStep[3][3] = {{1.45, 2.05, 2.85}, {1.65, 2.6, 2.6}, {2.6, 3.9, 3.9}};
+    static const int kOcc[3] = {3, 2, 2};
+    for (int t = 0; t < 3; ++t) {
+        const int64_t bm = 32 << t, blocks = E == 1 ? (m + bm - 1) / bm : m / bm + (m < E ? m : E), tiles = blocks * ((n + 255) / 256);
+        for (int64_t p = 1; p <= (E > 1 ? 1 : steps < 16 ? steps : 16); ++p) {
+            const int64_t spc = (steps + p - 1) / p, full = tiles * p / (256 * kOcc[t]), left = tiles * p - full * 256 * kOcc[t];
+            if ((steps + spc - 1) / spc != p) continue;
+            double us = 2.0 + (double)full * (3.0 + (double)spc * kStep[t][kOcc[t] - 1]);
+            if (left) us += 3.0 + (double)spc * kStep[t][(left + 255) / 256 - 1];
+            if (p > 1) us += 3.0 + (double)(p * m * n) * 1.6e-6;
+            if (us < least) {
+                least = us;
+                best = {t + 1, (int)p, (int)spc};
+            }
+        }
+    }
+    return best;
+}
+static int64_t g4_n4(int64_t n) { return (n + 3) & ~(int64_t)3; }
+static int64_t g4_part_bytes(const G4Plan& p, int64_t m, int64_t n) { return p.splits == 1 ? 0 : (int64_t)p.splits * m * g4_n4(n) * 4; }
+
 static int out_size(int t) { return t == EXL3_F32 ? 4 : 2; }
 
 static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, int64_t m, int64_t k, const uint8_t* codes,
                       const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const int32_t* ends,
-                      int64_t E, const float* bias, void* out, int64_t out_ld, int out_dtype, int rest, void* stream) {
+                      int64_t E, const float* bias, void* out, int64_t out_ld, int out_dtype, int rest, const CallScratch& s,
+                      void* stream) {
     EXL3_CHECK_ARG(m >= 0 && m <= 0x3FFFFFFF && n > 0 && n <= 0x3FFFFFFF && E > 0 && E <= 65536 && k > 0 && k <= (1 << 22) &&
                        k % 32 == 0 && n * E <= ((int64_t)1 << 42) / k,
                    "%s: bad sizes (%lld rows, %lld outputs, %lld inputs, %lld matrices; inputs a multiple of 32)", what,
@@ -80,11 +138,24 @@ static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, 
         else EXL3_LAUNCH("g4_tiny", g4_tiny_kernel<kRowBF16>, grid, dim3(256), 0, st, g, (int)group);
         return EXL3_OK;
     }
-    const int64_t mean = m / E;
-    int tile = mean <= 16 && k <= 8192 ? 0 : mean <= 48 ? 1 : mean <= 96 ? 2 : 3;
+    G4Plan plan = g4_plan(m, n, k, E);
     const int want = env_int("EXL3MI_G4_TILE", 0);
-    if (want > (k <= 8192 ? 0 : 1) && want <= 6) tile = want - 1;
-    return dtype == EXL3_F16 ? g4_run_f16(g, (int)group, tile, st) : g4_run_bf16(g, (int)group, tile, st);
+    if (want > (k <= 8192 ? 0 : 1) && want <= 4) plan = {want - 1, 1, (int)((k + 127) / 128)};
+    g.splits = plan.splits;
+    g.spc = plan.spc;
+    g.n4 = g4_n4(n);
+    if (plan.splits > 1) {
+        Carve c{};
+        const int rc = call_scratch(what, (size_t)g4_part_bytes(plan, m, n), s, st, &c);
+        if (rc) return rc;
+        g.part = reinterpret_cast<float*>(c.p);
+    }
+    const int rc = dtype == EXL3_F16 ? g4_run_f16(g, (int)group, plan.tile, st) : g4_run_bf16(g, (int)group, plan.tile, st);
+    if (rc || plan.splits == 1) return rc;
+    const int64_t wgs = (m * (g.n4 / 4) + 255) / 256;
+    EXL3_CHECK_ARG(wgs <= kMx4Grid, "%s: grid too large", what);
+    EXL3_LAUNCH("g4_reduce", g4_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, g);
+    return EXL3_OK;
 }
 
 }  // namespace exl3
@@ -93,11 +164,23 @@ extern "C" {
 
 using namespace exl3;
 
+int64_t exl3_g4_linear_scratch(int64_t m, int64_t k, int64_t n, int64_t group) {
+    if (m <= 0 || m > 0x3FFFFFFF || n <= 0 || n > 0x3FFFFFFF || k <= 0 || k > (1 << 22) || group <= 0 || n * (k / group) < 4) return 0;
+    return g4_part_bytes(g4_plan(m, n, k, 1), m, n);
+}
+
 int exl3_g4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const void* scales,
                    int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,
                    int c_dtype, void* stream) {
     return g4_product("exl3_g4_linear", x, x_ld, x_dtype, m, k, codes, scales, scale_dtype, zeros, group, n, nullptr, 1, bias, C, c_ld,
-                      c_dtype, 0, stream);
+                      c_dtype, 0, kLibScratch, stream);
+}
+
+int exl3_g4_linear_in(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const void* scales,
+                      int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,
+                      int c_dtype, void* scratch, int64_t scratch_bytes, void* stream) {
+    return g4_product("exl3_g4_linear", x, x_ld, x_dtype, m, k, codes, scales, scale_dtype, zeros, group, n, nullptr, 1, bias, C, c_ld,
+                      c_dtype, 0, CallScratch{scratch, scratch_bytes, false}, stream);
 }
 
 int exl3_grouped_g4(const void* x, int64_t x_ld, int x_dtype, int64_t T, int64_t k, const uint8_t* codes, const void* scales,
@@ -106,7 +189,7 @@ int exl3_grouped_g4(const void* x, int64_t x_ld, int x_dtype, int64_t T, int64_t
     EXL3_CHECK_ARG(ends, "exl3_grouped_g4: null pointer");
     EXL3_CHECK_ARG(rest == 0 || rest == 1, "exl3_grouped_g4: rest %d", rest);
     return g4_product("exl3_grouped_g4", x, x_ld, x_dtype, T, k, codes, scales, scale_dtype, zeros, group, n, ends, E, nullptr, out,
-                      out_ld, out_dtype, rest, stream);
+                      out_ld, out_dtype, rest, kLibScratch, stream);
 }
 
 }  // extern "C"

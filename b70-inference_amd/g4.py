@@ -8,14 +8,15 @@ w = (q - z) s: whole numbers q from 0 to 15, and for each `group` neighbouring i
     projection for ExpertTables or BC_GatedMLP)
   * grouped_mm(x, G4Tensor [E, n, k], ends)        rows sorted by expert
 No weight is rounded: q - z is exact in the rows' type and the scales multiply fp32 sums. Tensors live on the GPU; every op is
-asynchronous on the current stream of its tensors' device and needs no scratch. The reference has no counterpart: its weights are EXL3
+asynchronous on the current stream of its tensors' device and has scratch of its own where it needs some (calls may overlap on streams
+and threads, and can be captured without a warm-up). The reference has no counterpart: its weights are EXL3
 only.
 """
 from __future__ import annotations
 
 import torch
 
-from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, stream_of
+from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, scratch, stream_of
 from .mx4 import DTYPES, _bias, _out2, _rows
 
 _HALF = {torch.float16: EXL3_F16, torch.bfloat16: EXL3_BF16}
@@ -80,10 +81,11 @@ class G4Linear:
             x = x.half()
         x2, m, ld = _rows(x, k)
         y2, y_ld = _out2("G4Linear", y, m, n)
+        ws, need = scratch("exl3_g4_linear", x, m, k, n, w.group)
         with where:
-            rc = lib().exl3_g4_linear(x2.data_ptr(), ld, _HALF[x.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(),
-                                      _HALF[w.scales.dtype], ptr(w.zeros), w.group, n, ptr(self.bias), y2.data_ptr(), y_ld,
-                                      DTYPES[y.dtype], stream_of(x))
+            rc = lib().exl3_g4_linear_in(x2.data_ptr(), ld, _HALF[x.dtype], m, k, w.codes.data_ptr(), w.scales.data_ptr(),
+                                         _HALF[w.scales.dtype], ptr(w.zeros), w.group, n, ptr(self.bias), y2.data_ptr(), y_ld,
+                                         DTYPES[y.dtype], ptr(ws), need, stream_of(x))
         if rc:
             check(rc, "g4_linear")
 

@@ -408,7 +408,7 @@ int exl3_grouped_mm_dw(const void* dy, int64_t dy_ld, const void* x, int64_t x_l
  * (32, 64 or a multiple of 128, others EXL3_ERR_UNSUPPORTED) of an output one scale s (fp16 or bf16) and one z from 0 to 15 (8 with
  * zeros NULL). A matrix of n outputs and k inputs (k a multiple of the group) is codes uint8 [n, k / 2] (16-byte aligned), scales
  * [n, k / group], zeros uint8 [n, k / group], all contiguous. No weight is rounded: fp32 sums of exact products with q - z, times s,
- * in an order fixed by the sizes; one rounding. No scratch; calls may overlap. No reference counterpart. */
+ * in an order fixed by the sizes; one rounding. No reference counterpart. */
 
 /* C[m, n] = x @ W^T (+ bias) for x fp16 or bf16 [m, k] (row stride x_ld, rows 16-byte aligned), bias fp32 [n] or NULL, C fp16, bf16
  * or fp32 (row stride c_ld). */
@@ -416,8 +416,14 @@ int exl3_g4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t 
                    int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,
                    int c_dtype, void* stream);
 
+/* With scratch from the caller, as the _in calls above; calls of up to 16 rows and some others need none. */
+int64_t exl3_g4_linear_scratch(int64_t m, int64_t k, int64_t n, int64_t group);
+int exl3_g4_linear_in(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const void* scales,
+                      int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,
+                      int c_dtype, void* scratch, int64_t scratch_bytes, void* stream);
+
 /* exl3_grouped_mm over E such matrices, one behind the other: out[t, n] of the rows t of expert e = x[t] @ W_e^T, `ends` and `rest` as
- * there. */
+ * there; no scratch. */
 int exl3_grouped_g4(const void* x, int64_t x_ld, int x_dtype, int64_t T, int64_t k, const uint8_t* codes, const void* scales,
                     int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const int32_t* ends, int64_t E, void* out,
                     int64_t out_ld, int out_dtype, int rest, void* stream);
