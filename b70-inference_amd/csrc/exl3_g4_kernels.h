@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
     constexpr int kUnits = BM * 16, kLoads = kUnits / 256, RT = BM / 16;
     __shared__ u32x4_t lds[2 * kUnits + 4 * (Z ? 128 : 64)];   // x, and the waves' scales and zeros
     const int t = threadIdx.x, lane = t & 63, l = lane & 15, q4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const unsigned nnt = (unsigned)((g.n + 255) / 256), all = g.slots * nnt, id = grouped_place(kChunk);
+    const unsigned nnt = (unsigned)((g.n + 255) / 256), all = g.slots * nnt, id = grouped_place(kChunk, blockIdx.x);
     if (id >= all * g.splits) return;
     const unsigned sp = id / all;
     unsigned mt, nt;

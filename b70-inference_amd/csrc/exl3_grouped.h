@@ -64,11 +64,23 @@ __device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int 
     return s;
 }
 
-// This workgroup's place in a grid that takes `chunk` tiles after one another on an XCD, the XCDs in turn (workgroups go round robin over
+// The blocks there are, with `rest` those of the rows of none (wave-uniform).
+template <int BM>
+__device__ __forceinline__ unsigned group_blocks(const int32_t* ends, int E, int T, bool rest) {
+    int n = 0;
+    for (int i = 0; i < E + (rest ? 1 : 0); i += 64) {
+        const int e = i + (threadIdx.x & 63);
+        const int lo = e > 0 ? group_end(ends, e <= E ? e - 1 : E - 1, T) : 0, hi = e < E ? group_end(ends, e, T) : e == E && rest ? T : lo;
+        n += __builtin_amdgcn_readlane(wave_running_sum(hi > lo ? (hi - lo + BM - 1) / BM : 0), 63);
+    }
+    return (unsigned)n;
+}
+
+// A workgroup's place in a grid that takes `chunk` tiles after one another on an XCD, the XCDs in turn (workgroups go round robin over
 // them): what runs together on one shares operands in its L2, and tiles of little work (experts of few rows) spread over all.
-__device__ __forceinline__ unsigned grouped_place(unsigned chunk) {
-    const unsigned j = blockIdx.x >> 3, c = j / chunk;
-    return (c * 8 + (blockIdx.x & 7)) * chunk + j - c * chunk;
+__device__ __forceinline__ unsigned grouped_place(unsigned chunk, unsigned block) {
+    const unsigned j = block >> 3, c = j / chunk;
+    return (c * 8 + (block & 7)) * chunk + j - c * chunk;
 }
 // Tile `in` of nmt x nnt: eight rows of tiles after one another for each column.
 __device__ __forceinline__ void grouped_tile(unsigned in, unsigned nmt, unsigned nnt, unsigned& mt, unsigned& nt) {

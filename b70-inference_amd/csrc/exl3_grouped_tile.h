@@ -30,7 +30,6 @@ struct GroupedArgs {
     int out_dtype, vec;                // vec: eight neighbouring outputs may be stored as 16-byte pieces
     int rest;                          // rows of no expert become 0
     int accumulate;                    // the weights' gradient is added to what out holds
-    int slots;                         // row blocks of the grid
 };
 
 enum { kGroupRows = 0, kGroupWeights = 1 };
@@ -206,7 +205,8 @@ __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, i
     *o = r;
 }
 
-template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
+// ROUND: one workgroup to a CU, which goes round the tiles.
+template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT, bool ROUND>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs g) {
     constexpr int kThreads = 64 * WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
     static_assert(TM > 0 && TN > 1 && TN % 2 == 0, "pairs of tiles");
@@ -216,53 +216,63 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
     __shared__ u32x4_t lds[ST * kStep];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const unsigned nnt = (unsigned)((g.n + BN - 1) / BN);
-    unsigned mt, nt;
-    const unsigned id = grouped_place(kChunk);
-    GroupSlot s;
-    int64_t m0 = 0;
-    int have, left;
-    if constexpr (OP == kGroupRows) {
-        if (id >= g.slots * nnt) return;
-        grouped_tile(id, (unsigned)g.slots, nnt, mt, nt);
-        s = group_slot<BM>(g.ends, g.E, g.T, mt);
-        if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
-        have = s.rows;
-        left = s.e == g.E ? 0 : g.c;
-    } else {
-        const unsigned nmt = (unsigned)((g.m + BM - 1) / BM);
-        if (id >= nmt * nnt * g.E) return;
-        s.e = (int)(id / (nmt * nnt));
-        grouped_tile(id - s.e * (nmt * nnt), nmt, nnt, mt, nt);
-        const int lo = __builtin_amdgcn_readfirstlane(s.e > 0 ? group_end(g.ends, s.e - 1, g.T) : 0);
-        const int hi = __builtin_amdgcn_readfirstlane(group_end(g.ends, s.e, g.T));
-        s.row = lo;
-        s.rows = hi > lo ? hi - lo : 0;
-        if (g.accumulate && s.rows == 0) return;
-        m0 = (int64_t)mt * BM;
-        have = (int)(g.m - m0 < BM ? g.m - m0 : BM);
-        left = s.rows;
-    }
-    const int64_t n0 = (int64_t)nt * BN;
-    const int cols = (int)(g.n - n0 < BN ? g.n - n0 : BN);
+    // Blocks of rows there are; of the weights' gradient all tiles.
+    const unsigned nmt = OP == kGroupRows ? group_blocks<BM>(g.ends, g.E, g.T, g.rest) : (unsigned)((g.m + BM - 1) / BM);
+    const unsigned tiles = nmt * nnt * (OP == kGroupRows ? 1 : g.E);
+    // Where the grid goes round, what is left for the last round is taken in halves of BM / 2 rows if that fills it no more than once.
+    const unsigned left_over = tiles % gridDim.x, halves = ROUND && OP == kGroupRows && 2 * left_over <= gridDim.x ? left_over : 0,
+                   whole = tiles - halves;
+    struct Work {
+        int e, rows;                   // expert, rows of the contraction or of the block
+        int64_t row, m0, n0;           // first row of the expert or block, first outputs
+        int have, left, cols;          // rows and columns of outputs there are, contraction
+    };
+    // The tile of a place (uniform); false where there is none.
+    const auto work = [&](unsigned id, Work& w) {
+        if (id >= whole + 2 * halves) return false;
+        const unsigned tile = id < whole ? id : whole + (id - whole) / 2;
+        unsigned mt, nt;
+        if constexpr (OP == kGroupRows) {
+            grouped_tile(tile, nmt, nnt, mt, nt);
+            GroupSlot s = group_slot<BM>(g.ends, g.E, g.T, mt);
+            if (halves && id >= whole) {
+                const int skip = (id - whole) & 1 ? BM / 2 : 0, rest = s.rows - skip;
+                s.row += skip;
+                s.rows = rest < 0 ? 0 : rest < BM / 2 ? rest : BM / 2;
+            }
+            w.e = s.e;
+            w.row = s.row;
+            w.m0 = 0;
+            w.have = s.rows;
+            w.left = s.e < g.E ? g.c : 0;
+        } else {
+            w.e = (int)(tile / (nmt * nnt));
+            grouped_tile(tile - w.e * (nmt * nnt), nmt, nnt, mt, nt);
+            const int lo = __builtin_amdgcn_readfirstlane(w.e > 0 ? group_end(g.ends, w.e - 1, g.T) : 0);
+            const int hi = __builtin_amdgcn_readfirstlane(group_end(g.ends, w.e, g.T));
+            w.row = lo;
+            w.left = hi > lo ? hi - lo : 0;
+            w.m0 = (int64_t)mt * BM;
+            w.have = g.accumulate && w.left == 0 ? 0 : (int)(g.m - w.m0 < BM ? g.m - w.m0 : BM);
+        }
+        w.n0 = (int64_t)nt * BN;
+        w.cols = (int)(g.n - w.n0 < BN ? g.n - w.n0 : BN);
+        return true;
+    };
     A a;
     B b;
-    if constexpr (OP == kGroupRows) {
-        a.set(g.a + s.row * g.a_ld, g.a_ld, have, left, t);
-        const uint16_t* w = g.b + (s.e < g.E ? s.e : 0) * g.b_es;
-        b.set(w + (BACROSS ? n0 : n0 * g.b_ld), g.b_ld, cols, left, t);
-    } else {
-        a.set(g.a + s.row * g.a_ld + m0, g.a_ld, have, left, t);
-        b.set(g.b + s.row * g.b_ld + n0, g.b_ld, cols, left, t);
-    }
-    const int steps = (left + 63) / 64;
+    const auto set = [&](const Work& w) {
+        if constexpr (OP == kGroupRows) {
+            a.set(g.a + w.row * g.a_ld, g.a_ld, w.have, w.left, t);
+            const uint16_t* m = g.b + (w.e < g.E ? w.e : 0) * g.b_es;
+            b.set(m + (BACROSS ? w.n0 : w.n0 * g.b_ld), g.b_ld, w.cols, w.left, t);
+        } else {
+            a.set(g.a + w.row * g.a_ld + w.m0, g.a_ld, w.have, w.left, t);
+            b.set(g.b + w.row * g.b_ld + w.n0, g.b_ld, w.cols, w.left, t);
+        }
+    };
     const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-    const bool live = wm < have;                               // (uniform) this wave's rows are there
     f4_t acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{};
-
     constexpr int kLoads = A::kLoads + B::kLoads, kFrags = TM + TN, kMul = TM * TN;
     // Fragments of half a step (32) from `base`, with `loads` the loads of a step to `to`, and with `products` those of the half step
     // that ma and mb hold, in turn: reads or loads in a row wait for the LDS's and the caches' ports, and a wave issues in order, so
@@ -297,31 +307,65 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
     };
     const std::true_type yes;
     const std::false_type no;
-    if (steps > 0) {
-        u32x4_t fa[TM], fb[TN], ga[TM], gb[TN];
+    const auto start = [&] {                                   // the first steps' loads
         if constexpr (DIRECT) {
-            // Half a step's fragments are read while the half before is multiplied. The barrier is between the halves: behind it the
-            // next step lies in LDS, and the one whose second half is on its way to the MFMAs is loaded anew.
 #pragma unroll
             for (int c = 0; c < ST; ++c) {                     // (past the last: zeros)
                 a.load(lds + c * kStep, t);
                 b.load(lds + c * kStep + A::kUnits, t);
             }
+        } else {
+            a.load(nullptr, t);
+            b.load(nullptr, t);
+        }
+    };
+    const auto store = [&](const Work& w) {
+        int64_t at = (OP == kGroupRows ? w.row * g.out_ld : w.e * g.out_es + w.m0 * g.out_ld) + w.n0;
+        int m = wm + (lane & 15), n = wn + 16 * (lane >> 4 & 1) + 8 * (lane >> 5);
+        asm volatile("" : "+v"(m), "+v"(n));                   // (addresses are worked out here, not kept)
+        at += m * g.out_ld + n;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int j = 0; j < TN; j += 2) {
+                grouped_pair(acc[i][j], acc[i][j + 1]);
+                if (m + 16 * i < w.have && n + 16 * j < w.cols)
+                    grouped_store<OP>(g, at + 16 * j, w.cols - n - 16 * j, acc[i][j], acc[i][j + 1]);
+            }
+            at += 16 * g.out_ld;
+        }
+    };
+    unsigned block = blockIdx.x;
+    Work w, next;
+    if (!work(grouped_place(kChunk, block), w)) return;
+    set(w);
+    start();
+    for (;;) {
+        const int steps = (w.left + 63) / 64;
+        const bool live = wm < w.have;                         // (uniform) this wave's rows are there
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{};
+        u32x4_t fa[TM], fb[TN], ga[TM], gb[TN];
+        if constexpr (DIRECT) {
+            // Half a step's fragments are read while the half before is multiplied. The barrier is between the halves: behind it the
+            // next step lies in LDS, and the one whose second half is on its way to the MFMAs is loaded anew.
             wait_step<kLoads * (ST - 1)>();
             __builtin_amdgcn_s_barrier();
             int at = 0;
             if (live) {
                 half(no, no, lds, 0, fa, fb, nullptr, ga, gb);
                 for (int c = 0; c < steps; ++c) {
-                    const int next = at == ST - 1 ? 0 : at + 1;
+                    const int then = at == ST - 1 ? 0 : at + 1;
                     __builtin_amdgcn_sched_barrier(0);
                     half(no, yes, lds + at * kStep, 1, ga, gb, nullptr, fa, fb);
                     __builtin_amdgcn_sched_barrier(0);
                     wait_step<kLoads * (ST - 2)>();
                     __builtin_amdgcn_s_barrier();
                     __builtin_amdgcn_sched_barrier(0);
-                    half(yes, yes, lds + next * kStep, 0, fa, fb, lds + at * kStep, ga, gb);
-                    at = next;
+                    half(yes, yes, lds + then * kStep, 0, fa, fb, lds + at * kStep, ga, gb);
+                    at = then;
                 }
             } else {                                           // loads alone
                 for (int c = 0; c < steps; ++c) {
@@ -332,10 +376,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
                     at = at == ST - 1 ? 0 : at + 1;
                 }
             }
-            wait_step<0>();                                    // the LDS is the next workgroup's behind the end
+            wait_step<0>();                                    // the LDS is the next tile's, or behind the end the next workgroup's
+            if constexpr (ROUND) __builtin_amdgcn_s_barrier();
         } else {
-            a.load(nullptr, t);
-            b.load(nullptr, t);
             a.store(lds, t);
             b.store(lds + A::kUnits, t);
             __syncthreads();
@@ -354,19 +397,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
                 __syncthreads();
             }
         }
-    }
-    if (!live) return;
-    const int64_t row0 = OP == kGroupRows ? s.row : m0, base = OP == kGroupRows ? 0 : s.e * g.out_es;
-    const int g4 = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int m = wm + 16 * i + (lane & 15);
-#pragma unroll
-        for (int j = 0; j < TN; j += 2) {
-            grouped_pair(acc[i][j], acc[i][j + 1]);
-            const int n = wn + 16 * (j + (g4 & 1)) + 8 * (g4 >> 1);
-            if (m < have && n < cols) grouped_store<OP>(g, base + (row0 + m) * g.out_ld + n0 + n, cols - n, acc[i][j], acc[i][j + 1]);
+        block += gridDim.x;
+        const bool more = ROUND && work(grouped_place(kChunk, block), next);
+        if (more) {                                            // on their way while the outputs are stored
+            set(next);
+            start();
         }
+        if (live) store(w);
+        if (!more) return;
+        w = next;
     }
 }
 
@@ -375,14 +414,15 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
 enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTileAny128 = 4, kTileAny32 = 5 };
 
 template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
-static int launch_grouped(const char* name, GroupedArgs g, hipStream_t st) {
+static int launch_grouped(const char* name, const GroupedArgs& g, hipStream_t st) {
+    constexpr bool ROUND = BM == 256;
     const int64_t nmt = OP == kGroupRows ? group_slots(g.T, g.E, BM, g.rest) : (g.m + BM - 1) / BM * g.E;
-    g.slots = (int)nmt;
     const int64_t tiles = nmt * ((g.n + BN - 1) / BN);
     constexpr int64_t kRound = 8 * kChunk;
     EXL3_CHECK_ARG(tiles <= kMx4Grid * 256 / (64 * WM * WN) - kRound, "%s: grid too large", name);
-    EXL3_LAUNCH(name, (grouped_kernel<XT, OP, BACROSS, BM, BN, WM, WN, ST, OCC, DIRECT>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)),
-                dim3(64 * WM * WN), 0, st, g);
+    const int64_t grid = (tiles + kRound - 1) / kRound * kRound;
+    EXL3_LAUNCH(name, (grouped_kernel<XT, OP, BACROSS, BM, BN, WM, WN, ST, OCC, DIRECT, ROUND>),
+                dim3((unsigned)(ROUND && grid > kRound ? kRound : grid)), dim3(64 * WM * WN), 0, st, g);
     return EXL3_OK;
 }
 
