@@ -68,6 +68,8 @@ SIGNATURES = {
     "exl3_route_balance_scratch": [_i64, _i64],
     "exl3_grouped_mm": [_vp, _i64, _i32, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp],
     "exl3_grouped_mm_dw": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp],
+    "exl3_grouped_mm_dw_in": [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
+    "exl3_grouped_mm_dw_scratch": [_i64, _i64, _i64, _i64],
     "exl3_g4_linear": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp],
     "exl3_g4_linear_in": [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp],
     "exl3_g4_linear_scratch": [_i64, _i64, _i64, _i64],
@@ -77,7 +79,7 @@ SIGNATURES = {
     "exl3_router_logits": [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
 }
 _RESTYPE = {"exl3_last_error": ctypes.c_char_p, "exl3_mx4_linear_scratch": _i64, "exl3_mx4_gemm_scratch": _i64,
-            "exl3_mx4_moe_scratch": _i64, "exl3_g4_linear_scratch": _i64, "exl3_route_balance_scratch": _i64}
+            "exl3_mx4_moe_scratch": _i64, "exl3_g4_linear_scratch": _i64, "exl3_grouped_mm_dw_scratch": _i64, "exl3_route_balance_scratch": _i64}
 
 _lib = None
 

@@ -25,42 +25,60 @@ inline int64_t group_slots(int64_t T, int64_t E, int64_t BM, bool rest) {
     return T < n ? T : n;
 }
 
-// Sum over the lanes up to and with this one.
+// Sum over the lanes up to and with this one: shifts by 1, 2, 4, 8 inside the 16 lanes of a row, then the rows' sums on.
 __device__ __forceinline__ int wave_running_sum(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o);
-        v += lane >= o ? u : 0;
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast:15 into rows 1, 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast:31 into rows 2, 3
     return v;
+}
+
+// fn(first expert of 64, this lane's begin and end) for the experts and the rows of none as the last of all, until it returns true.
+// Five loads of either kind are under way: one after another they are a microsecond for every 64 experts and more.
+template <typename F>
+__device__ __forceinline__ void group_each(const int32_t* ends, int E, int T, F fn) {
+    constexpr int kBatch = 5;
+    const int lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 <= E; i0 += 64 * kBatch) {
+        int lo[kBatch], hi[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (i0 + 64 * i > E) break;                        // uniform
+            const int e = i0 + 64 * i + lane;
+            lo[i] = ldg(ends + (e < 1 ? 0 : e <= E ? e - 1 : E - 1));
+            hi[i] = ldg(ends + (e < E ? e : E - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (i0 + 64 * i > E) break;
+            const int e = i0 + 64 * i + lane;
+            const int l = e < 1 ? 0 : lo[i] < 0 ? 0 : lo[i] > T ? T : lo[i], h = e < E ? hi[i] < 0 ? 0 : hi[i] > T ? T : hi[i] : e == E ? T : l;
+            if (fn(i0 + 64 * i, l, h)) return;
+        }
+    }
 }
 
 // The same value in every lane (wave-uniform). Blocks behind the last one have no rows.
 template <int BM>
 __device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int T, unsigned slot) {
-    const int lane = threadIdx.x & 63;
-    GroupSlot s;
+    GroupSlot s = {E, 0, 0};
     unsigned first = 0;                // blocks of the experts before
-    for (int i = 0; i <= E; i += 64) {
-        const int e = i + lane;
-        const int lo = e > 0 ? group_end(ends, e <= E ? e - 1 : E - 1, T) : 0, hi = e < E ? group_end(ends, e, T) : e == E ? T : lo;
+    group_each(ends, E, T, [&](int i, int lo, int hi) {
         const int blocks = hi > lo ? (hi - lo + BM - 1) / BM : 0, sum = wave_running_sum(blocks);
         const uint64_t in = __ballot(first + (unsigned)sum > slot);
-        if (in) {                      // uniform
-            const int l = __builtin_ctzll(in);
-            s.e = i + l;
-            const int block = (int)(slot - first) - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(blocks, l));
-            const int row = __builtin_amdgcn_readlane(lo, l) + block * BM, left = __builtin_amdgcn_readlane(hi, l) - row;
-            s.row = row;
-            s.rows = left < BM ? left : BM;
-            return s;
-        }
         first += (unsigned)__builtin_amdgcn_readlane(sum, 63);
-    }
-    s.e = E;
-    s.row = 0;
-    s.rows = 0;
+        if (!in) return false;         // uniform
+        const int l = __builtin_ctzll(in), before = (int)first - __builtin_amdgcn_readlane(sum, 63);
+        const int block = (int)slot - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(blocks, l));
+        const int row = __builtin_amdgcn_readlane(lo, l) + block * BM, left = __builtin_amdgcn_readlane(hi, l) - row;
+        s.e = i + l;
+        s.row = row;
+        s.rows = left < BM ? left : BM;
+        return true;
+    });
     return s;
 }
 
@@ -68,11 +86,11 @@ __device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int 
 template <int BM>
 __device__ __forceinline__ unsigned group_blocks(const int32_t* ends, int E, int T, bool rest) {
     int n = 0;
-    for (int i = 0; i < E + (rest ? 1 : 0); i += 64) {
-        const int e = i + (threadIdx.x & 63);
-        const int lo = e > 0 ? group_end(ends, e <= E ? e - 1 : E - 1, T) : 0, hi = e < E ? group_end(ends, e, T) : e == E && rest ? T : lo;
-        n += __builtin_amdgcn_readlane(wave_running_sum(hi > lo ? (hi - lo + BM - 1) / BM : 0), 63);
-    }
+    group_each(ends, E, T, [&](int i, int lo, int hi) {
+        const bool in = hi > lo && (rest || i + (int)(threadIdx.x & 63) < E);
+        n += __builtin_amdgcn_readlane(wave_running_sum(in ? (hi - lo + BM - 1) / BM : 0), 63);
+        return false;
+    });
     return (unsigned)n;
 }
 

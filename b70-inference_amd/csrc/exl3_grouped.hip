@@ -30,6 +30,115 @@ static bool vec_out(const void* p, int dtype, int64_t ld, int64_t n) {
     return aligned(p, 16) && n % 8 == 0 && ld * out_size(dtype) % 16 == 0;
 }
 
+// Microseconds that `tiles` tiles of `steps` steps take by an estimate from measurements: a step and the rest of a tile, with `occ`
+// workgroups to a CU and with one, full rounds and what is left.
+struct TileCost {
+    int bm, bn, occ;
+    double step, step1, rest;
+};
+static const TileCost kTileCost[4] = {{256, 256, 1, 1.65, 1.65, 8.0}, {128, 128, 2, 1.1, 0.65, 5.0}, {64, 128, 2, 0.65, 0.42, 4.0}, {32, 128, 2, 0.5, 0.36, 4.0}};
+static double tile_time(const TileCost& t, double tiles, double steps) {
+    const int64_t n = (int64_t)(tiles + 0.999), full = n / (256 * t.occ), left = n - full * 256 * t.occ;
+    return (double)full * (steps * t.step + t.rest) + (left == 0 ? 0.0 : steps * (left > 256 ? t.step : t.step1) + t.rest);
+}
+
+// Tile of the products of T rows over E experts (few: the kernel of few rows is there for them).
+static int rows_tile(int64_t T, int64_t E, int64_t n, int64_t k, bool few) {
+    const double live = (double)(T < E ? T : E);
+    // blocks of 16 rows by 16 outputs, up to where their weights' bytes count (64 rows over 64 experts of 2048 -> 4096: 151 us against
+    // 115; 40 over 512 of 2048 -> 1024 28 against 34, one row of 4096 -> 4096 11 against 30)
+    if (few && T <= 16 * E && ((double)(T / 16) + live) * (double)n * (double)k <= (double)(1 << 27)) return kTileFew;
+    int best = 0;
+    double least = 1e30;
+    for (int i = 0; i < 4; ++i) {
+        const TileCost& t = kTileCost[i];
+        double blocks = (double)T / t.bm + 0.5 * live;
+        if (blocks < live) blocks = live;
+        const double us = tile_time(t, blocks * (double)((n + t.bn - 1) / t.bn), (double)((k + 63) / 64));
+        if (us < least) {
+            least = us;
+            best = i;
+        }
+    }
+    return best;
+}
+// Tile of the weights' gradient, and the parts of an expert's rows: few small matrices of many rows leave CUs idle.
+struct WeightsPlan {
+    int tile, splits;
+};
+static int64_t n8(int64_t n) { return (n + 7) & ~(int64_t)7; }
+static WeightsPlan weights_plan(int64_t T, int64_t E, int64_t n, int64_t k, bool direct) {
+    WeightsPlan best = {0, 1};
+    double least = 1e30;
+    for (int i = direct ? 0 : 1; i < 2; ++i) {
+        const TileCost& t = kTileCost[i];
+        const double tiles = (double)(E * ((n + t.bm - 1) / t.bm)) * (double)((k + t.bn - 1) / t.bn);
+        for (int p = 1; p <= 16; p *= 2) {
+            if (p > 1 && (tiles * p > 512.0 || (double)T / (double)E < 256.0 * p)) break;
+            double us = tile_time(t, tiles * p, (double)T / (double)(E * p) / 64.0 + 0.5);
+            if (p > 1) us += 3.0 + (double)p * (double)(E * n) * (double)n8(k) * 1.6e-6;
+            if (us < least) {
+                least = us;
+                best = {direct ? i == 0 ? kTile256 : kTile128 : kTileAny128, p};
+            }
+        }
+    }
+    return best;
+}
+static int64_t weights_part_bytes(const WeightsPlan& p, int64_t E, int64_t n, int64_t k) {
+    return p.splits == 1 ? 0 : (int64_t)p.splits * E * n * n8(k) * 4;
+}
+
+static int weights_gradient(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
+                            const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
+                            const CallScratch& s, void* stream) {
+    const char* what = "exl3_grouped_mm_dw";
+    const int rc = grouped_setup(what, dtype, T, n, k, ends, E, dw_dtype);
+    if (rc) return rc;
+    EXL3_CHECK_ARG(accumulate == 0 || accumulate == 1, "%s: accumulate %d", what, accumulate);
+    EXL3_CHECK_ARG((T <= 1 || (dy_ld >= n && x_ld >= k)) && dy_ld <= kMostWidth && x_ld <= kMostWidth && (n == 1 || dw_ld >= k) &&
+                       dw_ld <= ((int64_t)1 << 40) && dw_es >= 0 && dw_es <= ((int64_t)1 << 45) && (E == 1 || dw_es >= (n - 1) * dw_ld + k),
+                   "%s: bad strides (gradients %lld, rows %lld, output %lld and %lld)", what, (long long)dy_ld, (long long)x_ld,
+                   (long long)dw_ld, (long long)dw_es);
+    EXL3_CHECK_ARG((T == 0 || (dy && x && aligned(dy, 2) && aligned(x, 2))) && dw && aligned(dw, out_size(dw_dtype)),
+                   "%s: null or misaligned pointer", what);
+    GroupedArgs g{};
+    g.a = reinterpret_cast<const uint16_t*>(dy);
+    g.b = reinterpret_cast<const uint16_t*>(x);
+    g.out = dw;
+    g.a_ld = T <= 1 ? n : dy_ld;
+    g.b_ld = T <= 1 ? k : x_ld;
+    g.out_ld = n == 1 ? k : dw_ld;
+    g.out_es = dw_es;
+    g.ends = ends;
+    g.E = (int)E;
+    g.T = (int)T;
+    g.m = (int)n;
+    g.n = (int)k;
+    g.out_dtype = dw_dtype;
+    g.vec = vec_out(dw, dw_dtype, g.out_ld, k) && (E == 1 || dw_es * out_size(dw_dtype) % 16 == 0);
+    g.accumulate = accumulate;
+    const bool direct = units16(dy, g.a_ld, n) && units16(x, g.b_ld, k);
+    hipStream_t st = (hipStream_t)stream;
+    WeightsPlan plan = weights_plan(T, E, n, k, direct);
+    const int want = env_int("EXL3MI_GROUPED_TILE", 0);
+    if (direct && want > 0 && want <= 2) plan = {want - 1, 1};
+    g.splits = plan.splits;
+    if (plan.splits == 1) return grouped_weights(g, dtype, plan.tile, st);
+    Carve c{};
+    const int rs = call_scratch(what, (size_t)weights_part_bytes(plan, E, n, k), s, st, &c);
+    if (rs) return rs;
+    GroupedArgs h = g;                                         // the parts: fp32, padded rows
+    h.out = c.p;
+    h.out_ld = n8(k);
+    h.out_es = n * h.out_ld;
+    h.out_dtype = EXL3_F32;
+    h.vec = 1;
+    h.accumulate = 0;
+    const int rc2 = grouped_weights(h, dtype, plan.tile, st);
+    return rc2 ? rc2 : grouped_reduce(g, reinterpret_cast<const float*>(c.p), h.out_ld, E * h.out_es, st);
+}
+
 }  // namespace exl3
 
 extern "C" {
@@ -70,47 +179,32 @@ int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k
     g.rest = rest;
     const bool direct = units16(x, g.a_ld, k) && units16(w, w_ld, across ? n : k) && (E == 1 || w_es % 8 == 0);
     const int64_t mean = T / E;
-    int tile = !direct ? (mean <= 48 ? kTileAny32 : kTileAny128)
-             : mean <= 24 ? kTile32 : mean <= 64 ? kTile64 : mean <= 160 ? kTile128 : kTile256;
+    int tile = !direct ? (mean <= 48 ? kTileAny32 : kTileAny128) : rows_tile(T, E, n, k, !across && k <= 8192);
     const int want = env_int("EXL3MI_GROUPED_TILE", 0);
     if (direct && want > 0 && want <= 4) tile = want - 1;
+    if (direct && want == 5 && !across && k <= 8192) tile = kTileFew;
+    if (tile == kTileFew) return grouped_rows_few(g, dtype, (hipStream_t)stream);
     return (across ? grouped_rows_across : grouped_rows_along)(g, dtype, tile, (hipStream_t)stream);
+}
+
+// The plan does not know how the operands lie: the larger of both plans' scratch.
+int64_t exl3_grouped_mm_dw_scratch(int64_t T, int64_t n, int64_t k, int64_t E) {
+    if (T < 0 || T > kMostRows || n <= 0 || n > kMostWidth || k <= 0 || k > kMostWidth || E <= 0 || E > 65536) return 0;
+    const int64_t a = weights_part_bytes(weights_plan(T, E, n, k, true), E, n, k), b = weights_part_bytes(weights_plan(T, E, n, k, false), E, n, k);
+    return a > b ? a : b;
 }
 
 int exl3_grouped_mm_dw(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
                        const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
                        void* stream) {
-    const char* what = "exl3_grouped_mm_dw";
-    const int rc = grouped_setup(what, dtype, T, n, k, ends, E, dw_dtype);
-    if (rc) return rc;
-    EXL3_CHECK_ARG(accumulate == 0 || accumulate == 1, "%s: accumulate %d", what, accumulate);
-    EXL3_CHECK_ARG((T <= 1 || (dy_ld >= n && x_ld >= k)) && dy_ld <= kMostWidth && x_ld <= kMostWidth && (n == 1 || dw_ld >= k) &&
-                       dw_ld <= ((int64_t)1 << 40) && dw_es >= 0 && dw_es <= ((int64_t)1 << 45) && (E == 1 || dw_es >= (n - 1) * dw_ld + k),
-                   "%s: bad strides (gradients %lld, rows %lld, output %lld and %lld)", what, (long long)dy_ld, (long long)x_ld,
-                   (long long)dw_ld, (long long)dw_es);
-    EXL3_CHECK_ARG((T == 0 || (dy && x && aligned(dy, 2) && aligned(x, 2))) && dw && aligned(dw, out_size(dw_dtype)),
-                   "%s: null or misaligned pointer", what);
-    GroupedArgs g{};
-    g.a = reinterpret_cast<const uint16_t*>(dy);
-    g.b = reinterpret_cast<const uint16_t*>(x);
-    g.out = dw;
-    g.a_ld = T <= 1 ? n : dy_ld;
-    g.b_ld = T <= 1 ? k : x_ld;
-    g.out_ld = n == 1 ? k : dw_ld;
-    g.out_es = dw_es;
-    g.ends = ends;
-    g.E = (int)E;
-    g.T = (int)T;
-    g.m = (int)n;
-    g.n = (int)k;
-    g.out_dtype = dw_dtype;
-    g.vec = vec_out(dw, dw_dtype, g.out_ld, k) && (E == 1 || dw_es * out_size(dw_dtype) % 16 == 0);
-    g.accumulate = accumulate;
-    const bool direct = units16(dy, g.a_ld, n) && units16(x, g.b_ld, k);
-    int tile = !direct ? kTileAny128 : (n + 255) / 256 * ((k + 255) / 256) * E >= 512 ? kTile256 : kTile128;
-    const int want = env_int("EXL3MI_GROUPED_TILE", 0);
-    if (direct && want > 0 && want <= 2) tile = want - 1;
-    return grouped_weights(g, dtype, tile, (hipStream_t)stream);
+    return weights_gradient(dy, dy_ld, x, x_ld, dtype, T, n, k, ends, E, dw, dw_ld, dw_es, dw_dtype, accumulate, kLibScratch, stream);
+}
+
+int exl3_grouped_mm_dw_in(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
+                          const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
+                          void* scratch, int64_t scratch_bytes, void* stream) {
+    return weights_gradient(dy, dy_ld, x, x_ld, dtype, T, n, k, ends, E, dw, dw_ld, dw_es, dw_dtype, accumulate,
+                            CallScratch{scratch, scratch_bytes, false}, stream);
 }
 
 }  // extern "C"

@@ -30,6 +30,7 @@ struct GroupedArgs {
     int out_dtype, vec;                // vec: eight neighbouring outputs may be stored as 16-byte pieces
     int rest;                          // rows of no expert become 0
     int accumulate;                    // the weights' gradient is added to what out holds
+    int splits;                        // the weights' gradient: parts of an expert's rows, whose sums lie E out_es behind one another
 };
 
 enum { kGroupRows = 0, kGroupWeights = 1 };
@@ -218,12 +219,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
     const unsigned nnt = (unsigned)((g.n + BN - 1) / BN);
     // Blocks of rows there are; of the weights' gradient all tiles.
     const unsigned nmt = OP == kGroupRows ? group_blocks<BM>(g.ends, g.E, g.T, g.rest) : (unsigned)((g.m + BM - 1) / BM);
-    const unsigned tiles = nmt * nnt * (OP == kGroupRows ? 1 : g.E);
+    const unsigned tiles = nmt * nnt * (OP == kGroupRows ? 1 : g.E * g.splits);
     // Where the grid goes round, what is left for the last round is taken in halves of BM / 2 rows if that fills it no more than once.
     const unsigned left_over = tiles % gridDim.x, halves = ROUND && OP == kGroupRows && 2 * left_over <= gridDim.x ? left_over : 0,
                    whole = tiles - halves;
     struct Work {
-        int e, rows;                   // expert, rows of the contraction or of the block
+        int e;                         // expert (the weights' gradient: and E for each split before)
         int64_t row, m0, n0;           // first row of the expert or block, first outputs
         int have, left, cols;          // rows and columns of outputs there are, contraction
     };
@@ -248,10 +249,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
         } else {
             w.e = (int)(tile / (nmt * nnt));
             grouped_tile(tile - w.e * (nmt * nnt), nmt, nnt, mt, nt);
-            const int lo = __builtin_amdgcn_readfirstlane(w.e > 0 ? group_end(g.ends, w.e - 1, g.T) : 0);
-            const int hi = __builtin_amdgcn_readfirstlane(group_end(g.ends, w.e, g.T));
-            w.row = lo;
-            w.left = hi > lo ? hi - lo : 0;
+            const int sp = w.e / g.E, e = w.e - sp * g.E;
+            const int lo = __builtin_amdgcn_readfirstlane(e > 0 ? group_end(g.ends, e - 1, g.T) : 0);
+            const int hi = __builtin_amdgcn_readfirstlane(group_end(g.ends, e, g.T));
+            const int rows = hi > lo ? hi - lo : 0, per = ((rows + 63) / 64 + g.splits - 1) / g.splits * 64, skip = sp * per;
+            w.row = skip < rows ? lo + skip : 0;
+            w.left = skip < rows ? rows - skip < per ? rows - skip : per : 0;
             w.m0 = (int64_t)mt * BM;
             w.have = g.accumulate && w.left == 0 ? 0 : (int)(g.m - w.m0 < BM ? g.m - w.m0 : BM);
         }
@@ -411,12 +414,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void grouped_kernel(GroupedArgs 
 
 // ------------------------------------------------------------------------------------------------ launches
 // Tiles of a call: rows (and of the weights' gradient columns) of a workgroup; unaligned operands go through registers.
-enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTileAny128 = 4, kTileAny32 = 5 };
+enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTileAny128 = 4, kTileAny32 = 5, kTileFew = 6 };
 
 template <int XT, int OP, bool BACROSS, int BM, int BN, int WM, int WN, int ST, int OCC, bool DIRECT>
 static int launch_grouped(const char* name, const GroupedArgs& g, hipStream_t st) {
     constexpr bool ROUND = BM == 256;
-    const int64_t nmt = OP == kGroupRows ? group_slots(g.T, g.E, BM, g.rest) : (g.m + BM - 1) / BM * g.E;
+    const int64_t nmt = OP == kGroupRows ? group_slots(g.T, g.E, BM, g.rest) : (g.m + BM - 1) / BM * g.E * g.splits;
     const int64_t tiles = nmt * ((g.n + BN - 1) / BN);
     constexpr int64_t kRound = 8 * kChunk;
     EXL3_CHECK_ARG(tiles <= kMx4Grid * 256 / (64 * WM * WN) - kRound, "%s: grid too large", name);
@@ -439,8 +442,11 @@ static int launch_grouped_rows(const GroupedArgs& g, int tile, hipStream_t st) {
     }
 }
 
+int grouped_rows_few(const GroupedArgs& g, int dtype, hipStream_t st);   // aligned, at most 8192 inputs
 int grouped_rows_along(const GroupedArgs& g, int dtype, int tile, hipStream_t st);
 int grouped_rows_across(const GroupedArgs& g, int dtype, int tile, hipStream_t st);
 int grouped_weights(const GroupedArgs& g, int dtype, int tile, hipStream_t st);
+// out = the sum of g.splits parts [E m][n4] that lie `stride` behind one another
+int grouped_reduce(const GroupedArgs& g, const float* part, int64_t n4, int64_t stride, hipStream_t st);
 
 }  // namespace exl3

@@ -8,15 +8,15 @@ expert. moe_align sorts a routing: ends = counts.cumsum(0, dtype=torch.int32), x
   * grouped_mm_dx(dy, w, ends)   dx[t] = dy[t] @ w[e], the gradient with respect to the rows
   * grouped_mm_dw(dy, x, ends)   dw[e] = dy[rows of e]^T @ x[rows of e], the gradient with respect to the weights
 There is no autograd graph: pass the gradients on. Rows and weights fp16 or bf16, sums fp32 in an order fixed by the sizes, one rounding
-to out's type. Tensors live on the GPU; every op is asynchronous on the current stream of its tensors' device and needs no scratch
-(calls may overlap on streams and threads, and can be captured without a warm-up). The reference has no counterpart: its experts are
+to out's type. Tensors live on the GPU; every op is asynchronous on the current stream of its tensors' device and has scratch of its
+own where it needs some (calls may overlap on streams and threads, and can be captured without a warm-up). The reference has no counterpart: its experts are
 EXL3 only.
 """
 from __future__ import annotations
 
 import torch
 
-from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, stream_of
+from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, scratch, stream_of
 from .g4 import G4Tensor
 from .mx4 import DTYPES, _rows
 
@@ -168,9 +168,10 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
     es = se if E > 1 else m * ld
     if (k > 1 and sk != 1) or ld < k or es < (m - 1) * ld + k:
         raise Exl3Error(f"{what}: matrices of out must have contiguous rows or columns and must not overlap")
+    ws, need = scratch("exl3_grouped_mm_dw", x, T, m, k, E)
     with where:
-        rc = lib().exl3_grouped_mm_dw(a.data_ptr(), a_ld, b.data_ptr(), b_ld, _HALF[x.dtype], T, m, k, ends.data_ptr(), E,
-                                      out.data_ptr(), ld, es, DTYPES[out.dtype], int(bool(accumulate)), stream_of(x))
+        rc = lib().exl3_grouped_mm_dw_in(a.data_ptr(), a_ld, b.data_ptr(), b_ld, _HALF[x.dtype], T, m, k, ends.data_ptr(), E,
+                                         out.data_ptr(), ld, es, DTYPES[out.dtype], int(bool(accumulate)), ptr(ws), need, stream_of(x))
     if rc:
         check(rc, what)
     return out

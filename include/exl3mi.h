@@ -385,13 +385,13 @@ int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t 
  * ascending, at most T (other values lead to no access out of range, but to rows that belong to no or to several experts). An
  * expert may have no rows; rows from ends[E - 1] on belong to none. Any sizes (columns at most 2^22, as the row strides);
  * operands of 16-byte aligned rows of whole multiples of eight values are read fastest. Sums are fp32 in an order fixed by the
- * sizes, with one rounding. No scratch; calls may overlap. No reference counterpart (the reference's experts are EXL3 only). */
+ * sizes, with one rounding. No reference counterpart (the reference's experts are EXL3 only). */
 enum exl3_grouped_w { EXL3_GROUPED_W_NK = 0, EXL3_GROUPED_W_KN = 1 };
 
 /* out[t, n] = sum over k of x[t, k] W_e(n, k) for the rows t of every expert e: x fp16 or bf16 (`dtype`) [T, k] (row stride x_ld), W
  * of the same type, an expert's matrix w_es elements behind the one before: [n, k] (EXL3_GROUPED_W_NK, row stride w_ld >= k) or
  * [k, n] (EXL3_GROUPED_W_KN, w_ld >= n). out fp16, bf16 or fp32 [T, n] (row stride out_ld). Rows of no expert: left as they are
- * (rest 0) or set to 0 (rest 1). The gradient with respect to x is the same product of the output's gradient in the other layout. */
+ * (rest 0) or set to 0 (rest 1). The gradient with respect to x is the same product of the output's gradient in the other layout. No scratch: calls may overlap. */
 int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k, const void* w, int64_t w_ld, int64_t w_es,
                     int w_layout, int64_t n, const int32_t* ends, int64_t E, void* out, int64_t out_ld, int out_dtype, int rest,
                     void* stream);
@@ -402,6 +402,12 @@ int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k
 int exl3_grouped_mm_dw(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
                        const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
                        void* stream);
+
+/* With scratch from the caller, as the _in calls above; few calls need any (small matrices of many rows). */
+int64_t exl3_grouped_mm_dw_scratch(int64_t T, int64_t n, int64_t k, int64_t E);
+int exl3_grouped_mm_dw_in(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
+                          const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
+                          void* scratch, int64_t scratch_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------ 4-bit weights with group scales (G4)
  * w = (q - z) s: whole numbers q from 0 to 15, two to a byte, the even one in the low half; for each `group` neighbouring inputs

@@ -44,11 +44,11 @@ def test_products_and_gradients(exl3, T, E, N, K, pad, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("tile", (1, 2, 3, 4))
+@pytest.mark.parametrize("tile", (1, 2, 3, 4, 5))
 def test_every_tile(exl3, monkeypatch, tile, dtype):
     """Each tile over blocks that are full, end early, or hold a row, a contraction of one step and of many, and its tail."""
     monkeypatch.setenv("EXL3MI_GROUPED_TILE", str(tile))
-    for sizes, N, K in (([256, 1, 0, 300, 31], 272, 64), ([3, 0, 65, 129, 600], 520, 408), ([0, 0, 40], 8, 8)):
+    for sizes, N, K in (([256, 1, 0, 300, 31], 272, 64), ([3, 0, 65, 129, 600], 520, 408), ([0, 0, 40], 8, 8), ([16, 1, 0, 33], 24, 5000)):
         ends = ends_of(sizes)
         x, dy, w = _data(sum(sizes), len(sizes), N, K, dtype, tile + N)
         y = exl3.grouped_mm(x, w, ends)
@@ -57,6 +57,22 @@ def test_every_tile(exl3, monkeypatch, tile, dtype):
         check(dx, *rows_product(dy, w.transpose(1, 2), ends, len(x)), N, "dx")
         dw = exl3.grouped_mm_dw(dy, x, ends)
         check(dw, *weights_gradient(dy, x, ends), max(sizes), "dw")
+
+
+@pytest.mark.parametrize("N,K", ((64, 96), (33, 57)))
+def test_rows_in_parts(exl3, N, K):
+    """Small matrices of many rows: an expert's rows go to several workgroups, some of which have none."""
+    sizes = [3000, 0, 20, 64]
+    ends = ends_of(sizes)
+    x, dy, w = _data(sum(sizes), 4, N, K, torch.bfloat16, 2)
+    assert exl3.lib().exl3_grouped_mm_dw_scratch(sum(sizes), N, K, 4) > 0
+    ref, mag = weights_gradient(dy, x, ends)
+    for out_dtype in OUTS:
+        check(exl3.grouped_mm_dw(dy, x, ends, out_dtype=out_dtype), ref, mag, 3000 + 16, "parts")
+    old = torch.randn(4, N, K, device="cuda")
+    out = old.clone()
+    exl3.grouped_mm_dw(dy, x, ends, out=out, accumulate=True)
+    check(out, ref + old.double(), mag + old.double().abs(), 3000 + 17, "sum")
 
 
 def test_given_out_keeps_other_rows(exl3):
