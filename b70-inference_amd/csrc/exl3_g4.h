@@ -53,9 +53,9 @@ __device__ __forceinline__ uint32_t g4_zero(int z) {
     if constexpr (XT == kRowF16) return 0xE400E400u + (uint32_t)z * 0x10001u;
     else return Z ? (uint32_t)(128 - z) * 0x01010101u : 0u;
 }
-// The factor of the scale that g4_frag leaves out.
+// The factor that g4_frag leaves out: the sums' (a scale's might leave its type).
 template <int XT, bool Z>
-constexpr float kG4Scale = XT == kRowBF16 && !Z ? 16.f : 1.f;
+constexpr float kG4Factor = XT == kRowBF16 && !Z ? 16.f : 1.f;
 
 // The signed 4-bit number in the low bits of byte B, as sixteenths of 16 (the compiler shifts the byte down first, mostly).
 template <int B>

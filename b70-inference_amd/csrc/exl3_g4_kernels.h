@@ -46,7 +46,7 @@ struct G4Scales {
     }
     // scale i of the four; `in`: 0 for those that are not there, beside x that is 0
     __device__ __forceinline__ float scale(int i, bool in, int bf16) const {
-        return g4_scale((uint32_t)(s >> (16 * i)) & 0xFFFFu, bf16, in) * kG4Scale<XT, Z>;
+        return g4_scale((uint32_t)(s >> (16 * i)) & 0xFFFFu, bf16, in);
     }
     __device__ __forceinline__ uint32_t zero(int i) const { return g4_zero<XT, Z>(Z ? z >> (8 * i) & 15 : 8); }
 };
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
         asm volatile("" : "+v"(m));                            // (the rows' addresses are worked out here, not kept)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (m + e < s.rows) store_as(g.out, (s.row + m + e) * g.out_ld + n, acc[e] + b, g.out_dtype);
+            if (m + e < s.rows) store_as(g.out, (s.row + m + e) * g.out_ld + n, __builtin_fmaf(kG4Factor<XT, Z>, acc[e], b), g.out_dtype);
     }
 }
 
@@ -323,7 +323,9 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int m = 16 * r + 4 * q4 + e;
-            if (m < s.rows) g4_put4(g, sp, s.row + m, n0 + 4 * l, f4_t{acc[r][0][e], acc[r][1][e], acc[r][2][e], acc[r][3][e]});
+            constexpr float k = kG4Factor<XT, Z>;
+            if (m < s.rows)
+                g4_put4(g, sp, s.row + m, n0 + 4 * l, f4_t{k * acc[r][0][e], k * acc[r][1][e], k * acc[r][2][e], k * acc[r][3][e]});
         }
 }
 

@@ -21,6 +21,7 @@ import torch
 from ._lib import (ACT_GELU_TANH, ACT_SILU, EXL3_F16, EXL3_F32, EXL3_WORDS_PLANAR4, EXL3_WORDS_TILE_ORDER, Exl3Error,
                    check, lib, on_device, ptr, require_device, scratch, stream_of)
 from .linear import BC_LinearEXL3
+from .g4 import G4Linear, G4Tensor
 from .mx4 import ACTS, MX4Experts, MX4Linear, mx4_moe_forward
 
 
@@ -58,6 +59,8 @@ class MixedEXL3:
 def _proj_K(p) -> int:
     if isinstance(p, MX4Linear):
         raise NotImplementedError("ExpertTables: EXL3 projections expected; MX4 ones go into MX4Experts")
+    if isinstance(p, (G4Linear, G4Tensor)):
+        raise NotImplementedError("ExpertTables: EXL3 projections expected; G4 ones are multiplied by grouped_mm")
     return 0 if isinstance(p, MixedEXL3) else p.Ki
 
 
@@ -600,6 +603,8 @@ class BlockSparseMLP:
                  selection_bias: torch.Tensor | None = None, scoring: str = "softmax", routed_scaling: float = 1.0,
                  renormalize: bool = True, bias_select_only: bool = False, router_layout: str = "he",
                  router_round_fp16: bool = False):
+        if isinstance(experts, G4Tensor):
+            raise NotImplementedError("BlockSparseMLP: ExpertTables or MX4Experts expected; G4 experts are multiplied by grouped_mm")
         self.experts = experts
         self.num_experts = experts.E - (1 if has_shared else 0)
         self.num_experts_per_tok = num_experts_per_tok

@@ -266,6 +266,8 @@ class MX4Experts:
                     if p.bias is not None:
                         raise NotImplementedError("MX4Experts: experts with biases")
                     p = p.weight
+                if not isinstance(p, MX4Tensor):
+                    raise NotImplementedError(f"MX4Experts: MX4 projections expected, got {type(p).__name__}")
                 ts.append(p)
             projs.append(ts)
         shape = projs[0][0].shape

@@ -129,6 +129,18 @@ def test_every_code_and_zero_is_exact(exl3, zeros, dtype):
         assert torch.equal(y.double(), values(packed, scales, z)[:, :m].t())
 
 
+def test_scales_near_the_types_ends(exl3):
+    """bf16 scales of 2^125 beside rows of 2^-100, and of 2^-120 beside rows of 2^60."""
+    for s, x0 in ((2.0 ** 125, 2.0 ** -100), (2.0 ** -120, 2.0 ** 60)):
+        for zeros in (False, True):
+            codes, scales, z = make((), 20, 128, 64, zeros, torch.bfloat16, 3)
+            scales = torch.full_like(scales, s)
+            for m in (2, 40):
+                x = (rows(m, 128, torch.float32, m) * x0).to(torch.bfloat16)
+                y = exl3.G4Linear(exl3.G4Tensor(codes, scales, z)).run_alloc(x, 20, True)
+                check(y, *product(x, values(codes, scales, z)), 128)
+
+
 @pytest.mark.parametrize("dtype", HALF)
 def test_rows_do_not_mix(exl3, dtype):
     """Infinities and NaN of a row, and of another output's scales, stay where they are; an infinite input gives what the sum does."""
