@@ -47,10 +47,10 @@ __device__ __forceinline__ void g4_turn(u32x4_t& w) {
     w = u32x4_t{c[0], c[1], d[0], d[1]};
 }
 
-// What takes a word's codes to q - z: fp16 as packed -(1024 + z); bf16 with zeros as bytes 128 - z.
+// What takes a word's codes to q - z: fp16 as -(1024 + z) and -(64 + z); bf16 with zeros as bytes 128 - z.
 template <int XT, bool Z>
 __device__ __forceinline__ uint32_t g4_zero(int z) {
-    if constexpr (XT == kRowF16) return 0xE400E400u + (uint32_t)z * 0x10001u;
+    if constexpr (XT == kRowF16) return 0xD400E400u + (uint32_t)z * 0x00100001u;
     else return Z ? (uint32_t)(128 - z) * 0x01010101u : 0u;
 }
 // The factor that g4_frag leaves out: the sums' (a scale's might leave its type).
@@ -68,18 +68,26 @@ __device__ __forceinline__ float g4_off(uint32_t w) {
     return f;
 }
 
-// Eight q - z of a word, exact, in order: fp16 by setting the codes below 1024 and subtracting 1024 + z; bf16 by way of fp32, where
-// a conversion takes signed 4-bit numbers to sixteenths of them (z = 8), or signed bytes.
+// x & mask | bits (of two constants the compiler makes two instructions).
+__device__ __forceinline__ uint32_t g4_and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(bits));
+    return r;
+}
+
+// Eight q - z of a word, exact, in order. fp16: a byte in both halves, of which the lower keeps its low four bits below 1024 and the
+// upper its high ones, so that they are 1024 + q and 1024 + 16 q; one multiply-add takes them to q - z. bf16 by way of fp32, where a
+// conversion takes signed 4-bit numbers to sixteenths of them (z = 8), or signed bytes.
 template <int XT, bool Z>
 __device__ __forceinline__ u32x4_t g4_frag(uint32_t w, uint32_t zero) {
     u32x4_t r;
     if constexpr (XT == kRowF16) {
-        const uint32_t lo = w & 0xFFFFu, hi = w >> 16, a = lo | lo << 12, b = hi | hi << 12;
-        const uint32_t p[4] = {a, a >> 8, b, b >> 8};
+        const h2_t k = {(_Float16)1.f, (_Float16)0.0625f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, (p[i] & 0x000F000Fu) | 0x64006400u) +
-                                                    __builtin_bit_cast(h2_t, zero));
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t p = g4_and_or(__builtin_amdgcn_perm(w, w, 0x00000000u + 0x01010101u * i), 0x00F0000Fu, 0x64006400u);
+            r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2_t, p), k, __builtin_bit_cast(h2_t, zero)));
+        }
     } else if constexpr (!Z) {
         const uint32_t e = w ^ 0x88888888u, o = e >> 4;
         r[0] = __builtin_bit_cast(uint32_t, b2_t{(__bf16)g4_off<0>(e), (__bf16)g4_off<0>(o)});

@@ -52,20 +52,29 @@ struct G4Scales {
 };
 
 // ------------------------------------------------------------------------------------------------ few rows
-// Blocks of up to 16 rows. A wave takes 512 inputs (four chunks) of the block's rows, which stay in its registers, and of one tile of
-// 16 weight rows after another; the waves of a workgroup share the inputs and are added in order through LDS. Bound by the
-// weights' bytes, for small matrices by the chain of load, sum and store.
+// Blocks of up to 16 rows; tiles of 16 weight rows whose inputs the waves of a workgroup share, groups of 512 (four chunks) in turn,
+// added in order through LDS. A group's weights and scales are asked for as soon as those of the one before are used, the next tile's
+// behind the last.
+//   XL: x lies in LDS, and eight waves go round a tile's groups: two workgroups to a CU, one of which works while the other waits
+//   for its barrier (one row of 4096 -> 4096 7.0 us, 8.0 without; ten rows of 512 experts of 2048 -> 1024 8.9 and 9.8).
+//   Not XL, where x leaves room for one workgroup: a wave has one group of every tile, whose x stays in its registers.
+// Bound by the weights' bytes (6 rows of 5376 -> 21504, fp16 with zeros: 61 MB in 23.5 us, 2.6 TB/s, of which the instructions that
+// take the codes apart are a third), for small matrices by the chain of launch, load, sum and store.
 constexpr int kG4Waves = 16, kG4Slice = 512;
+constexpr int kG4Lds = 163840;         // of a CU
 
-template <int XT, int SG, bool Z>
-__global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split) {
+// Bytes from row to row of x in LDS: whole chunks, and 16 bytes to spread the rows over the banks.
+__host__ __device__ constexpr int64_t g4_x_stride(int64_t k) { return (k + 127) / 128 * 256 + 16; }
+
+template <int XT, int SG, bool Z, bool XL>
+__global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g, int split) {
     extern __shared__ f4_t red[];
     const int lane = threadIdx.x & 63, l = lane & 15, q4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
               waves = blockDim.x >> 6;
     const unsigned slot = blockIdx.x / (unsigned)split, first = blockIdx.x - slot * (unsigned)split;
     const GroupSlot s = g4_slot<16>(g, slot);
     if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
-    const int tiles = (g.n + 15) / 16, kb = g.k / 32, c0 = 4 * wave;
+    const int tiles = (g.n + 15) / 16, kb = g.k / 32, groups = (kb + 15) / 16;
     if (s.e == g.E) {                                          // rows of no expert
         for (int tile = first; tile < tiles; tile += split)
             if (wave == 0)
@@ -77,7 +86,7 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
     }
     // a tile's weights and scales; a chunk's are asked for anew for the next tile as soon as they are used
     const int64_t row0 = (int64_t)s.e * g.n, rows = (int64_t)g.E * g.n;
-    const uint32_t off = (uint32_t)l * (uint32_t)(kb * 16) + 64 * c0 + 16 * q4;
+    const uint32_t off = (uint32_t)l * (uint32_t)(kb * 16) + 16 * q4;
     typedef G4Scales<XT, SG, Z> S;
     struct Tile {
         __amdgpu_buffer_rsrc_t w;
@@ -90,63 +99,93 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
             srow = (l < left ? l : left - 1) * g.groups;
         }
     };
-    const auto load_w = [&](const Tile& d, int u) { return mx4_buffer16(d.w, 4 * (c0 + u) + q4 < kb ? off + 64 * u : kMx4Out); };
+    const auto load_w = [&](const Tile& d, int c) { return mx4_buffer16(d.w, 4 * c + q4 < kb ? off + 64 * c : kMx4Out); };
     // Scales: lane group u brings the four of chunks 4 / SG u .. of its row and lays them out in LDS as they are used, [16][16 rows].
     u32x4_t w[4];
     S raw;
-    const int set = q4 < SG ? q4 : SG - 1, cf = c0 + set * (4 / SG);
+    const int set = q4 < SG ? q4 : SG - 1, cs = set * (4 / SG);
     float* const ls = reinterpret_cast<float*>(red + (waves > 1 ? 2 * waves * 64 : 0)) + wave * (Z ? 512 : 256) + l;
     uint32_t* const lz = reinterpret_cast<uint32_t*>(ls + 256);
     {
         const Tile d(g, row0, rows, first * 16, kb, l);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) w[u] = load_w(d, u);
-        raw.load(g, d.b, d.srow, cf);
+        for (int u = 0; u < 4; ++u) w[u] = load_w(d, 4 * wave + u);
+        raw.load(g, d.b, d.srow, 4 * wave + cs);
     }
     // x: of lane l the row l, inputs 32 v + 8 (lane >> 4) of each chunk; 0 behind the row's end
-    u32x4_t x[4][4];
-    {
-        const __amdgpu_buffer_rsrc_t r = mx4_rsrc(reinterpret_cast<const uint8_t*>(g.x + s.row * g.x_ld), 0xE0000000LL);
-        const uint32_t at = (uint32_t)(l < s.rows ? l : 0) * (uint32_t)(2 * g.x_ld) + 256 * c0 + 16 * q4;
+    u32x4_t x[XL ? 1 : 4][4];
+    const int stride = (int)g4_x_stride(g.k);
+    char* const xl = reinterpret_cast<char*>(red + (waves > 1 ? 2 * waves * 64 : 0)) + waves * (Z ? 2048 : 1024);
+    const __amdgpu_buffer_rsrc_t xr = mx4_rsrc(reinterpret_cast<const uint8_t*>(g.x + s.row * g.x_ld), 0xE0000000LL);
+    if constexpr (XL) {
+        // all rows' units in one run over the threads, eight loads under way
+        const unsigned units = (unsigned)(kb + 3) / 4 * 16, all = units * s.rows, T = blockDim.x;
+        for (unsigned u0 = threadIdx.x; u0 < all; u0 += 8 * T) {
+            u32x4_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned u = u0 + i * T, r = u / units, c = u - r * units;
+                v[i] = mx4_buffer16(xr, u < all && c < (unsigned)kb * 4 ? r * (uint32_t)(2 * g.x_ld) + 16 * c : kMx4Out);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned u = u0 + i * T, r = u / units, c = u - r * units;
+                if (u < all) *reinterpret_cast<u32x4_t*>(xl + r * stride + 16 * c) = v[i];
+            }
+        }
+        __syncthreads();
+    } else {
+        const uint32_t at = (uint32_t)(l < s.rows ? l : 0) * (uint32_t)(2 * g.x_ld) + 1024 * wave + 16 * q4;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) x[u][v] = mx4_buffer16(r, 4 * (c0 + u) + v < kb ? at + 256 * u + 64 * v : kMx4Out);
+            for (int v = 0; v < 4; ++v) x[u][v] = mx4_buffer16(xr, 4 * (4 * wave + u) + v < kb ? at + 256 * u + 64 * v : kMx4Out);
     }
+    const char* const xrow = xl + (l < s.rows ? l : s.rows - 1) * stride + 16 * q4;
     int buf = 0;
 #pragma unroll 1
     for (int tile = first; tile < tiles; tile += split, buf ^= 1) {
-        const bool last = tile + split >= tiles;               // (the last tile's weights are read again and not used)
-        const Tile next(g, row0, rows, 16 * (last ? tile : tile + split), kb, l);
-        {
-            const Tile d(g, row0, rows, 16 * tile, kb, l);
-            raw.fix(g, d.b, d.srow, cf);
-        }
-        if (q4 < SG)
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int k = S::index(g, cf, cf + p / SG, p % SG);
-                ls[(4 * set + p) * 16] = raw.scale(k, S::first(g, cf) + k < g.groups, g.scale_bf16);
-                if constexpr (Z) lz[(4 * set + p) * 16] = raw.zero(k);
-            }
-        raw.load(g, next.b, next.srow, cf);
-        __builtin_amdgcn_wave_barrier();
         f4_t acc = {};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            g4_turn(w[u]);
-#pragma unroll
-            for (int i = 0; i < SG; ++i) {
-                const float f = ls[(u * SG + i) * 16];
-                const uint32_t zero = Z ? lz[(u * SG + i) * 16] : g4_zero<XT, Z>(8);
-                f4_t part = {};
-#pragma unroll
-                for (int v = i * (4 / SG); v < (i + 1) * (4 / SG); ++v)
-                    part = mfma16<XT>(x[u][v], g4_frag<XT, Z>(w[u][v], zero), part);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(f, part[e], acc[e]);
+#pragma unroll 1
+        for (int gi = wave; gi < groups; gi += waves) {        // (waves <= groups: every wave has a group of every tile)
+            // the next group: this tile's, or the next tile's first (the last tile's is read again and not used)
+            const bool on = gi + waves < groups;
+            const int c0 = 4 * gi, cn = 4 * (on ? gi + waves : wave), tn = on || tile + split >= tiles ? tile : tile + split;
+            const Tile next(g, row0, rows, 16 * tn, kb, l);
+            {
+                const Tile d(g, row0, rows, 16 * tile, kb, l);
+                raw.fix(g, d.b, d.srow, c0 + cs);
             }
-            w[u] = load_w(next, u);
+            if (q4 < SG)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const int k = S::index(g, c0 + cs, c0 + cs + p / SG, p % SG);
+                    ls[(4 * set + p) * 16] = raw.scale(k, S::first(g, c0 + cs) + k < g.groups, g.scale_bf16);
+                    if constexpr (Z) lz[(4 * set + p) * 16] = raw.zero(k);
+                }
+            raw.load(g, next.b, next.srow, cn + cs);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (4 * (c0 + u) < kb) {                       // uniform
+                    if constexpr (XL)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) x[0][v] = *reinterpret_cast<const u32x4_t*>(xrow + 256 * (c0 + u) + 64 * v);
+                    g4_turn(w[u]);
+#pragma unroll
+                    for (int i = 0; i < SG; ++i) {
+                        const float f = ls[(u * SG + i) * 16];
+                        const uint32_t zero = Z ? lz[(u * SG + i) * 16] : g4_zero<XT, Z>(8);
+                        f4_t part = {};
+#pragma unroll
+                        for (int v = i * (4 / SG); v < (i + 1) * (4 / SG); ++v)
+                            part = mfma16<XT>(x[XL ? 0 : u][v], g4_frag<XT, Z>(w[u][v], zero), part);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(f, part[e], acc[e]);
+                    }
+                }
+                w[u] = load_w(next, cn + u);
+            }
         }
         if (waves > 1) {
             f4_t* o = red + buf * waves * 64;                  // two, so that one barrier a tile is enough
@@ -176,14 +215,27 @@ __global__ __launch_bounds__(1024, 4) void g4_decode_kernel(G4Args g, int split)
 
 template <int XT, int SG, bool Z>
 static int launch_g4_decode(G4Args g, hipStream_t st) {
-    const int waves = (g.k + kG4Slice - 1) / kG4Slice;
+    const int groups = (g.k + kG4Slice - 1) / kG4Slice, few = g.T < 16 ? g.T : 16;
+    const int64_t own = Z ? 2048 : 1024, xb = few * g4_x_stride(g.k);
+    // x in LDS where two workgroups of eight waves fit a CU: as few rounds of groups as eight waves take, with as few waves as do them
+    int waves = (groups + 7) / 8;
+    waves = (groups + waves - 1) / waves;
+    const bool xl = 2 * (xb + waves * (2048 + own)) <= kG4Lds;
+    if (!xl) waves = groups;
+    EXL3_CHECK_ARG(waves <= kG4Waves, "g4: too many inputs");
+    const int64_t lds = (waves > 1 ? 2 * waves * 1024 : 0) + waves * own + (xl ? xb : 0);
     g.slots = (int)(g.ends ? group_slots(g.T, g.E, 16, g.rest) : (g.T + 15) / 16);
-    // row blocks that have work: no more than there are rows, nor than slots
-    const int64_t tiles = (g.n + 15) / 16, room = 256 * (16 / waves > 4 ? 4 : 16 / waves), live = g.slots;
-    const int64_t rounds = (tiles * live + room - 1) / room, split = (tiles + rounds - 1) / rounds;
+    const int64_t by_lds = kG4Lds / lds, by_waves = 16 / waves, fit = by_lds < by_waves ? by_lds : by_waves;
+    // workgroups: as few as need no more rounds
+    const int64_t tiles = (g.n + 15) / 16, room = 256 * (fit > 4 ? 4 : fit);
+    const int64_t rounds = (tiles * g.slots + room - 1) / room, split = (tiles + rounds - 1) / rounds;
     EXL3_CHECK_ARG(g.slots * split <= kMx4Grid / 4, "g4: grid too large");
-    EXL3_LAUNCH("g4_decode", (g4_decode_kernel<XT, SG, Z>), dim3((unsigned)(g.slots * split)), dim3(64 * waves),
-                (size_t)(waves > 1 ? 2 * waves * 1024 : 0) + waves * (Z ? 2048 : 1024), st, g, (int)split);
+    if (xl)
+        EXL3_LAUNCH("g4_decode", (g4_decode_kernel<XT, SG, Z, true>), dim3((unsigned)(g.slots * split)), dim3(64 * waves), (size_t)lds, st,
+                    g, (int)split);
+    else
+        EXL3_LAUNCH("g4_decode", (g4_decode_kernel<XT, SG, Z, false>), dim3((unsigned)(g.slots * split)), dim3(64 * waves), (size_t)lds,
+                    st, g, (int)split);
     return EXL3_OK;
 }
 

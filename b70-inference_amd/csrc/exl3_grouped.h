@@ -37,10 +37,10 @@ __device__ __forceinline__ int wave_running_sum(int v) {
 }
 
 // fn(first expert of 64, this lane's begin and end) for the experts and the rows of none as the last of all, until it returns true.
-// Five loads of either kind are under way: one after another they are a microsecond for every 64 experts and more.
+// Nine loads of either kind are under way: one after another they are a microsecond for every 64 experts and more.
 template <typename F>
 __device__ __forceinline__ void group_each(const int32_t* ends, int E, int T, F fn) {
-    constexpr int kBatch = 5;
+    constexpr int kBatch = 9;
     const int lane = threadIdx.x & 63;
     for (int i0 = 0; i0 <= E; i0 += 64 * kBatch) {
         int lo[kBatch], hi[kBatch];
