@@ -51,11 +51,12 @@ __global__ __launch_bounds__(256) void g4_reduce_kernel(G4Args g) {
 
 // Kernel and splits of a call: the least time by an estimate from measurements (1 to 512 rows of nine shapes from 640 -> 2560 to
 // 8192 -> 8192 and 5376 -> 21504), in microseconds for 256 CUs. Six rows of 8192 -> 8192, fp16: 16 with the kernel of few rows, 18
-// with the other; of 5376 -> 21504 24 and 22, in groups of 32 24 and 27; 24 rows of it 42 and 25; of 4096 -> 4096 13 and 17. Splits are the linear's alone (experts have workgroups enough, or few rows).
+// with the other; of 5376 -> 21504 24 and 22, in groups of 32 24 and 27; 24 rows of it 42 and 25; of 4096 -> 4096 13 and 17. Splits are the linear's alone: experts have workgroups enough, or few
+// rows, and rows of no expert have no sums.
 struct G4Plan {
     int tile, splits, spc;
 };
-static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E) {
+static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E, bool split) {
     const int64_t steps = (k + 127) / 128;
     G4Plan best = {0, 1, (int)steps};
     double least = 1e30;
@@ -69,7 +70,7 @@ static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E)
     const double scales = group >= 128 ? 0.95 : group == 64 ? 1.05 : 1.25;
     for (int t = 0; t < 3; ++t) {
         const int64_t bm = 32 << t, blocks = E == 1 ? (m + bm - 1) / bm : m / bm + (m < E ? m : E), tiles = blocks * ((n + 255) / 256);
-        for (int64_t p = 1; p <= (E > 1 ? 1 : steps < 16 ? steps : 16); ++p) {
+        for (int64_t p = 1; p <= (!split ? 1 : steps < 16 ? steps : 16); ++p) {
             const int64_t spc = (steps + p - 1) / p, full = tiles * p / (256 * kOcc[t]), left = tiles * p - full * 256 * kOcc[t];
             if ((steps + spc - 1) / spc != p) continue;
             double us = 2.0 + (double)full * (3.0 + scales * (double)spc * kStep[t][kOcc[t] - 1]);
@@ -138,7 +139,7 @@ static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, 
         else EXL3_LAUNCH("g4_tiny", g4_tiny_kernel<kRowBF16>, grid, dim3(256), 0, st, g, (int)group);
         return EXL3_OK;
     }
-    G4Plan plan = g4_plan(m, n, k, group, E);
+    G4Plan plan = g4_plan(m, n, k, group, E, !ends);
     const int want = env_int("EXL3MI_G4_TILE", 0);
     if (want > (k <= 8192 ? 0 : 1) && want <= 4) plan = {want - 1, 1, (int)((k + 127) / 128)};
     g.splits = plan.splits;
@@ -166,7 +167,7 @@ using namespace exl3;
 
 int64_t exl3_g4_linear_scratch(int64_t m, int64_t k, int64_t n, int64_t group) {
     if (m <= 0 || m > 0x3FFFFFFF || n <= 0 || n > 0x3FFFFFFF || k <= 0 || k > (1 << 22) || group <= 0 || n * (k / group) < 4) return 0;
-    return g4_part_bytes(g4_plan(m, n, k, group, 1), m, n);
+    return g4_part_bytes(g4_plan(m, n, k, group, 1, true), m, n);
 }
 
 int exl3_g4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const void* scales,

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(256) void grouped_reduce_kernel(GroupedArgs g, cons
 int grouped_reduce(const GroupedArgs& g, const float* part, int64_t n4, int64_t stride, hipStream_t st) {
     const int64_t wgs = ((int64_t)g.E * g.m * (n4 / 4) + 255) / 256;
     EXL3_CHECK_ARG(wgs <= kMx4Grid, "grouped_reduce: grid too large");
-    EXL3_LAUNCH("grouped_reduce", grouped_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, g, part, n4, stride);
+    GROUPED_LAUNCH("grouped_reduce", grouped_reduce_kernel, dim3((unsigned)wgs), dim3(256), g.accumulate, st, g, part, n4, stride);
     return EXL3_OK;
 }
 

@@ -65,8 +65,8 @@ int exl3_release_workspace(void);
 int exl3_device_status(int* status);
 
 /* Kernel timing: while enabled (on != 0), every kernel the library launches is bracketed by a HIP event pair on its
- * stream; with on = R > 1 each launch runs R times inside its pair (the kernels are idempotent) to amortise the event
- * overhead. exl3_profile_read writes "name count avg_us" lines (per-launch averages) since the last enable.
+ * stream; with on = R > 1 each launch runs R times inside its pair (the kernels are idempotent; exl3_grouped_mm_dw's
+ * with accumulate, which are not, run once and untimed) to amortise the event overhead. exl3_profile_read writes "name count avg_us" lines (per-launch averages) since the last enable.
  * Not for use under graph capture. No reference counterpart (the reference times with torch.profiler). */
 int exl3_profile_enable(int on);
 int exl3_profile_read(char* out, int64_t cap);
@@ -384,7 +384,7 @@ int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t 
  * Rows t with ends[e - 1] <= t < ends[e] (0 for ends[-1]) of a matrix of T rows belong to expert e; ends int32 [E] on the device,
  * ascending, at most T (other values lead to no access out of range, but to rows that belong to no or to several experts). An
  * expert may have no rows; rows from ends[E - 1] on belong to none. Any sizes (columns at most 2^22, as the row strides);
- * operands of 16-byte aligned rows of whole multiples of eight values are read fastest. Sums are fp32 in an order fixed by the
+ * operands of 16-byte aligned rows of whole multiples of eight values are read fastest. Outputs must not overlap operands. Sums are fp32 in an order fixed by the
  * sizes, with one rounding. No reference counterpart (the reference's experts are EXL3 only). */
 enum exl3_grouped_w { EXL3_GROUPED_W_NK = 0, EXL3_GROUPED_W_KN = 1 };
 
@@ -422,7 +422,7 @@ int exl3_g4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t 
                    int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,
                    int c_dtype, void* stream);
 
-/* With scratch from the caller, as the _in calls above; calls of up to 16 rows and some others need none. */
+/* With scratch from the caller, as the _in calls above; most calls of up to 16 rows need none. */
 int64_t exl3_g4_linear_scratch(int64_t m, int64_t k, int64_t n, int64_t group);
 int exl3_g4_linear_in(const void* x, int64_t x_ld, int x_dtype, int64_t m, int64_t k, const uint8_t* codes, const void* scales,
                       int scale_dtype, const uint8_t* zeros, int64_t group, int64_t n, const float* bias, void* C, int64_t c_ld,

@@ -175,3 +175,52 @@ def test_strided_rows_and_outputs(exl3):
     assert lin.run_alloc(x[:0], 40, True).shape == (0, 40)
     x32 = x.float()
     check(lin.run_alloc(x32, 40, True), *product(x32.half(), values(*w)), 256)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("T", (40, 130))
+def test_one_expert_keeps_rows_of_none(exl3, T, dtype):
+    """One expert of few outputs and many inputs, where a linear's inputs would be split over workgroups."""
+    codes, scales, z = make((1,), 256, 4096, 128, True, dtype, T)
+    x = rows(T + 9, 4096, dtype, T)
+    ends = ends_of([T])
+    y = torch.full((T + 9, 256), 5.0, device="cuda")
+    exl3.grouped_mm(x, exl3.G4Tensor(codes, scales, z), ends, out=y)
+    check(y[:T], *product(x[:T], values(codes[0], scales[0], z[0])), 4096)
+    assert bool((y[T:] == 5).all())
+    y = exl3.grouped_mm(x, exl3.G4Tensor(codes, scales, z), ends)
+    assert bool((y[T:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m,n,k,group,zeros", ((15, 40, 2048, 128, False), (14, 50, 2048, 64, True), (6, 33, 4608, 32, False), (1, 700, 8192, 64, True),
+                                               (3, 4200, 1536, 128, True), (9, 70, 512, 512, False)))
+def test_few_rows(exl3, m, n, k, group, zeros, dtype):
+    """Rows that fill their share of a CU's LDS and rows that do not, groups of inputs that waves take in turn, many tiles."""
+    w = make((), n, k, group, zeros, dtype, m + n)
+    x = rows(m, k, dtype, m)
+    y = torch.full((m, n), float("nan"), device="cuda")
+    exl3.G4Linear(exl3.G4Tensor(*w)).run(x, y)
+    check(y, *product(x, values(*w)), k)
+
+
+def test_offsets_past_32_bits(exl3):
+    """Codes of 5.4 GB, rows and outputs of more than 4 GB."""
+    E, n, k, m = 640, 4096, 4096, 20
+    codes = torch.zeros(E, n, k // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(E, n, k // 128, dtype=torch.float16, device="cuda")
+    w = make((), n, k, 128, False, torch.float16, 1)
+    codes[-1], scales[-1] = w[0], w[1]
+    x = rows(m, k, torch.float16, 2)
+    ref, mag = product(x, values(*w))
+    for T in (m, 600):                                         # few rows of the last expert, and all experts in blocks of them
+        xs = torch.cat((torch.ones(T - m, k, dtype=torch.float16, device="cuda"), x))
+        ends = ends_of([0] * (E - 2) + [T - m, m])
+        check(exl3.grouped_mm(xs, exl3.G4Tensor(codes, scales), ends)[T - m:], ref, mag, k)
+    T = (1 << 31) // k + 1000                                  # x 4.3 GB, y 4.3 GB
+    xs = torch.zeros(T, k, dtype=torch.float16, device="cuda")
+    xs[-m:] = x
+    y = torch.empty(T, n, dtype=torch.float16, device="cuda")
+    exl3.G4Linear(exl3.G4Tensor(*w)).run(xs, y)
+    check(y[-m:], ref, mag, k)
+    assert not bool(y[:-m].any())

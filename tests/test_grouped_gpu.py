@@ -215,3 +215,51 @@ def test_repeats_and_permutations(exl3):
     assert torch.equal(dw, exl3.grouped_mm_dw(dy, x, ends))
     order = torch.cat([a + torch.randperm(b - a) for _, a, b in spans(ends)]).cuda()
     assert torch.equal(exl3.grouped_mm(x[order], w, ends), y[order])
+
+
+def test_timing_that_repeats_launches_adds_once(exl3):
+    from importlib import import_module
+    lib = import_module(exl3.__name__ + "._lib")
+    for N, K in ((96, 40), (256, 264)):                        # in one part and in parts
+        ends = ends_of([3000, 20])
+        x, dy, _ = _data(3020, 2, N, K, torch.bfloat16, N)
+        dw = torch.ones(2, N, K, device="cuda")
+        lib.profile_enable(True, repeat=3)
+        try:
+            exl3.grouped_mm_dw(dy, x, ends, out=dw, accumulate=True)
+            torch.cuda.synchronize()
+        finally:
+            lib.profile_enable(False)
+        ref, mag = weights_gradient(dy, x, ends)
+        check(dw, ref + 1, mag + 1, 3001, f"{N} x {K}")
+
+
+@pytest.mark.parametrize("m", (10, 300))
+def test_offsets_past_32_bits(exl3, m):
+    """Weights of 9 GB, then rows and outputs of more than 4 GB each, whose last expert's rows lie at the end."""
+    E, N, K = 1100, 2048, 2048
+    w = torch.zeros(E, N, K, dtype=torch.bfloat16, device="cuda")
+    x, dy, last = _data(m, 1, N, K, torch.bfloat16, m)
+    w[-1] = last[0]
+    ends, one = ends_of([0] * (E - 1) + [m]), ends_of([m])
+    ref, mag = rows_product(x, last, one, m)
+    rdx, mdx = rows_product(dy, last.transpose(1, 2), one, m)
+    check(exl3.grouped_mm(x, w, ends), ref, mag, K, "forward")
+    check(exl3.grouped_mm_dx(dy, w, ends), rdx, mdx, N, "dx")
+    rdw, mdw = weights_gradient(dy, x, one)
+    exl3.grouped_mm_dw(dy, x, ends, out=w)
+    check(w[-1:], rdw, mdw, m, "dw")
+    assert not bool(w[:-1].any())
+    del w
+    T = (1 << 31) // K + 700
+    xs, dys = (torch.cat((torch.zeros(T - m, K, dtype=torch.bfloat16, device="cuda"), v)) for v in (x, dy))
+    two = torch.cat((torch.zeros_like(last), last))
+    ends = ends_of([T - m, m])
+    y = exl3.grouped_mm(xs, two, ends)
+    check(y[-m:], ref, mag, K, "forward, many rows")
+    assert not bool(y[:-m].any())
+    y = exl3.grouped_mm_dx(dys, two, ends)
+    check(y[-m:], rdx, mdx, N, "dx, many rows")
+    dw = exl3.grouped_mm_dw(dys, xs, ends)
+    check(dw[1:], rdw, mdw, m, "dw, many rows")
+    assert not bool(dw[0].any())
