@@ -32,10 +32,10 @@ struct G4Args {
     int groups, per;                   // scales of a row; chunks of 128 that share one (groups of 32 and 64: 1)
     int scale_bf16, out_dtype, vec, rest;
     int slots;                         // row blocks of the grid
-    // steps of 128 inputs split over workgroups: `splits` of `spc`, their sums in part [splits][T][n4] (n4: n rounded up to 4)
-    int splits, spc;
+    // The steps of 128 inputs of the tiles from `whole` on are split over workgroups, `splits` of `spc`. Their sums lie in
+    // part [splits][tiles from whole on][part_rows][256].
+    int whole, splits, spc, part_rows;
     float* part;
-    int64_t n4;
 };
 
 // 4 x 4 words of lane groups and blocks turned.
@@ -133,12 +133,6 @@ __device__ __forceinline__ void g4_store4(const G4Args& g, int64_t m, int64_t n,
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         if (n + q < g.n) store_as(g.out, m * g.out_ld + n + q, v[q], g.out_dtype);
-}
-
-// The same of split sp: the output, or its sums.
-__device__ __forceinline__ void g4_put4(const G4Args& g, unsigned sp, int64_t m, int64_t n, f4_t v) {
-    if (!g.part) g4_store4(g, m, n, v);
-    else if (n < g.n4) *reinterpret_cast<f4_t*>(g.part + ((int64_t)sp * g.T + m) * g.n4 + n) = v;
 }
 
 // tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows

@@ -29,17 +29,21 @@ __global__ __launch_bounds__(256) void g4_tiny_kernel(G4Args g, int group) {
     store_as(g.out, m * g.out_ld + n, sum + (g.bias ? ldg(g.bias + n) : 0.f), g.out_dtype);
 }
 
-// The splits' sums in order, the bias, one rounding.
-__global__ __launch_bounds__(256) void g4_reduce_kernel(G4Args g) {
-    const int64_t q4 = g.n4 / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / q4, n = 4 * (i - m * q4);
-    if (m >= g.T) return;
-    const float* p = g.part + m * g.n4 + n;
+// The splits' sums in order, the bias, one rounding: four neighbours per thread, four rows of a tile per workgroup.
+__global__ __launch_bounds__(256) void g4_reduce_kernel(G4Args g, int bm) {
+    const unsigned nnt = (unsigned)((g.n + 255) / 256), all = g.slots * nnt, tail = all - g.whole, groups = (g.part_rows + 3) / 4,
+                   at = blockIdx.x / groups, r = (blockIdx.x - at * groups) * 4 + threadIdx.x / 64;
+    unsigned mt, nt;
+    grouped_tile(g.whole + at, (unsigned)g.slots, nnt, mt, nt);
+    const int64_t m = (int64_t)mt * bm + r, n = (int64_t)nt * 256 + 4 * (threadIdx.x & 63);
+    if ((int)r >= g.part_rows || m >= g.T || n >= g.n) return;
+    const int64_t stride = (int64_t)tail * g.part_rows * 256;
+    const float* p = g.part + ((int64_t)at * g.part_rows + r) * 256 + 4 * (threadIdx.x & 63);
     f4_t v = {};
     for (int s0 = 0; s0 < g.splits; s0 += 4) {
         f4_t t[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-            t[s] = ldg(reinterpret_cast<const f4_t*>(p + (int64_t)(s0 + s < g.splits ? s0 + s : s0) * g.T * g.n4));
+        for (int s = 0; s < 4; ++s) t[s] = ldg(reinterpret_cast<const f4_t*>(p + (s0 + s < g.splits ? s0 + s : s0) * stride));
 #pragma unroll
         for (int s = 0; s < 4; ++s)
             if (s0 + s < g.splits)
@@ -54,38 +58,53 @@ __global__ __launch_bounds__(256) void g4_reduce_kernel(G4Args g) {
 // with the other; of 5376 -> 21504 24 and 22, in groups of 32 24 and 27; 24 rows of it 42 and 25; of 4096 -> 4096 13 and 17. Splits are the linear's alone: experts have workgroups enough, or few
 // rows, and rows of no expert have no sums.
 struct G4Plan {
-    int tile, splits, spc;
+    int tile;
+    int64_t whole, splits, spc;
 };
+static int64_t g4_rows(int tile) { return 16 << tile; }
+static int64_t g4_tiles(int tile, int64_t m, int64_t n) { return (m + g4_rows(tile) - 1) / g4_rows(tile) * ((n + 255) / 256); }
 static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E, bool split) {
     const int64_t steps = (k + 127) / 128;
-    G4Plan best = {0, 1, (int)steps};
+    G4Plan best = {0, 0, 1, steps};
     double least = 1e30;
     // blocks of 16 rows: the groups of 512 inputs of all tiles, spread over the CUs
     const int64_t live = E == 1 ? (m + 15) / 16 : m / 16 + (m < E ? m : E);
     if (k <= 8192 && (E == 1 || m <= 16 * E))
         least = 6.5 + (double)(live * ((n + 15) / 16) * ((k + 511) / 512)) / 256.0 * (0.265 + 0.003 * (double)(m < 16 ? m : 16));
-    // blocks of 32, 64, 128 rows: time of a step with one, two, three workgroups to a CU, full rounds and what is left
+    // blocks of 32, 64, 128 rows: time of a step with one, two, three workgroups to a CU; all tiles in splits, or full rounds of whole
+    // tiles and the rest in splits (1021 rows of 5376 -> 21504, 672 tiles for 512 places: 250 us whole, 223 with the last 160 in three)
     static const double kStep[3][3] = {{1.45, 2.05, 2.85}, {1.65, 2.6, 2.6}, {2.6, 3.9, 3.9}};
     static const int kOcc[3] = {3, 2, 2};
     const double scales = group >= 128 ? 0.95 : group == 64 ? 1.05 : 1.25;
     for (int t = 0; t < 3; ++t) {
-        const int64_t bm = 32 << t, blocks = E == 1 ? (m + bm - 1) / bm : m / bm + (m < E ? m : E), tiles = blocks * ((n + 255) / 256);
-        for (int64_t p = 1; p <= (!split ? 1 : steps < 16 ? steps : 16); ++p) {
-            const int64_t spc = (steps + p - 1) / p, full = tiles * p / (256 * kOcc[t]), left = tiles * p - full * 256 * kOcc[t];
-            if ((steps + spc - 1) / spc != p) continue;
-            double us = 2.0 + (double)full * (3.0 + scales * (double)spc * kStep[t][kOcc[t] - 1]);
-            if (left) us += 3.0 + scales * (double)spc * kStep[t][(left + 255) / 256 - 1];
-            if (p > 1) us += 3.0 + (double)(p * m * n) * 1.2e-6;
-            if (us < least) {
-                least = us;
-                best = {t + 1, (int)p, (int)spc};
+        const int64_t bm = 32 << t, room = 256 * kOcc[t], blocks = E == 1 ? (m + bm - 1) / bm : m / bm + (m < E ? m : E),
+                      tiles = blocks * ((n + 255) / 256), rounds = tiles / room;
+        const auto time = [&](int64_t wgs, int64_t spc) {
+            const int64_t full = wgs / room, left = wgs - full * room;
+            return (double)full * (3.0 + scales * (double)spc * kStep[t][kOcc[t] - 1]) +
+                   (left ? 3.0 + scales * (double)spc * kStep[t][(left + 255) / 256 - 1] : 0.0);
+        };
+        for (int tail = 0; tail < (split && rounds ? 2 : 1); ++tail) {
+            const int64_t whole = tail ? rounds * room : 0, rest = tiles - whole;
+            if (rest == 0) break;
+            for (int64_t p = tail ? 2 : 1; p <= (!split ? 1 : steps < 16 ? steps : 16); ++p) {
+                const int64_t spc = (steps + p - 1) / p;
+                if ((steps + spc - 1) / spc != p) continue;
+                double us = 2.0 + time(whole, steps) + time(rest * p, spc);
+                if (p > 1) us += 3.0 + (tail ? (double)(p * rest * bm * 256) : (double)(p * m * n)) * 1.2e-6;
+                if (us < least) {
+                    least = us;
+                    best = {t + 1, whole, p, spc};
+                }
             }
         }
     }
     return best;
 }
-static int64_t g4_n4(int64_t n) { return (n + 3) & ~(int64_t)3; }
-static int64_t g4_part_bytes(const G4Plan& p, int64_t m, int64_t n) { return p.splits == 1 ? 0 : (int64_t)p.splits * m * g4_n4(n) * 4; }
+static int64_t g4_part_rows(const G4Plan& p, int64_t m) { return m < g4_rows(p.tile) ? m : g4_rows(p.tile); }
+static int64_t g4_part_bytes(const G4Plan& p, int64_t m, int64_t n) {
+    return p.splits == 1 ? 0 : p.splits * (g4_tiles(p.tile, m, n) - p.whole) * g4_part_rows(p, m) * 1024;
+}
 
 static int out_size(int t) { return t == EXL3_F32 ? 4 : 2; }
 
@@ -141,10 +160,11 @@ static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, 
     }
     G4Plan plan = g4_plan(m, n, k, group, E, !ends);
     const int want = env_int("EXL3MI_G4_TILE", 0);
-    if (want > (k <= 8192 ? 0 : 1) && want <= 4) plan = {want - 1, 1, (int)((k + 127) / 128)};
-    g.splits = plan.splits;
-    g.spc = plan.spc;
-    g.n4 = g4_n4(n);
+    if (want > (k <= 8192 ? 0 : 1) && want <= 4) plan = {want - 1, 0, 1, (k + 127) / 128};
+    g.whole = (int)plan.whole;
+    g.splits = (int)plan.splits;
+    g.spc = (int)plan.spc;
+    g.part_rows = (int)g4_part_rows(plan, m);
     if (plan.splits > 1) {
         Carve c{};
         const int rc = call_scratch(what, (size_t)g4_part_bytes(plan, m, n), s, st, &c);
@@ -153,9 +173,10 @@ static int g4_product(const char* what, const void* x, int64_t x_ld, int dtype, 
     }
     const int rc = dtype == EXL3_F16 ? g4_run_f16(g, (int)group, plan.tile, st) : g4_run_bf16(g, (int)group, plan.tile, st);
     if (rc || plan.splits == 1) return rc;
-    const int64_t wgs = (m * (g.n4 / 4) + 255) / 256;
+    g.slots = (int)((m + g4_rows(plan.tile) - 1) / g4_rows(plan.tile));
+    const int64_t wgs = (g4_tiles(plan.tile, m, n) - plan.whole) * ((g.part_rows + 3) / 4);
     EXL3_CHECK_ARG(wgs <= kMx4Grid, "%s: grid too large", what);
-    EXL3_LAUNCH("g4_reduce", g4_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, g);
+    EXL3_LAUNCH("g4_reduce", g4_reduce_kernel, dim3((unsigned)wgs), dim3(256), 0, st, g, (int)g4_rows(plan.tile));
     return EXL3_OK;
 }
 

@@ -240,8 +240,8 @@ static int launch_g4_decode(G4Args g, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// Tiles of BM rows x 256 outputs, 64 of them per wave, in steps of a chunk; the steps of a tile may be split over workgroups, whose sums
-// g4_reduce_kernel adds. x goes to LDS by direct loads (eight values a unit, permuted as in the 16-bit products), the weights
+// Tiles of BM rows x 256 outputs, 64 of them per wave, in steps of a chunk; the steps of the last tiles, or of all, may be split over
+// workgroups, whose sums g4_reduce_kernel adds. x goes to LDS by direct loads (eight values a unit, permuted as in the 16-bit products), the weights
 // straight to the registers of the one wave that converts them, the scales four at a time. Tile j of a wave has outputs
 // 4 (lane & 15) + j, so that a lane stores four neighbours. Two of the four are converted and multiplied at a time, and
 // their registers take the next step's weights.
@@ -250,14 +250,16 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
     constexpr int kUnits = BM * 16, kLoads = kUnits / 256, RT = BM / 16;
     __shared__ u32x4_t lds[2 * kUnits + 4 * (Z ? 128 : 64)];   // x, and the waves' scales and zeros
     const int t = threadIdx.x, lane = t & 63, l = lane & 15, q4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const unsigned nnt = (unsigned)((g.n + 255) / 256), all = g.slots * nnt, id = grouped_place(kChunk, blockIdx.x);
-    if (id >= all * g.splits) return;
-    const unsigned sp = id / all;
+    const unsigned nnt = (unsigned)((g.n + 255) / 256), whole = (unsigned)g.whole, tail = g.slots * nnt - whole,
+                   id = grouped_place(kChunk, blockIdx.x);
+    if (id >= whole + tail * g.splits) return;
+    const bool parted = id >= whole;                           // uniform
+    const unsigned sp = parted ? (id - whole) / tail : 0, tile = parted ? id - sp * tail : id;
     unsigned mt, nt;
-    grouped_tile(id - sp * all, (unsigned)g.slots, nnt, mt, nt);
+    grouped_tile(tile, (unsigned)g.slots, nnt, mt, nt);
     const GroupSlot s = g4_slot<BM>(g, mt);
     if (s.rows == 0 || (s.e == g.E && !g.rest)) return;
-    const int kb = g.k / 32, c0 = (int)sp * g.spc, end = (kb + 3) / 4 - c0 < g.spc ? (kb + 3) / 4 : c0 + g.spc,
+    const int kb = g.k / 32, c0 = (int)sp * g.spc, end = !parted || (kb + 3) / 4 - c0 < g.spc ? (kb + 3) / 4 : c0 + g.spc,
               steps = s.e == g.E ? 0 : end - c0;
     const int64_t n0 = (int64_t)nt * 256 + 64 * wave, row0 = (int64_t)(s.e < g.E ? s.e : 0) * g.n, rows = (int64_t)g.E * g.n;
     f4_t acc[RT][4];
@@ -376,15 +378,17 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
         for (int e = 0; e < 4; ++e) {
             const int m = 16 * r + 4 * q4 + e;
             constexpr float k = kG4Factor<XT, Z>;
-            if (m < s.rows)
-                g4_put4(g, sp, s.row + m, n0 + 4 * l, f4_t{k * acc[r][0][e], k * acc[r][1][e], k * acc[r][2][e], k * acc[r][3][e]});
+            if (m >= s.rows) continue;
+            const f4_t v = {k * acc[r][0][e], k * acc[r][1][e], k * acc[r][2][e], k * acc[r][3][e]};
+            if (parted && g.splits > 1) *reinterpret_cast<f4_t*>(g.part + ((int64_t)(sp * tail + tile - whole) * g.part_rows + m) * 256 + 64 * wave + 4 * l) = v;
+            else g4_store4(g, s.row + m, n0 + 4 * l, v);
         }
 }
 
 template <int XT, int SG, bool Z, int BM, int OCC>
 static int launch_g4_wide(G4Args g, hipStream_t st) {
     g.slots = (int)(g.ends ? group_slots(g.T, g.E, BM, g.rest) : (g.T + BM - 1) / BM);
-    const int64_t tiles = (int64_t)g.slots * ((g.n + 255) / 256) * g.splits;
+    const int64_t all = (int64_t)g.slots * ((g.n + 255) / 256), tiles = g.whole + (all - g.whole) * g.splits;
     constexpr int64_t kRound = 8 * kChunk;
     EXL3_CHECK_ARG(tiles <= kMx4Grid - kRound, "g4: grid too large");
     EXL3_LAUNCH("g4_wide", (g4_wide_kernel<XT, SG, Z, BM, OCC>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)), dim3(256), 0,

@@ -224,3 +224,17 @@ def test_offsets_past_32_bits(exl3):
     exl3.G4Linear(exl3.G4Tensor(*w)).run(xs, y)
     check(y[-m:], ref, mag, k)
     assert not bool(y[:-m].any())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_last_tiles_in_splits(exl3, dtype):
+    """More tiles than the CUs take in a round: the last ones' inputs are split over workgroups, the others' are not."""
+    m, n, k = 1037, 14850, 4096
+    need = exl3.lib().exl3_g4_linear_scratch(m, k, n, 128)
+    assert 0 < need < 2 * 4 * m * n
+    w = make((), n, k, 128, True, torch.float16, 3)
+    x, bias = rows(m, k, dtype, 4), torch.randn(n, device="cuda")
+    ref, mag = product(x, values(*w))
+    y = torch.full((m, n), float("nan"), device="cuda")
+    exl3.G4Linear(exl3.G4Tensor(*w), bias).run(x, y)
+    check(y, ref + bias.double(), mag + bias.double().abs(), k)
