@@ -73,8 +73,9 @@ static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E,
         least = 6.5 + (double)(live * ((n + 15) / 16) * ((k + 511) / 512)) / 256.0 * (0.265 + 0.003 * (double)(m < 16 ? m : 16));
     // blocks of 32, 64, 128 rows: time of a step with one, two, three workgroups to a CU; all tiles in splits, or full rounds of whole
     // tiles and the rest in splits (1021 rows of 5376 -> 21504, 672 tiles for 512 places: 250 us whole, 223 with the last 160 in three)
-    static const double kStep[3][3] = {{1.45, 2.05, 2.85}, {1.65, 2.6, 2.6}, {2.6, 3.9, 3.9}};
-    static const int kOcc[3] = {3, 2, 2};
+    static const double kStep[3][4] = {{1.45, 2.05, 2.85, 3.7}, {1.65, 2.6, 4.2}, {2.6, 3.9}};
+    const bool more = !split && group >= 128;                  // experts: a workgroup more to a CU
+    const int kOcc[3] = {more ? 4 : 3, more ? 3 : 2, 2};
     const double scales = group >= 128 ? 0.95 : group == 64 ? 1.05 : 1.25;
     for (int t = 0; t < 3; ++t) {
         const int64_t bm = 32 << t, room = 256 * kOcc[t], blocks = E == 1 ? (m + bm - 1) / bm : m / bm + (m < E ? m : E),

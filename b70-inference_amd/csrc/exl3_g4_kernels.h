@@ -243,9 +243,11 @@ static int launch_g4_decode(G4Args g, hipStream_t st) {
 // Tiles of BM rows x 256 outputs, 64 of them per wave, in steps of a chunk; the steps of the last tiles, or of all, may be split over
 // workgroups, whose sums g4_reduce_kernel adds. x goes to LDS by direct loads (eight values a unit, permuted as in the 16-bit products), the weights
 // straight to the registers of the one wave that converts them, the scales four at a time. Tile j of a wave has outputs
-// 4 (lane & 15) + j, so that a lane stores four neighbours. Two of the four are converted and multiplied at a time, and
-// their registers take the next step's weights.
-template <int XT, int SG, bool Z, int BM, int OCC>
+// 4 (lane & 15) + j, so that a lane stores four neighbours. JN of the four are converted and multiplied at a time, and
+// their registers take the next step's weights: two, or one for smaller tiles of experts, whose tiles are many and of few steps, so
+// that one workgroup more fits a CU and hides their starts (10240 rows over 512 experts of 640 -> 2560 168 -> 150 us, 40000 rows 333 ->
+// 289; of 2560 -> 640 151 -> 154; a linear's splits are slower by it, and so are groups of 32 and 64, whose products are short then).
+template <int XT, int SG, bool Z, int BM, int OCC, int JN>
 __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
     constexpr int kUnits = BM * 16, kLoads = kUnits / 256, RT = BM / 16;
     __shared__ u32x4_t lds[2 * kUnits + 4 * (Z ? 128 : 64)];   // x, and the waves' scales and zeros
@@ -320,32 +322,33 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
                 for (int v = 0; v < 4; ++v) x[v] = xb[(16 * r + l) * 16 + ((4 * v + q4) ^ l)];
             };
 #pragma unroll
-            for (int jp = 0; jp < 4; jp += 2) {
-                u32x4_t f[2][4], x[2][4];
+            for (int jp = 0; jp < 4; jp += JN) {
+                u32x4_t f[JN][4], x[2][4];
                 read_x(0, x[0]);
-                f2_t scale[SG];
-                uint2 zero[SG];
+                float scale[SG][JN];
+                uint32_t zero[SG][JN];
 #pragma unroll
-                for (int i = 0; i < SG; ++i) {
-                    scale[i] = *reinterpret_cast<const f2_t*>(ls + 64 * (at + i) + 4 * l + jp);
-                    if constexpr (Z) zero[i] = *reinterpret_cast<const uint2*>(lz + 64 * (at + i) + 4 * l + jp);
-                    else zero[i] = make_uint2(g4_zero<XT, Z>(8), g4_zero<XT, Z>(8));
-                }
+                for (int i = 0; i < SG; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                    for (int j = 0; j < JN; ++j) {
+                        scale[i][j] = ls[64 * (at + i) + 4 * l + jp + j];
+                        zero[i][j] = Z ? lz[64 * (at + i) + 4 * l + jp + j] : g4_zero<XT, Z>(8);
+                    }
+#pragma unroll
+                for (int j = 0; j < JN; ++j) {
                     g4_turn(w[jp + j]);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) f[j][v] = g4_frag<XT, Z>(w[jp + j][v], j ? zero[v / (4 / SG)].y : zero[v / (4 / SG)].x);
+                    for (int v = 0; v < 4; ++v) f[j][v] = g4_frag<XT, Z>(w[jp + j][v], zero[v / (4 / SG)][j]);
                     w[jp + j] = next_w(c + 1, jp + j);
                 }
                 __builtin_amdgcn_s_setprio(1);                 // the other waves convert meanwhile
                 __builtin_amdgcn_sched_barrier(0);
                 // a product's sums are scaled behind the next one's MFMAs, where there are registers for it
                 constexpr bool kLate = SG == 1 || BM < 128;
-                f4_t part[kLate ? 2 : 1][2];
+                f4_t part[kLate ? 2 : 1][JN];
                 const auto scaled = [&](int q) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < JN; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             acc[q / SG][jp + j][e] = __builtin_fmaf(scale[q % SG][j], part[kLate ? q & 1 : 0][j][e], acc[q / SG][jp + j][e]);
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
 #pragma unroll
                     for (int v = q % SG * V; v < (q % SG + 1) * V; ++v)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                        for (int j = 0; j < JN; ++j)
                             part[kLate ? q & 1 : 0][j] = mfma16<XT>(x[r & 1][v], f[j][v], v == q % SG * V ? f4_t{} : part[kLate ? q & 1 : 0][j]);
                     if (!kLate) scaled(q);
                     else if (q > 0) scaled(q - 1);
@@ -385,21 +388,24 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
         }
 }
 
-template <int XT, int SG, bool Z, int BM, int OCC>
+template <int XT, int SG, bool Z, int BM, int OCC, int JN>
 static int launch_g4_wide(G4Args g, hipStream_t st) {
     g.slots = (int)(g.ends ? group_slots(g.T, g.E, BM, g.rest) : (g.T + BM - 1) / BM);
     const int64_t all = (int64_t)g.slots * ((g.n + 255) / 256), tiles = g.whole + (all - g.whole) * g.splits;
     constexpr int64_t kRound = 8 * kChunk;
     EXL3_CHECK_ARG(tiles <= kMx4Grid - kRound, "g4: grid too large");
-    EXL3_LAUNCH("g4_wide", (g4_wide_kernel<XT, SG, Z, BM, OCC>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)), dim3(256), 0,
+    EXL3_LAUNCH("g4_wide", (g4_wide_kernel<XT, SG, Z, BM, OCC, JN>), dim3((unsigned)((tiles + kRound - 1) / kRound * kRound)), dim3(256), 0,
                 st, g);
     return EXL3_OK;
 }
 
 template <int XT, int SG, bool Z>
 static int launch_g4(const G4Args& g, int tile, hipStream_t st) {
-    return tile == 0 ? launch_g4_decode<XT, SG, Z>(g, st) : tile == 1 ? launch_g4_wide<XT, SG, Z, 32, 3>(g, st)
-         : tile == 2 ? launch_g4_wide<XT, SG, Z, 64, 2>(g, st) : launch_g4_wide<XT, SG, Z, 128, 2>(g, st);
+    if (tile == 0) return launch_g4_decode<XT, SG, Z>(g, st);
+    if constexpr (SG == 1)
+        if (g.ends && tile < 3) return tile == 1 ? launch_g4_wide<XT, SG, Z, 32, 4, 1>(g, st) : launch_g4_wide<XT, SG, Z, 64, 3, 1>(g, st);
+    return tile == 1 ? launch_g4_wide<XT, SG, Z, 32, 3, 2>(g, st) : tile == 2 ? launch_g4_wide<XT, SG, Z, 64, 2, 2>(g, st)
+                                                                              : launch_g4_wide<XT, SG, Z, 128, 2, 2>(g, st);
 }
 
 // tile: 0 few rows, 1, 2, 3 blocks of 32, 64, 128 rows
