@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void g4_reduce_kernel(G4Args g, int bm) {
 
 // Kernel and splits of a call: the least time by an estimate from measurements (1 to 512 rows of nine shapes from 640 -> 2560 to
 // 8192 -> 8192 and 5376 -> 21504), in microseconds for 256 CUs. Six rows of 8192 -> 8192, fp16: 16 with the kernel of few rows, 18
-// with the other; of 5376 -> 21504 24 and 22, in groups of 32 24 and 27; 24 rows of it 42 and 25; of 4096 -> 4096 13 and 17. Splits are the linear's alone: experts have workgroups enough, or few
+// with the other; of 5376 -> 21504 21 and 22, in groups of 32 21 and 27; 24 rows of it 36 and 25; of 4096 -> 4096 13 and 17. Splits are the linear's alone: experts have workgroups enough, or few
 // rows, and rows of no expert have no sums.
 struct G4Plan {
     int tile;
@@ -70,7 +70,7 @@ static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E,
     // blocks of 16 rows: the groups of 512 inputs of all tiles, spread over the CUs
     const int64_t live = E == 1 ? (m + 15) / 16 : m / 16 + (m < E ? m : E);
     if (k <= 8192 && (E == 1 || m <= 16 * E))
-        least = 6.5 + (double)(live * ((n + 15) / 16) * ((k + 511) / 512)) / 256.0 * (0.265 + 0.003 * (double)(m < 16 ? m : 16));
+        least = 6.5 + (double)(live * ((n + 15) / 16) * ((k + 511) / 512)) / 256.0 * (0.245 + 0.003 * (double)(m < 16 ? m : 16));
     // blocks of 32, 64, 128 rows: time of a step with one, two, three workgroups to a CU; all tiles in splits, or full rounds of whole
     // tiles and the rest in splits (1021 rows of 5376 -> 21504, 672 tiles for 512 places: 250 us whole, 223 with the last 160 in three)
     static const double kStep[3][4] = {{1.45, 2.05, 2.85, 3.7}, {1.65, 2.6, 4.2}, {2.6, 3.9}};

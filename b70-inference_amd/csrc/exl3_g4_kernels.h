@@ -58,9 +58,12 @@ struct G4Scales {
 //   XL: x lies in LDS, and eight waves go round a tile's groups: two workgroups to a CU, one of which works while the other waits
 //   for its barrier (one row of 4096 -> 4096 7.0 us, 8.0 without; ten rows of 512 experts of 2048 -> 1024 8.9 and 9.8).
 //   Not XL, where x leaves room for one workgroup: a wave has one group of every tile, whose x stays in its registers.
-// Bound by the weights' bytes (6 rows of 5376 -> 21504, fp16 with zeros: 61 MB in 23.5 us, 2.6 TB/s, of which the instructions that
-// take the codes apart are a third), for small matrices by the chain of launch, load, sum and store.
+// Bound by the weights' bytes (6 rows of 5376 -> 21504, fp16 with zeros: 61 MB in 21.2 us, 2.9 TB/s) and by the instructions that take
+// the codes apart (9 us of each SIMD), for small matrices by the chain of launch, load, sum and store.
 constexpr int kG4Waves = 16, kG4Slice = 512;
+// Tiles between two barriers, each added by another wave: where all waves of a CU wait for one barrier (6 rows of 5376 -> 21504 with one
+// tile 23.8 us, with two 21.1, with three 21.2; 6 rows of 4096 -> 21504 19.8 and 19.4).
+__host__ __device__ constexpr int g4_tiles_held(bool xl) { return xl ? 1 : 3; }
 constexpr int kG4Lds = 163840;         // of a CU
 
 // Bytes from row to row of x in LDS: whole chunks, and 16 bytes to spread the rows over the banks.
@@ -69,6 +72,7 @@ __host__ __device__ constexpr int64_t g4_x_stride(int64_t k) { return (k + 127) 
 template <int XT, int SG, bool Z, bool XL>
 __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g, int split) {
     extern __shared__ f4_t red[];
+    constexpr int kTiles = g4_tiles_held(XL);
     const int lane = threadIdx.x & 63, l = lane & 15, q4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
               waves = blockDim.x >> 6;
     const unsigned slot = blockIdx.x / (unsigned)split, first = blockIdx.x - slot * (unsigned)split;
@@ -104,7 +108,7 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
     u32x4_t w[4];
     S raw;
     const int set = q4 < SG ? q4 : SG - 1, cs = set * (4 / SG);
-    float* const ls = reinterpret_cast<float*>(red + (waves > 1 ? 2 * waves * 64 : 0)) + wave * (Z ? 512 : 256) + l;
+    float* const ls = reinterpret_cast<float*>(red + (waves > 1 ? 2 * kTiles * waves * 64 : 0)) + wave * (Z ? 512 : 256) + l;
     uint32_t* const lz = reinterpret_cast<uint32_t*>(ls + 256);
     {
         const Tile d(g, row0, rows, first * 16, kb, l);
@@ -115,7 +119,7 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
     // x: of lane l the row l, inputs 32 v + 8 (lane >> 4) of each chunk; 0 behind the row's end
     u32x4_t x[XL ? 1 : 4][4];
     const int stride = (int)g4_x_stride(g.k);
-    char* const xl = reinterpret_cast<char*>(red + (waves > 1 ? 2 * waves * 64 : 0)) + waves * (Z ? 2048 : 1024);
+    char* const xl = reinterpret_cast<char*>(red + (waves > 1 ? 2 * kTiles * waves * 64 : 0)) + waves * (Z ? 2048 : 1024);
     const __amdgpu_buffer_rsrc_t xr = mx4_rsrc(reinterpret_cast<const uint8_t*>(g.x + s.row * g.x_ld), 0xE0000000LL);
     if constexpr (XL) {
         // all rows' units in one run over the threads, eight loads under way
@@ -142,10 +146,11 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
             for (int v = 0; v < 4; ++v) x[u][v] = mx4_buffer16(xr, 4 * (4 * wave + u) + v < kb ? at + 256 * u + 64 * v : kMx4Out);
     }
     const char* const xrow = xl + (l < s.rows ? l : s.rows - 1) * stride + 16 * q4;
-    int buf = 0;
+    int buf = 0, held = 0;                                     // tiles in LDS behind the last barrier
 #pragma unroll 1
-    for (int tile = first; tile < tiles; tile += split, buf ^= 1) {
+    for (int tile = first; tile < tiles; tile += split) {
         f4_t acc = {};
+        int n0 = 16 * tile;
 #pragma unroll 1
         for (int gi = wave; gi < groups; gi += waves) {        // (waves <= groups: every wave has a group of every tile)
             // the next group: this tile's, or the next tile's first (the last tile's is read again and not used)
@@ -188,10 +193,19 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
             }
         }
         if (waves > 1) {
-            f4_t* o = red + buf * waves * 64;                  // two, so that one barrier a tile is enough
-            o[wave * 64 + lane] = acc;
+            red[((buf * kTiles + held) * waves + wave) * 64 + lane] = acc;
+            if (held + 1 < kTiles && tile + split < tiles) {
+                ++held;
+                continue;
+            }
             __syncthreads();
-            if (wave != 0) continue;
+            const int back = held - wave;                      // each of these tiles is a wave's
+            const f4_t* o = red + (buf * kTiles + wave) * waves * 64;
+            held = 0;
+            buf ^= 1;                                          // two, so that one barrier is enough
+            if (back < 0) continue;
+            n0 -= 16 * back * split;
+            acc = o[lane];
             for (int w0 = 1; w0 < waves; w0 += 5) {            // five reads under way
                 f4_t t[5];
 #pragma unroll
@@ -202,7 +216,7 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
                     for (int e = 0; e < 4; ++e) acc[e] += w0 + i < waves ? t[i][e] : 0.f;
             }
         }
-        const int n = 16 * tile + l;
+        const int n = n0 + l;
         if (n >= g.n) continue;
         const float b = g.bias ? ldg(g.bias + n) : 0.f;
         int m = 4 * q4;
@@ -223,7 +237,7 @@ static int launch_g4_decode(G4Args g, hipStream_t st) {
     const bool xl = 2 * (xb + waves * (2048 + own)) <= kG4Lds;
     if (!xl) waves = groups;
     EXL3_CHECK_ARG(waves <= kG4Waves, "g4: too many inputs");
-    const int64_t lds = (waves > 1 ? 2 * waves * 1024 : 0) + waves * own + (xl ? xb : 0);
+    const int64_t lds = (waves > 1 ? 2 * g4_tiles_held(xl) * waves * 1024 : 0) + waves * own + (xl ? xb : 0);
     g.slots = (int)(g.ends ? group_slots(g.T, g.E, 16, g.rest) : (g.T + 15) / 16);
     const int64_t by_lds = kG4Lds / lds, by_waves = 16 / waves, fit = by_lds < by_waves ? by_lds : by_waves;
     // workgroups: as few as need no more rounds
