@@ -240,9 +240,7 @@ static int launch_g4_decode(G4Args g, hipStream_t st) {
     const int64_t lds = (waves > 1 ? 2 * g4_tiles_held(xl) * waves * 1024 : 0) + waves * own + (xl ? xb : 0);
     g.slots = (int)(g.ends ? group_slots(g.T, g.E, 16, g.rest) : (g.T + 15) / 16);
     const int64_t by_lds = kG4Lds / lds, by_waves = 16 / waves, fit = by_lds < by_waves ? by_lds : by_waves;
-    // workgroups: as few as need no more rounds
-    const int64_t tiles = (g.n + 15) / 16, room = 256 * (fit > 4 ? 4 : fit);
-    const int64_t rounds = (tiles * g.slots + room - 1) / room, split = (tiles + rounds - 1) / rounds;
+    const int64_t split = group_split(g.T, g.E, (g.n + 15) / 16, waves, fit > 4 ? 4 : fit, 8, (double)g.k * 8 / 12e3);
     EXL3_CHECK_ARG(g.slots * split <= kMx4Grid / 4, "g4: grid too large");
     if (xl)
         EXL3_LAUNCH("g4_decode", (g4_decode_kernel<XT, SG, Z, true>), dim3((unsigned)(g.slots * split)), dim3(64 * waves), (size_t)lds, st,

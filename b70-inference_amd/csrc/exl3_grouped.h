@@ -3,6 +3,8 @@
 // finds the expert of its block in a running sum of the experts' blocks, 64 experts at a time.
 #pragma once
 
+#include <cmath>
+
 #include "exl3_mx4.h"
 
 namespace exl3 {
@@ -23,6 +25,29 @@ __device__ __forceinline__ int group_end(const int32_t* ends, int e, int T) {
 inline int64_t group_slots(int64_t T, int64_t E, int64_t BM, bool rest) {
     const int64_t n = T / BM + E + (rest ? 1 : 0);
     return T < n ? T : n;
+}
+
+// Workgroups to a block of rows for kernels of few rows, whose workgroups go round the block's tiles: as many as fill the CUs by the
+// estimate that is least for the CU with most tiles. `us`: what a tile's weights take a CU without a pause, which takes `need` waves (16-bit
+// weights six; 4-bit ones, which are converted, eight); a workgroup that waits for another's end starts late. As many as need no more
+// rounds, without regard to the tiles of a CU, were slower: ten rows of 512 experts of 2048 -> 1024, 16-bit weights, 14.2 against 11.8 us;
+// 4-bit, 16 rows of 4096 -> 6144 15.5 and 11.1.
+inline int64_t group_split(int64_t T, int64_t E, int64_t tiles, int64_t waves, int64_t fit, int64_t need, double us) {
+    // blocks of 16 rows: the full ones, and a part of each expert's that has rows if all are as likely
+    const int64_t slots = E == 1 ? (T + 15) / 16 : T / 16 + (int64_t)std::ceil((double)E * (1.0 - std::pow(1.0 - 1.0 / (double)E, (double)T)));
+    int64_t best = 1;
+    double least = 1e30;
+    const int64_t mean = slots * tiles / 256 + 1;
+    for (int64_t q = 1; q <= (tiles < 32 ? tiles : 32); ++q) {
+        const int64_t n = (slots * ((tiles + q - 1) / q) + 255) / 256, rounds = (n + fit - 1) / fit, busy = (n < fit ? n : fit) * waves;
+        const double t = (double)(n * q) * us * (busy < need ? (double)need / (double)busy : 1.0) + 4.0 * (double)(rounds - 1);
+        if (t > least) continue;
+        least = t;
+        best = n * 256 / slots;
+    }
+    // (as few as fill the CUs where a workgroup has more tiles than that)
+    if (mean > 16 * fit) best = 256 * fit / slots;
+    return best < 1 ? 1 : best < tiles ? best : tiles;
 }
 
 // Sum over the lanes up to and with this one: shifts by 1, 2, 4, 8 inside the 16 lanes of a row, then the rows' sums on.
