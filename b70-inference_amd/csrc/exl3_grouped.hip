@@ -45,9 +45,6 @@ static double tile_time(const TileCost& t, double tiles, double steps) {
 // Tile of the products of T rows over E experts (few: the kernel of few rows is there for them).
 static int rows_tile(int64_t T, int64_t E, int64_t n, int64_t k, bool few) {
     const double live = (double)(T < E ? T : E);
-    // blocks of 16 rows by 16 outputs, up to where their weights' bytes count (64 rows over 64 experts of 2048 -> 4096: 151 us against
-    // 115; 40 over 512 of 2048 -> 1024 28 against 34, one row of 4096 -> 4096 11 against 30)
-    if (few && T <= 16 * E && ((double)(T / 16) + live) * (double)n * (double)k <= (double)(1 << 27)) return kTileFew;
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < 4; ++i) {
@@ -59,6 +56,15 @@ static int rows_tile(int64_t T, int64_t E, int64_t n, int64_t k, bool few) {
             least = us;
             best = i;
         }
+    }
+    // Blocks of 16 rows by 16 outputs: the weights at the rate that a CU with most of them reaches, against the tiles' time or the bytes'
+    // (us, few rows' kernel and the best tile: one row of 4096 -> 4096 11 and 30, 40 over 512 experts of 2048 -> 1024 28 and 35, 24
+    // over 64 of 4096 -> 4096 114 and 130, 300 over 64 of 512 -> 512 10 and 7). Above 4096 inputs one workgroup fills a CU, and its
+    // waves wait for each other: 8 rows over 16 experts of 7168 -> 4096 88 and 70.
+    if (few && T <= 16 * E && (k <= 4096 || live * (double)(n * k) <= (double)(1 << 27))) {
+        const double used = group_live(T, E), load = std::ceil((used + (double)(T / 16)) * (double)((n + 15) / 16) / 256.0),
+                     bytes = 2.0 + used * (double)(n * k) * 2.0 / 5.5e6;
+        if (4.0 + 0.72 * load * (double)k * 32.0 / 19.5e3 <= (least > bytes ? least : bytes)) return kTileFew;
     }
     return best;
 }
