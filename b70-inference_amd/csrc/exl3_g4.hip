@@ -71,6 +71,7 @@ static G4Plan g4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int64_t E,
     const int64_t live = E == 1 ? (m + 15) / 16 : m / 16 + (m < E ? m : E);
     if (k <= 8192 && (E == 1 || m <= 16 * E))
         least = 6.5 + (double)(live * ((n + 15) / 16) * ((k + 511) / 512)) / 256.0 * (0.245 + 0.003 * (double)(m < 16 ? m : 16));
+    if (least <= 8.0 + 1.35 * (double)((steps + 15) / 16) && least <= 5.0 + 1.35 * (double)steps) return best;   // none below is less
     // blocks of 32, 64, 128 rows: time of a step with one, two, three workgroups to a CU; all tiles in splits, or full rounds of whole
     // tiles and the rest in splits (1021 rows of 5376 -> 21504, 672 tiles for 512 places: 250 us whole, 223 with the last 160 in three)
     static const double kStep[3][4] = {{1.45, 2.05, 2.85, 3.7}, {1.65, 2.6, 4.2}, {2.6, 3.9}};

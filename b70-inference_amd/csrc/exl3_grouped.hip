@@ -26,10 +26,6 @@ static int grouped_setup(const char* what, int dtype, int64_t T, int64_t n, int6
 
 static bool units16(const void* p, int64_t ld, int64_t cols) { return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0; }
 
-static bool vec_out(const void* p, int dtype, int64_t ld, int64_t n) {
-    return aligned(p, 16) && n % 8 == 0 && ld * out_size(dtype) % 16 == 0;
-}
-
 // Microseconds that `tiles` tiles of `steps` steps take by an estimate from measurements: a step and the rest of a tile, with `occ`
 // workgroups to a CU and with one, full rounds and what is left.
 struct TileCost {
@@ -122,7 +118,6 @@ static int weights_gradient(const void* dy, int64_t dy_ld, const void* x, int64_
     g.m = (int)n;
     g.n = (int)k;
     g.out_dtype = dw_dtype;
-    g.vec = vec_out(dw, dw_dtype, g.out_ld, k) && (E == 1 || dw_es * out_size(dw_dtype) % 16 == 0);
     g.accumulate = accumulate;
     const bool direct = units16(dy, g.a_ld, n) && units16(x, g.b_ld, k);
     hipStream_t st = (hipStream_t)stream;
@@ -139,7 +134,6 @@ static int weights_gradient(const void* dy, int64_t dy_ld, const void* x, int64_
     h.out_ld = n8(k);
     h.out_es = n * h.out_ld;
     h.out_dtype = EXL3_F32;
-    h.vec = 1;
     h.accumulate = 0;
     const int rc2 = grouped_weights(h, dtype, plan.tile, st);
     return rc2 ? rc2 : grouped_reduce(g, reinterpret_cast<const float*>(c.p), h.out_ld, E * h.out_es, st);
@@ -181,7 +175,7 @@ int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k
     g.c = (int)k;
     g.n = (int)n;
     g.out_dtype = out_dtype;
-    g.vec = vec_out(out, out_dtype, g.out_ld, n);
+    g.vec = n % 4 == 0 && g.out_ld % 4 == 0 && aligned(out, 4 * out_size(out_dtype));
     g.rest = rest;
     const bool direct = units16(x, g.a_ld, k) && units16(w, w_ld, across ? n : k) && (E == 1 || w_es % 8 == 0);
     const int64_t mean = T / E;

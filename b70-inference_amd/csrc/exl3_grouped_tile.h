@@ -27,7 +27,7 @@ struct GroupedArgs {
     int E, T;
     int c;                             // contraction (the weights' gradient: the expert's rows)
     int m, n;                          // outputs: columns n; the weights' gradient has m rows
-    int out_dtype, vec;                // vec: eight neighbouring outputs may be stored as 16-byte pieces
+    int out_dtype, vec;                // vec: the kernel of few rows may store four neighbouring outputs at once
     int rest;                          // rows of no expert become 0
     int accumulate;                    // the weights' gradient is added to what out holds
     int splits;                        // the weights' gradient: parts of an expert's rows, whose sums lie E out_es behind one another
@@ -146,6 +146,9 @@ __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
     return dtype == EXL3_F16 ? h2f(v) : bf2f(v);
 }
 
+typedef f4_t f4_any_t __attribute__((aligned(4)));
+typedef u32x4_t u4_any_t __attribute__((aligned(2)));
+
 // The outputs of two tiles of 16 n, four neighbours of each per lane, to eight neighbours: of lane groups 0 and 2 the first tile's n 0 .. 7
 // and 8 .. 15, of 1 and 3 the second's.
 __device__ __forceinline__ void grouped_pair(f4_t& v, f4_t& w) {
@@ -158,10 +161,13 @@ __device__ __forceinline__ void grouped_pair(f4_t& v, f4_t& w) {
     }
 }
 
-// Eight neighbouring outputs at element i, `left` of which are there.
+// Eight neighbouring outputs at element i, `left` of which are there. Whole pieces at any alignment, which global memory takes (200 rows
+// over 64 experts, gradient of 2049 -> 2048 weights: 548 us by single values).
 template <int OP>
 __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, int left, f4_t v, f4_t w) {
-    if (!g.vec) {                      // uniform
+    typedef __attribute__((address_space(1))) f4_any_t f4_g;
+    typedef __attribute__((address_space(1))) u4_any_t u4_g;
+    if (left < 8) {
 #pragma unroll 1
         for (int q = 0; q < (left < 8 ? left : 8); ++q) {
             float f = q < 4 ? v[q & 3] : w[q & 3];
@@ -171,9 +177,9 @@ __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, i
         return;
     }
     if (g.out_dtype == EXL3_F32) {
-        f4_t* o = reinterpret_cast<f4_t*>(reinterpret_cast<float*>(g.out) + i);
+        f4_g* o = (f4_g*)(reinterpret_cast<float*>(g.out) + i);
         if (OP == kGroupWeights && g.accumulate) {
-            const f4_t p = ldg(o), r = ldg(o + 1);
+            const f4_t p = o[0], r = o[1];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 v[q] += p[q];
@@ -184,9 +190,9 @@ __device__ __forceinline__ void grouped_store(const GroupedArgs& g, int64_t i, i
         o[1] = w;
         return;
     }
-    u32x4_t* o = reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(g.out) + i);
+    u4_g* o = (u4_g*)(reinterpret_cast<uint16_t*>(g.out) + i);
     if (OP == kGroupWeights && g.accumulate) {
-        const u32x4_t p = ldg(o);
+        const u32x4_t p = *o;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             const uint16_t h = (uint16_t)(p[q >> 1] >> (16 * (q & 1)));
