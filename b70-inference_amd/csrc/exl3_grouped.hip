@@ -28,6 +28,7 @@ static bool units16(const void* p, int64_t ld, int64_t cols) { return aligned(p,
 
 // Microseconds that `tiles` tiles of `steps` steps take by an estimate from measurements: a step and the rest of a tile, with `occ`
 // workgroups to a CU and with one, full rounds and what is left.
+// (Times of 16384 rows over 8 to 512 experts of 512 to 7168 columns: the least of the four within 10 %.)
 struct TileCost {
     int bm, bn, occ;
     double step, step1, rest;
@@ -64,7 +65,8 @@ static int rows_tile(int64_t T, int64_t E, int64_t n, int64_t k, bool few) {
     }
     return best;
 }
-// Tile of the weights' gradient, and the parts of an expert's rows: few small matrices of many rows leave CUs idle.
+// Tile of the weights' gradient, and the parts of an expert's rows: few small matrices of many rows leave CUs idle (16384 rows over 8
+// experts of 512 x 512: 65 us whole, 44 in parts).
 struct WeightsPlan {
     int tile, splits;
 };
