@@ -1,6 +1,6 @@
 // Rows grouped by expert: rows ends[e - 1] .. ends[e] - 1 of a matrix (from 0 for e = 0) belong to expert e, rows behind the last end
 // to none. The ends lie on the GPU, so the grid holds as many blocks of BM rows as T rows over E experts can need, and a workgroup
-// finds the expert of its block in a running sum of the experts' blocks, 64 experts at a time.
+// finds the expert of its block in a running sum of the experts' blocks, 576 experts at a time.
 #pragma once
 
 #include <cmath>
@@ -33,7 +33,7 @@ inline double group_live(int64_t T, int64_t E) { return E == 1 ? 1.0 : (double)E
 // Workgroups to a block of rows for kernels of few rows, whose workgroups go round the block's tiles: as many as fill the CUs by the
 // estimate that is least for the CU with most tiles. `us`: what a tile's weights take a CU without a pause, which takes `need` waves (16-bit
 // weights six; 4-bit ones, which are converted, eight); a workgroup that waits for another's end starts late. As many as need no more
-// rounds, without regard to the tiles of a CU, were slower: ten rows of 512 experts of 2048 -> 1024, 16-bit weights, 14.2 against 11.8 us;
+// rounds, without regard to the tiles of a CU, were slower: ten rows of 512 experts of 2048 -> 1024, 16-bit weights, 14.2 against 11.8 us (with the search of then);
 // 4-bit, 16 rows of 4096 -> 6144 15.5 and 11.1.
 inline int64_t group_split(int64_t T, int64_t E, int64_t tiles, int64_t waves, int64_t fit, int64_t need, double us) {
     const int64_t slots = E == 1 ? (T + 15) / 16 : T / 16 + (int64_t)std::ceil(group_live(T, E));   // blocks of 16 rows
@@ -63,62 +63,84 @@ __device__ __forceinline__ int wave_running_sum(int v) {
     return v;
 }
 
-// fn(first expert of 64, this lane's begin and end) for the experts and the rows of none as the last of all, until it returns true.
-// Nine loads of either kind are under way: one after another they are a microsecond for every 64 experts and more.
-template <typename F>
-__device__ __forceinline__ void group_each(const int32_t* ends, int E, int T, F fn) {
-    constexpr int kBatch = 9;
-    const int lane = threadIdx.x & 63;
-    for (int i0 = 0; i0 <= E; i0 += 64 * kBatch) {
-        int lo[kBatch], hi[kBatch];
+// Where the K experts of a lane end, from `e0` on: v[i] .. v[i + 1] the rows of expert e0 + i; expert E has the rows of none, those
+// behind it no rows. The loads are under way together.
+template <int K>
+__device__ __forceinline__ void group_ends(const int32_t* ends, int E, int T, int e0, int (&v)[K + 1]) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (i0 + 64 * i > E) break;                        // uniform
-            const int e = i0 + 64 * i + lane;
-            lo[i] = ldg(ends + (e < 1 ? 0 : e <= E ? e - 1 : E - 1));
-            hi[i] = ldg(ends + (e < E ? e : E - 1));
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (i0 + 64 * i > E) break;
-            const int e = i0 + 64 * i + lane;
-            const int l = e < 1 ? 0 : lo[i] < 0 ? 0 : lo[i] > T ? T : lo[i], h = e < E ? hi[i] < 0 ? 0 : hi[i] > T ? T : hi[i] : e == E ? T : l;
-            if (fn(i0 + 64 * i, l, h)) return;
-        }
+    for (int i = 0; i <= K; ++i) {
+        const int e = e0 + i - 1;
+        v[i] = ldg(ends + (e < 0 ? 0 : e < E ? e : E - 1));
     }
+#pragma unroll
+    for (int i = 0; i <= K; ++i) {
+        const int e = e0 + i - 1, c = v[i] < 0 ? 0 : v[i] > T ? T : v[i];
+        v[i] = e < 0 ? 0 : e < E ? c : T;
+    }
+}
+template <int BM>
+__device__ __forceinline__ int group_blocks_of(int lo, int hi) {
+    return hi > lo ? (hi - lo + BM - 1) / BM : 0;
 }
 
 // The same value in every lane (wave-uniform). Blocks behind the last one have no rows.
+template <int BM, int K>
+__device__ __forceinline__ GroupSlot group_slot_of(const int32_t* ends, int E, int T, unsigned slot) {
+    const int lane = threadIdx.x & 63;
+    unsigned first = 0;                // blocks of the experts before
+    for (int i0 = 0; i0 <= E; i0 += 64 * K) {
+        const int e0 = i0 + lane * K;
+        int v[K + 1], upto[K], sum = 0;
+        group_ends<K>(ends, E, T, e0, v);
+#pragma unroll
+        for (int i = 0; i < K; ++i) upto[i] = sum += group_blocks_of<BM>(v[i], v[i + 1]);
+        const int run = wave_running_sum(sum);
+        const uint64_t in = __ballot(first + (unsigned)run > slot);
+        if (!in) {                     // uniform
+            first += (unsigned)__builtin_amdgcn_readlane(run, 63);
+            continue;
+        }
+        // every lane looks as if the block were its own, the one that has it is right
+        const int l = __builtin_ctzll(in), at = (int)(slot - first) - (run - sum);
+        int e = e0, row = 0, left = 0;
+#pragma unroll
+        for (int i = K - 1; i >= 0; --i)
+            if (upto[i] > at) {
+                e = e0 + i;
+                row = v[i] + (at - (i ? upto[i - 1] : 0)) * BM;
+                left = v[i + 1] - row;
+            }
+        GroupSlot s;
+        s.e = __builtin_amdgcn_readlane(e, l);
+        s.row = __builtin_amdgcn_readlane(row, l);
+        left = __builtin_amdgcn_readlane(left, l);
+        s.rows = left < BM ? left : BM;
+        return s;
+    }
+    return GroupSlot{E, 0, 0};
+}
+
+// Nine experts to a lane, one of fewer than 64 (64 rows over 512 experts of 512 -> 512 7.1 us; with one expert to a lane, and the lanes' sums
+// for each, 8.7. One row of one matrix of 4096 -> 4096 10.5; with nine 11.2).
+constexpr int kLaneExperts = 9;
 template <int BM>
 __device__ __forceinline__ GroupSlot group_slot(const int32_t* ends, int E, int T, unsigned slot) {
-    GroupSlot s = {E, 0, 0};
-    unsigned first = 0;                // blocks of the experts before
-    group_each(ends, E, T, [&](int i, int lo, int hi) {
-        const int blocks = hi > lo ? (hi - lo + BM - 1) / BM : 0, sum = wave_running_sum(blocks);
-        const uint64_t in = __ballot(first + (unsigned)sum > slot);
-        first += (unsigned)__builtin_amdgcn_readlane(sum, 63);
-        if (!in) return false;         // uniform
-        const int l = __builtin_ctzll(in), before = (int)first - __builtin_amdgcn_readlane(sum, 63);
-        const int block = (int)slot - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(blocks, l));
-        const int row = __builtin_amdgcn_readlane(lo, l) + block * BM, left = __builtin_amdgcn_readlane(hi, l) - row;
-        s.e = i + l;
-        s.row = row;
-        s.rows = left < BM ? left : BM;
-        return true;
-    });
-    return s;
+    return E < 64 ? group_slot_of<BM, 1>(ends, E, T, slot) : group_slot_of<BM, kLaneExperts>(ends, E, T, slot);
 }
 
 // The blocks there are, with `rest` those of the rows of none (wave-uniform).
 template <int BM>
 __device__ __forceinline__ unsigned group_blocks(const int32_t* ends, int E, int T, bool rest) {
-    int n = 0;
-    group_each(ends, E, T, [&](int i, int lo, int hi) {
-        const bool in = hi > lo && (rest || i + (int)(threadIdx.x & 63) < E);
-        n += __builtin_amdgcn_readlane(wave_running_sum(in ? (hi - lo + BM - 1) / BM : 0), 63);
-        return false;
-    });
-    return (unsigned)n;
+    unsigned n = 0;
+    for (int i0 = 0; i0 <= E; i0 += 64 * kLaneExperts) {
+        const int e0 = i0 + (int)(threadIdx.x & 63) * kLaneExperts;
+        int v[kLaneExperts + 1], sum = 0;
+        group_ends<kLaneExperts>(ends, E, T, e0, v);
+#pragma unroll
+        for (int i = 0; i < kLaneExperts; ++i) sum += rest || e0 + i < E ? group_blocks_of<BM>(v[i], v[i + 1]) : 0;
+        n += (unsigned)__builtin_amdgcn_readlane(wave_running_sum(sum), 63);
+    }
+    return n;
 }
 
 // A workgroup's place in a grid that takes `chunk` tiles after one another on an XCD, the XCDs in turn (workgroups go round robin over

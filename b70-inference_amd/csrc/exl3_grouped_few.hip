@@ -2,7 +2,7 @@
 // has SLICE inputs of the block's rows and of one tile of 16 outputs after another; the waves of a workgroup share the inputs and
 // are added in order through LDS. A load takes 64 neighbouring bytes of 16 weight rows, eight of them are under way per wave, those of
 // the next tile behind the last of this one. Bound by the weights' bytes, of a few experts by the chain of ends, weights, sum and
-// store: ten rows of 512 experts of 2048 -> 1024, 42 MB, in 11.8 us as one of a graph's nodes.
+// store: ten rows of 512 experts of 2048 -> 1024, 42 MB, in 11.4 us as one of a graph's nodes.
 #include "exl3_grouped.h"
 #include "exl3_grouped_tile.h"
 

@@ -12,8 +12,8 @@
 // the end, so that a lane has eight neighbours and stores 16 bytes (or 32).
 //
 // Bound by the MFMAs for many rows (8192 x 8192 x 8192 bf16 1.36 to 1.40 PFLOP/s, as a large library product; 16384 rows over 16 experts of
-// 7168 -> 4096 906 us, 1.06, with the experts' partial blocks and 4.5 rounds of tiles), by the weights' or outputs' bytes for few (2085
-// rows over 512 experts of 2560 -> 1280 497 us). Tiles of 256 x 256 read each operand's LDS half as often as 128 x 128 and leave room
+// 7168 -> 4096 903 us, 1.07, with the experts' partial blocks and 4.5 rounds of tiles), by the weights' or outputs' bytes for few (2085
+// rows over 512 experts of 2560 -> 1280 500 us). Tiles of 256 x 256 read each operand's LDS half as often as 128 x 128 and leave room
 // for one workgroup to a CU, so that workgroup goes round the tiles and loads the next behind the stores (985 us with a workgroup for
 // each tile); of the smaller tiles two fit a CU, one of which computes while the other begins or ends.
 #pragma once

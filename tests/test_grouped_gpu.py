@@ -263,3 +263,19 @@ def test_offsets_past_32_bits(exl3, m):
     dw = exl3.grouped_mm_dw(dys, xs, ends)
     check(dw[1:], rdw, mdw, m, "dw, many rows")
     assert not bool(dw[0].any())
+
+
+@pytest.mark.parametrize("tile", ("0", "1", "4", "5"))
+def test_many_experts(exl3, monkeypatch, tile):
+    """As many experts as a step of the search for a block's takes, and one more or less, with rows of none behind them."""
+    monkeypatch.setenv("EXL3MI_GROUPED_TILE", tile)
+    N, K, pad = 16, 32, 3
+    for E in (63, 64, 65, 575, 576, 577, 1152, 2500):
+        sizes = sizes_for(3 * E // 2, E, E, empty=range(0, E, 5))
+        T, ends = sum(sizes), ends_of(sizes)
+        x, _, w = _data(T + pad, E, N, K, torch.float16, E)
+        of = torch.repeat_interleave(torch.arange(E), torch.tensor(sizes)).cuda()
+        prod = w.double()[of] * x[:T].double()[:, None]
+        for y in (exl3.grouped_mm(x, w, ends), exl3.grouped_mm(x, w, ends, out=torch.full((T + pad, N), 7.0, device="cuda"))):
+            check(y[:T], prod.sum(-1), prod.abs().sum(-1), K, f"{E} experts")
+            assert bool((y[T:] == (7 if y.dtype == torch.float32 else 0)).all())
