@@ -33,7 +33,7 @@ inline double group_live(int64_t T, int64_t E) { return E == 1 ? 1.0 : (double)E
 // Workgroups to a block of rows for kernels of few rows, whose workgroups go round the block's tiles: as many as fill the CUs by the
 // estimate that is least for the CU with most tiles. `us`: what a tile's weights take a CU without a pause, which takes `need` waves (16-bit
 // weights six; 4-bit ones, which are converted, eight); a workgroup that waits for another's end starts late. As many as need no more
-// rounds, without regard to the tiles of a CU, were slower: ten rows of 512 experts of 2048 -> 1024, 16-bit weights, 14.2 against 11.8 us (with the search of then);
+// rounds, without regard to the tiles of a CU, were slower: ten rows of 512 experts of 2048 -> 1024, 16-bit weights, 14.2 against 11.8 us;
 // 4-bit, 16 rows of 4096 -> 6144 15.5 and 11.1.
 inline int64_t group_split(int64_t T, int64_t E, int64_t tiles, int64_t waves, int64_t fit, int64_t need, double us) {
     const int64_t slots = E == 1 ? (T + 15) / 16 : T / 16 + (int64_t)std::ceil(group_live(T, E));   // blocks of 16 rows
