@@ -124,18 +124,25 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
     if constexpr (XL) {
         // all rows' units in one run over the threads, eight loads under way
         const unsigned units = (unsigned)(kb + 3) / 4 * 16, all = units * s.rows, T = blockDim.x;
+        const unsigned dr = T / units, dc = T - dr * units;
+        unsigned r = threadIdx.x / units, c = threadIdx.x - r * units;
         for (unsigned u0 = threadIdx.x; u0 < all; u0 += 8 * T) {
             u32x4_t v[8];
+            unsigned to[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const unsigned u = u0 + i * T, r = u / units, c = u - r * units;
-                v[i] = mx4_buffer16(xr, u < all && c < (unsigned)kb * 4 ? r * (uint32_t)(2 * g.x_ld) + 16 * c : kMx4Out);
+                v[i] = mx4_buffer16(xr, u0 + i * T < all && c < (unsigned)kb * 4 ? r * (uint32_t)(2 * g.x_ld) + 16 * c : kMx4Out);
+                to[i] = r * stride + 16 * c;
+                r += dr;
+                c += dc;
+                if (c >= units) {
+                    c -= units;
+                    ++r;
+                }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned u = u0 + i * T, r = u / units, c = u - r * units;
-                if (u < all) *reinterpret_cast<u32x4_t*>(xl + r * stride + 16 * c) = v[i];
-            }
+            for (int i = 0; i < 8; ++i)
+                if (u0 + i * T < all) *reinterpret_cast<u32x4_t*>(xl + to[i]) = v[i];
         }
         __syncthreads();
     } else {
