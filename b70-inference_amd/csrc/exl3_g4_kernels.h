@@ -58,7 +58,7 @@ struct G4Scales {
 //   XL: x lies in LDS, and eight waves go round a tile's groups: two workgroups to a CU, one of which works while the other waits
 //   for its barrier (one row of 4096 -> 4096 7.0 us, 8.0 without; ten rows of 512 experts of 2048 -> 1024 8.9 and 9.8).
 //   Not XL, where x leaves room for one workgroup: a wave has one group of every tile, whose x stays in its registers.
-// Bound by the weights' bytes (6 rows of 5376 -> 21504, fp16 with zeros: 61 MB in 21.2 us, 2.9 TB/s) and by the instructions that take
+// Bound by the weights' bytes (6 rows of 5376 -> 21504, fp16 with zeros: 61 MB in 20.7 us, 3.0 TB/s) and by the instructions that take
 // the codes apart (9 us of each SIMD), for small matrices by the chain of launch, load, sum and store.
 constexpr int kG4Waves = 16, kG4Slice = 512;
 // Tiles between two barriers, each added by another wave: where all waves of a CU wait for one barrier (6 rows of 5376 -> 21504 with one
