@@ -530,6 +530,8 @@ def _act_mul(x, y, z, act, act_limit):
     require_device(x, y, z)
     if x.shape != y.shape or x.numel() != z.numel() or x.dtype != y.dtype or z.dtype != torch.float16:
         raise Exl3Error("act_mul: x, y same shape and dtype, z fp16 with as many elements")
+    if x.dtype not in (torch.float16, torch.float32):
+        raise Exl3Error(f"act_mul: x and y must be fp16 or fp32, got {x.dtype}")
     if not (x.is_contiguous() and y.is_contiguous() and z.is_contiguous()):
         raise Exl3Error("act_mul: tensors must be contiguous")
     dt = EXL3_F16 if x.dtype == torch.float16 else EXL3_F32
@@ -537,12 +539,12 @@ def _act_mul(x, y, z, act, act_limit):
 
 
 def silu_mul(x, y, z, act_limit):
-    """z = min(silu(x), L) * clamp(y, -L, L) (L = act_limit, 0 disables), written into z (fp16)."""
+    """z = min(silu(x), L) * clamp(y, -L, L) (L = act_limit, 0 disables) for x and y fp16 or fp32, written into z (fp16)."""
     _act_mul(x, y, z, ACT_SILU, act_limit)
 
 
 def gelu_mul(x, y, z, act_limit=0.0):
-    """z = gelu_tanh(x) * y, written into z (fp16)."""
+    """z = gelu_tanh(x) * y for x and y fp16 or fp32, written into z (fp16)."""
     _act_mul(x, y, z, ACT_GELU_TANH, 0.0)
 
 
