@@ -20,6 +20,13 @@ from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, sc
 from .mx4 import DTYPES, _bias, _out2, _rows
 
 _HALF = {torch.float16: EXL3_F16, torch.bfloat16: EXL3_BF16}
+_MOST_LD = 1 << 22                     # elements from row to row that the kernels' 32-bit offsets inside a block of rows allow
+
+
+def _g4_rows(x: torch.Tensor, k: int):
+    """_rows, in the kernels' reach (a copy where the rows are further apart)."""
+    x2, m, ld = _rows(x, k)
+    return (x2, m, ld) if ld <= _MOST_LD or ld == k else (x2.contiguous(), m, k)
 
 
 class G4Tensor:
@@ -79,7 +86,7 @@ class G4Linear:
         where = on_device("G4Linear", x, y, w.codes, self.bias)
         if x.dtype not in _HALF:
             x = x.half()
-        x2, m, ld = _rows(x, k)
+        x2, m, ld = _g4_rows(x, k)
         y2, y_ld = _out2("G4Linear", y, m, n)
         ws, need = scratch("exl3_g4_linear", x, m, k, n, w.group)
         with where:

@@ -17,8 +17,8 @@ from __future__ import annotations
 import torch
 
 from ._lib import EXL3_BF16, EXL3_F16, Exl3Error, check, lib, on_device, ptr, scratch, stream_of
-from .g4 import G4Tensor
-from .mx4 import DTYPES, _rows
+from .g4 import _MOST_LD, G4Tensor, _g4_rows
+from .mx4 import DTYPES
 
 _HALF = {torch.float16: EXL3_F16, torch.bfloat16: EXL3_BF16}
 _W_NK, _W_KN = 0, 1                    # exl3_grouped_w
@@ -31,14 +31,14 @@ def _ends(what: str, ends: torch.Tensor, E: int) -> torch.Tensor:
 
 
 def _rows2(what: str, name: str, x: torch.Tensor):
-    """x [T, k] with contiguous, non-overlapping rows (a copy where they are not) and their stride."""
+    """x [T, k] with contiguous, non-overlapping rows in the kernels' reach (a copy where they are not) and their stride."""
     if x.dim() != 2 or x.dtype not in _HALF:
         raise Exl3Error(f"{what}: {name} must be fp16 or bf16 [T, columns], got {x.dtype} {tuple(x.shape)}")
     T, k = x.shape
     if k == 0:
         raise Exl3Error(f"{what}: {name} has no columns")
     ld = x.stride(0) if T > 1 else k
-    if (k > 1 and x.stride(1) != 1) or ld < k:
+    if (k > 1 and x.stride(1) != 1) or ld < k or ld > _MOST_LD:
         x = x.contiguous()
         ld = k
     return x, ld
@@ -46,14 +46,14 @@ def _rows2(what: str, name: str, x: torch.Tensor):
 
 def _matrices(what: str, w: torch.Tensor):
     """w [E, N, K] as (tensor, layout, row stride, expert stride): rows of K or, for transposed matrices, of N (a copy of w where
-    neither is contiguous)."""
+    neither is contiguous, or where they are further apart than the kernels reach)."""
     E, n, k = w.shape
     se, sn, sk = w.stride()
     se = se if E > 1 else 0
     if se >= 0:
-        if (sk == 1 or k == 1) and (n == 1 or sn >= k):
+        if (sk == 1 or k == 1) and (n == 1 or k <= sn <= _MOST_LD):
             return w, _W_NK, sn if n > 1 else k, se
-        if (sn == 1 or n == 1) and (k == 1 or sk >= n):
+        if (sn == 1 or n == 1) and (k == 1 or n <= sk <= _MOST_LD):
             return w, _W_KN, sk if k > 1 else n, se
     return w.contiguous(), _W_NK, k, n * k
 
@@ -108,7 +108,7 @@ def _mm_g4(what: str, x, w: G4Tensor, ends, out, out_dtype):
         raise Exl3Error(f"{what}: x must be fp16 or bf16 [T, {k}], got {x.dtype} {tuple(x.shape)}")
     ends = _ends(what, ends, E)
     rest = out is None
-    x2, T, ld = _rows(x, k)
+    x2, T, ld = _g4_rows(x, k)
     out, o_ld = _out_rows(what, x, T, n, out, out_dtype)
     with on_device(what, x, w.codes, ends, out):
         rc = lib().exl3_grouped_g4(x2.data_ptr(), ld, _HALF[x.dtype], T, k, w.codes.data_ptr(), w.scales.data_ptr(),
