@@ -24,6 +24,11 @@ static int grouped_setup(const char* what, int dtype, int64_t T, int64_t n, int6
     return EXL3_OK;
 }
 
+// Matrices of n x k behind one another, or whose rows lie between one another's.
+static bool apart(int64_t E, int64_t n, int64_t k, int64_t ld, int64_t es) {
+    return E == 1 || es >= (n - 1) * ld + k || (es >= k && ld >= (E - 1) * es + k);
+}
+
 static bool units16(const void* p, int64_t ld, int64_t cols) { return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0; }
 
 // Microseconds that `tiles` tiles of `steps` steps take by an estimate from measurements: a step and the rest of a tile, with `occ`
@@ -103,7 +108,7 @@ static int weights_gradient(const void* dy, int64_t dy_ld, const void* x, int64_
     if (rc) return rc;
     EXL3_CHECK_ARG(accumulate == 0 || accumulate == 1, "%s: accumulate %d", what, accumulate);
     EXL3_CHECK_ARG((T <= 1 || (dy_ld >= n && x_ld >= k)) && dy_ld <= kMostWidth && x_ld <= kMostWidth && (n == 1 || dw_ld >= k) &&
-                       dw_ld <= ((int64_t)1 << 40) && dw_es >= 0 && dw_es <= ((int64_t)1 << 45) && (E == 1 || dw_es >= (n - 1) * dw_ld + k),
+                       dw_ld <= ((int64_t)1 << 40) && dw_es >= 0 && dw_es <= ((int64_t)1 << 45) && apart(E, n, k, dw_ld, dw_es),
                    "%s: bad strides (gradients %lld, rows %lld, output %lld and %lld)", what, (long long)dy_ld, (long long)x_ld,
                    (long long)dw_ld, (long long)dw_es);
     EXL3_CHECK_ARG((T == 0 || (dy && x && aligned(dy, 2) && aligned(x, 2))) && dw && aligned(dw, out_size(dw_dtype)),

@@ -166,7 +166,7 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
         a, a_ld, b, b_ld, m, k, sn, sk = x, x_ld, dy, dy_ld, k, n, sk, sn
     ld = sn if m > 1 else k
     es = se if E > 1 else m * ld
-    if (k > 1 and sk != 1) or ld < k or es < (m - 1) * ld + k:
+    if (k > 1 and sk != 1) or ld < k or (es < (m - 1) * ld + k and (es < k or ld < (E - 1) * es + k)):
         raise Exl3Error(f"{what}: matrices of out must have contiguous rows or columns and must not overlap")
     ws, need = scratch("exl3_grouped_mm_dw", x, T, m, k, E)
     with where:

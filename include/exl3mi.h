@@ -398,7 +398,8 @@ int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k
 
 /* Gradient with respect to the weights: dw[e, n, k] = sum over the rows t of expert e of dy[t, n] x[t, k], 0 for an expert without
  * rows; with accumulate 1 added to what dw holds (one rounding of the sum). dy [T, n] and x [T, k] fp16 or bf16 (`dtype`), dw fp16,
- * bf16 or fp32 [E, n, k] (row stride dw_ld, expert stride dw_es >= (n - 1) dw_ld + k). */
+ * bf16 or fp32 [E, n, k] (row stride dw_ld, expert stride dw_es; matrices one behind the other, dw_es >= (n - 1) dw_ld + k, or with rows
+ * between one another's, dw_ld >= (E - 1) dw_es + k). */
 int exl3_grouped_mm_dw(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, int64_t T, int64_t n, int64_t k,
                        const int32_t* ends, int64_t E, void* dw, int64_t dw_ld, int64_t dw_es, int dw_dtype, int accumulate,
                        void* stream);
