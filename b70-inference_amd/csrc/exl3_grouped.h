@@ -161,7 +161,7 @@ constexpr unsigned kChunk = 32;        // the CUs of an XCD
 // the compiler waits for the load before every transposing read, whatever it reads. What it brings is waited for by wait_step.
 __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint32_t at, const void* lds) {
     const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(r));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(r) : "m0", "memory");
 }
 
 }  // namespace exl3
