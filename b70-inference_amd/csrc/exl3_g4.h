@@ -109,6 +109,14 @@ __device__ __forceinline__ float g4_scale(uint32_t v, int bf16, bool in = true) 
     return __builtin_bit_cast(float, ((v << 16 & m) | (__builtin_bit_cast(uint32_t, h2f((uint16_t)v)) & ~m)) & k);
 }
 
+// Values that lanes of a wave pass one another through LDS: what was stored or read before is so for all of them. A wave's LDS accesses
+// are carried out in order, so this costs no instruction; it keeps the compiler from moving them past one another.
+__device__ __forceinline__ void g4_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // Block of rows, and its expert's first matrix row: slot s of blocks of BM rows.
 template <int BM>
 __device__ __forceinline__ GroupSlot g4_slot(const G4Args& g, unsigned slot) {

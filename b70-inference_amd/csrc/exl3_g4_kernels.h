@@ -168,6 +168,7 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
                 const Tile d(g, row0, rows, 16 * tile, kb, l);
                 raw.fix(g, d.b, d.srow, c0 + cs);
             }
+            g4_wave_sync();                                    // the group before is read
             if (q4 < SG)
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(XL ? 512 : 1024, 4) void g4_decode_kernel(G4Args g,
                     if constexpr (Z) lz[(4 * set + p) * 16] = raw.zero(k);
                 }
             raw.load(g, next.b, next.srow, cn + cs);
-            __builtin_amdgcn_wave_barrier();
+            g4_wave_sync();
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (4 * (c0 + u) < kb) {                       // uniform
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(256, OCC) void g4_wide_kernel(G4Args g) {
                     if constexpr (Z) lz[64 * i + lane] = raw.zero(k);
                 }
                 raw.load(g, sb, srow, c + 4 / SG);             // (past the last: not used)
-                __builtin_amdgcn_wave_barrier();
+                g4_wave_sync();
             }
             load_x(c + 1);
             const u32x4_t* xb = lds + ((c - c0) & 1) * kUnits;
