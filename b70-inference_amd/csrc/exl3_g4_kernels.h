@@ -56,7 +56,8 @@ struct G4Scales {
 // added in order through LDS. A group's weights and scales are asked for as soon as those of the one before are used, the next tile's
 // behind the last.
 //   XL: x lies in LDS, and eight waves go round a tile's groups: two workgroups to a CU, one of which works while the other waits
-//   for its barrier (one row of 4096 -> 4096 7.0 us, 8.0 without; ten rows of 512 experts of 2048 -> 1024 8.9 and 9.8).
+//   for its barrier (replayed from a graph, with and without: ten rows of 512 experts of 2048 -> 1024 7.6 and 7.9 us, six rows of
+//   4096 -> 4096 7.7 and 7.9, one row of it 5.9 and 5.6).
 //   Not XL, where x leaves room for one workgroup: a wave has one group of every tile, whose x stays in its registers.
 // Bound by the weights' bytes (6 rows of 5376 -> 21504, fp16 with zeros: 61 MB in 20.7 us, 3.0 TB/s) and by the instructions that take
 // the codes apart (9 us of each SIMD), for small matrices by the chain of launch, load, sum and store.

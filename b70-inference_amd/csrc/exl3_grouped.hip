@@ -73,7 +73,7 @@ static int rows_tile(int64_t T, int64_t E, int64_t n, int64_t k, bool few) {
     return best;
 }
 // Tile of the weights' gradient, and the parts of an expert's rows: few small matrices of many rows leave CUs idle (16384 rows over 8
-// experts of 512 x 512: 65 us whole, 44 in parts).
+// experts of 512 x 512, replayed from a graph: 41 us whole and 32 in parts where a router leans towards some experts, 28 and 25 where not).
 struct WeightsPlan {
     int tile, splits;
 };
@@ -187,6 +187,10 @@ int exl3_grouped_mm(const void* x, int64_t x_ld, int dtype, int64_t T, int64_t k
     g.vec = n % 4 == 0 && g.out_ld % 4 == 0 && aligned(out, 4 * out_size(out_dtype));
     g.rest = rest;
     const bool direct = units16(x, g.a_ld, k) && units16(w, w_ld, across ? n : k) && (E == 1 || w_es % 8 == 0);
+    // Tiles of operands that go through registers: 32 rows, or 128 where an expert has more than 48 on average (us, 32 and 128 rows: 40
+    // rows for each of 64 experts of 2049 -> 2048 176 and 186, 64 rows 215 and 194; of 4097 -> 4096 639 and 571, 804 and 616; for
+    // each of 16 experts 184 and 207, 240 and 223, of 1025 -> 513 20 and 28, 20 and 29). By rows alone, so not the faster one everywhere:
+    // 256 rows of one matrix of 4097 -> 4096 60 and 85.
     const int64_t mean = T / E;
     int tile = !direct ? (mean <= 48 ? kTileAny32 : kTileAny128) : rows_tile(T, E, n, k, !across && k <= 8192);
     const int want = env_int("EXL3MI_GROUPED_TILE", 0);

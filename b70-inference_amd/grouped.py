@@ -7,7 +7,7 @@ expert. moe_align sorts a routing: ends = counts.cumsum(0, dtype=torch.int32), x
   * grouped_mm(x, w, ends)       y[t] = w[e] @ x[t]; w 16-bit [E, N, K] or a G4Tensor (4-bit weights with group scales)
   * grouped_mm_dx(dy, w, ends)   dx[t] = dy[t] @ w[e], the gradient with respect to the rows
   * grouped_mm_dw(dy, x, ends)   dw[e] = dy[rows of e]^T @ x[rows of e], the gradient with respect to the weights
-There is no autograd graph: pass the gradients on. Rows and weights fp16 or bf16, sums fp32 in an order fixed by the sizes, one rounding
+There is no autograd graph: pass the gradients on. Rows and weights fp16 or bf16, sums fp32 in an order fixed by the sizes, layouts and alignments, one rounding
 to out's type. Tensors live on the GPU; every op is asynchronous on the current stream of its tensors' device and has scratch of its
 own where it needs some (calls may overlap on streams and threads, and can be captured without a warm-up). The reference has no counterpart: its experts are
 EXL3 only.

@@ -385,7 +385,7 @@ int exl3_route_balance_grad(const float* logits, int64_t ld, int64_t M, int64_t 
  * ascending, at most T (other values lead to no access out of range, but to rows that belong to no or to several experts). An
  * expert may have no rows; rows from ends[E - 1] on belong to none. Any sizes (columns at most 2^22, as the row strides);
  * operands of 16-byte aligned rows of whole multiples of eight values are read fastest. Outputs must not overlap operands. Sums are fp32 in an order fixed by the
- * sizes, with one rounding. No reference counterpart (the reference's experts are EXL3 only). */
+ * sizes, layouts and alignments, with one rounding. No reference counterpart (the reference's experts are EXL3 only). */
 enum exl3_grouped_w { EXL3_GROUPED_W_NK = 0, EXL3_GROUPED_W_KN = 1 };
 
 /* out[t, n] = sum over k of x[t, k] W_e(n, k) for the rows t of every expert e: x fp16 or bf16 (`dtype`) [T, k] (row stride x_ld), W
@@ -415,7 +415,8 @@ int exl3_grouped_mm_dw_in(const void* dy, int64_t dy_ld, const void* x, int64_t 
  * (32, 64 or a multiple of 128, others EXL3_ERR_UNSUPPORTED) of an output one scale s (fp16 or bf16) and one z from 0 to 15 (8 with
  * zeros NULL). A matrix of n outputs and k inputs (k a multiple of the group) is codes uint8 [n, k / 2] (16-byte aligned), scales
  * [n, k / group], zeros uint8 [n, k / group], all contiguous. No weight is rounded: fp32 sums of exact products with q - z, times s,
- * in an order fixed by the sizes; one rounding. No reference counterpart. */
+ * in an order fixed by the sizes; one rounding. (The sums are taken before s: bf16 rows of magnitudes above 2^100 may leave fp32 there.) No
+ * reference counterpart. */
 
 /* C[m, n] = x @ W^T (+ bias) for x fp16 or bf16 [m, k] (row stride x_ld, rows 16-byte aligned), bias fp32 [n] or NULL, C fp16, bf16
  * or fp32 (row stride c_ld). */
